@@ -176,6 +176,7 @@ def prepare(case, seed):
         opt = AdamW(params, lr=LR, betas=BETAS, eps=ADAM_EPS, weight_decay=WD,
                     state_bits=c["bits"], stochastic_rounding=c["sr"], seed=SEED0)
         for p, (s, at, k) in zip(params, lay):
+            p.grad_dtype = gt        # the gradients may be wider than the weights
             p.grad = st["G"][at: at + k].view(s)
             if c["bits"] == 32:
                 state = dict(exp_avg=st["M"][at: at + k].view(s), exp_avg_sq=st["V"][at: at + k].view(s))
