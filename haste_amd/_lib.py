@@ -34,6 +34,17 @@ class SgdTensor(ctypes.Structure):
     _fields_ = [("w", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p),
                 ("n", ctypes.c_int64), ("offset0", ctypes.c_uint64)]
 
+class GradTensor(ctypes.Structure):
+    """haste_grad_tensor of include/haste_ffi.h."""
+    _fields_ = [("g", ctypes.c_void_p), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """haste_adamw_tensor of include/haste_ffi.h."""
+    _fields_ = [("w", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("n", ctypes.c_int64), ("stream", ctypes.c_uint32)]
+
 
 # Every symbol declared in include/haste_ffi.h: name -> (restype, argtypes).
 _P = ctypes.c_void_p
@@ -41,6 +52,7 @@ _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _U64 = ctypes.c_uint64
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 SIGNATURES = {
     "haste_last_error": (ctypes.c_char_p, []),
     "haste_abi_version": (ctypes.c_int, []),
@@ -127,6 +139,15 @@ SIGNATURES = {
     "haste_rewire_ex": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _I64, _I64,
                                        _I64, _I64, _I32, _F32, _I64, _I32, _I32, _F32, _U64,
                                        _P]),
+    "haste_layer_norm": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _F64,
+                                        _I32, _I32, _P]),
+    "haste_layer_norm_bwd_workspace_size": (_I64, [_I64, _I64]),
+    "haste_layer_norm_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P,
+                                            _I64, _I64, _I64, _I32, _I32, _P]),
+    "haste_grad_norm_workspace_size": (_I64, [_I32]),
+    "haste_grad_norm": (ctypes.c_int, [_P, _I32, _F64, _P, _P, _I64, _P]),
+    "haste_adamw_step": (ctypes.c_int, [_P, _I32, _I32, _I32, _I32, _F64, _F64, _F64, _F64, _F64,
+                                        _I64, _I32, _U64, _P, _P]),
 }
 
 _lib = None

@@ -1,11 +1,13 @@
-"""Public op ``group_ffi_mul`` (reference: shared_ffi/ops.py:7-24)."""
+"""Public ops: ``group_ffi_mul`` (reference: shared_ffi/ops.py:7-24), ``head_tail_logits``, and
+``layer_norm`` for the encoder in front of an FFI layer."""
 from typing import Optional
 
 import torch
 
 from . import bindings as _bindings
+from .layer_norm import layer_norm
 
-__all__ = ["group_ffi_mul", "head_tail_logits"]
+__all__ = ["group_ffi_mul", "head_tail_logits", "layer_norm"]
 
 
 def group_ffi_mul(features: torch.Tensor,

@@ -1,0 +1,209 @@
+"""AdamW over many tensors at once, for the encoder in front of an FFI layer, and the norm that
+clips its gradients.
+
+``AdamW`` takes the place of torch.optim.AdamW (decoupled weight decay, bias-corrected
+moments, in fp32); beside it:
+  * bfloat16 and float16 parameters are stepped in place, with stochastic rounding (as
+    SRSgd does; per param group ``seed`` is read and then incremented every step), so that no
+    fp32 copy of them is needed; float32 parameters are rounded to nearest;
+  * ``state_bits=8`` keeps the first moment and the root of the second as float8_e4m3fn with
+    one power-of-two scale (float8_e8m0fnu) for each 128 elements, rounded stochastically:
+    2.03 bytes an element instead of 8;
+  * ``step(grad_scale=...)`` takes a factor for all gradients that is on the device, such as
+    ``grad_norm``'s; a NaN there leaves parameters and states as they are.
+The tensors of a group are stepped by one launch for each 60 of them (and for each dtype of
+parameters and gradients, and each count of steps).  Random bits: Philox4x32-10 keyed by the
+seed, with the position of a tensor in its group and of an element in it as counters, so a step's
+results depend on nothing else.
+
+State of a parameter (created at its first step): ``step``, an int; with 32 bits ``exp_avg`` and
+``exp_avg_sq``, fp32 of its shape; with 8 bits ``exp_avg`` and ``rms`` (codes, of its elements in
+order, padded to a multiple of 128) with ``exp_avg_scale`` and ``rms_scale``.
+"""
+from __future__ import annotations
+
+import math
+from typing import Iterable, Tuple
+
+import torch
+from torch.optim import Optimizer
+
+from . import _C, _lib
+from .optim_sr import run_hooked
+
+__all__ = ["AdamW", "grad_norm"]
+
+STATE_BLOCK = 128  # elements of an 8-bit state that share a scale
+_STATE = {32: {"exp_avg": torch.float32, "exp_avg_sq": torch.float32},
+          8: {"exp_avg": torch.float8_e4m3fn, "rms": torch.float8_e4m3fn,
+              "exp_avg_scale": torch.float8_e8m0fnu, "rms_scale": torch.float8_e8m0fnu}}
+
+
+def _dense(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t with its values in memory in order, as the kernels read it."""
+    if t.layout is not torch.strided:
+        raise RuntimeError(f"{name} must be dense (got {t.layout})")
+    if t.is_neg():
+        t = t.resolve_neg()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def grad_norm(tensors: Iterable[torch.Tensor], max_norm: float = math.inf
+              ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(norm, coef): the 2-norm over all the tensors and min(1, max_norm / (norm + 1e-6)), the
+    factor of torch.nn.utils.clip_grad_norm_, as fp32 scalars on their device, without a
+    sync and without touching the tensors: ``AdamW.step(grad_scale=coef)`` applies it.
+    coef is NaN where norm is not finite."""
+    tensors = [_dense(t, "gradients") for t in tensors]
+    if not tensors:
+        raise RuntimeError("grad_norm: no tensors")
+    dev = tensors[0].device
+    for t in tensors:
+        _C.require_device(t, "gradients")
+        if t.device != dev:
+            raise RuntimeError(f"grad_norm: tensors must be on one device (got {dev}, {t.device})")
+    n = len(tensors)
+    arr = (_lib.GradTensor * n)(*[(t.data_ptr(), t.numel(), _C.dtype_code(t.dtype))
+                                  for t in tensors])
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    size = _lib.lib().haste_grad_norm_workspace_size(n)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _lib.call("haste_grad_norm", arr, n, float(max_norm), out.data_ptr(), ws.data_ptr(), size,
+              _C.stream_of(out))
+    return out[0], out[1]
+
+
+class AdamW(Optimizer):
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
+                 stochastic_rounding: bool = True, seed: int = 123):
+        if not lr >= 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not eps >= 0.0:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"Invalid beta parameters: {betas}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if state_bits not in _STATE:
+            raise ValueError(f"state_bits must be 8 or 32 (got {state_bits})")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
+                                      weight_decay=weight_decay, state_bits=state_bits,
+                                      stochastic_rounding=stochastic_rounding, seed=seed))
+
+    @staticmethod
+    def _state_size(key: str, bits: int, p: torch.Tensor) -> int:
+        blocks = -(-p.numel() // STATE_BLOCK)
+        return p.numel() if bits == 32 else blocks if key.endswith("_scale") else blocks * STATE_BLOCK
+
+    def _new_state(self, p: torch.Tensor, bits: int) -> dict:
+        state = self.state[p]
+        state["step"] = 0
+        for key, dtype in _STATE[bits].items():
+            if bits == 32:
+                state[key] = torch.zeros(p.shape, dtype=dtype, device=p.device)
+            else:  # code 127 of a scale is 1
+                fill = 127 if key.endswith("_scale") else 0
+                state[key] = torch.full((self._state_size(key, bits, p),), fill, dtype=torch.uint8,
+                                        device=p.device).view(dtype)
+        return state
+
+    def load_state_dict(self, state_dict) -> None:
+        # torch casts floating-point state to the parameter's dtype: put the states back as they
+        # were saved
+        saved = {k: dict(v) for k, v in state_dict["state"].items()}
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            want = _STATE[group["state_bits"]]
+            for p in group["params"]:
+                got = saved.get(ids.pop(0))
+                if not got:
+                    continue
+                for key, dtype in want.items():
+                    t = got.get(key)
+                    if not isinstance(t, torch.Tensor) or t.dtype != dtype or \
+                            t.numel() != self._state_size(key, group["state_bits"], p):
+                        raise ValueError(f"AdamW: saved state {key} does not fit a parameter of "
+                                         f"shape {list(p.shape)} with {group['state_bits']}-bit states")
+                    self.state[p][key] = t.to(device=p.device).clone()
+                self.state[p]["step"] = int(got["step"])
+
+    def step(self, closure=None, *, grad_scale=None):
+        """One step, torch.optim.Optimizer.step semantics, hooks included.  ``grad_scale``: an
+        fp32 tensor of one element on the parameters' device that multiplies every gradient
+        as it is read (1 when None); where it is NaN the kernels change no parameter and no
+        moment (the counts of steps and the seed go on)."""
+        return run_hooked(self, "_adamw_step", (closure,),
+                          {} if grad_scale is None else {"grad_scale": grad_scale})
+
+    step.hooked = True  # Optimizer.__init__ then leaves it unwrapped
+
+    @torch.no_grad()
+    def _adamw_step(self, closure=None, *, grad_scale=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured: the count of steps and the seed "
+                               "are the host's, and a replay would repeat one step's")
+        if grad_scale is not None:
+            _C.require_device(grad_scale, "grad_scale")
+            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
+                raise RuntimeError(f"grad_scale must be one float32 (got {list(grad_scale.shape)} "
+                                   f"{grad_scale.dtype})")
+        for group in self.param_groups:
+            self._step_group(group, grad_scale)
+        return loss
+
+    def _step_group(self, group, grad_scale) -> None:
+        bits, device = group["state_bits"], None
+        batches, stepped, copies, keep = {}, [], [], []
+        for index, p in enumerate(group["params"]):
+            grad = p.grad
+            if grad is None:
+                continue
+            _C.require_device(p, "parameters")
+            device = p.device if device is None else device
+            for t, name in ((grad, "gradient"), (grad_scale, "grad_scale"), (p, "parameter")):
+                if t is not None and t.device != device:
+                    raise RuntimeError(f"AdamW: {name} is on {t.device}, its group on {device}")
+            if grad.numel() != p.numel():
+                raise RuntimeError(f"AdamW: gradient {list(grad.shape)} of a parameter "
+                                   f"{list(p.shape)}")
+            w, g = _dense(p.detach(), "parameters"), _dense(grad, "gradients")
+            state = self.state[p]
+            if "step" not in state:
+                state = self._new_state(p, bits)
+            tensors = []
+            for key, dtype in _STATE[bits].items():
+                t = state[key]
+                if t.dtype != dtype or t.device != device or not t.is_contiguous() or \
+                        t.numel() != self._state_size(key, bits, p):
+                    raise RuntimeError(f"AdamW: state {key} does not fit a parameter of shape "
+                                       f"{list(p.shape)} with {bits}-bit states")
+                tensors.append(t.data_ptr())
+            if bits == 32:
+                tensors += [None, None]
+            state["step"] += 1
+            rows = batches.setdefault((_C.dtype_code(w.dtype), _C.dtype_code(g.dtype),
+                                       state["step"]), [])
+            rows.append((w.data_ptr(), g.data_ptr(), *tensors, p.numel(), index))
+            keep.append((w, g))
+            stepped.append(p)
+            if w.data_ptr() != p.data_ptr():
+                copies.append((p, w))
+        seed = group["seed"]
+        group["seed"] += 1
+        scale = None if grad_scale is None else grad_scale.data_ptr()
+        for (wd, gd, step), rows in batches.items():
+            arr = (_lib.AdamwTensor * len(rows))(*rows)
+            _lib.call("haste_adamw_step", arr, len(rows), wd, gd, bits, float(group["lr"]),
+                      float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
+                      float(group["weight_decay"]), step, int(bool(group["stochastic_rounding"])),
+                      int(seed), scale, _C.stream_of(keep[0][0]))
+        for p, w in copies:
+            p.copy_(w)
+        if stepped:  # written through raw pointers: move the version counters as torch would
+            torch.autograd.graph.increment_version(stepped)

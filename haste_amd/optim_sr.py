@@ -131,6 +131,30 @@ def _step_f32(f32s, lr, wd, mu, mom_on) -> None:
         [t for p, _, m in f32s for t in ((p,) if m is None else (p, m))])
 
 
+def run_hooked(optimizer, inner: str, args: tuple, kwargs: dict):
+    """Call the optimizer's method ``inner`` between its step hooks in torch's order: the
+    pre-hooks (global, then its own) first, which may replace the arguments, the
+    post-hooks (its own, then global) after."""
+    pre = _torch_optimizer._global_optimizer_pre_hooks
+    post = _torch_optimizer._global_optimizer_post_hooks
+    if not (pre or post or optimizer._optimizer_step_pre_hooks
+            or optimizer._optimizer_step_post_hooks):
+        return getattr(optimizer, inner)(*args, **kwargs)
+    args = (optimizer, *args)
+    for hook in chain(pre.values(), optimizer._optimizer_step_pre_hooks.values()):
+        result = hook(optimizer, args, kwargs)
+        if result is not None:
+            if isinstance(result, tuple) and len(result) == 2:
+                args, kwargs = result
+            else:
+                raise RuntimeError(f"{hook} must return None or a tuple of (new_args, "
+                                   f"new_kwargs), but got {result}.")
+    out = getattr(args[0], inner)(*args[1:], **kwargs)
+    for hook in chain(optimizer._optimizer_step_post_hooks.values(), post.values()):
+        hook(optimizer, args, kwargs)
+    return out
+
+
 class SRSgd(Optimizer):
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.0,
                  momentum: float = 0.0, use_momentum: bool = True,
@@ -196,23 +220,7 @@ class SRSgd(Optimizer):
         which saves about 15 us of host time per step, and runs the hooks
         itself.  The step shows in a torch profile through its kernels and
         library calls, without an ``Optimizer.step#SRSgd.step`` scope."""
-        pre = _torch_optimizer._global_optimizer_pre_hooks
-        post = _torch_optimizer._global_optimizer_post_hooks
-        if not (pre or post or self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks):
-            return self._sr_step(closure)
-        args, kwargs = (self, closure), {}
-        for hook in chain(pre.values(), self._optimizer_step_pre_hooks.values()):
-            result = hook(self, args, kwargs)
-            if result is not None:
-                if isinstance(result, tuple) and len(result) == 2:
-                    args, kwargs = result
-                else:
-                    raise RuntimeError(f"{hook} must return None or a tuple of (new_args, "
-                                       f"new_kwargs), but got {result}.")
-        out = args[0]._sr_step(*args[1:], **kwargs)
-        for hook in chain(self._optimizer_step_post_hooks.values(), post.values()):
-            hook(self, args, kwargs)
-        return out
+        return run_hooked(self, "_sr_step", (closure,), {})
 
     step.hooked = True  # Optimizer.__init__ then leaves it unwrapped
 

@@ -576,6 +576,91 @@ int haste_rewire_ex(void* W, int32_t w_dtype, int32_t* idx, const void* grad, in
                     int32_t regrow_mode, int32_t init_mode, float bound, uint64_t seed,
                     void* stream);
 
+/*
+ * Layer norm over the last axis of rows [N, D], fp32 statistics:
+ *   h = RNE(x + res) if res, else x;  mean, var = moments of the row's h (var / D)
+ *   y = RNE((h - mean) * rstd * w + b),  rstd = 1 / sqrt(var + eps)
+ * x and res have row pitches ldx and ldres (elements, >= D; 0 reads one row for all),
+ * y and h are [N, D] contiguous.  dtype of x, res, y, h: bf16, f16 or f32; w_dtype of w
+ * and b: the same or f32.  res, b may be NULL; h is required with res and unused
+ * without.  stats [N, 2] (mean, rstd) is written where not NULL.  Element
+ * alignment is enough for every tensor.
+ */
+int haste_layer_norm(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w,
+                     const void* b, void* y, void* h, float* stats, int64_t N, int64_t D,
+                     double eps, int32_t dtype, int32_t w_dtype, void* stream);
+
+/*
+ * Its gradients, from the h, w and stats of the forward:
+ *   n = (h - mean) * rstd;  a = dy * w
+ *   dx = RNE(rstd * (a - mean_D(a) - n * mean_D(a * n)) + dh)   (dh the gradient of h, or NULL)
+ *   dw = sum_N(dy * n), db = sum_N(dy)                          (fp32 sums in a fixed order)
+ * dy, dh, h have row pitches; dx is [N, D] contiguous (the gradient of x, and of res).
+ * Any of dx, dw and db may be NULL (not computed).  dtype and w_dtype as above.  ws: workspace of
+ * haste_layer_norm_bwd_workspace_size(N, D) bytes (16-byte aligned), needed for dw or db.
+ */
+int64_t haste_layer_norm_bwd_workspace_size(int64_t N, int64_t D);
+int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                         const void* h, int64_t ldh, const void* w, const float* stats, void* dx,
+                         void* dw, void* db, void* ws, int64_t ws_bytes, int64_t N, int64_t D,
+                         int32_t dtype, int32_t w_dtype, void* stream);
+
+/*
+ * The 2-norm over all of several tensors, and the factor that clips it:
+ *   out[0] = norm = sqrt(sum g^2),  out[1] = min(1, max_norm / (norm + 1e-6)),
+ * out[1] = NaN where norm is not finite (haste_adamw_step then skips its step).
+ * dtype of each tensor: bf16, f16 or f32.  Sums are in a fixed order.  ws: workspace of
+ * haste_grad_norm_workspace_size(count) bytes (8-byte aligned).
+ */
+typedef struct haste_grad_tensor {
+    const void* g;
+    int64_t n;
+    int32_t dtype;
+} haste_grad_tensor;
+
+int64_t haste_grad_norm_workspace_size(int32_t count);
+int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, double max_norm, float* out,
+                    void* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * One AdamW step of several tensors, in place, all after `step` steps (this one counted):
+ *   g  = grad * (*grad_scale)              (1 where grad_scale is NULL)
+ *   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2
+ *   w' = w (1 - lr wd) - lr / (1 - beta1^step) m' / (sqrt(v' / (1 - beta2^step)) + eps)
+ * in fp32.  Where *grad_scale is NaN the kernels change nothing.  w_dtype and g_dtype: bf16,
+ * f16 or f32 for all of the call's tensors.  With do_sr 16-bit weights are rounded
+ * stochastically, else to nearest.
+ * state_bits 32: m and v are fp32 [n], m_scale and v_scale unused.
+ * state_bits 8: m holds m and v holds u = sqrt(v), both as e4m3 codes [ceil(n / 128) * 128] with
+ * one E8M0 scale (2^(code - 127)) for each 128 elements in m_scale and v_scale
+ * [ceil(n / 128)]: the power of two that puts the block's largest value in [128, 256).  Both
+ * are rounded stochastically whatever do_sr is; u > 0 is kept above 0; what is not finite
+ * becomes e4m3's NaN and does not count for the scale.
+ * Random bits: Philox4x32-10 with key `seed` and counter (k low, k high, t.stream, 0).  With
+ * 32-bit states element i takes half i & 1 (0: the low one) of word (i & 7) / 2 for k = i / 8.
+ * With 8-bit states it takes, for k = i / 4, the low half of word i & 3 for w, its high half for
+ * m, and the high half of word (i + 1) & 3 for u.  A draw r in [0, 2^16) rounds up where
+ * what is cut off, in units of the result's last place, plus r / 2^16 (f16 weights: the upper 13
+ * bits of r over 2^13) reaches 1.
+ * w and g need the alignment of their elements, m and v 16 bytes (8-bit: 8 bytes).  n == 0
+ * entries are skipped.
+ */
+typedef struct haste_adamw_tensor {
+    void* w;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* m_scale;
+    uint8_t* v_scale;
+    int64_t n;
+    uint32_t stream;
+} haste_adamw_tensor;
+
+int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count, int32_t w_dtype,
+                     int32_t g_dtype, int32_t state_bits, double lr, double beta1, double beta2,
+                     double eps, double wd, int64_t step, int32_t do_sr, uint64_t seed,
+                     const float* grad_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
