@@ -8,7 +8,11 @@ namespace haste {
 namespace {
 
 constexpr int kBlock = 128;    // elements of an 8-bit state that share a scale
-constexpr int kMaxSegs = 60;   // tensors of one launch: their table fills its 4 KB of arguments
+constexpr int kMaxSegs = 64;   // tensors of one launch: a lane to each when a wave looks its own up,
+                               // and their table stays within 4 KB of kernel arguments
+constexpr int kThreads = 256;
+constexpr int kPiece = kThreads * 8;  // elements that a workgroup steps at a time
+constexpr int kPieces = 2;            // pieces of a workgroup
 
 struct AdamSeg {
     void* w;
@@ -17,16 +21,16 @@ struct AdamSeg {
     void* v;
     uint8_t* ms;
     uint8_t* vs;
-    int64_t n;
-    uint32_t blk0;    // first workgroup of this tensor
-    uint32_t stream;
+    uint64_t n_stream;  // elements, and the tensor's stream << 40
 };
 struct AdamBatch {
+    uint32_t blk0[kMaxSegs];  // first workgroup of each tensor
     AdamSeg s[kMaxSegs];
     int32_t count;
 };
 struct AdamArgs {
     float b1, c1, b2, c2;  // beta1, 1 - beta1, beta2, 1 - beta2
+    float root_b2;         // sqrt(beta2)
     float decay, lr, rcorr, eps;  // 1 - lr wd, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
     uint32_t k0, k1;
     int32_t do_sr;
@@ -37,12 +41,20 @@ struct GradSeg {
     const void* g;
     int64_t n;
     int32_t dtype;
-    uint32_t blk0;
 };
 struct GradBatch {
+    uint32_t blk0[kMaxSegs];
     GradSeg s[kMaxSegs];
     int32_t count;
 };
+
+// The tensor that workgroup (or piece) `blk` belongs to: every lane compares one start.
+template <typename B>
+__device__ __forceinline__ int find_seg(const B& b, uint32_t blk) {
+    const int lane = threadIdx.x & 63;
+    const bool at = lane < b.count && b.blk0[lane] <= blk;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(at)) - 1);
+}
 
 // The four words of Philox4x32-10 (philox_w0's function).
 __device__ __forceinline__ u32x4 philox_words(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t k0,
@@ -61,121 +73,240 @@ __device__ __forceinline__ u32x4 philox_words(uint32_t c0, uint32_t c1, uint32_t
     return u32x4{c0, c1, c2, c3};
 }
 
-// |x| in units of its spacing with MANT mantissa bits and smallest normal 2^LOW, plus `up` in
-// [0, 1), cut to a whole number; `unit` is that spacing.
-template <int MANT, int LOW>
-__device__ __forceinline__ float cut_units(float x, float up, float* unit) {
-    const uint32_t e = max(__float_as_uint(x) & 0x7F800000u, (uint32_t)(127 + LOW) << 23);
-    *unit = __uint_as_float(e - ((uint32_t)MANT << 23));
-    return floorf(fabsf(x) * __uint_as_float((254u << 23) - (e - ((uint32_t)MANT << 23))) + up);
+// w as fp16, rounded by the 16 bits r: |w| in units of its spacing (10 mantissa bits, smallest
+// normal 2^-14) plus the upper 13 bits of r over 2^13, cut to a whole number.
+__device__ __forceinline__ uint32_t sr_f16(float w, uint32_t r) {
+    const uint32_t e = max(__float_as_uint(w) & 0x7F800000u, (uint32_t)(127 - 14) << 23);
+    const float unit = __uint_as_float(e - (10u << 23));
+    const float t = floorf(fabsf(w) * __uint_as_float((264u << 23) - e) + (float)(r >> 3) * 0x1p-13f);
+    return f32_to_f16_rne(fabsf(w) < 65536.f ? copysignf(t * unit, w) : w);
 }
 
-// x as an e4m3 code, rounded by the 16 bits r; with KEEP what is above zero stays so.  |x| is
-// below 2^8 or not finite (NaN then).
+template <int C>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+    return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, C, 0xF, 0xF, true));
+}
+// The maximum over the 16 lanes of a row, in all of them (rotations by 8, 4, 2 and 1).
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+    return dpp_max<0x121>(dpp_max<0x122>(dpp_max<0x124>(dpp_max<0x128>(x))));
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// The E8M0 code of the power of two that puts the row's largest |x| in [128, 256).  As whole
+// numbers the patterns of |x| are in its order, with infinities and NaN above all others: only
+// where one is met are the finite ones looked for.
+__device__ __forceinline__ uint32_t scale_code(const float* x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    top = row_max(top);
+    if (__any(top >= kInfBits)) {
+        top = 0;
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t a = __float_as_uint(x[e]) & 0x7FFFFFFFu;
+            top = max(top, a < kInfBits ? a : 0u);
+        }
+        top = row_max(top);
+    }
+    return (uint32_t)max((int)(top >> 23) - 7, 1);
+}
+
+__device__ __forceinline__ float pow2_code(uint32_t code) { return __uint_as_float(code << 23); }
+
+// Eight values as e4m3 codes under the scale of `code`, x[e] rounded up by the upper half of
+// seed[e]: v_cvt_sr_fp8_f32 adds the seed's upper 20 bits to what it cuts off, subnormals
+// included, and makes NaN of what is not finite.  KEEP: x > 0 does not become 0.
 template <bool KEEP>
-__device__ __forceinline__ uint32_t cut_e4m3(float x, uint32_t r) {
-    float unit;
-    float t = cut_units<3, -6>(x, (float)r * 0x1p-16f, &unit);
-    if (KEEP && x > 0.f) t = fmaxf(t, 1.f);
-    t = copysignf(t * unit, x);
-    if (!(fabsf(x) < 512.f)) return 0x7Fu;
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false) & 0xFFu;
+__device__ __forceinline__ u32x2 cut_e4m3(const float* x, uint32_t code, const uint32_t* seed) {
+    const float inv = pow2_code(254u - code);
+    u32x2 out = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float s = x[e] * inv;
+        if (KEEP) s = x[e] > 0.f && s < 0x1p-9f ? 0x1p-9f : s;
+        const int sd = (int)(seed[e] & 0xFFFF0000u);
+        int& o = reinterpret_cast<int*>(&out)[e / 4];
+        switch (e & 3) {
+        case 0: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 0); break;
+        case 1: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 1); break;
+        case 2: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 2); break;
+        default: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 3);
+        }
+    }
+    return out;
 }
 
-__device__ __forceinline__ float e4m3_to_f32(uint32_t c) {
-    return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
+__device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], true);
+        f[4 * h] = lo[0];
+        f[4 * h + 1] = lo[1];
+        f[4 * h + 2] = hi[0];
+        f[4 * h + 3] = hi[1];
+    }
 }
 
-// w as 16 bits of type WT, rounded by the 16 bits r.
-template <int WT>
-__device__ __forceinline__ uint32_t cut_16(float w, uint32_t r) {
-    if constexpr (WT == HASTE_DTYPE_BF16) return sr_bf16(w, r);
-    if (!(fabsf(w) < 65536.f)) return f32_to_f16_rne(w);
-    float unit;
-    const float t = cut_units<10, -14>(w, (float)(r >> 3) * 0x1p-13f, &unit);
-    return f32_to_f16_rne(copysignf(t * unit, w));
-}
-
-template <typename B>
-__device__ __forceinline__ int find_seg(const B& b, uint32_t blk) {
-    int t = 0;
-    for (int k = 1; k < b.count; ++k)
-        if (blk >= b.s[k].blk0) t = k;
-    return t;
-}
-
-// A thread to an element, a workgroup to a block of 128.
+// Eight consecutive elements of a tensor, as loaded.
 template <int WT, int GT, bool Q8>
-__global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamBatch b, const AdamArgs a) {
-    __shared__ float top[2][kBlock / 64];
+struct AdamElems {
+    Elems8<WT> w;
+    Elems8<GT> g;
+    Elems8<HASTE_DTYPE_F32> m, v;  // fp32 states
+    u32x2 m8, u8;                  // codes
+    uint32_t ms, us;
+};
+
+// FULL: all of the workgroup's elements are the tensor's; else `count` (of eight) are.
+template <int WT, int GT, bool Q8, bool FULL>
+__device__ __forceinline__ void adam_load(AdamElems<WT, GT, Q8>& x, const AdamSeg& s, int64_t i,
+                                          int64_t count) {
+    if constexpr (FULL) {
+        x.w = load8<WT>(s.w, i);
+        x.g = load8<GT>(s.g, i);
+    } else {
+        x.w = load8_part<WT>(s.w, i, count);
+        x.g = load8_part<GT>(s.g, i, count);
+    }
+    if constexpr (Q8) {
+        x.m8 = x.u8 = u32x2{0, 0};
+        x.ms = x.us = 127;
+        if (FULL || count > 0) {
+            x.m8 = *reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.m) + i);
+            x.u8 = *reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.v) + i);
+            x.ms = s.ms[i / kBlock];
+            x.us = s.vs[i / kBlock];
+        }
+    } else if constexpr (FULL) {
+        x.m = load8<HASTE_DTYPE_F32>(s.m, i);
+        x.v = load8<HASTE_DTYPE_F32>(s.v, i);
+    } else {
+        x.m = load8_part<HASTE_DTYPE_F32>(s.m, i, count);
+        x.v = load8_part<HASTE_DTYPE_F32>(s.v, i, count);
+    }
+}
+
+template <int WT, int GT, bool Q8, bool FULL>
+__device__ __forceinline__ void adam_step(const AdamElems<WT, GT, Q8>& x, const AdamSeg& s,
+                                          const AdamArgs& a, float gs, int64_t i, int64_t count) {
+    float w[8], g[8], m[8], v[8], u[8];
+    unpack8<WT>(x.w, w);
+    unpack8<GT>(x.g, g);
+    if constexpr (Q8) {
+        from_e4m3(x.m8, m);
+        from_e4m3(x.u8, u);
+        const float fm = a.b1 * pow2_code(x.ms), fu = a.root_b2 * pow2_code(x.us);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!FULL && e >= count) m[e] = u[e] = 0.f;
+            g[e] *= gs;
+            m[e] = m[e] * fm + a.c1 * g[e];
+            u[e] *= fu;
+            u[e] = u[e] * u[e] + a.c2 * g[e] * g[e];
+        }
+    } else {
+        unpack8<HASTE_DTYPE_F32>(x.m, m);
+        unpack8<HASTE_DTYPE_F32>(x.v, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            g[e] *= gs;
+            m[e] = a.b1 * m[e] + a.c1 * g[e];
+            u[e] = v[e] = a.b2 * v[e] + a.c2 * g[e] * g[e];
+        }
+        if constexpr (FULL) {
+            store8<HASTE_DTYPE_F32>(s.m, i, pack8<HASTE_DTYPE_F32>(m));
+            store8<HASTE_DTYPE_F32>(s.v, i, pack8<HASTE_DTYPE_F32>(v));
+        } else {
+            store8_part<HASTE_DTYPE_F32>(s.m, i, pack8<HASTE_DTYPE_F32>(m), count);
+            store8_part<HASTE_DTYPE_F32>(s.v, i, pack8<HASTE_DTYPE_F32>(v), count);
+        }
+    }
+    // the hardware's root and reciprocal are within 1 ulp
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        u[e] = __builtin_amdgcn_sqrtf(u[e]);
+        w[e] = w[e] * a.decay - a.lr * m[e] * __builtin_amdgcn_rcpf(u[e] * a.rcorr + a.eps);
+    }
+    uint32_t r[8];
+    const uint32_t stream = (uint32_t)(s.n_stream >> 40);
+    if constexpr (Q8) {
+        const uint64_t k = (uint64_t)i / 4;
+        const u32x4 q0 = philox_words((uint32_t)k, (uint32_t)(k >> 32), stream, a.k0, a.k1);
+        const u32x4 q1 = philox_words((uint32_t)k + 1, (uint32_t)(k >> 32), stream, a.k0, a.k1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r[e] = q0[e];
+            r[4 + e] = q1[e];
+        }
+    } else if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+        const uint64_t k = (uint64_t)i / 8;
+        const u32x4 q = philox_words((uint32_t)k, (uint32_t)(k >> 32), stream, a.k0, a.k1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r[2 * e] = q[e];
+            r[2 * e + 1] = q[e] >> 16;
+        }
+    }
+    Elems8<WT> out;
+    if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t lo = r[e] & 0xFFFFu, hi = r[e + 1] & 0xFFFFu;
+            out.q[0][e / 2] = WT == HASTE_DTYPE_BF16 ? sr_bf16(w[e], lo) | sr_bf16(w[e + 1], hi) << 16
+                                                     : sr_f16(w[e], lo) | sr_f16(w[e + 1], hi) << 16;
+        }
+    } else {
+        out = pack8<WT>(w);
+    }
+    if constexpr (FULL) store8<WT>(s.w, i, out);
+    else store8_part<WT>(s.w, i, out, count);
+    if constexpr (Q8) {
+        const uint32_t cm = scale_code(m), cu = scale_code(u);
+        const uint32_t ru[8] = {r[1], r[2], r[3], r[0], r[5], r[6], r[7], r[4]};
+        const u32x2 m8 = cut_e4m3<false>(m, cm, r), u8 = cut_e4m3<true>(u, cu, ru);
+        // (the states are padded to whole blocks of 128)
+        if (FULL || (i & ~(int64_t)(kBlock - 1)) < i + count) {
+            *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.m) + i) = m8;
+            *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.v) + i) = u8;
+            if ((threadIdx.x & 15) == 0) {
+                s.ms[i / kBlock] = (uint8_t)cm;
+                s.vs[i / kBlock] = (uint8_t)cu;
+            }
+        }
+    }
+}
+
+// A thread to eight elements, so 16 lanes (one DPP row) to a block of an 8-bit state: its maxima
+// need no LDS.
+template <int WT, int GT, bool Q8>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, const AdamArgs a) {
     float gs = 1.f;
     if (a.grad_scale) {
         gs = *a.grad_scale;
         if (gs != gs) return;
     }
-    const AdamSeg& s = b.s[find_seg(b, blockIdx.x)];
-    const int64_t blk = blockIdx.x - s.blk0;
-    const int64_t i = blk * kBlock + threadIdx.x;
-    const bool in = i < s.n;
-    const float g = in ? load_elem<GT>(s.g, i) * gs : 0.f;
-    float w = in ? load_elem<WT>(s.w, i) : 0.f;
-    float m = 0.f, u;
-    if constexpr (Q8) {
-        m = e4m3_to_f32(static_cast<uint8_t*>(s.m)[i]) *
-            __uint_as_float((uint32_t)s.ms[blk] << 23);
-        u = e4m3_to_f32(static_cast<uint8_t*>(s.v)[i]) *
-            __uint_as_float((uint32_t)s.vs[blk] << 23);
-        m = a.b1 * m + a.c1 * g;
-        u = sqrtf(a.b2 * (u * u) + a.c2 * (g * g));
+    const int t = find_seg(b, blockIdx.x);
+    const AdamSeg& s = b.s[t];
+    const int64_t n = (int64_t)(s.n_stream & 0xFFFFFFFFFFull);
+    const int64_t i0 = (int64_t)(blockIdx.x - b.blk0[t]) * (kPiece * kPieces);
+    const int64_t i = i0 + threadIdx.x * 8;
+    if (i0 + kPiece * kPieces <= n) {
+        AdamElems<WT, GT, Q8> x[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+            adam_load<WT, GT, Q8, true>(x[p], s, i + p * kPiece, 8);
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+            adam_step<WT, GT, Q8, true>(x[p], s, a, gs, i + p * kPiece, 8);
     } else {
-        float v = 0.f;
-        if (in) {
-            m = a.b1 * static_cast<float*>(s.m)[i] + a.c1 * g;
-            v = a.b2 * static_cast<float*>(s.v)[i] + a.c2 * (g * g);
-            static_cast<float*>(s.m)[i] = m;
-            static_cast<float*>(s.v)[i] = v;
-        }
-        u = sqrtf(v);
-    }
-    w = w * a.decay - a.lr * (m / (u * a.rcorr + a.eps));
-    uint32_t r = 0, rm = 0, ru = 0;
-    if constexpr (Q8) {
-        const int64_t k = i / 4;
-        const u32x4 q = philox_words((uint32_t)k, (uint32_t)(k >> 32), s.stream, a.k0, a.k1);
-        r = q[i & 3] & 0xFFFFu;
-        rm = q[i & 3] >> 16;
-        ru = q[(i + 1) & 3] >> 16;
-    } else if (WT != HASTE_DTYPE_F32 && a.do_sr) {
-        const int64_t k = i / 8;
-        const u32x4 q = philox_words((uint32_t)k, (uint32_t)(k >> 32), s.stream, a.k0, a.k1);
-        r = (q[(i & 7) >> 1] >> (16 * (i & 1))) & 0xFFFFu;
-    }
-    if (in) {
-        if (WT != HASTE_DTYPE_F32 && a.do_sr)
-            static_cast<uint16_t*>(s.w)[i] = (uint16_t)cut_16<WT>(w, r);
-        else
-            store_elem<WT>(s.w, i, w);
-    }
-    if constexpr (Q8) {
-        float tm = fabsf(m) < INFINITY ? fabsf(m) : 0.f, tu = u < INFINITY ? u : 0.f;
-        for (int o = 32; o; o >>= 1) {
-            tm = fmaxf(tm, __shfl_xor(tm, o));
-            tu = fmaxf(tu, __shfl_xor(tu, o));
-        }
-        if ((threadIdx.x & 63) == 0) {
-            top[0][threadIdx.x >> 6] = tm;
-            top[1][threadIdx.x >> 6] = tu;
-        }
-        __syncthreads();
-        const int em = max((int)(__float_as_uint(fmaxf(top[0][0], top[0][1])) >> 23) - 7, 1);
-        const int eu = max((int)(__float_as_uint(fmaxf(top[1][0], top[1][1])) >> 23) - 7, 1);
-        static_cast<uint8_t*>(s.m)[i] =
-            (uint8_t)cut_e4m3<false>(m * __uint_as_float((uint32_t)(254 - em) << 23), rm);
-        static_cast<uint8_t*>(s.v)[i] =
-            (uint8_t)cut_e4m3<true>(u * __uint_as_float((uint32_t)(254 - eu) << 23), ru);
-        if (threadIdx.x == 0) {
-            s.ms[blk] = (uint8_t)em;
-            s.vs[blk] = (uint8_t)eu;
+        for (int p = 0; p < kPieces; ++p) {
+            const int64_t at = i + p * kPiece, count = n - at;
+            AdamElems<WT, GT, Q8> x;
+            adam_load<WT, GT, Q8, false>(x, s, at, count);
+            adam_step<WT, GT, Q8, false>(x, s, a, gs, at, count);
         }
     }
 }
@@ -189,21 +320,46 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
+// This thread's share of the squares of elements i0 .. i0 + kNormElems of n: fp32 over its 64,
+// four sums side by side.
+template <int DT>
+__device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_t n) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[8];
+    const int64_t i = i0 + threadIdx.x * 8;
+    constexpr int K = kNormElems / (kNormThreads * 8);
+    if (i0 + kNormElems <= n) {
+        Elems8<DT> x[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k] = load8<DT>(g, i + k * (kNormThreads * 8));
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            unpack8<DT>(x[k], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
+        }
+    } else {
+        for (int k = 0; k < K; ++k) {
+            const int64_t at = i + k * (kNormThreads * 8);
+            unpack8<DT>(load8_part<DT>(g, at, n - at), f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
+        }
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 // part[block] = the sum of squares of the block's pieces, every gridDim.x-th of the launch's.
 __global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const GradBatch b, uint32_t pieces,
                                                                  double* part) {
     __shared__ double sums[kNormThreads / 64];
     double total = 0.0;
     for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
-        const GradSeg& s = b.s[find_seg(b, p)];
-        const int64_t i0 = (int64_t)(p - s.blk0) * kNormElems;
-        const int64_t i1 = min(s.n, i0 + kNormElems);
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += kNormThreads) {
-            const float g = s.dtype == HASTE_DTYPE_BF16  ? load_elem<HASTE_DTYPE_BF16>(s.g, i)
-                            : s.dtype == HASTE_DTYPE_F16 ? load_elem<HASTE_DTYPE_F16>(s.g, i)
-                                                         : load_elem<HASTE_DTYPE_F32>(s.g, i);
-            total += (double)g * (double)g;
-        }
+        const int t = find_seg(b, p);
+        const GradSeg& s = b.s[t];
+        const int64_t i0 = (int64_t)(p - b.blk0[t]) * kNormElems;
+        total += s.dtype == HASTE_DTYPE_BF16  ? piece_squares<HASTE_DTYPE_BF16>(s.g, i0, s.n)
+                 : s.dtype == HASTE_DTYPE_F16 ? piece_squares<HASTE_DTYPE_F16>(s.g, i0, s.n)
+                                              : piece_squares<HASTE_DTYPE_F32>(s.g, i0, s.n);
     }
     total = wave_sum(total);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
@@ -238,13 +394,14 @@ int launch_adamw(const haste_adamw_tensor* ts, int count, const AdamArgs& a, hip
         for (; base < count && b.count < kMaxSegs; ++base) {
             const haste_adamw_tensor& t = ts[base];
             if (t.n == 0) continue;
-            b.s[b.count++] = AdamSeg{t.w, t.g, t.m, t.v, t.m_scale, t.v_scale, t.n,
-                                     (uint32_t)blocks, t.stream};
-            blocks += ceil_div(t.n, kBlock);
+            b.blk0[b.count] = (uint32_t)blocks;
+            b.s[b.count++] = AdamSeg{t.w, t.g, t.m, t.v, t.m_scale, t.v_scale,
+                                     (uint64_t)t.n | (uint64_t)t.stream << 40};
+            blocks += ceil_div(t.n, (int64_t)kPiece * kPieces);
             HASTE_CHECK_ARG(blocks < (int64_t)1 << 31, "haste_adamw_step: tensors too large");
         }
         if (b.count == 0) break;
-        adamw_kernel<WT, GT, Q8><<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(b, a);
+        adamw_kernel<WT, GT, Q8><<<dim3((unsigned)blocks), dim3(kThreads), 0, st>>>(b, a);
         HASTE_CHECK_LAUNCH("haste_adamw_step");
     }
     return HASTE_OK;
@@ -272,7 +429,9 @@ extern "C" int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count
     const bool q8 = state_bits == 8;
     for (int k = 0; k < count; ++k) {
         const haste_adamw_tensor& t = tensors[k];
-        HASTE_CHECK_ARG(t.n >= 0, "%s: tensor %d: n must be >= 0", fn, k);
+        HASTE_CHECK_ARG(t.n >= 0 && t.n < (int64_t)1 << 40,
+                        "%s: tensor %d: n must be >= 0 and below 2^40", fn, k);
+        HASTE_CHECK_ARG(t.stream < 1u << 24, "%s: tensor %d: stream must be below 2^24", fn, k);
         if (t.n == 0) continue;
         HASTE_CHECK_ARG(t.w && t.g && t.m && t.v && (!q8 || (t.m_scale && t.v_scale)),
                         "%s: tensor %d: null pointer", fn, k);
@@ -286,6 +445,7 @@ extern "C" int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count
     a.c1 = (float)(1.0 - beta1);
     a.b2 = (float)beta2;
     a.c2 = (float)(1.0 - beta2);
+    a.root_b2 = (float)std::sqrt(beta2);
     a.decay = (float)(1.0 - lr * wd);
     a.lr = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     a.rcorr = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
@@ -351,7 +511,8 @@ extern "C" int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, 
         for (; base < count && b.count < haste::kMaxSegs; ++base) {
             const haste_grad_tensor& t = tensors[base];
             if (t.n == 0) continue;
-            b.s[b.count++] = haste::GradSeg{t.g, t.n, t.dtype, (uint32_t)pieces};
+            b.blk0[b.count] = (uint32_t)pieces;
+            b.s[b.count++] = haste::GradSeg{t.g, t.n, t.dtype};
             pieces += haste::ceil_div(t.n, (int64_t)haste::kNormElems);
             HASTE_CHECK_ARG(pieces < (int64_t)1 << 31, "%s: tensors too large", fn);
         }

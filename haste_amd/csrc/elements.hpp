@@ -34,6 +34,91 @@ __device__ __forceinline__ float round_elem(float f) {
                                   : f16_bits_to_f32(f32_to_f16_rne(f));
 }
 
+// Eight elements as they lie in memory, read and written with the alignment of one element
+// (gfx950 takes 16-byte accesses at any address).
+template <int DT>
+struct Elems8 {
+    u32x4 q[DT == HASTE_DTYPE_F32 ? 2 : 1];
+};
+typedef u32x4 __attribute__((aligned(2))) u32x4_a2;
+
+template <int DT>
+__device__ __forceinline__ Elems8<DT> load8(const void* p, int64_t i) {
+    const u32x4_a2* a =
+        reinterpret_cast<const u32x4_a2*>(static_cast<const char*>(p) + i * kElemBytes<DT>);
+    Elems8<DT> v;
+    v.q[0] = a[0];
+    if constexpr (DT == HASTE_DTYPE_F32) v.q[1] = a[1];
+    return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t i, const Elems8<DT>& v) {
+    u32x4_a2* a = reinterpret_cast<u32x4_a2*>(static_cast<char*>(p) + i * kElemBytes<DT>);
+    a[0] = v.q[0];
+    if constexpr (DT == HASTE_DTYPE_F32) a[1] = v.q[1];
+}
+
+// The first `count` of eight elements, zeros after them; none where count <= 0.
+template <int DT>
+__device__ __forceinline__ Elems8<DT> load8_part(const void* p, int64_t i, int64_t count) {
+    if (count >= 8) return load8<DT>(p, i);
+    Elems8<DT> v;
+    v.q[0] = u32x4{0, 0, 0, 0};
+    if constexpr (DT == HASTE_DTYPE_F32) v.q[1] = v.q[0];
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < count) {
+            if constexpr (DT == HASTE_DTYPE_F32)
+                v.q[e / 4][e & 3] = static_cast<const uint32_t*>(p)[i + e];
+            else
+                v.q[0][e / 2] |= (uint32_t)static_cast<const uint16_t*>(p)[i + e] << (16 * (e & 1));
+        }
+    return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void store8_part(void* p, int64_t i, const Elems8<DT>& v, int64_t count) {
+    if (count >= 8) return store8<DT>(p, i, v);
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < count) {
+            if constexpr (DT == HASTE_DTYPE_F32)
+                static_cast<uint32_t*>(p)[i + e] = v.q[e / 4][e & 3];
+            else
+                static_cast<uint16_t*>(p)[i + e] = (uint16_t)(v.q[0][e / 2] >> (16 * (e & 1)));
+        }
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack8(const Elems8<DT>& v, float* f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (DT == HASTE_DTYPE_F32) {
+            f[e] = __uint_as_float(v.q[e / 4][e & 3]);
+        } else {
+            const uint32_t h = (e & 1) ? v.q[0][e / 2] >> 16 : v.q[0][e / 2] & 0xFFFFu;
+            f[e] = DT == HASTE_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+        }
+    }
+}
+
+// Rounded to nearest even.
+template <int DT>
+__device__ __forceinline__ Elems8<DT> pack8(const float* f) {
+    Elems8<DT> v;
+    if constexpr (DT == HASTE_DTYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.q[e / 4][e & 3] = __float_as_uint(f[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v.q[0][e] = DT == HASTE_DTYPE_BF16 ? pack2_rne<BF16>(f[2 * e], f[2 * e + 1])
+                                               : f32_to_f16_rne(f[2 * e]) | f32_to_f16_rne(f[2 * e + 1]) << 16;
+    }
+    return v;
+}
+
 inline bool elem_dtype(int32_t dt) {
     return dt == HASTE_DTYPE_BF16 || dt == HASTE_DTYPE_F16 || dt == HASTE_DTYPE_F32;
 }
