@@ -31,6 +31,12 @@ from torch.optim import Optimizer
 from . import _C, _lib
 from .optim_sr import run_hooked
 
+try:
+    from . import _host
+except ImportError as e:
+    raise ImportError("haste_amd: host module not built (haste_amd/_host.so); run "
+                      f"__graft_entry__.build() or `make -C haste_amd` ({e})") from e
+
 __all__ = ["AdamW", "grad_norm"]
 
 STATE_BLOCK = 128  # elements of an 8-bit state that share a scale
@@ -54,17 +60,23 @@ def grad_norm(tensors: Iterable[torch.Tensor], max_norm: float = math.inf
     factor of torch.nn.utils.clip_grad_norm_, as fp32 scalars on their device, without a
     sync and without touching the tensors: ``AdamW.step(grad_scale=coef)`` applies it.
     coef is NaN where norm is not finite."""
-    tensors = [_dense(t, "gradients") for t in tensors]
+    tensors = list(tensors)
     if not tensors:
         raise RuntimeError("grad_norm: no tensors")
-    dev = tensors[0].device
-    for t in tensors:
-        _C.require_device(t, "gradients")
-        if t.device != dev:
-            raise RuntimeError(f"grad_norm: tensors must be on one device (got {dev}, {t.device})")
-    n = len(tensors)
-    arr = (_lib.GradTensor * n)(*[(t.data_ptr(), t.numel(), _C.dtype_code(t.dtype))
-                                  for t in tensors])
+    n, rows = len(tensors), _host.grad_rows(tensors)
+    if rows is not None:
+        arr, index = rows
+        dev = torch.device("cuda", index)
+    else:
+        for t in tensors:
+            _C.require_device(t, "gradients")
+        tensors, dev = [_dense(t, "gradients") for t in tensors], tensors[0].device
+        for t in tensors:
+            if t.device != dev:
+                raise RuntimeError(f"grad_norm: tensors must be on one device (got {dev}, "
+                                   f"{t.device})")
+        arr = (_lib.GradTensor * n)(*[(t.data_ptr(), t.numel(), _C.dtype_code(t.dtype))
+                                      for t in tensors])
     out = torch.empty(2, dtype=torch.float32, device=dev)
     size = _lib.lib().haste_grad_norm_workspace_size(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
@@ -158,52 +170,71 @@ class AdamW(Optimizer):
         return loss
 
     def _step_group(self, group, grad_scale) -> None:
-        bits, device = group["state_bits"], None
-        batches, stepped, copies, keep = {}, [], [], []
-        for index, p in enumerate(group["params"]):
+        bits, copies = group["state_bits"], []
+        got = _host.adamw_rows(group["params"], self.state, bits)
+        if got is None:
+            batches, device, keep, copies = self._rows(group["params"], bits)
+        else:
+            batches, device = got
+        seed, (beta1, beta2) = group["seed"], group["betas"]
+        group["seed"] += 1
+        if not batches:
+            return
+        scale = None
+        if grad_scale is not None:
+            if grad_scale.get_device() != device:
+                raise RuntimeError(f"AdamW: grad_scale is on {grad_scale.device}, the parameters "
+                                   f"on cuda:{device}")
+            scale = grad_scale.data_ptr()
+        stream = torch._C._cuda_getCurrentRawStream(device)
+        for w_code, g_code, step, count, rows in batches:
+            _lib.call("haste_adamw_step", rows, count, w_code, g_code, bits, float(group["lr"]),
+                      float(beta1), float(beta2), float(group["eps"]),
+                      float(group["weight_decay"]), step, int(bool(group["stochastic_rounding"])),
+                      int(seed), scale, stream)
+        for p, w in copies:
+            p.copy_(w)
+
+    def _rows(self, params, bits):
+        """_host.adamw_rows for any parameters: ([(w dtype, g dtype, step, tensors, rows)],
+        device, tensors to keep until the launch, [(parameter, contiguous copy to step)]),
+        with states made where there are none yet."""
+        batches, stepped, copies, keep, device = {}, [], [], [], None
+        for index, p in enumerate(params):
             grad = p.grad
             if grad is None:
                 continue
             _C.require_device(p, "parameters")
             device = p.device if device is None else device
-            for t, name in ((grad, "gradient"), (grad_scale, "grad_scale"), (p, "parameter")):
-                if t is not None and t.device != device:
+            for t, name in ((grad, "a gradient"), (p, "a parameter")):
+                if t.device != device:
                     raise RuntimeError(f"AdamW: {name} is on {t.device}, its group on {device}")
             if grad.numel() != p.numel():
                 raise RuntimeError(f"AdamW: gradient {list(grad.shape)} of a parameter "
                                    f"{list(p.shape)}")
             w, g = _dense(p.detach(), "parameters"), _dense(grad, "gradients")
+            codes = _C.dtype_code(w.dtype), _C.dtype_code(g.dtype)
             state = self.state[p]
             if "step" not in state:
                 state = self._new_state(p, bits)
-            tensors = []
+            row = [w.data_ptr(), g.data_ptr()]
             for key, dtype in _STATE[bits].items():
                 t = state[key]
                 if t.dtype != dtype or t.device != device or not t.is_contiguous() or \
                         t.numel() != self._state_size(key, bits, p):
                     raise RuntimeError(f"AdamW: state {key} does not fit a parameter of shape "
                                        f"{list(p.shape)} with {bits}-bit states")
-                tensors.append(t.data_ptr())
-            if bits == 32:
-                tensors += [None, None]
-            state["step"] += 1
-            rows = batches.setdefault((_C.dtype_code(w.dtype), _C.dtype_code(g.dtype),
-                                       state["step"]), [])
-            rows.append((w.data_ptr(), g.data_ptr(), *tensors, p.numel(), index))
+                row.append(t.data_ptr())
+            row += [None] * (6 - len(row)) + [p.numel(), index]
+            stepped.append((state, codes, row, p))
             keep.append((w, g))
-            stepped.append(p)
             if w.data_ptr() != p.data_ptr():
                 copies.append((p, w))
-        seed = group["seed"]
-        group["seed"] += 1
-        scale = None if grad_scale is None else grad_scale.data_ptr()
-        for (wd, gd, step), rows in batches.items():
-            arr = (_lib.AdamwTensor * len(rows))(*rows)
-            _lib.call("haste_adamw_step", arr, len(rows), wd, gd, bits, float(group["lr"]),
-                      float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
-                      float(group["weight_decay"]), step, int(bool(group["stochastic_rounding"])),
-                      int(seed), scale, _C.stream_of(keep[0][0]))
-        for p, w in copies:
-            p.copy_(w)
+        for state, codes, row, p in stepped:
+            state["step"] += 1
+            batches.setdefault((*codes, state["step"]), []).append(tuple(row))
         if stepped:  # written through raw pointers: move the version counters as torch would
-            torch.autograd.graph.increment_version(stepped)
+            torch.autograd.graph.increment_version([s[3] for s in stepped])
+        return ([(*key, len(rows), (_lib.AdamwTensor * len(rows))(*rows))
+                 for key, rows in batches.items()], None if device is None else device.index, keep,
+                copies)
