@@ -1,5 +1,6 @@
 // Layer norm over rows, forward and backward.
 #include <algorithm>
+#include <type_traits>
 
 #include "elements.hpp"
 
@@ -20,9 +21,11 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
     return v;
 }
 
-// A workgroup to a row; the row is read again from cache for each of its passes.
+// ---------------------------------------------------------------- any width ----
+// For rows under 8 elements or past what registers hold: a workgroup to a row, which is read
+// again from cache for each of its passes.
 template <int DT, int WT>
-__global__ __launch_bounds__(kRowThreads) void ln_fwd_kernel(
+__global__ __launch_bounds__(kRowThreads) void ln_fwd_any_kernel(
     const char* x, int64_t ldx, const char* res, int64_t ldres, const void* w, const void* b,
     char* y, char* h, float* stats, int64_t D, float eps) {
     __shared__ float part[kRowThreads / 64];
@@ -60,7 +63,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_kernel(
 }
 
 template <int DT, int WT>
-__global__ __launch_bounds__(kRowThreads) void ln_dx_kernel(
+__global__ __launch_bounds__(kRowThreads) void ln_dx_any_kernel(
     const char* dy, int64_t lddy, const char* dh, int64_t lddh, const char* h, int64_t ldh,
     const void* w, const float* stats, char* dx, int64_t D) {
     __shared__ float part[kRowThreads / 64];
@@ -86,18 +89,19 @@ __global__ __launch_bounds__(kRowThreads) void ln_dx_kernel(
     }
 }
 
-// 64 columns to a workgroup, four rows at a time.
-template <int DT, int WT>
-__global__ __launch_bounds__(kRowThreads) void ln_dw_kernel(const char* dy, int64_t lddy,
-                                                            const char* h, int64_t ldh,
-                                                            const float* stats, void* dw, void* db,
-                                                            int64_t N, int64_t D) {
+// sums[blockIdx.y] = dw and db of every gridDim.y-th four rows: 64 columns to a workgroup.
+template <int DT>
+__global__ __launch_bounds__(kRowThreads) void ln_dw_any_kernel(const char* dy, int64_t lddy,
+                                                                const char* h, int64_t ldh,
+                                                                const float* stats, float* sums,
+                                                                int64_t N, int64_t D) {
     __shared__ float part[2][kRowThreads];
     constexpr int S = kElemBytes<DT>;
+    constexpr int R = kRowThreads / 64;
     const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     float sw = 0.f, sb = 0.f;
     if (c < D)
-        for (int64_t r = threadIdx.x >> 6; r < N; r += kRowThreads / 64) {
+        for (int64_t r = (int64_t)blockIdx.y * R + (threadIdx.x >> 6); r < N; r += gridDim.y * R) {
             const float g = load_elem<DT>(dy + r * lddy * S, c);
             sw += g * ((load_elem<DT>(h + r * ldh * S, c) - stats[2 * r]) * stats[2 * r + 1]);
             sb += g;
@@ -106,12 +110,328 @@ __global__ __launch_bounds__(kRowThreads) void ln_dw_kernel(const char* dy, int6
     part[1][threadIdx.x] = sb;
     __syncthreads();
     if (threadIdx.x >= 64 || c >= D) return;
-    for (int k = 1; k < kRowThreads / 64; ++k) {
+    for (int k = 1; k < R; ++k) {
         sw += part[0][k * 64 + threadIdx.x];
         sb += part[1][k * 64 + threadIdx.x];
     }
-    if (dw) store_elem<WT>(dw, c, sw);
-    if (db) store_elem<WT>(db, c, sb);
+    sums += (int64_t)blockIdx.y * 2 * D;
+    sums[c] = sw;
+    sums[D + c] = sb;
+}
+
+// ------------------------------------------------------- rows in registers ----
+// `tpr` threads (a power of two from 16) hold a row, 8 elements in each of C slots: thread t has
+// elements 8 (c tpr + t) + 0..7 of it in slot c.  Only the last slot can pass the row's end:
+// there a thread reads and writes the row's last 8 elements instead, of which it shares the
+// first `skip` with other threads (which compute the same values) and leaves them out of sums;
+// with skip >= 8 it has none of its own.
+struct Slot {
+    int64_t at;  // first element
+    int skip;
+};
+__device__ __forceinline__ Slot row_slot(int c, int C, int tpr, int lane, int64_t D) {
+    const int64_t e = 8 * ((int64_t)c * tpr + lane);
+    if (c < C - 1) return Slot{e, 0};
+    const int64_t at = min(e, D - 8);
+    return Slot{at, (int)(e - at)};
+}
+
+template <int C>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), C, 0xF, 0xF, true));
+}
+// The sum over groups of min(tpr, 64) lanes, in all of them: rotations within 16 lanes, then
+// rows and halves of the wave swapped with their neighbours.
+__device__ __forceinline__ float lanes_sum(float x, int tpr) {
+    x = dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x))));
+    if (tpr >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (tpr >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return x;
+}
+
+// Sums of a and b over the row's threads, in all of them.  Rows of several waves meet in
+// part[2][2 * 16], whose halves take turns (`turn`): one barrier a sum.
+__device__ __forceinline__ void row_sums(float& a, float& b, int tpr, float (*part)[32], int& turn) {
+    a = lanes_sum(a, tpr);
+    b = lanes_sum(b, tpr);
+    if (tpr <= 64) return;
+    const int wave = threadIdx.x >> 6, waves = tpr >> 6;
+    float* p = part[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+        p[wave] = a;
+        p[16 + wave] = b;
+    }
+    __syncthreads();
+    const int first = wave & ~(waves - 1);
+    a = b = 0.f;
+    for (int k = 0; k < waves; ++k) {
+        a += p[first + k];
+        b += p[16 + first + k];
+    }
+}
+
+template <int DT, int WT, int C>
+__global__ __launch_bounds__(1024) void ln_fwd_kernel(
+    const char* __restrict__ x, int64_t ldx, const char* __restrict__ res, int64_t ldres,
+    const void* __restrict__ w, const void* __restrict__ b, char* __restrict__ y,
+    char* __restrict__ h, float* __restrict__ stats, int64_t N, int64_t D, float eps, int tpr) {
+    __shared__ float part[2][32];
+    constexpr int S = kElemBytes<DT>;
+    const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+    const int64_t want = (int64_t)blockIdx.x * (blockDim.x / tpr) + group;
+    const int64_t row = min(want, N - 1);
+    const bool live = want < N;
+    int turn = 0;
+    x += row * ldx * S;
+    if (res) res += row * ldres * S;
+    Elems8<DT> raw[C], add[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[c] = load8<DT>(x, row_slot(c, C, tpr, lane, D).at);
+    if (res) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) add[c] = load8<DT>(res, row_slot(c, C, tpr, lane, D).at);
+    }
+    float f[C][8], s = 0.f, none = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const Slot at = row_slot(c, C, tpr, lane, D);
+        unpack8<DT>(raw[c], f[c]);
+        if (res) {
+            float g[8];
+            unpack8<DT>(add[c], g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[c][e] += g[e];
+            const Elems8<DT> sum = pack8<DT>(f[c]);
+            if (live && at.skip < 8) store8<DT>(h + row * D * S, at.at, sum);
+            unpack8<DT>(sum, f[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += c < C - 1 || e >= at.skip ? f[c][e] : 0.f;
+    }
+    row_sums(s, none, tpr, part, turn);
+    const float mean = s / (float)D;
+    s = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int skip = row_slot(c, C, tpr, lane, D).skip;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f[c][e] -= mean;
+            s += c < C - 1 || e >= skip ? f[c][e] * f[c][e] : 0.f;
+        }
+    }
+    row_sums(s, none, tpr, part, turn);
+    const float rstd = 1.f / sqrtf(s / (float)D + eps);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const Slot at = row_slot(c, C, tpr, lane, D);
+        float g[8];
+        unpack8<WT>(load8<WT>(w, at.at), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[c][e] = f[c][e] * rstd * g[e];
+        if (b) {
+            unpack8<WT>(load8<WT>(b, at.at), g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[c][e] += g[e];
+        }
+        if (live && at.skip < 8) store8<DT>(y + row * D * S, at.at, pack8<DT>(f[c]));
+    }
+    if (stats && lane == 0 && live) {
+        stats[2 * row] = mean;
+        stats[2 * row + 1] = rstd;
+    }
+}
+
+constexpr int kBwdThreads = 512;
+constexpr int kBwdBlocks = 512;  // partial sums of dw and db: one pair of rows a workgroup
+
+template <int DT, int C>
+struct BwdRow {
+    Elems8<DT> dy[C], h[C], dh[C];
+    float mean, rstd;
+};
+
+// Every group of tpr threads takes each (gridDim groups)-th row: one read of dy, h and dh gives
+// dx, and what the row adds to dw and db stays in registers until the end.  The next row's
+// loads are under way while a row is reduced.
+template <int DT, int WT, int C>
+__global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
+    const char* __restrict__ dy, int64_t lddy, const char* __restrict__ dh, int64_t lddh,
+    const char* __restrict__ h, int64_t ldh, const void* __restrict__ w,
+    const float* __restrict__ stats, char* __restrict__ dx, float* __restrict__ sums, int64_t N,
+    int64_t D, int tpr) {
+    extern __shared__ float lds[];
+    __shared__ float part[2][32];
+    constexpr int S = kElemBytes<DT>;
+    const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+    const int groups = kBwdThreads / tpr;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    int turn = 0;
+    float g[C][8], aw[C][8], ab[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        unpack8<WT>(load8<WT>(w, row_slot(c, C, tpr, lane, D).at), g[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) aw[c][e] = ab[c][e] = 0.f;
+    }
+    auto load = [&](BwdRow<DT, C>& r, int64_t want) __attribute__((always_inline)) {
+        const int64_t row = min(want, N - 1);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int64_t at = row_slot(c, C, tpr, lane, D).at;
+            r.dy[c] = load8<DT>(dy + row * lddy * S, at);
+            r.h[c] = load8<DT>(h + row * ldh * S, at);
+            if (dh) r.dh[c] = load8<DT>(dh + row * lddh * S, at);
+        }
+        r.mean = stats[2 * row];
+        r.rstd = stats[2 * row + 1];
+    };
+    // (all groups make the same number of turns: rows_sums may hold a barrier)
+    const int64_t turns = (N + step - 1) / step;
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    BwdRow<DT, C> next;
+    load(next, row);
+    for (int64_t k = 0; k < turns; ++k, row += step) {
+        const BwdRow<DT, C> r = next;
+        if (k + 1 < turns) load(next, row + step);
+        const bool live = row < N;
+        float s1 = 0.f, s2 = 0.f, n[C][8];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int skip = row_slot(c, C, tpr, lane, D).skip;
+            float d[8];
+            unpack8<DT>(r.dy[c], d);
+            unpack8<DT>(r.h[c], n[c]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n[c][e] = (n[c][e] - r.mean) * r.rstd;
+                const bool own = live && (c < C - 1 || e >= skip);
+                const float a = d[e] * g[c][e];
+                s1 += own ? a : 0.f;
+                s2 += own ? a * n[c][e] : 0.f;
+                aw[c][e] += own ? d[e] * n[c][e] : 0.f;
+                ab[c][e] += own ? d[e] : 0.f;
+            }
+        }
+        row_sums(s1, s2, tpr, part, turn);
+        if (!dx) continue;
+        const float c1 = s1 / (float)D, c2 = s2 / (float)D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const Slot at = row_slot(c, C, tpr, lane, D);
+            float d[8];
+            unpack8<DT>(r.dy[c], d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = r.rstd * (d[e] * g[c][e] - c1 - n[c][e] * c2);
+            if (dh) {
+                float q[8];
+                unpack8<DT>(r.dh[c], q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] += q[e];
+            }
+            if (live && at.skip < 8) store8<DT>(dx + row * D * S, at.at, pack8<DT>(d));
+        }
+    }
+    if (!sums) return;
+    // the groups' sums, halved until the first has them all
+    for (int half = groups / 2; half; half /= 2) {
+        __syncthreads();
+        float* p = lds + (group & (half - 1)) * (16 * C * tpr) + lane;
+        if (group >= half && group < 2 * half) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[(16 * c + e) * tpr] = aw[c][e];
+                    p[(16 * c + 8 + e) * tpr] = ab[c][e];
+                }
+        }
+        __syncthreads();
+        if (group < half) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    aw[c][e] += p[(16 * c + e) * tpr];
+                    ab[c][e] += p[(16 * c + 8 + e) * tpr];
+                }
+        }
+    }
+    if (group) return;
+    float* out = sums + (int64_t)blockIdx.x * 2 * D;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const Slot at = row_slot(c, C, tpr, lane, D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c < C - 1 || e >= at.skip) {
+                out[at.at + e] = aw[c][e];
+                out[D + at.at + e] = ab[c][e];
+            }
+    }
+}
+
+// dw (blockIdx.y 0) and db (1) from the workgroups' sums: 64 columns a workgroup, 16 sums of
+// each side by side, joined in order.
+template <int WT>
+__global__ __launch_bounds__(1024) void ln_sums_kernel(const float* __restrict__ sums, int blocks,
+                                                       void* dw, void* db, int64_t D) {
+    __shared__ float part[16][64];
+    const int x = threadIdx.x & 63, k = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + x;
+    void* out = blockIdx.y ? db : dw;
+    float s = 0.f;
+    if (c < D) {
+        const float* p = sums + blockIdx.y * D + c;
+#pragma unroll 8
+        for (int b = k; b < blocks; b += 16) s += p[(int64_t)b * 2 * D];
+    }
+    part[k][x] = s;
+    __syncthreads();
+    if (k || c >= D || !out) return;
+    for (int j = 1; j < 16; ++j) s += part[j][x];
+    store_elem<WT>(out, c, s);
+}
+
+// How the threads hold rows of D elements in up to `slots` slots: the fewest threads left over,
+// then the fewest threads to a row.  C == 0: they do not fit `most` threads, or are under 8
+// elements.
+struct RowShape {
+    int tpr, C;
+};
+RowShape row_shape(int64_t D, int most, int slots) {
+    RowShape best{0, 0};
+    int64_t over = 0;
+    if (D < 8) return best;
+    for (int tpr = 16; tpr <= most; tpr *= 2) {
+        const int64_t C = ceil_div(D, (int64_t)8 * tpr);
+        if (C > slots) continue;
+        const int64_t o = C * 8 * tpr - D;
+        if (best.C == 0 || o < over) {
+            best = RowShape{tpr, (int)C};
+            over = o;
+        }
+    }
+    return best;
+}
+RowShape fwd_shape(int64_t D) { return row_shape(D, 1024, 4); }
+// (the registers of a backward slot: 16-bit rows 56 and fp32 rows 80, of 256)
+constexpr int bwd_slots(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 2 : 3; }
+RowShape bwd_shape(int64_t D, int32_t dtype) { return row_shape(D, kBwdThreads, bwd_slots(dtype)); }
+
+// The partial sums of dw and db.
+int bwd_blocks(int64_t N, int64_t D, const RowShape& r) {
+    const int64_t rows = r.C ? kBwdThreads / r.tpr : 64, most = r.C ? kBwdBlocks : 64;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(N, rows), most));
 }
 
 int ln_types(const char* fn, int32_t dtype, int32_t w_dtype) {
@@ -130,6 +450,15 @@ int ln_rows(const char* fn, const char* what, const void* p, int64_t ld, int64_t
     HASTE_CHECK_ARG(ld == 0 || ld >= D, "%s: row pitch of %s is short (%lld < %lld)", fn, what,
                     (long long)ld, (long long)D);
     return HASTE_OK;
+}
+
+// f with C as a constant.
+template <typename F>
+void with_slots(int C, F f) {
+    if (C == 1) f(std::integral_constant<int, 1>());
+    else if (C == 2) f(std::integral_constant<int, 2>());
+    else if (C == 3) f(std::integral_constant<int, 3>());
+    else f(std::integral_constant<int, 4>());
 }
 
 #define HASTE_TRY(expr)                        \
@@ -171,11 +500,24 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
     HASTE_CHECK_ARG(haste::elem_aligned(b, w_dtype), "%s: b is not aligned to its elements", fn);
     HASTE_TRY(haste::ln_rows(fn, "y", y, D, D, dtype));
     HASTE_CHECK_ARG(haste::elem_aligned(stats, HASTE_DTYPE_F32), "%s: stats is misaligned", fn);
+    const haste::RowShape r = haste::fwd_shape(D);
+    const int threads = std::max(r.tpr, 256), rows = r.C ? threads / r.tpr : 1;
+    const dim3 grid((unsigned)haste::ceil_div(N, (int64_t)rows));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const char *xc = static_cast<const char*>(x), *rc = static_cast<const char*>(res);
+    char *yc = static_cast<char*>(y), *hc = static_cast<char*>(h);
 #define HASTE_LN_FWD(DT, WT)                                                                   \
-    haste::ln_fwd_kernel<DT, WT><<<dim3((unsigned)N), dim3(haste::kRowThreads), 0,             \
-                                   static_cast<hipStream_t>(stream)>>>(                        \
-        static_cast<const char*>(x), ldx, static_cast<const char*>(res), ldres, w, b,          \
-        static_cast<char*>(y), static_cast<char*>(h), stats, D, (float)eps)
+    do {                                                                                       \
+        auto slots = [&](auto c) {                                                             \
+            haste::ln_fwd_kernel<DT, WT, decltype(c)::value><<<grid, dim3(threads), 0, st>>>(  \
+                xc, ldx, rc, ldres, w, b, yc, hc, stats, N, D, (float)eps, r.tpr);             \
+        };                                                                                     \
+        if (r.C)                                                                               \
+            haste::with_slots(r.C, slots);                                                     \
+        else                                                                                   \
+            haste::ln_fwd_any_kernel<DT, WT><<<grid, dim3(haste::kRowThreads), 0, st>>>(       \
+                xc, ldx, rc, ldres, w, b, yc, hc, stats, D, (float)eps);                       \
+    } while (0)
     HASTE_LN_TYPES(HASTE_LN_FWD);
 #undef HASTE_LN_FWD
     HASTE_CHECK_LAUNCH(fn);
@@ -183,7 +525,12 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
 }
 
 extern "C" int64_t haste_layer_norm_bwd_workspace_size(int64_t N, int64_t D) {
-    return N < 0 || D < 0 ? HASTE_ERR_INVALID_ARG : 16;
+    if (N < 0 || D < 0) return HASTE_ERR_INVALID_ARG;
+    // (the larger of the two shapes that the rows' dtypes may take)
+    int most = 1;
+    for (int32_t dt : {HASTE_DTYPE_BF16, HASTE_DTYPE_F32})
+        most = std::max(most, haste::bwd_blocks(N, D, haste::bwd_shape(D, dt)));
+    return most * 2 * std::max<int64_t>(D, 8) * (int64_t)sizeof(float);
 }
 
 extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh,
@@ -217,17 +564,36 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
         }
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
+    const haste::RowShape r = haste::bwd_shape(D, dtype);
+    const int blocks = haste::bwd_blocks(N, D, r);
+    const char *dyc = static_cast<const char*>(dy), *dhc = static_cast<const char*>(dh),
+               *hc = static_cast<const char*>(h);
+    float* sums = dw || db ? static_cast<float*>(ws) : nullptr;
+    const dim3 columns((unsigned)haste::ceil_div(D, 64), 2);
 #define HASTE_LN_BWD(DT, WT)                                                                     \
     do {                                                                                         \
-        if (dx && N > 0)                                                                         \
-            haste::ln_dx_kernel<DT, WT><<<dim3((unsigned)N), dim3(haste::kRowThreads), 0, st>>>( \
-                static_cast<const char*>(dy), lddy, static_cast<const char*>(dh), lddh,          \
-                static_cast<const char*>(h), ldh, w, stats, static_cast<char*>(dx), D);          \
-        if (dw || db)                                                                            \
-            haste::ln_dw_kernel<DT, WT><<<dim3((unsigned)haste::ceil_div(D, 64)),                \
-                                          dim3(haste::kRowThreads), 0, st>>>(                    \
-                static_cast<const char*>(dy), lddy, static_cast<const char*>(h), ldh, stats, dw, \
-                db, N, D);                                                                       \
+        auto slots = [&](auto c) {                                                               \
+            constexpr int C = std::min(decltype(c)::value, haste::bwd_slots(DT));                \
+            const size_t lds = r.tpr < haste::kBwdThreads && sums                                \
+                                   ? sizeof(float) * 8 * C * haste::kBwdThreads                  \
+                                   : 0;                                                          \
+            haste::ln_bwd_kernel<DT, WT, C><<<dim3(blocks), dim3(haste::kBwdThreads), lds, st>>>(\
+                dyc, lddy, dhc, lddh, hc, ldh, w, stats, static_cast<char*>(dx), sums, N, D,     \
+                r.tpr);                                                                          \
+        };                                                                                       \
+        if (N > 0 && r.C) {                                                                      \
+            haste::with_slots(r.C, slots);                                                       \
+        } else {                                                                                 \
+            if (N > 0 && dx)                                                                     \
+                haste::ln_dx_any_kernel<DT, WT><<<dim3((unsigned)N), dim3(haste::kRowThreads),   \
+                                                  0, st>>>(dyc, lddy, dhc, lddh, hc, ldh, w,     \
+                                                           stats, static_cast<char*>(dx), D);    \
+            if (sums)                                                                            \
+                haste::ln_dw_any_kernel<DT><<<dim3(columns.x, blocks), dim3(haste::kRowThreads), \
+                                              0, st>>>(dyc, lddy, hc, ldh, stats, sums, N, D);   \
+        }                                                                                        \
+        if (sums)                                                                                \
+            haste::ln_sums_kernel<WT><<<columns, dim3(1024), 0, st>>>(sums, blocks, dw, db, D);  \
     } while (0)
     HASTE_LN_TYPES(HASTE_LN_BWD);
 #undef HASTE_LN_BWD
