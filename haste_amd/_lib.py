@@ -7,6 +7,7 @@ or ``make -C haste_amd``.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 
@@ -176,6 +177,21 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = L
     return _lib
+
+
+_host = None
+
+
+def host():
+    """Load (once) and return the native module haste_amd._host; raises if it is absent."""
+    global _host
+    if _host is None:
+        try:
+            _host = importlib.import_module("haste_amd._host")
+        except ImportError as e:
+            raise ImportError(f"haste_amd: host module not built ({_HERE}/_host.so); run "
+                              f"__graft_entry__.build() or `make -C haste_amd` ({e})") from e
+    return _host
 
 
 def last_error() -> str:

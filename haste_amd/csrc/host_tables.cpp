@@ -1,8 +1,8 @@
-// haste_amd._host: tables of many tensors for the C ABI, made without a Python call for each
-// attribute of each tensor.  An AdamW step of 195 tensors with 8-bit states reads some 40
+// haste_amd._host, the Python module.  Here: tables of many tensors for the C ABI, made without a
+// Python call for each attribute of each tensor.  An AdamW step of 195 tensors with 8-bit states reads some 40
 // attributes of each: 0.9 ms in Python, more than its kernels take.
 //
-// Both functions return None where a tensor is not plain (dense, contiguous, not negated, no
+// grad_rows and adamw_rows return None where a tensor is not plain (dense, contiguous, not negated, no
 // subclass with a dispatch of its own, on the first one's HIP device) or its state does not
 // fit: the callers' Python paths then copy, create or refuse.
 #define PY_SSIZE_T_CLEAN
@@ -15,17 +15,13 @@
 #include <vector>
 
 #include "../../include/haste_ffi.h"
+#include "host_tables.hpp"
 
 namespace {
 
 constexpr int64_t kStateBlock = 128;  // elements of an 8-bit state that share a scale
 
-int dtype_code(at::ScalarType t) {
-    return t == at::kBFloat16 ? HASTE_DTYPE_BF16
-           : t == at::kHalf   ? HASTE_DTYPE_F16
-           : t == at::kFloat  ? HASTE_DTYPE_F32
-                              : -1;
-}
+using haste_host::dtype_code;
 
 bool plain(const at::Tensor& t, int64_t* device) {
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_neg() ||
@@ -199,8 +195,10 @@ PyMethodDef methods[] = {
     {"grad_rows", grad_rows, METH_O, "grad_rows(tensors) -> (rows, device) or None"},
     {"adamw_rows", adamw_rows, METH_VARARGS,
      "adamw_rows(params, state, bits) -> ([(w, g, step, count, rows)], device) or None"},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(haste_host::layer_norm)),
+     METH_FASTCALL, "layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual"},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Tables of tensors for libhaste_ffi.so.", -1,
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of libhaste_ffi.so's entry points that take torch tensors.", -1,
                       methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

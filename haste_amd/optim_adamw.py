@@ -31,12 +31,6 @@ from torch.optim import Optimizer
 from . import _C, _lib
 from .optim_sr import run_hooked
 
-try:
-    from . import _host
-except ImportError as e:
-    raise ImportError("haste_amd: host module not built (haste_amd/_host.so); run "
-                      f"__graft_entry__.build() or `make -C haste_amd` ({e})") from e
-
 __all__ = ["AdamW", "grad_norm"]
 
 STATE_BLOCK = 128  # elements of an 8-bit state that share a scale
@@ -63,7 +57,7 @@ def grad_norm(tensors: Iterable[torch.Tensor], max_norm: float = math.inf
     tensors = list(tensors)
     if not tensors:
         raise RuntimeError("grad_norm: no tensors")
-    n, rows = len(tensors), _host.grad_rows(tensors)
+    n, rows = len(tensors), _lib.host().grad_rows(tensors)
     if rows is not None:
         arr, index = rows
         dev = torch.device("cuda", index)
@@ -171,7 +165,7 @@ class AdamW(Optimizer):
 
     def _step_group(self, group, grad_scale) -> None:
         bits, copies = group["state_bits"], []
-        got = _host.adamw_rows(group["params"], self.state, bits)
+        got = _lib.host().adamw_rows(group["params"], self.state, bits)
         if got is None:
             batches, device, keep, copies = self._rows(group["params"], bits)
         else:
@@ -196,7 +190,7 @@ class AdamW(Optimizer):
             p.copy_(w)
 
     def _rows(self, params, bits):
-        """_host.adamw_rows for any parameters: ([(w dtype, g dtype, step, tensors, rows)],
+        """adamw_rows of the native module for any parameters: ([(w dtype, g dtype, step, tensors, rows)],
         device, tensors to keep until the launch, [(parameter, contiguous copy to step)]),
         with states made where there are none yet."""
         batches, stepped, copies, keep, device = {}, [], [], [], None

@@ -310,3 +310,22 @@ def test_refusals(dev):
     for bad in (dict(normalized_shape=(4, 64)), dict(normalized_shape=64, elementwise_affine=False)):
         with pytest.raises(ValueError, match="one normalised axis"):
             LayerNorm(**bad)
+
+
+def test_its_backward_is_not_differentiable(dev):
+    x = torch.randn(4, 64, device=dev, requires_grad=True)
+    w = torch.ones(64, device=dev, requires_grad=True)
+    y = ops.layer_norm(x, w)
+    gx, gw = torch.autograd.grad(y.square().sum(), [x, w], create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        (gx.sum() + gw.sum()).backward()
+
+
+def test_saved_rows_changed_in_place_are_noticed(dev):
+    x = torch.randn(4, 64, device=dev)
+    w = torch.ones(64, device=dev, requires_grad=True)
+    y, h = ops.layer_norm(x, w, residual=x)
+    with torch.no_grad():
+        h.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
