@@ -37,20 +37,17 @@ struct AdamArgs {
     const float* grad_scale;
 };
 
-struct GradSeg {
-    const void* g;
-    int64_t n;
-    int32_t dtype;
-};
+// 200 tensors fill 4 KB of kernel arguments.
+constexpr int kMaxGrads = 200;
 struct GradBatch {
-    uint32_t blk0[kMaxSegs];
-    GradSeg s[kMaxSegs];
-    int32_t count;
+    uint32_t piece0[kMaxGrads];   // first piece of each tensor
+    const void* g[kMaxGrads];
+    uint64_t n_dtype[kMaxGrads];  // elements, and the dtype << 56
+    int32_t count, pieces;
 };
 
-// The tensor that workgroup (or piece) `blk` belongs to: every lane compares one start.
-template <typename B>
-__device__ __forceinline__ int find_seg(const B& b, uint32_t blk) {
+// The tensor that workgroup `blk` belongs to: every lane compares one start.
+__device__ __forceinline__ int find_seg(const AdamBatch& b, uint32_t blk) {
     const int lane = threadIdx.x & 63;
     const bool at = lane < b.count && b.blk0[lane] <= blk;
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(at)) - 1);
@@ -312,34 +309,35 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, cons
 }
 
 constexpr int kNormThreads = 256;
-constexpr int kNormElems = 16384;       // elements of a workgroup
-constexpr int kNormParts = 2048;        // partial sums of a launch
+constexpr int kNormLoads = 8;                                  // 16-byte (fp32: 32) loads in flight
+constexpr int kNormPiece = kNormThreads * 8 * kNormLoads;      // elements of a piece
+constexpr int kNormParts = 1024;                               // workgroups of a launch, 4 to a CU
 
 __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-// This thread's share of the squares of elements i0 .. i0 + kNormElems of n: fp32 over its 64,
+// This thread's share of the squares of elements i0 .. i0 + kNormPiece of n: fp32 over its 64,
 // four sums side by side.
 template <int DT>
 __device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_t n) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[8];
     const int64_t i = i0 + threadIdx.x * 8;
-    constexpr int K = kNormElems / (kNormThreads * 8);
-    if (i0 + kNormElems <= n) {
-        Elems8<DT> x[K];
+    if (i0 + kNormPiece <= n) {
+        Elems8<DT> x[kNormLoads];
 #pragma unroll
-        for (int k = 0; k < K; ++k) x[k] = load8<DT>(g, i + k * (kNormThreads * 8));
+        for (int k = 0; k < kNormLoads; ++k) x[k] = load8<DT>(g, i + k * (kNormThreads * 8));
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+        for (int k = 0; k < kNormLoads; ++k) {
             unpack8<DT>(x[k], f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
         }
     } else {
-        for (int k = 0; k < K; ++k) {
+        for (int k = 0; k < kNormLoads; ++k) {
             const int64_t at = i + k * (kNormThreads * 8);
+            if (at >= n) break;
             unpack8<DT>(load8_part<DT>(g, at, n - at), f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
@@ -348,38 +346,49 @@ __device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// part[block] = the sum of squares of the block's pieces, every gridDim.x-th of the launch's.
-__global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const GradBatch b, uint32_t pieces,
-                                                                 double* part) {
+// part[workgroup] = the sum of squares of every gridDim-th piece, the launch's last pieces first:
+// the first tensors' gradients are then what the last-level cache holds when a step reads them
+// again from the start.
+__global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const GradBatch b, double* part) {
     __shared__ double sums[kNormThreads / 64];
+    __shared__ uint32_t piece0[kMaxGrads];
+    for (int k = threadIdx.x; k < b.count; k += kNormThreads) piece0[k] = b.piece0[k];
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
     double total = 0.0;
-    for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
-        const int t = find_seg(b, p);
-        const GradSeg& s = b.s[t];
-        const int64_t i0 = (int64_t)(p - b.blk0[t]) * kNormElems;
-        total += s.dtype == HASTE_DTYPE_BF16  ? piece_squares<HASTE_DTYPE_BF16>(s.g, i0, s.n)
-                 : s.dtype == HASTE_DTYPE_F16 ? piece_squares<HASTE_DTYPE_F16>(s.g, i0, s.n)
-                                              : piece_squares<HASTE_DTYPE_F32>(s.g, i0, s.n);
+    for (int p = b.pieces - 1 - (int)blockIdx.x; p >= 0; p -= (int)gridDim.x) {
+        int t = -1;
+        for (int k = 0; k < b.count; k += 64)
+            t += __popcll(__ballot(k + lane < b.count && piece0[k + lane] <= (uint32_t)p));
+        t = __builtin_amdgcn_readfirstlane(t);
+        const void* g = b.g[t];
+        const int64_t n = (int64_t)(b.n_dtype[t] & 0xFFFFFFFFFFFFFFull);
+        const int dtype = (int)(b.n_dtype[t] >> 56);
+        const int64_t i0 = (int64_t)((uint32_t)p - b.piece0[t]) * kNormPiece;
+        total += dtype == HASTE_DTYPE_BF16  ? piece_squares<HASTE_DTYPE_BF16>(g, i0, n)
+                 : dtype == HASTE_DTYPE_F16 ? piece_squares<HASTE_DTYPE_F16>(g, i0, n)
+                                            : piece_squares<HASTE_DTYPE_F32>(g, i0, n);
     }
     total = wave_sum(total);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
+    if (lane == 0) sums[threadIdx.x >> 6] = total;
     __syncthreads();
     if (threadIdx.x) return;
     for (int k = 1; k < kNormThreads / 64; ++k) total += sums[k];
     part[blockIdx.x] = total;
 }
 
-__global__ __launch_bounds__(kNormThreads) void grad_norm_final_kernel(const double* part,
-                                                                       int64_t parts, float max_norm,
-                                                                       float* out) {
-    __shared__ double sums[kNormThreads / 64];
+constexpr int kFinalThreads = 1024;
+__global__ __launch_bounds__(kFinalThreads) void grad_norm_final_kernel(const double* part,
+                                                                        int64_t parts,
+                                                                        float max_norm, float* out) {
+    __shared__ double sums[kFinalThreads / 64];
     double total = 0.0;
-    for (int64_t i = threadIdx.x; i < parts; i += kNormThreads) total += part[i];
+    for (int64_t i = threadIdx.x; i < parts; i += kFinalThreads) total += part[i];
     total = wave_sum(total);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int k = 1; k < kNormThreads / 64; ++k) total += sums[k];
+    for (int k = 1; k < kFinalThreads / 64; ++k) total += sums[k];
     const float norm = (float)sqrt(total);
     out[0] = norm;
     out[1] = norm < INFINITY ? fminf(1.f, max_norm / (norm + 1e-6f)) : NAN;
@@ -474,7 +483,7 @@ extern "C" int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count
 
 extern "C" int64_t haste_grad_norm_workspace_size(int32_t count) {
     if (count < 0) return HASTE_ERR_INVALID_ARG;
-    return haste::ceil_div(std::max(count, 1), haste::kMaxSegs) * haste::kNormParts *
+    return haste::ceil_div(std::max(count, 1), haste::kMaxGrads) * haste::kNormParts *
            (int64_t)sizeof(double);
 }
 
@@ -494,7 +503,8 @@ extern "C" int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, 
     }
     for (int k = 0; k < count; ++k) {
         const haste_grad_tensor& t = tensors[k];
-        HASTE_CHECK_ARG(t.n >= 0, "%s: tensor %d: n must be >= 0", fn, k);
+        HASTE_CHECK_ARG(t.n >= 0 && t.n < (int64_t)1 << 44,
+                        "%s: tensor %d: n must be >= 0 and below 2^44", fn, k);
         HASTE_CHECK_ARG(haste::elem_dtype(t.dtype),
                         "%s: tensor %d must be bf16, fp16 or fp32 (dtype code %d)", fn, k,
                         (int)t.dtype);
@@ -508,22 +518,24 @@ extern "C" int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, 
         haste::GradBatch b;
         b.count = 0;
         int64_t pieces = 0;
-        for (; base < count && b.count < haste::kMaxSegs; ++base) {
+        for (; base < count && b.count < haste::kMaxGrads; ++base) {
             const haste_grad_tensor& t = tensors[base];
             if (t.n == 0) continue;
-            b.blk0[b.count] = (uint32_t)pieces;
-            b.s[b.count++] = haste::GradSeg{t.g, t.n, t.dtype};
-            pieces += haste::ceil_div(t.n, (int64_t)haste::kNormElems);
-            HASTE_CHECK_ARG(pieces < (int64_t)1 << 31, "%s: tensors too large", fn);
+            b.piece0[b.count] = (uint32_t)pieces;
+            b.g[b.count] = t.g;
+            b.n_dtype[b.count++] = (uint64_t)t.n | (uint64_t)t.dtype << 56;
+            pieces += haste::ceil_div(t.n, (int64_t)haste::kNormPiece);
+            HASTE_CHECK_ARG(pieces < (int64_t)1 << 30, "%s: tensors too large", fn);
         }
         if (b.count == 0) break;
+        b.pieces = (int32_t)pieces;
         const int64_t blocks = std::min<int64_t>(pieces, haste::kNormParts);
         haste::grad_norm_kernel<<<dim3((unsigned)blocks), dim3(haste::kNormThreads), 0, st>>>(
-            b, (uint32_t)pieces, part + parts);
+            b, part + parts);
         HASTE_CHECK_LAUNCH(fn);
         parts += blocks;
     }
-    haste::grad_norm_final_kernel<<<dim3(1), dim3(haste::kNormThreads), 0, st>>>(
+    haste::grad_norm_final_kernel<<<dim3(1), dim3(haste::kFinalThreads), 0, st>>>(
         part, parts, (float)max_norm, out);
     HASTE_CHECK_LAUNCH(fn);
     return HASTE_OK;
