@@ -1,6 +1,7 @@
 // The norm of many gradients, and AdamW steps of many tensors with states in 32 or in 8 bits.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "elements.hpp"
 
@@ -11,8 +12,7 @@ constexpr int kBlock = 128;    // elements of an 8-bit state that share a scale
 constexpr int kMaxSegs = 64;   // tensors of one launch: a lane to each when a wave looks its own up,
                                // and their table stays within 4 KB of kernel arguments
 constexpr int kThreads = 256;
-constexpr int kPiece = kThreads * 8;  // elements that a workgroup steps at a time
-constexpr int kPieces = 2;            // pieces of a workgroup
+constexpr int kPiece = kThreads * 8;  // elements of a workgroup
 
 struct AdamSeg {
     void* w;
@@ -147,139 +147,182 @@ __device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
     }
 }
 
-// Eight consecutive elements of a tensor, as loaded.
-template <int WT, int GT, bool Q8>
-struct AdamElems {
-    Elems8<WT> w;
-    Elems8<GT> g;
-    Elems8<HASTE_DTYPE_F32> m, v;  // fp32 states
-    u32x2 m8, u8;                  // codes
-    uint32_t ms, us;
-};
-
-// FULL: all of the workgroup's elements are the tensor's; else `count` (of eight) are.
-template <int WT, int GT, bool Q8, bool FULL>
-__device__ __forceinline__ void adam_load(AdamElems<WT, GT, Q8>& x, const AdamSeg& s, int64_t i,
-                                          int64_t count) {
-    if constexpr (FULL) {
-        x.w = load8<WT>(s.w, i);
-        x.g = load8<GT>(s.g, i);
-    } else {
-        x.w = load8_part<WT>(s.w, i, count);
-        x.g = load8_part<GT>(s.g, i, count);
-    }
-    if constexpr (Q8) {
-        x.m8 = x.u8 = u32x2{0, 0};
-        x.ms = x.us = 127;
-        if (FULL || count > 0) {
-            x.m8 = *reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.m) + i);
-            x.u8 = *reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.v) + i);
-            x.ms = s.ms[i / kBlock];
-            x.us = s.vs[i / kBlock];
-        }
-    } else if constexpr (FULL) {
-        x.m = load8<HASTE_DTYPE_F32>(s.m, i);
-        x.v = load8<HASTE_DTYPE_F32>(s.v, i);
-    } else {
-        x.m = load8_part<HASTE_DTYPE_F32>(s.m, i, count);
-        x.v = load8_part<HASTE_DTYPE_F32>(s.v, i, count);
-    }
+// w' of one element; u = sqrt(v').  The hardware's root and reciprocal are within 1 ulp.
+__device__ __forceinline__ float adam_weight(float w, float m, float u, const AdamArgs& a) {
+    return w * a.decay - a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps);
 }
 
-template <int WT, int GT, bool Q8, bool FULL>
-__device__ __forceinline__ void adam_step(const AdamElems<WT, GT, Q8>& x, const AdamSeg& s,
-                                          const AdamArgs& a, float gs, int64_t i, int64_t count) {
-    float w[8], g[8], m[8], v[8], u[8];
-    unpack8<WT>(x.w, w);
-    unpack8<GT>(x.g, g);
-    if constexpr (Q8) {
-        from_e4m3(x.m8, m);
-        from_e4m3(x.u8, u);
-        const float fm = a.b1 * pow2_code(x.ms), fu = a.root_b2 * pow2_code(x.us);
+template <int WT>
+__device__ __forceinline__ uint32_t sr_pair(float lo, float hi, uint32_t r_lo, uint32_t r_hi) {
+    r_lo &= 0xFFFFu;
+    r_hi &= 0xFFFFu;
+    return WT == HASTE_DTYPE_BF16 ? sr_bf16(lo, r_lo) | sr_bf16(hi, r_hi) << 16
+                                  : sr_f16(lo, r_lo) | sr_f16(hi, r_hi) << 16;
+}
+
+// 32-bit states: a piece's thread has two runs of four elements, a piece's half apart, so that every
+// 16-byte access of fp32 is next to its neighbour lane's.
+template <int WT, int GT>
+struct AdamElems32 {
+    static constexpr int kRun = kThreads * 4;
+    Elems4<WT> w[2];
+    Elems4<GT> g[2];
+    Elems4<HASTE_DTYPE_F32> m[2], v[2];
+
+    // FULL: all of the workgroup's elements are the tensor's; else those below n are.
+    template <bool FULL>
+    __device__ __forceinline__ void load(const AdamSeg& s, int64_t piece, int64_t n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (!FULL && e >= count) m[e] = u[e] = 0.f;
-            g[e] *= gs;
-            m[e] = m[e] * fm + a.c1 * g[e];
-            u[e] *= fu;
-            u[e] = u[e] * u[e] + a.c2 * g[e] * g[e];
+        for (int k = 0; k < 2; ++k) {
+            const int64_t i = piece + k * kRun + threadIdx.x * 4;
+            if constexpr (FULL) {
+                w[k] = load4<WT, true>(s.w, i);
+                g[k] = load4<GT, true>(s.g, i);
+                m[k] = load4<HASTE_DTYPE_F32, true>(s.m, i);
+                v[k] = load4<HASTE_DTYPE_F32, true>(s.v, i);
+            } else {
+                w[k] = load4_part<WT>(s.w, i, n - i);
+                g[k] = load4_part<GT>(s.g, i, n - i);
+                m[k] = load4_part<HASTE_DTYPE_F32>(s.m, i, n - i);
+                v[k] = load4_part<HASTE_DTYPE_F32>(s.v, i, n - i);
+            }
         }
-    } else {
-        unpack8<HASTE_DTYPE_F32>(x.m, m);
-        unpack8<HASTE_DTYPE_F32>(x.v, v);
+    }
+
+    template <bool FULL>
+    __device__ __forceinline__ void step(const AdamSeg& s, const AdamArgs& a, float gs,
+                                         int64_t piece, int64_t n) const {
+        const uint32_t stream = (uint32_t)(s.n_stream >> 40);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            g[e] *= gs;
-            m[e] = a.b1 * m[e] + a.c1 * g[e];
-            u[e] = v[e] = a.b2 * v[e] + a.c2 * g[e] * g[e];
+        for (int k = 0; k < 2; ++k) {
+            const int64_t i = piece + k * kRun + threadIdx.x * 4;
+            float wf[4], gf[4], mf[4], vf[4];
+            unpack4<WT>(w[k], wf);
+            unpack4<GT>(g[k], gf);
+            unpack4<HASTE_DTYPE_F32>(m[k], mf);
+            unpack4<HASTE_DTYPE_F32>(v[k], vf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                gf[e] *= gs;
+                mf[e] = a.b1 * mf[e] + a.c1 * gf[e];
+                vf[e] = a.b2 * vf[e] + a.c2 * gf[e] * gf[e];
+                wf[e] = adam_weight(wf[e], mf[e], __builtin_amdgcn_sqrtf(vf[e]), a);
+            }
+            Elems4<WT> out;
+            if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+                const uint64_t c = (uint64_t)i / 8;
+                const u32x4 q = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
+                const uint32_t r0 = i & 4 ? q[2] : q[0], r1 = i & 4 ? q[3] : q[1];
+                out.q[0] = sr_pair<WT>(wf[0], wf[1], r0, r0 >> 16);
+                out.q[1] = sr_pair<WT>(wf[2], wf[3], r1, r1 >> 16);
+            } else {
+                out = pack4<WT>(wf);
+            }
+            const Elems4<HASTE_DTYPE_F32> mo = pack4<HASTE_DTYPE_F32>(mf),
+                                          vo = pack4<HASTE_DTYPE_F32>(vf);
+            if constexpr (FULL) {
+                store4<WT, true>(s.w, i, out);
+                store4<HASTE_DTYPE_F32, true>(s.m, i, mo);
+                store4<HASTE_DTYPE_F32, true>(s.v, i, vo);
+            } else {
+                store4_part<WT>(s.w, i, out, n - i);
+                store4_part<HASTE_DTYPE_F32>(s.m, i, mo, n - i);
+                store4_part<HASTE_DTYPE_F32>(s.v, i, vo, n - i);
+            }
         }
+    }
+};
+
+// 8-bit states: a thread has eight elements, so 16 lanes (one DPP row) a block of 128, whose
+// maxima need no LDS.  The states are padded to whole blocks.
+template <int WT, int GT>
+struct AdamElems8 {
+    Elems8<WT> w;
+    Elems8<GT> g;
+    u32x2 m, u;
+    uint32_t ms, us;
+
+    template <bool FULL>
+    __device__ __forceinline__ void load(const AdamSeg& s, int64_t piece, int64_t n) {
+        const int64_t i = piece + threadIdx.x * 8;
         if constexpr (FULL) {
-            store8<HASTE_DTYPE_F32>(s.m, i, pack8<HASTE_DTYPE_F32>(m));
-            store8<HASTE_DTYPE_F32>(s.v, i, pack8<HASTE_DTYPE_F32>(v));
+            w = load8<WT, WT != HASTE_DTYPE_F32>(s.w, i);
+            g = load8<GT, GT != HASTE_DTYPE_F32>(s.g, i);
         } else {
-            store8_part<HASTE_DTYPE_F32>(s.m, i, pack8<HASTE_DTYPE_F32>(m), count);
-            store8_part<HASTE_DTYPE_F32>(s.v, i, pack8<HASTE_DTYPE_F32>(v), count);
+            w = load8_part<WT>(s.w, i, n - i);
+            g = load8_part<GT>(s.g, i, n - i);
+        }
+        m = u = u32x2{0, 0};
+        ms = us = 127;
+        if (FULL || i < n) {
+            const u32x2* mp = reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.m) + i);
+            const u32x2* up = reinterpret_cast<const u32x2*>(static_cast<uint8_t*>(s.v) + i);
+            m = __builtin_nontemporal_load(mp);
+            u = __builtin_nontemporal_load(up);
+            ms = s.ms[i / kBlock];
+            us = s.vs[i / kBlock];
         }
     }
-    // the hardware's root and reciprocal are within 1 ulp
+
+    template <bool FULL>
+    __device__ __forceinline__ void step(const AdamSeg& s, const AdamArgs& a, float gs,
+                                         int64_t piece, int64_t n) const {
+        const int64_t i = piece + threadIdx.x * 8;
+        float wf[8], gf[8], mf[8], uf[8];
+        unpack8<WT>(w, wf);
+        unpack8<GT>(g, gf);
+        from_e4m3(m, mf);
+        from_e4m3(u, uf);
+        const float fm = a.b1 * pow2_code(ms), fu = a.root_b2 * pow2_code(us);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        u[e] = __builtin_amdgcn_sqrtf(u[e]);
-        w[e] = w[e] * a.decay - a.lr * m[e] * __builtin_amdgcn_rcpf(u[e] * a.rcorr + a.eps);
-    }
-    uint32_t r[8];
-    const uint32_t stream = (uint32_t)(s.n_stream >> 40);
-    if constexpr (Q8) {
-        const uint64_t k = (uint64_t)i / 4;
-        const u32x4 q0 = philox_words((uint32_t)k, (uint32_t)(k >> 32), stream, a.k0, a.k1);
-        const u32x4 q1 = philox_words((uint32_t)k + 1, (uint32_t)(k >> 32), stream, a.k0, a.k1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            r[e] = q0[e];
-            r[4 + e] = q1[e];
+        for (int e = 0; e < 8; ++e) {
+            if (!FULL && i + e >= n) mf[e] = uf[e] = 0.f;
+            gf[e] *= gs;
+            mf[e] = mf[e] * fm + a.c1 * gf[e];
+            uf[e] *= fu;
+            uf[e] = __builtin_amdgcn_sqrtf(uf[e] * uf[e] + a.c2 * gf[e] * gf[e]);
+            wf[e] = adam_weight(wf[e], mf[e], uf[e], a);
         }
-    } else if (WT != HASTE_DTYPE_F32 && a.do_sr) {
-        const uint64_t k = (uint64_t)i / 8;
-        const u32x4 q = philox_words((uint32_t)k, (uint32_t)(k >> 32), stream, a.k0, a.k1);
+        const uint32_t stream = (uint32_t)(s.n_stream >> 40);
+        const uint64_t c = (uint64_t)i / 4;
+        const u32x4 q0 = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
+        const u32x4 q1 = philox_words((uint32_t)c + 1, (uint32_t)(c >> 32), stream, a.k0, a.k1);
+        const uint32_t r[8] = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
+        Elems8<WT> out;
+        if (WT != HASTE_DTYPE_F32 && a.do_sr) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            r[2 * e] = q[e];
-            r[2 * e + 1] = q[e] >> 16;
+            for (int e = 0; e < 4; ++e)
+                out.q[0][e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
+        } else {
+            out = pack8<WT>(wf);
         }
-    }
-    Elems8<WT> out;
-    if (WT != HASTE_DTYPE_F32 && a.do_sr) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const uint32_t lo = r[e] & 0xFFFFu, hi = r[e + 1] & 0xFFFFu;
-            out.q[0][e / 2] = WT == HASTE_DTYPE_BF16 ? sr_bf16(w[e], lo) | sr_bf16(w[e + 1], hi) << 16
-                                                     : sr_f16(w[e], lo) | sr_f16(w[e + 1], hi) << 16;
-        }
-    } else {
-        out = pack8<WT>(w);
-    }
-    if constexpr (FULL) store8<WT>(s.w, i, out);
-    else store8_part<WT>(s.w, i, out, count);
-    if constexpr (Q8) {
-        const uint32_t cm = scale_code(m), cu = scale_code(u);
+        if constexpr (FULL) store8<WT, WT != HASTE_DTYPE_F32>(s.w, i, out);
+        else store8_part<WT>(s.w, i, out, n - i);
+        const uint32_t cm = scale_code(mf), cu = scale_code(uf);
         const uint32_t ru[8] = {r[1], r[2], r[3], r[0], r[5], r[6], r[7], r[4]};
-        const u32x2 m8 = cut_e4m3<false>(m, cm, r), u8 = cut_e4m3<true>(u, cu, ru);
-        // (the states are padded to whole blocks of 128)
-        if (FULL || (i & ~(int64_t)(kBlock - 1)) < i + count) {
-            *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.m) + i) = m8;
-            *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.v) + i) = u8;
+        const u32x2 mo = cut_e4m3<false>(mf, cm, r), uo = cut_e4m3<true>(uf, cu, ru);
+        if (FULL || (i & ~(int64_t)(kBlock - 1)) < n) {
+            u32x2* mp = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.m) + i);
+            u32x2* up = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.v) + i);
+            __builtin_nontemporal_store(mo, mp);
+            __builtin_nontemporal_store(uo, up);
             if ((threadIdx.x & 15) == 0) {
                 s.ms[i / kBlock] = (uint8_t)cm;
                 s.vs[i / kBlock] = (uint8_t)cu;
             }
         }
     }
-}
+};
 
-// A thread to eight elements, so 16 lanes (one DPP row) to a block of an 8-bit state: its maxima
-// need no LDS.
+// Bound by HBM: every byte is met once.  All accesses are non-temporal (but 8-wide ones of fp32, of
+// which each touches half a line), which leaves the last-level cache to the gradients that the
+// norm has just read, and not to dirty lines: 12 layers of 768 in bf16 with 8-bit states (92 M
+// weights, norm included) 221 -> 188 us, 670 M weights 1497 -> 1350; with 32-bit states in runs of
+// four 424 -> 345 (5.8 TB/s), fp32 352 -> 281.  One piece to a workgroup and two take the same
+// within 3 %.
 template <int WT, int GT, bool Q8>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, const AdamArgs a) {
+    using Elems = std::conditional_t<Q8, AdamElems8<WT, GT>, AdamElems32<WT, GT>>;
     float gs = 1.f;
     if (a.grad_scale) {
         gs = *a.grad_scale;
@@ -288,23 +331,14 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, cons
     const int t = find_seg(b, blockIdx.x);
     const AdamSeg& s = b.s[t];
     const int64_t n = (int64_t)(s.n_stream & 0xFFFFFFFFFFull);
-    const int64_t i0 = (int64_t)(blockIdx.x - b.blk0[t]) * (kPiece * kPieces);
-    const int64_t i = i0 + threadIdx.x * 8;
-    if (i0 + kPiece * kPieces <= n) {
-        AdamElems<WT, GT, Q8> x[kPieces];
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p)
-            adam_load<WT, GT, Q8, true>(x[p], s, i + p * kPiece, 8);
-#pragma unroll
-        for (int p = 0; p < kPieces; ++p)
-            adam_step<WT, GT, Q8, true>(x[p], s, a, gs, i + p * kPiece, 8);
+    const int64_t i0 = (int64_t)(blockIdx.x - b.blk0[t]) * kPiece;
+    Elems x;
+    if (i0 + kPiece <= n) {
+        x.template load<true>(s, i0, n);
+        x.template step<true>(s, a, gs, i0, n);
     } else {
-        for (int p = 0; p < kPieces; ++p) {
-            const int64_t at = i + p * kPiece, count = n - at;
-            AdamElems<WT, GT, Q8> x;
-            adam_load<WT, GT, Q8, false>(x, s, at, count);
-            adam_step<WT, GT, Q8, false>(x, s, a, gs, at, count);
-        }
+        x.template load<false>(s, i0, n);
+        x.template step<false>(s, a, gs, i0, n);
     }
 }
 
@@ -406,7 +440,7 @@ int launch_adamw(const haste_adamw_tensor* ts, int count, const AdamArgs& a, hip
             b.blk0[b.count] = (uint32_t)blocks;
             b.s[b.count++] = AdamSeg{t.w, t.g, t.m, t.v, t.m_scale, t.v_scale,
                                      (uint64_t)t.n | (uint64_t)t.stream << 40};
-            blocks += ceil_div(t.n, (int64_t)kPiece * kPieces);
+            blocks += ceil_div(t.n, (int64_t)kPiece);
             HASTE_CHECK_ARG(blocks < (int64_t)1 << 31, "haste_adamw_step: tensors too large");
         }
         if (b.count == 0) break;

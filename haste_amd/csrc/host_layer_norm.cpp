@@ -6,7 +6,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -20,12 +19,6 @@ namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-void* stream_of(const at::Tensor& t) {
-    return c10::hip::getCurrentHIPStream(t.get_device()).stream();
-}
-
-void call(int rc) { TORCH_CHECK(rc == HASTE_OK, haste_last_error()); }
 
 // t as rows [N, D] with contiguous columns, `ld` elements apart (0: one row for all), copied only
 // where it has no such view.
@@ -223,12 +216,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
             h = f.h;
         }
     }
-    if (!h.defined()) return THPVariable_Wrap(y);
-    PyObject *a = THPVariable_Wrap(y), *b = a ? THPVariable_Wrap(h) : nullptr;
-    PyObject* pair = b ? PyTuple_Pack(2, a, b) : nullptr;
-    Py_XDECREF(a);
-    Py_XDECREF(b);
-    return pair;
+    return h.defined() ? pair_of(y, h) : THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS
 }
 

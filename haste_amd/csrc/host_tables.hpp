@@ -3,7 +3,9 @@
 
 #include <Python.h>
 
-#include <c10/core/ScalarType.h>
+#include <ATen/core/Tensor.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/haste_ffi.h"
 
@@ -15,6 +17,21 @@ inline int dtype_code(c10::ScalarType t) {
            : t == c10::kHalf   ? HASTE_DTYPE_F16
            : t == c10::kFloat  ? HASTE_DTYPE_F32
                                : -1;
+}
+
+inline void* stream_of(const at::Tensor& t) {
+    return c10::hip::getCurrentHIPStream(t.get_device()).stream();
+}
+
+inline void call(int rc) { TORCH_CHECK(rc == HASTE_OK, haste_last_error()); }
+
+// (a, b) as Python tensors.
+inline PyObject* pair_of(const at::Tensor& a, const at::Tensor& b) {
+    PyObject *x = THPVariable_Wrap(a), *y = x ? THPVariable_Wrap(b) : nullptr;
+    PyObject* pair = y ? PyTuple_Pack(2, x, y) : nullptr;
+    Py_XDECREF(x);
+    Py_XDECREF(y);
+    return pair;
 }
 
 // layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual

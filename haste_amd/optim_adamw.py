@@ -57,20 +57,18 @@ def grad_norm(tensors: Iterable[torch.Tensor], max_norm: float = math.inf
     tensors = list(tensors)
     if not tensors:
         raise RuntimeError("grad_norm: no tensors")
-    n, rows = len(tensors), _lib.host().grad_rows(tensors)
-    if rows is not None:
-        arr, index = rows
-        dev = torch.device("cuda", index)
-    else:
-        for t in tensors:
-            _C.require_device(t, "gradients")
-        tensors, dev = [_dense(t, "gradients") for t in tensors], tensors[0].device
-        for t in tensors:
-            if t.device != dev:
-                raise RuntimeError(f"grad_norm: tensors must be on one device (got {dev}, "
-                                   f"{t.device})")
-        arr = (_lib.GradTensor * n)(*[(t.data_ptr(), t.numel(), _C.dtype_code(t.dtype))
-                                      for t in tensors])
+    got = _lib.host().grad_norm(tensors, float(max_norm))
+    if got is not None:
+        return got
+    for t in tensors:
+        _C.require_device(t, "gradients")
+    n, dev = len(tensors), tensors[0].device
+    tensors = [_dense(t, "gradients") for t in tensors]
+    for t in tensors:
+        if t.device != dev:
+            raise RuntimeError(f"grad_norm: tensors must be on one device (got {dev}, {t.device})")
+    arr = (_lib.GradTensor * n)(*[(t.data_ptr(), t.numel(), _C.dtype_code(t.dtype))
+                                  for t in tensors])
     out = torch.empty(2, dtype=torch.float32, device=dev)
     size = _lib.lib().haste_grad_norm_workspace_size(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
@@ -164,14 +162,14 @@ class AdamW(Optimizer):
         return loss
 
     def _step_group(self, group, grad_scale) -> None:
-        bits, copies = group["state_bits"], []
-        got = _lib.host().adamw_rows(group["params"], self.state, bits)
-        if got is None:
-            batches, device, keep, copies = self._rows(group["params"], bits)
-        else:
-            batches, device = got
-        seed, (beta1, beta2) = group["seed"], group["betas"]
+        bits, seed = group["state_bits"], group["seed"]
+        (beta1, beta2), sr = group["betas"], bool(group["stochastic_rounding"])
+        args = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]),
+                float(group["weight_decay"]))
         group["seed"] += 1
+        if _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, grad_scale):
+            return
+        batches, device, keep, copies = self._rows(group["params"], bits)
         if not batches:
             return
         scale = None
@@ -182,15 +180,13 @@ class AdamW(Optimizer):
             scale = grad_scale.data_ptr()
         stream = torch._C._cuda_getCurrentRawStream(device)
         for w_code, g_code, step, count, rows in batches:
-            _lib.call("haste_adamw_step", rows, count, w_code, g_code, bits, float(group["lr"]),
-                      float(beta1), float(beta2), float(group["eps"]),
-                      float(group["weight_decay"]), step, int(bool(group["stochastic_rounding"])),
+            _lib.call("haste_adamw_step", rows, count, w_code, g_code, bits, *args, step, int(sr),
                       int(seed), scale, stream)
         for p, w in copies:
             p.copy_(w)
 
     def _rows(self, params, bits):
-        """adamw_rows of the native module for any parameters: ([(w dtype, g dtype, step, tensors, rows)],
+        """The table of the step of any parameters: ([(w dtype, g dtype, step, tensors, rows)],
         device, tensors to keep until the launch, [(parameter, contiguous copy to step)]),
         with states made where there are none yet."""
         batches, stepped, copies, keep, device = {}, [], [], [], None
