@@ -165,26 +165,26 @@ __device__ __forceinline__ uint32_t sr_pair(float lo, float hi, uint32_t r_lo, u
 template <int WT, int GT>
 struct AdamElems32 {
     static constexpr int kRun = kThreads * 4;
-    Elems4<WT> w[2];
-    Elems4<GT> g[2];
-    Elems4<HASTE_DTYPE_F32> m[2], v[2];
+    Elems<WT, 4> w[2];
+    Elems<GT, 4> g[2];
+    Elems<HASTE_DTYPE_F32, 4> m[2], v[2];
 
     // FULL: all of the workgroup's elements are the tensor's; else those below n are.
     template <bool FULL>
-    __device__ __forceinline__ void load(const AdamSeg& s, int64_t piece, int64_t n) {
+    __device__ __forceinline__ void fetch(const AdamSeg& s, int64_t piece, int64_t n) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t i = piece + k * kRun + threadIdx.x * 4;
             if constexpr (FULL) {
-                w[k] = load4<WT, true>(s.w, i);
-                g[k] = load4<GT, true>(s.g, i);
-                m[k] = load4<HASTE_DTYPE_F32, true>(s.m, i);
-                v[k] = load4<HASTE_DTYPE_F32, true>(s.v, i);
+                w[k] = load<WT, 4, true>(s.w, i);
+                g[k] = load<GT, 4, true>(s.g, i);
+                m[k] = load<HASTE_DTYPE_F32, 4, true>(s.m, i);
+                v[k] = load<HASTE_DTYPE_F32, 4, true>(s.v, i);
             } else {
-                w[k] = load4_part<WT>(s.w, i, n - i);
-                g[k] = load4_part<GT>(s.g, i, n - i);
-                m[k] = load4_part<HASTE_DTYPE_F32>(s.m, i, n - i);
-                v[k] = load4_part<HASTE_DTYPE_F32>(s.v, i, n - i);
+                w[k] = load_part<WT, 4>(s.w, i, n - i);
+                g[k] = load_part<GT, 4>(s.g, i, n - i);
+                m[k] = load_part<HASTE_DTYPE_F32, 4>(s.m, i, n - i);
+                v[k] = load_part<HASTE_DTYPE_F32, 4>(s.v, i, n - i);
             }
         }
     }
@@ -197,10 +197,10 @@ struct AdamElems32 {
         for (int k = 0; k < 2; ++k) {
             const int64_t i = piece + k * kRun + threadIdx.x * 4;
             float wf[4], gf[4], mf[4], vf[4];
-            unpack4<WT>(w[k], wf);
-            unpack4<GT>(g[k], gf);
-            unpack4<HASTE_DTYPE_F32>(m[k], mf);
-            unpack4<HASTE_DTYPE_F32>(v[k], vf);
+            unpack<WT, 4>(w[k], wf);
+            unpack<GT, 4>(g[k], gf);
+            unpack<HASTE_DTYPE_F32, 4>(m[k], mf);
+            unpack<HASTE_DTYPE_F32, 4>(v[k], vf);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 gf[e] *= gs;
@@ -208,7 +208,7 @@ struct AdamElems32 {
                 vf[e] = a.b2 * vf[e] + a.c2 * gf[e] * gf[e];
                 wf[e] = adam_weight(wf[e], mf[e], __builtin_amdgcn_sqrtf(vf[e]), a);
             }
-            Elems4<WT> out;
+            Elems<WT, 4> out;
             if (WT != HASTE_DTYPE_F32 && a.do_sr) {
                 const uint64_t c = (uint64_t)i / 8;
                 const u32x4 q = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
@@ -216,18 +216,18 @@ struct AdamElems32 {
                 out.q[0] = sr_pair<WT>(wf[0], wf[1], r0, r0 >> 16);
                 out.q[1] = sr_pair<WT>(wf[2], wf[3], r1, r1 >> 16);
             } else {
-                out = pack4<WT>(wf);
+                out = pack<WT, 4>(wf);
             }
-            const Elems4<HASTE_DTYPE_F32> mo = pack4<HASTE_DTYPE_F32>(mf),
-                                          vo = pack4<HASTE_DTYPE_F32>(vf);
+            const Elems<HASTE_DTYPE_F32, 4> mo = pack<HASTE_DTYPE_F32, 4>(mf),
+                                          vo = pack<HASTE_DTYPE_F32, 4>(vf);
             if constexpr (FULL) {
-                store4<WT, true>(s.w, i, out);
-                store4<HASTE_DTYPE_F32, true>(s.m, i, mo);
-                store4<HASTE_DTYPE_F32, true>(s.v, i, vo);
+                store<WT, 4, true>(s.w, i, out);
+                store<HASTE_DTYPE_F32, 4, true>(s.m, i, mo);
+                store<HASTE_DTYPE_F32, 4, true>(s.v, i, vo);
             } else {
-                store4_part<WT>(s.w, i, out, n - i);
-                store4_part<HASTE_DTYPE_F32>(s.m, i, mo, n - i);
-                store4_part<HASTE_DTYPE_F32>(s.v, i, vo, n - i);
+                store_part<WT, 4>(s.w, i, out, n - i);
+                store_part<HASTE_DTYPE_F32, 4>(s.m, i, mo, n - i);
+                store_part<HASTE_DTYPE_F32, 4>(s.v, i, vo, n - i);
             }
         }
     }
@@ -237,20 +237,20 @@ struct AdamElems32 {
 // maxima need no LDS.  The states are padded to whole blocks.
 template <int WT, int GT>
 struct AdamElems8 {
-    Elems8<WT> w;
-    Elems8<GT> g;
+    Elems<WT, 8> w;
+    Elems<GT, 8> g;
     u32x2 m, u;
     uint32_t ms, us;
 
     template <bool FULL>
-    __device__ __forceinline__ void load(const AdamSeg& s, int64_t piece, int64_t n) {
+    __device__ __forceinline__ void fetch(const AdamSeg& s, int64_t piece, int64_t n) {
         const int64_t i = piece + threadIdx.x * 8;
         if constexpr (FULL) {
-            w = load8<WT, WT != HASTE_DTYPE_F32>(s.w, i);
-            g = load8<GT, GT != HASTE_DTYPE_F32>(s.g, i);
+            w = load<WT, 8, WT != HASTE_DTYPE_F32>(s.w, i);
+            g = load<GT, 8, GT != HASTE_DTYPE_F32>(s.g, i);
         } else {
-            w = load8_part<WT>(s.w, i, n - i);
-            g = load8_part<GT>(s.g, i, n - i);
+            w = load_part<WT, 8>(s.w, i, n - i);
+            g = load_part<GT, 8>(s.g, i, n - i);
         }
         m = u = u32x2{0, 0};
         ms = us = 127;
@@ -269,8 +269,8 @@ struct AdamElems8 {
                                          int64_t piece, int64_t n) const {
         const int64_t i = piece + threadIdx.x * 8;
         float wf[8], gf[8], mf[8], uf[8];
-        unpack8<WT>(w, wf);
-        unpack8<GT>(g, gf);
+        unpack<WT, 8>(w, wf);
+        unpack<GT, 8>(g, gf);
         from_e4m3(m, mf);
         from_e4m3(u, uf);
         const float fm = a.b1 * pow2_code(ms), fu = a.root_b2 * pow2_code(us);
@@ -288,16 +288,16 @@ struct AdamElems8 {
         const u32x4 q0 = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
         const u32x4 q1 = philox_words((uint32_t)c + 1, (uint32_t)(c >> 32), stream, a.k0, a.k1);
         const uint32_t r[8] = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
-        Elems8<WT> out;
+        Elems<WT, 8> out;
         if (WT != HASTE_DTYPE_F32 && a.do_sr) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                out.q[0][e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
+                out.q[e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
         } else {
-            out = pack8<WT>(wf);
+            out = pack<WT, 8>(wf);
         }
-        if constexpr (FULL) store8<WT, WT != HASTE_DTYPE_F32>(s.w, i, out);
-        else store8_part<WT>(s.w, i, out, n - i);
+        if constexpr (FULL) store<WT, 8, WT != HASTE_DTYPE_F32>(s.w, i, out);
+        else store_part<WT, 8>(s.w, i, out, n - i);
         const uint32_t cm = scale_code(mf), cu = scale_code(uf);
         const uint32_t ru[8] = {r[1], r[2], r[3], r[0], r[5], r[6], r[7], r[4]};
         const u32x2 mo = cut_e4m3<false>(mf, cm, r), uo = cut_e4m3<true>(uf, cu, ru);
@@ -334,10 +334,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, cons
     const int64_t i0 = (int64_t)(blockIdx.x - b.blk0[t]) * kPiece;
     Elems x;
     if (i0 + kPiece <= n) {
-        x.template load<true>(s, i0, n);
+        x.template fetch<true>(s, i0, n);
         x.template step<true>(s, a, gs, i0, n);
     } else {
-        x.template load<false>(s, i0, n);
+        x.template fetch<false>(s, i0, n);
         x.template step<false>(s, a, gs, i0, n);
     }
 }
@@ -359,12 +359,12 @@ __device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_
     float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[8];
     const int64_t i = i0 + threadIdx.x * 8;
     if (i0 + kNormPiece <= n) {
-        Elems8<DT> x[kNormLoads];
+        Elems<DT, 8> x[kNormLoads];
 #pragma unroll
-        for (int k = 0; k < kNormLoads; ++k) x[k] = load8<DT>(g, i + k * (kNormThreads * 8));
+        for (int k = 0; k < kNormLoads; ++k) x[k] = load<DT, 8>(g, i + k * (kNormThreads * 8));
 #pragma unroll
         for (int k = 0; k < kNormLoads; ++k) {
-            unpack8<DT>(x[k], f);
+            unpack<DT, 8>(x[k], f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
         }
@@ -372,7 +372,7 @@ __device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_
         for (int k = 0; k < kNormLoads; ++k) {
             const int64_t at = i + k * (kNormThreads * 8);
             if (at >= n) break;
-            unpack8<DT>(load8_part<DT>(g, at, n - at), f);
+            unpack<DT, 8>(load_part<DT, 8>(g, at, n - at), f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
         }

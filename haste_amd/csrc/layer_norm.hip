@@ -4,6 +4,18 @@
 
 #include "elements.hpp"
 
+#ifndef NTX
+#define NTX 0
+#endif
+#ifndef NTB
+#define NTB 0
+#endif
+#ifndef NTH
+#define NTH 0
+#endif
+#ifndef NTY
+#define NTY 0
+#endif
 namespace haste {
 namespace {
 
@@ -120,19 +132,21 @@ __global__ __launch_bounds__(kRowThreads) void ln_dw_any_kernel(const char* dy, 
 }
 
 // ------------------------------------------------------- rows in registers ----
-// `tpr` threads (a power of two from 16) hold a row, 8 elements in each of C slots: thread t has
-// elements 8 (c tpr + t) + 0..7 of it in slot c.  Only the last slot can pass the row's end:
-// there a thread reads and writes the row's last 8 elements instead, of which it shares the
-// first `skip` with other threads (which compute the same values) and leaves them out of sums;
-// with skip >= 8 it has none of its own.
+// `tpr` threads (a power of two from 16) hold a row, V elements (16 bytes) in each of C slots:
+// thread t has elements V (c tpr + t) + 0..V-1 of it in slot c.  Only the last slot can pass the
+// row's end: there a thread reads and writes the row's last V elements instead, of which it
+// shares the first `skip` with other threads (which compute the same values) and leaves them out
+// of sums; with skip >= V it has none of its own.
+constexpr int row_vec(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 8; }
 struct Slot {
     int64_t at;  // first element
     int skip;
 };
+template <int V>
 __device__ __forceinline__ Slot row_slot(int c, int C, int tpr, int lane, int64_t D) {
-    const int64_t e = 8 * ((int64_t)c * tpr + lane);
+    const int64_t e = V * ((int64_t)c * tpr + lane);
     if (c < C - 1) return Slot{e, 0};
-    const int64_t at = min(e, D - 8);
+    const int64_t at = min(e, D - V);
     return Slot{at, (int)(e - at)};
 }
 
@@ -185,7 +199,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_kernel(
     const void* __restrict__ w, const void* __restrict__ b, char* __restrict__ y,
     char* __restrict__ h, float* __restrict__ stats, int64_t N, int64_t D, float eps, int tpr) {
     __shared__ float part[2][32];
-    constexpr int S = kElemBytes<DT>;
+    constexpr int S = kElemBytes<DT>, V = row_vec(DT);
     const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
     const int64_t want = (int64_t)blockIdx.x * (blockDim.x / tpr) + group;
     const int64_t row = min(want, N - 1);
@@ -193,38 +207,38 @@ __global__ __launch_bounds__(1024) void ln_fwd_kernel(
     int turn = 0;
     x += row * ldx * S;
     if (res) res += row * ldres * S;
-    Elems8<DT> raw[C], add[C];
+    Elems<DT, V> raw[C], add[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) raw[c] = load8<DT>(x, row_slot(c, C, tpr, lane, D).at);
+    for (int c = 0; c < C; ++c) raw[c] = load<DT, V, NTX>(x, row_slot<V>(c, C, tpr, lane, D).at);
     if (res) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) add[c] = load8<DT>(res, row_slot(c, C, tpr, lane, D).at);
+        for (int c = 0; c < C; ++c) add[c] = load<DT, V, NTX>(res, row_slot<V>(c, C, tpr, lane, D).at);
     }
-    float f[C][8], s = 0.f, none = 0.f;
+    float f[C][V], s = 0.f, none = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const Slot at = row_slot(c, C, tpr, lane, D);
-        unpack8<DT>(raw[c], f[c]);
+        const Slot at = row_slot<V>(c, C, tpr, lane, D);
+        unpack<DT, V>(raw[c], f[c]);
         if (res) {
-            float g[8];
-            unpack8<DT>(add[c], g);
+            float g[V];
+            unpack<DT, V>(add[c], g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[c][e] += g[e];
-            const Elems8<DT> sum = pack8<DT>(f[c]);
-            if (live && at.skip < 8) store8<DT>(h + row * D * S, at.at, sum);
-            unpack8<DT>(sum, f[c]);
+            for (int e = 0; e < V; ++e) f[c][e] += g[e];
+            const Elems<DT, V> sum = pack<DT, V>(f[c]);
+            if (live && at.skip < V) store<DT, V, NTH>(h + row * D * S, at.at, sum);
+            unpack<DT, V>(sum, f[c]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += c < C - 1 || e >= at.skip ? f[c][e] : 0.f;
+        for (int e = 0; e < V; ++e) s += c < C - 1 || e >= at.skip ? f[c][e] : 0.f;
     }
     row_sums(s, none, tpr, part, turn);
     const float mean = s / (float)D;
     s = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int skip = row_slot(c, C, tpr, lane, D).skip;
+        const int skip = row_slot<V>(c, C, tpr, lane, D).skip;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < V; ++e) {
             f[c][e] -= mean;
             s += c < C - 1 || e >= skip ? f[c][e] * f[c][e] : 0.f;
         }
@@ -233,17 +247,17 @@ __global__ __launch_bounds__(1024) void ln_fwd_kernel(
     const float rstd = 1.f / sqrtf(s / (float)D + eps);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const Slot at = row_slot(c, C, tpr, lane, D);
-        float g[8];
-        unpack8<WT>(load8<WT>(w, at.at), g);
+        const Slot at = row_slot<V>(c, C, tpr, lane, D);
+        float g[V];
+        unpack<WT, V>(load<WT, V>(w, at.at), g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[c][e] = f[c][e] * rstd * g[e];
+        for (int e = 0; e < V; ++e) f[c][e] = f[c][e] * rstd * g[e];
         if (b) {
-            unpack8<WT>(load8<WT>(b, at.at), g);
+            unpack<WT, V>(load<WT, V>(b, at.at), g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[c][e] += g[e];
+            for (int e = 0; e < V; ++e) f[c][e] += g[e];
         }
-        if (live && at.skip < 8) store8<DT>(y + row * D * S, at.at, pack8<DT>(f[c]));
+        if (live && at.skip < V) store<DT, V, NTY>(y + row * D * S, at.at, pack<DT, V>(f[c]));
     }
     if (stats && lane == 0 && live) {
         stats[2 * row] = mean;
@@ -256,7 +270,8 @@ constexpr int kBwdBlocks = 512;  // partial sums of dw and db: one pair of rows 
 
 template <int DT, int C>
 struct BwdRow {
-    Elems8<DT> dy[C], h[C], dh[C];
+    static constexpr int V = row_vec(DT);
+    Elems<DT, V> dy[C], h[C], dh[C];
     float mean, rstd;
 };
 
@@ -271,26 +286,26 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     int64_t D, int tpr) {
     extern __shared__ float lds[];
     __shared__ float part[2][32];
-    constexpr int S = kElemBytes<DT>;
+    constexpr int S = kElemBytes<DT>, V = row_vec(DT);
     const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
     const int groups = kBwdThreads / tpr;
     const int64_t step = (int64_t)gridDim.x * groups;
     int turn = 0;
-    float g[C][8], aw[C][8], ab[C][8];
+    float g[C][V], aw[C][V], ab[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        unpack8<WT>(load8<WT>(w, row_slot(c, C, tpr, lane, D).at), g[c]);
+        unpack<WT, V>(load<WT, V>(w, row_slot<V>(c, C, tpr, lane, D).at), g[c]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) aw[c][e] = ab[c][e] = 0.f;
+        for (int e = 0; e < V; ++e) aw[c][e] = ab[c][e] = 0.f;
     }
-    auto load = [&](BwdRow<DT, C>& r, int64_t want) __attribute__((always_inline)) {
+    auto fetch = [&](BwdRow<DT, C>& r, int64_t want) __attribute__((always_inline)) {
         const int64_t row = min(want, N - 1);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int64_t at = row_slot(c, C, tpr, lane, D).at;
-            r.dy[c] = load8<DT>(dy + row * lddy * S, at);
-            r.h[c] = load8<DT>(h + row * ldh * S, at);
-            if (dh) r.dh[c] = load8<DT>(dh + row * lddh * S, at);
+            const int64_t at = row_slot<V>(c, C, tpr, lane, D).at;
+            r.dy[c] = load<DT, V, NTB>(dy + row * lddy * S, at);
+            r.h[c] = load<DT, V, NTB>(h + row * ldh * S, at);
+            if (dh) r.dh[c] = load<DT, V, NTB>(dh + row * lddh * S, at);
         }
         r.mean = stats[2 * row];
         r.rstd = stats[2 * row + 1];
@@ -299,20 +314,20 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     const int64_t turns = (N + step - 1) / step;
     int64_t row = (int64_t)blockIdx.x * groups + group;
     BwdRow<DT, C> next;
-    load(next, row);
+    fetch(next, row);
     for (int64_t k = 0; k < turns; ++k, row += step) {
         const BwdRow<DT, C> r = next;
-        if (k + 1 < turns) load(next, row + step);
+        if (k + 1 < turns) fetch(next, row + step);
         const bool live = row < N;
-        float s1 = 0.f, s2 = 0.f, n[C][8];
+        float s1 = 0.f, s2 = 0.f, n[C][V];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int skip = row_slot(c, C, tpr, lane, D).skip;
-            float d[8];
-            unpack8<DT>(r.dy[c], d);
-            unpack8<DT>(r.h[c], n[c]);
+            const int skip = row_slot<V>(c, C, tpr, lane, D).skip;
+            float d[V];
+            unpack<DT, V>(r.dy[c], d);
+            unpack<DT, V>(r.h[c], n[c]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < V; ++e) {
                 n[c][e] = (n[c][e] - r.mean) * r.rstd;
                 const bool own = live && (c < C - 1 || e >= skip);
                 const float a = d[e] * g[c][e];
@@ -327,32 +342,32 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
         const float c1 = s1 / (float)D, c2 = s2 / (float)D;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const Slot at = row_slot(c, C, tpr, lane, D);
-            float d[8];
-            unpack8<DT>(r.dy[c], d);
+            const Slot at = row_slot<V>(c, C, tpr, lane, D);
+            float d[V];
+            unpack<DT, V>(r.dy[c], d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = r.rstd * (d[e] * g[c][e] - c1 - n[c][e] * c2);
+            for (int e = 0; e < V; ++e) d[e] = r.rstd * (d[e] * g[c][e] - c1 - n[c][e] * c2);
             if (dh) {
-                float q[8];
-                unpack8<DT>(r.dh[c], q);
+                float q[V];
+                unpack<DT, V>(r.dh[c], q);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] += q[e];
+                for (int e = 0; e < V; ++e) d[e] += q[e];
             }
-            if (live && at.skip < 8) store8<DT>(dx + row * D * S, at.at, pack8<DT>(d));
+            if (live && at.skip < V) store<DT, V, NTY>(dx + row * D * S, at.at, pack<DT, V>(d));
         }
     }
     if (!sums) return;
     // the groups' sums, halved until the first has them all
     for (int half = groups / 2; half; half /= 2) {
         __syncthreads();
-        float* p = lds + (group & (half - 1)) * (16 * C * tpr) + lane;
+        float* p = lds + (group & (half - 1)) * (2 * V * C * tpr) + lane;
         if (group >= half && group < 2 * half) {
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[(16 * c + e) * tpr] = aw[c][e];
-                    p[(16 * c + 8 + e) * tpr] = ab[c][e];
+                for (int e = 0; e < V; ++e) {
+                    p[(2 * V * c + e) * tpr] = aw[c][e];
+                    p[(2 * V * c + V + e) * tpr] = ab[c][e];
                 }
         }
         __syncthreads();
@@ -360,9 +375,9 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    aw[c][e] += p[(16 * c + e) * tpr];
-                    ab[c][e] += p[(16 * c + 8 + e) * tpr];
+                for (int e = 0; e < V; ++e) {
+                    aw[c][e] += p[(2 * V * c + e) * tpr];
+                    ab[c][e] += p[(2 * V * c + V + e) * tpr];
                 }
         }
     }
@@ -370,9 +385,9 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     float* out = sums + (int64_t)blockIdx.x * 2 * D;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const Slot at = row_slot(c, C, tpr, lane, D);
+        const Slot at = row_slot<V>(c, C, tpr, lane, D);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < V; ++e)
             if (c < C - 1 || e >= at.skip) {
                 out[at.at + e] = aw[c][e];
                 out[D + at.at + e] = ab[c][e];
@@ -403,19 +418,20 @@ __global__ __launch_bounds__(1024) void ln_sums_kernel(const float* __restrict__
 }
 
 // How the threads hold rows of D elements in up to `slots` slots: the fewest threads left over,
-// then the fewest threads to a row.  C == 0: they do not fit `most` threads, or are under 8
-// elements.
+// then the fewest threads to a row.  C == 0: they do not fit `most` threads, or are shorter than
+// a slot.
 struct RowShape {
     int tpr, C;
 };
-RowShape row_shape(int64_t D, int most, int slots) {
+RowShape row_shape(int64_t D, int32_t dtype, int most, int slots) {
+    const int64_t V = row_vec(dtype);
     RowShape best{0, 0};
     int64_t over = 0;
-    if (D < 8) return best;
+    if (D < V) return best;
     for (int tpr = 16; tpr <= most; tpr *= 2) {
-        const int64_t C = ceil_div(D, (int64_t)8 * tpr);
+        const int64_t C = ceil_div(D, V * tpr);
         if (C > slots) continue;
-        const int64_t o = C * 8 * tpr - D;
+        const int64_t o = C * V * tpr - D;
         if (best.C == 0 || o < over) {
             best = RowShape{tpr, (int)C};
             over = o;
@@ -423,10 +439,13 @@ RowShape row_shape(int64_t D, int most, int slots) {
     }
     return best;
 }
-RowShape fwd_shape(int64_t D) { return row_shape(D, 1024, 4); }
-// (the registers of a backward slot: 16-bit rows 56 and fp32 rows 80, of 256)
-constexpr int bwd_slots(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 2 : 3; }
-RowShape bwd_shape(int64_t D, int32_t dtype) { return row_shape(D, kBwdThreads, bwd_slots(dtype)); }
+constexpr int kFwdSlots = 4;
+RowShape fwd_shape(int64_t D, int32_t dtype) { return row_shape(D, dtype, 1024, kFwdSlots); }
+// (the registers of a backward slot: 56 with 16-bit rows and 40 with fp32 ones, of 256)
+constexpr int bwd_slots(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 3; }
+RowShape bwd_shape(int64_t D, int32_t dtype) {
+    return row_shape(D, dtype, kBwdThreads, bwd_slots(dtype));
+}
 
 // The partial sums of dw and db.
 int bwd_blocks(int64_t N, int64_t D, const RowShape& r) {
@@ -500,7 +519,7 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
     HASTE_CHECK_ARG(haste::elem_aligned(b, w_dtype), "%s: b is not aligned to its elements", fn);
     HASTE_TRY(haste::ln_rows(fn, "y", y, D, D, dtype));
     HASTE_CHECK_ARG(haste::elem_aligned(stats, HASTE_DTYPE_F32), "%s: stats is misaligned", fn);
-    const haste::RowShape r = haste::fwd_shape(D);
+    const haste::RowShape r = haste::fwd_shape(D, dtype);
     const int threads = std::max(r.tpr, 256), rows = r.C ? threads / r.tpr : 1;
     const dim3 grid((unsigned)haste::ceil_div(N, (int64_t)rows));
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -575,7 +594,7 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
         auto slots = [&](auto c) {                                                               \
             constexpr int C = std::min(decltype(c)::value, haste::bwd_slots(DT));                \
             const size_t lds = r.tpr < haste::kBwdThreads && sums                                \
-                                   ? sizeof(float) * 8 * C * haste::kBwdThreads                  \
+                                   ? sizeof(float) * haste::row_vec(DT) * C * haste::kBwdThreads                  \
                                    : 0;                                                          \
             haste::ln_bwd_kernel<DT, WT, C><<<dim3(blocks), dim3(haste::kBwdThreads), lds, st>>>(\
                 dyc, lddy, dhc, lddh, hc, ldh, w, stats, static_cast<char*>(dx), sums, N, D,     \
