@@ -21,10 +21,36 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
     return v;
 }
 
+// Rows are met V elements (16 bytes) at a time.  Where V does not divide D, the thread of the last
+// ones takes the row's last V elements instead, of which it shares the first `skip` with another
+// thread (which computes the same values) and leaves them out of sums; with skip >= V it has none
+// of its own.
+constexpr int row_vec(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 8; }
+struct Slot {
+    int64_t at;  // first element
+    int skip;
+};
+template <int V>
+__device__ __forceinline__ Slot last_slot(int64_t e, int64_t D) {
+    const int64_t at = min(e, D - V);
+    return Slot{at, (int)(e - at)};
+}
+
 // ---------------------------------------------------------------- any width ----
-// For rows under 8 elements or past what registers hold: a workgroup to a row, which is read
-// again from cache for each of its passes.
-template <int DT, int WT>
+// For rows shorter than a slot (V = 1) or past what registers hold: a workgroup to a row, which
+// is read again from cache for each of its passes.
+template <int DT, int V>
+__device__ __forceinline__ void get(const void* p, int64_t i, float* f) {
+    if constexpr (V == 1) f[0] = load_elem<DT>(p, i);
+    else unpack<DT, V>(load<DT, V>(p, i), f);
+}
+template <int DT, int V>
+__device__ __forceinline__ void put(void* p, int64_t i, const float* f) {
+    if constexpr (V == 1) store_elem<DT>(p, i, f[0]);
+    else store<DT, V>(p, i, pack<DT, V>(f));
+}
+
+template <int DT, int WT, int V>
 __global__ __launch_bounds__(kRowThreads) void ln_fwd_any_kernel(
     const char* x, int64_t ldx, const char* res, int64_t ldres, const void* w, const void* b,
     char* y, char* h, float* stats, int64_t D, float eps) {
@@ -37,24 +63,43 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_any_kernel(
         res += row * ldres * S;
         h += row * D * S;
     }
-    auto get = [&](int64_t i) {
-        const float f = load_elem<DT>(x, i);
-        return res ? round_elem<DT>(f + load_elem<DT>(res, i)) : f;
+    auto rows = [&](int64_t at, float* f) __attribute__((always_inline)) {
+        get<DT, V>(x, at, f);
+        if (!res) return;
+        float g[V];
+        get<DT, V>(res, at, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = round_elem<DT>(f[e] + g[e]);
     };
-    float s = 0.f;
-    for (int64_t i = threadIdx.x; i < D; i += kRowThreads) s += get(i);
+    float s = 0.f, f[V], g[V];
+    for (int64_t i = threadIdx.x * V; i < D; i += kRowThreads * V) {
+        const Slot t = last_slot<V>(i, D);
+        rows(t.at, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += e >= t.skip ? f[e] : 0.f;
+    }
     const float mean = group_sum(s, part) / (float)D;
     s = 0.f;
-    for (int64_t i = threadIdx.x; i < D; i += kRowThreads) {
-        const float d = get(i) - mean;
-        s += d * d;
+    for (int64_t i = threadIdx.x * V; i < D; i += kRowThreads * V) {
+        const Slot t = last_slot<V>(i, D);
+        rows(t.at, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += e >= t.skip ? (f[e] - mean) * (f[e] - mean) : 0.f;
     }
     const float rstd = 1.f / sqrtf(group_sum(s, part) / (float)D + eps);
-    for (int64_t i = threadIdx.x; i < D; i += kRowThreads) {
-        const float f = get(i);
-        if (res) store_elem<DT>(h, i, f);
-        const float n = (f - mean) * rstd * load_elem<WT>(w, i);
-        store_elem<DT>(y, i, b ? n + load_elem<WT>(b, i) : n);
+    for (int64_t i = threadIdx.x * V; i < D; i += kRowThreads * V) {
+        const int64_t at = last_slot<V>(i, D).at;
+        rows(at, f);
+        if (res) put<DT, V>(h, at, f);
+        get<WT, V>(w, at, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = (f[e] - mean) * rstd * g[e];
+        if (b) {
+            get<WT, V>(b, at, g);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] += g[e];
+        }
+        put<DT, V>(y, at, f);
     }
     if (stats && threadIdx.x == 0) {
         stats[2 * row] = mean;
@@ -62,7 +107,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_any_kernel(
     }
 }
 
-template <int DT, int WT>
+template <int DT, int WT, int V>
 __global__ __launch_bounds__(kRowThreads) void ln_dx_any_kernel(
     const char* dy, int64_t lddy, const char* dh, int64_t lddh, const char* h, int64_t ldh,
     const void* w, const float* stats, char* dx, int64_t D) {
@@ -74,78 +119,105 @@ __global__ __launch_bounds__(kRowThreads) void ln_dx_any_kernel(
     dx += row * D * S;
     if (dh) dh += row * lddh * S;
     const float mean = stats[2 * row], rstd = stats[2 * row + 1];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t i = threadIdx.x; i < D; i += kRowThreads) {
-        const float a = load_elem<DT>(dy, i) * load_elem<WT>(w, i);
-        s1 += a;
-        s2 += a * ((load_elem<DT>(h, i) - mean) * rstd);
+    float s1 = 0.f, s2 = 0.f, a[V], n[V], g[V];
+    auto rows = [&](int64_t at) __attribute__((always_inline)) {
+        get<DT, V>(dy, at, a);
+        get<DT, V>(h, at, n);
+        get<WT, V>(w, at, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            a[e] *= g[e];
+            n[e] = (n[e] - mean) * rstd;
+        }
+    };
+    for (int64_t i = threadIdx.x * V; i < D; i += kRowThreads * V) {
+        const Slot t = last_slot<V>(i, D);
+        rows(t.at);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            s1 += e >= t.skip ? a[e] : 0.f;
+            s2 += e >= t.skip ? a[e] * n[e] : 0.f;
+        }
     }
     const float c1 = group_sum(s1, part) / (float)D, c2 = group_sum(s2, part) / (float)D;
-    for (int64_t i = threadIdx.x; i < D; i += kRowThreads) {
-        const float n = (load_elem<DT>(h, i) - mean) * rstd;
-        float d = rstd * (load_elem<DT>(dy, i) * load_elem<WT>(w, i) - c1 - n * c2);
-        if (dh) d += load_elem<DT>(dh, i);
-        store_elem<DT>(dx, i, d);
+    for (int64_t i = threadIdx.x * V; i < D; i += kRowThreads * V) {
+        const int64_t at = last_slot<V>(i, D).at;
+        rows(at);
+#pragma unroll
+        for (int e = 0; e < V; ++e) a[e] = rstd * (a[e] - c1 - n[e] * c2);
+        if (dh) {
+            get<DT, V>(dh, at, g);
+#pragma unroll
+            for (int e = 0; e < V; ++e) a[e] += g[e];
+        }
+        put<DT, V>(dx, at, a);
     }
 }
 
-// sums[blockIdx.y] = dw and db of every gridDim.y-th four rows: 64 columns to a workgroup.
-template <int DT>
+// sums[blockIdx.y] = dw and db of every gridDim.y-th 16 rows: 16 V columns to a workgroup.
+constexpr int kAnyRows = 16;
+template <int DT, int V>
 __global__ __launch_bounds__(kRowThreads) void ln_dw_any_kernel(const char* dy, int64_t lddy,
                                                                 const char* h, int64_t ldh,
                                                                 const float* stats, float* sums,
                                                                 int64_t N, int64_t D) {
-    __shared__ float part[2][kRowThreads];
+    __shared__ float part[2 * V][kRowThreads];
     constexpr int S = kElemBytes<DT>;
-    constexpr int R = kRowThreads / 64;
-    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    float sw = 0.f, sb = 0.f;
-    if (c < D)
-        for (int64_t r = (int64_t)blockIdx.y * R + (threadIdx.x >> 6); r < N; r += gridDim.y * R) {
-            const float g = load_elem<DT>(dy + r * lddy * S, c);
-            sw += g * ((load_elem<DT>(h + r * ldh * S, c) - stats[2 * r]) * stats[2 * r + 1]);
-            sb += g;
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int64_t i = ((int64_t)blockIdx.x * 16 + x) * V;
+    const Slot t = last_slot<V>(i, D);
+    float sw[V] = {}, sb[V] = {}, a[V], n[V];
+    if (i < D)
+        for (int64_t r = (int64_t)blockIdx.y * kAnyRows + y; r < N; r += gridDim.y * kAnyRows) {
+            get<DT, V>(dy + r * lddy * S, t.at, a);
+            get<DT, V>(h + r * ldh * S, t.at, n);
+            const float mean = stats[2 * r], rstd = stats[2 * r + 1];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sw[e] += a[e] * ((n[e] - mean) * rstd);
+                sb[e] += a[e];
+            }
         }
-    part[0][threadIdx.x] = sw;
-    part[1][threadIdx.x] = sb;
-    __syncthreads();
-    if (threadIdx.x >= 64 || c >= D) return;
-    for (int k = 1; k < R; ++k) {
-        sw += part[0][k * 64 + threadIdx.x];
-        sb += part[1][k * 64 + threadIdx.x];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        part[e][threadIdx.x] = sw[e];
+        part[V + e][threadIdx.x] = sb[e];
     }
+    __syncthreads();
+    if (y || i >= D) return;
     sums += (int64_t)blockIdx.y * 2 * D;
-    sums[c] = sw;
-    sums[D + c] = sb;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        if (e < t.skip) continue;
+        for (int k = 1; k < kRowThreads / 16; ++k) {
+            sw[e] += part[e][k * 16 + x];
+            sb[e] += part[V + e][k * 16 + x];
+        }
+        sums[t.at + e] = sw[e];
+        sums[D + t.at + e] = sb[e];
+    }
 }
 
 // ------------------------------------------------------- rows in registers ----
-// `tpr` threads (a power of two from 16) hold a row, V elements (16 bytes) in each of C slots:
-// thread t has elements V (c tpr + t) + 0..V-1 of it in slot c.  Only the last slot can pass the
-// row's end: there a thread reads and writes the row's last V elements instead, of which it
-// shares the first `skip` with other threads (which compute the same values) and leaves them out
-// of sums; with skip >= V it has none of its own.
-constexpr int row_vec(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 8; }
-struct Slot {
-    int64_t at;  // first element
-    int skip;
-};
+// `tpr` threads (a power of two) hold a row in C slots: thread t has elements
+// V (c tpr + t) + 0..V-1 of it in slot c.  Only the last slot can pass the row's end.
 template <int V>
 __device__ __forceinline__ Slot row_slot(int c, int C, int tpr, int lane, int64_t D) {
     const int64_t e = V * ((int64_t)c * tpr + lane);
-    if (c < C - 1) return Slot{e, 0};
-    const int64_t at = min(e, D - V);
-    return Slot{at, (int)(e - at)};
+    return c < C - 1 ? Slot{e, 0} : last_slot<V>(e, D);
 }
 
 template <int C>
 __device__ __forceinline__ float dpp_add(float x) {
     return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), C, 0xF, 0xF, true));
 }
-// The sum over groups of min(tpr, 64) lanes, in all of them: rotations within 16 lanes, then
-// rows and halves of the wave swapped with their neighbours.
+// The sum over groups of min(tpr, 64) lanes, in all of them: neighbours, pairs, quads mirrored
+// within 8 and 16 lanes, then rows and halves of the wave swapped.
 __device__ __forceinline__ float lanes_sum(float x, int tpr) {
-    x = dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x))));
+    if (tpr >= 2) x = dpp_add<0xB1>(x);
+    if (tpr >= 4) x = dpp_add<0x4E>(x);
+    if (tpr >= 8) x = dpp_add<0x141>(x);
+    if (tpr >= 16) x = dpp_add<0x140>(x);
     if (tpr >= 32) {
         const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
                                                         false, false);
@@ -281,10 +353,11 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     const int groups = kBwdThreads / tpr;
     const int64_t step = (int64_t)gridDim.x * groups;
     int turn = 0;
-    float g[C][V], aw[C][V], ab[C][V];
+    Elems<WT, V> gamma[C];
+    float aw[C][V], ab[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        unpack<WT, V>(load<WT, V>(w, row_slot<V>(c, C, tpr, lane, D).at), g[c]);
+        gamma[c] = load<WT, V>(w, row_slot<V>(c, C, tpr, lane, D).at);
 #pragma unroll
         for (int e = 0; e < V; ++e) aw[c][e] = ab[c][e] = 0.f;
     }
@@ -306,24 +379,25 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     BwdRow<DT, C> next;
     fetch(next, row);
     for (int64_t k = 0; k < turns; ++k, row += step) {
-        const BwdRow<DT, C> r = next;
+        BwdRow<DT, C> r = next;
         if (k + 1 < turns) fetch(next, row + step);
         const bool live = row < N;
-        float s1 = 0.f, s2 = 0.f, n[C][V];
+        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int skip = row_slot<V>(c, C, tpr, lane, D).skip;
-            float d[V];
+            float d[V], n[V], g[V];
             unpack<DT, V>(r.dy[c], d);
-            unpack<DT, V>(r.h[c], n[c]);
+            unpack<DT, V>(r.h[c], n);
+            unpack<WT, V>(gamma[c], g);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                n[c][e] = (n[c][e] - r.mean) * r.rstd;
+                n[e] = (n[e] - r.mean) * r.rstd;
                 const bool own = live && (c < C - 1 || e >= skip);
-                const float a = d[e] * g[c][e];
+                const float a = d[e] * g[e];
                 s1 += own ? a : 0.f;
-                s2 += own ? a * n[c][e] : 0.f;
-                aw[c][e] += own ? d[e] * n[c][e] : 0.f;
+                s2 += own ? a * n[e] : 0.f;
+                aw[c][e] += own ? d[e] * n[e] : 0.f;
                 ab[c][e] += own ? d[e] : 0.f;
             }
         }
@@ -333,10 +407,13 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const Slot at = row_slot<V>(c, C, tpr, lane, D);
-            float d[V];
+            float d[V], n[V], g[V];
             unpack<DT, V>(r.dy[c], d);
+            unpack<DT, V>(r.h[c], n);
+            unpack<WT, V>(gamma[c], g);
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = r.rstd * (d[e] * g[c][e] - c1 - n[c][e] * c2);
+            for (int e = 0; e < V; ++e)
+                d[e] = r.rstd * (d[e] * g[e] - c1 - (n[e] - r.mean) * r.rstd * c2);
             if (dh) {
                 float q[V];
                 unpack<DT, V>(r.dh[c], q);
@@ -407,34 +484,37 @@ __global__ __launch_bounds__(1024) void ln_sums_kernel(const float* __restrict__
     store_elem<WT>(out, c, s);
 }
 
-// How the threads hold rows of D elements in up to `slots` slots: the fewest threads left over,
-// then the fewest threads to a row.  C == 0: they do not fit `most` threads, or are shorter than
-// a slot.
+// How the threads hold rows of D elements: the fewest threads left over in up to `slots` slots of
+// `most` threads; among those the most threads up to `wide`, and never several slots of under
+// `narrow` threads, whose accesses would touch only part of their lines (2^26 elements of fp32 in
+// rows of 16 with one thread to a row 445 us, with four 108; rows of 100 with eight threads 231,
+// with 16 128).  The forward takes several slots where it can (rows of 512 in bf16: 43 us with
+// four, 52 with one, whose threads have one load under way), the backward, which has the next
+// row's loads under way, one (70 and 73).  C == 0: rows that do not fit, or shorter than a slot.
 struct RowShape {
     int tpr, C;
 };
-RowShape row_shape(int64_t D, int32_t dtype, int most, int slots) {
+RowShape row_shape(int64_t D, int32_t dtype, int most, int slots, int narrow, int wide) {
     const int64_t V = row_vec(dtype);
     RowShape best{0, 0};
     int64_t over = 0;
     if (D < V) return best;
-    for (int tpr = 16; tpr <= most; tpr *= 2) {
+    for (int tpr = 1; tpr <= most; tpr *= 2) {
         const int64_t C = ceil_div(D, V * tpr);
-        if (C > slots) continue;
+        if (C > slots || (tpr < narrow && C > 1)) continue;
         const int64_t o = C * V * tpr - D;
-        if (best.C == 0 || o < over) {
+        if (best.C == 0 || o < over || (o == over && tpr <= wide)) {
             best = RowShape{tpr, (int)C};
             over = o;
         }
     }
     return best;
 }
-constexpr int kFwdSlots = 4;
-RowShape fwd_shape(int64_t D, int32_t dtype) { return row_shape(D, dtype, 1024, kFwdSlots); }
+RowShape fwd_shape(int64_t D, int32_t dtype) { return row_shape(D, dtype, 1024, 4, 16, 0); }
 // (the registers of a backward slot: 56 with 16-bit rows and 40 with fp32 ones, of 256)
 constexpr int bwd_slots(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 3; }
 RowShape bwd_shape(int64_t D, int32_t dtype) {
-    return row_shape(D, dtype, kBwdThreads, bwd_slots(dtype));
+    return row_shape(D, dtype, kBwdThreads, bwd_slots(dtype), 8, 64);
 }
 
 // Whether a matrix of rows is no more in the last-level cache when it is met again: half of it,
@@ -445,7 +525,7 @@ bool past_cache(int64_t N, int64_t D, int32_t dtype) {
 
 // The partial sums of dw and db.
 int bwd_blocks(int64_t N, int64_t D, const RowShape& r) {
-    const int64_t rows = r.C ? kBwdThreads / r.tpr : 64, most = r.C ? kBwdBlocks : 64;
+    const int64_t rows = r.C ? kBwdThreads / r.tpr : 4 * kAnyRows, most = r.C ? kBwdBlocks : 64;
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(N, rows), most));
 }
 
@@ -522,6 +602,10 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
     const bool nt = haste::past_cache(N, D, dtype);
     const char *xc = static_cast<const char*>(x), *rc = static_cast<const char*>(res);
     char *yc = static_cast<char*>(y), *hc = static_cast<char*>(h);
+    auto any = [&](auto kernel) {
+        kernel<<<grid, dim3(haste::kRowThreads), 0, st>>>(xc, ldx, rc, ldres, w, b, yc, hc, stats, D,
+                                                          (float)eps);
+    };
 #define HASTE_LN_FWD(DT, WT)                                                                   \
     do {                                                                                       \
         auto slots = [&](auto c) {                                                             \
@@ -536,8 +620,8 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
         if (r.C)                                                                               \
             haste::with_slots(r.C, slots);                                                     \
         else                                                                                   \
-            haste::ln_fwd_any_kernel<DT, WT><<<grid, dim3(haste::kRowThreads), 0, st>>>(       \
-                xc, ldx, rc, ldres, w, b, yc, hc, stats, D, (float)eps);                       \
+            any(D < haste::row_vec(DT) ? haste::ln_fwd_any_kernel<DT, WT, 1>                   \
+                                       : haste::ln_fwd_any_kernel<DT, WT, haste::row_vec(DT)>); \
     } while (0)
     HASTE_LN_TYPES(HASTE_LN_FWD);
 #undef HASTE_LN_FWD
@@ -592,6 +676,14 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
                *hc = static_cast<const char*>(h);
     float* sums = dw || db ? static_cast<float*>(ws) : nullptr;
     const dim3 columns((unsigned)haste::ceil_div(D, 64), 2);
+    auto any_dx = [&](auto kernel) {
+        kernel<<<dim3((unsigned)N), dim3(haste::kRowThreads), 0, st>>>(
+            dyc, lddy, dhc, lddh, hc, ldh, w, stats, static_cast<char*>(dx), D);
+    };
+    auto any_dw = [&](auto kernel, int V) {
+        kernel<<<dim3((unsigned)haste::ceil_div(D, (int64_t)16 * V), blocks),
+                 dim3(haste::kRowThreads), 0, st>>>(dyc, lddy, hc, ldh, stats, sums, N, D);
+    };
 #define HASTE_LN_BWD(DT, WT)                                                                     \
     do {                                                                                         \
         auto slots = [&](auto c) {                                                               \
@@ -608,13 +700,14 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
         if (N > 0 && r.C) {                                                                      \
             haste::with_slots(r.C, slots);                                                       \
         } else {                                                                                 \
+            constexpr int V = haste::row_vec(DT);                                                \
             if (N > 0 && dx)                                                                     \
-                haste::ln_dx_any_kernel<DT, WT><<<dim3((unsigned)N), dim3(haste::kRowThreads),   \
-                                                  0, st>>>(dyc, lddy, dhc, lddh, hc, ldh, w,     \
-                                                           stats, static_cast<char*>(dx), D);    \
-            if (sums)                                                                            \
-                haste::ln_dw_any_kernel<DT><<<dim3(columns.x, blocks), dim3(haste::kRowThreads), \
-                                              0, st>>>(dyc, lddy, hc, ldh, stats, sums, N, D);   \
+                any_dx(D < V ? haste::ln_dx_any_kernel<DT, WT, 1>                                \
+                             : haste::ln_dx_any_kernel<DT, WT, V>);                              \
+            if (sums && D < V)                                                                   \
+                any_dw(haste::ln_dw_any_kernel<DT, 1>, 1);                                       \
+            else if (sums)                                                                       \
+                any_dw(haste::ln_dw_any_kernel<DT, V>, V);                                       \
         }                                                                                        \
         if (sums)                                                                                \
             haste::ln_sums_kernel<WT><<<columns, dim3(1024), 0, st>>>(sums, blocks, dw, db, D);  \
