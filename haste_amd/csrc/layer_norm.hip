@@ -328,6 +328,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_kernel(
 }
 
 constexpr int kBwdThreads = 512;
+constexpr int kWideThreads = 1024;  // (rows of fp32 past 8192)
 constexpr int kBwdBlocks = 512;  // partial sums of dw and db: one pair of rows a workgroup
 
 template <int DT, int C>
@@ -339,9 +340,9 @@ struct BwdRow {
 
 // Every group of tpr threads takes each (gridDim groups)-th row: one read of dy, h and dh, their
 // last and non-temporal, gives dx, and what the row adds to dw and db stays in registers until
-// the end.  The next row's loads are under way while a row is reduced.
-template <int DT, int WT, int C, bool NT>
-__global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
+// the end.  The next row's loads are under way while a row is reduced, but with T = kWideThreads.
+template <int DT, int WT, int C, bool NT, int T>
+__global__ __launch_bounds__(T) void ln_bwd_kernel(
     const char* __restrict__ dy, int64_t lddy, const char* __restrict__ dh, int64_t lddh,
     const char* __restrict__ h, int64_t ldh, const void* __restrict__ w,
     const float* __restrict__ stats, char* __restrict__ dx, float* __restrict__ sums, int64_t N,
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     __shared__ float part[2][32];
     constexpr int S = kElemBytes<DT>, V = row_vec(DT);
     const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
-    const int groups = kBwdThreads / tpr;
+    const int groups = T / tpr;
     const int64_t step = (int64_t)gridDim.x * groups;
     int turn = 0;
     Elems<WT, V> gamma[C];
@@ -376,11 +377,13 @@ __global__ __launch_bounds__(kBwdThreads) void ln_bwd_kernel(
     // (all groups make the same number of turns: rows_sums may hold a barrier)
     const int64_t turns = (N + step - 1) / step;
     int64_t row = (int64_t)blockIdx.x * groups + group;
+    constexpr bool AHEAD = T == kBwdThreads;
     BwdRow<DT, C> next;
-    fetch(next, row);
+    if (AHEAD) fetch(next, row);
     for (int64_t k = 0; k < turns; ++k, row += step) {
-        BwdRow<DT, C> r = next;
-        if (k + 1 < turns) fetch(next, row + step);
+        if (!AHEAD) fetch(next, row);
+        const BwdRow<DT, C> r = next;
+        if (AHEAD && k + 1 < turns) fetch(next, row + step);
         const bool live = row < N;
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -513,7 +516,13 @@ RowShape row_shape(int64_t D, int32_t dtype, int most, int slots, int narrow, in
 RowShape fwd_shape(int64_t D, int32_t dtype) { return row_shape(D, dtype, 1024, 4, 16, 0); }
 // (the registers of a backward slot: 56 with 16-bit rows and 40 with fp32 ones, of 256)
 constexpr int bwd_slots(int32_t dtype) { return dtype == HASTE_DTYPE_F32 ? 4 : 3; }
+// Wider fp32 rows take 1024 threads, with half the registers and no loads ahead of their row: rows
+// of 12,000, 2^26 elements, 295 -> 162 us; of 16,384 (33 registers spilled) 321 -> 210.  With
+// 16-bit rows, whose slots hold twice the elements, the any-width passes are as fast.
+constexpr bool wide(int32_t dtype, int C) { return dtype == HASTE_DTYPE_F32 && C >= 3; }
 RowShape bwd_shape(int64_t D, int32_t dtype) {
+    const int64_t C = ceil_div(D, (int64_t)kWideThreads * row_vec(dtype));
+    if (C <= 4 && wide(dtype, (int)C)) return RowShape{kWideThreads, (int)C};
     return row_shape(D, dtype, kBwdThreads, bwd_slots(dtype), 8, 64);
 }
 
@@ -525,7 +534,7 @@ bool past_cache(int64_t N, int64_t D, int32_t dtype) {
 
 // The partial sums of dw and db.
 int bwd_blocks(int64_t N, int64_t D, const RowShape& r) {
-    const int64_t rows = r.C ? kBwdThreads / r.tpr : 4 * kAnyRows, most = r.C ? kBwdBlocks : 64;
+    const int64_t rows = r.C ? std::max(kBwdThreads / r.tpr, 1) : 4 * kAnyRows, most = r.C ? kBwdBlocks : 64;
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(N, rows), most));
 }
 
@@ -691,9 +700,13 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
             const size_t lds = r.tpr < haste::kBwdThreads && sums                                \
                                    ? sizeof(float) * haste::row_vec(DT) * C * haste::kBwdThreads                  \
                                    : 0;                                                          \
-            auto kernel = nt ? haste::ln_bwd_kernel<DT, WT, C, true>                             \
-                             : haste::ln_bwd_kernel<DT, WT, C, false>;                           \
-            kernel<<<dim3(blocks), dim3(haste::kBwdThreads), lds, st>>>(                         \
+            auto kernel = nt ? haste::ln_bwd_kernel<DT, WT, C, true, haste::kBwdThreads>         \
+                             : haste::ln_bwd_kernel<DT, WT, C, false, haste::kBwdThreads>;       \
+            if constexpr (haste::wide(DT, C))                                                    \
+                if (r.tpr == haste::kWideThreads)                                                \
+                    kernel = nt ? haste::ln_bwd_kernel<DT, WT, C, true, haste::kWideThreads>     \
+                                : haste::ln_bwd_kernel<DT, WT, C, false, haste::kWideThreads>;   \
+            kernel<<<dim3(blocks), dim3(std::max(r.tpr, haste::kBwdThreads)), lds, st>>>(        \
                 dyc, lddy, dhc, lddh, hc, ldh, w, stats, static_cast<char*>(dx), sums, N, D,     \
                 r.tpr);                                                                          \
         };                                                                                       \
