@@ -30,7 +30,6 @@ struct AdamBatch {
 };
 struct AdamArgs {
     float b1, c1, b2, c2;  // beta1, 1 - beta1, beta2, 1 - beta2
-    float root_b2;         // sqrt(beta2)
     float decay, lr, rcorr, eps;  // 1 - lr wd, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
     uint32_t k0, k1;
     int32_t do_sr;
@@ -90,48 +89,58 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-// The E8M0 code of the power of two that puts the row's largest |x| in [128, 256).  As whole
-// numbers the patterns of |x| are in its order, with infinities and NaN above all others: only
-// where one is met are the finite ones looked for.
-__device__ __forceinline__ uint32_t scale_code(const float* x) {
+// The largest |x| of a row as a bit pattern.  As whole numbers the patterns of |x| are in its order,
+// with infinities and NaN above all others; FINITE leaves those out.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t row_top(const float* x) {
     uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-    top = row_max(top);
-    if (__any(top >= kInfBits)) {
-        top = 0;
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t a = __float_as_uint(x[e]) & 0x7FFFFFFFu;
-            top = max(top, a < kInfBits ? a : 0u);
-        }
-        top = row_max(top);
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t a = __float_as_uint(x[e]) & 0x7FFFFFFFu;
+        top = max(top, FINITE && a >= kInfBits ? 0u : a);
     }
+    return row_max(top);
+}
+
+// The E8M0 code of the power of two that puts what has these bits in [128, 256).
+__device__ __forceinline__ uint32_t scale_code(uint32_t top) {
     return (uint32_t)max((int)(top >> 23) - 7, 1);
 }
 
 __device__ __forceinline__ float pow2_code(uint32_t code) { return __uint_as_float(code << 23); }
 
-// Eight values as e4m3 codes under the scale of `code`, x[e] rounded up by the upper half of
-// seed[e]: v_cvt_sr_fp8_f32 adds the seed's upper 20 bits to what it cuts off, subnormals
-// included, and makes NaN of what is not finite.  KEEP: x > 0 does not become 0.
-template <bool KEEP>
-__device__ __forceinline__ u32x2 cut_e4m3(const float* x, uint32_t code, const uint32_t* seed) {
-    const float inv = pow2_code(254u - code);
-    u32x2 out = {0, 0};
+// Eight m and u as e4m3 codes under the scales of cm and cu, m[e] rounded up by the upper half of
+// r[e] and u[e] by that of its quad's next: v_cvt_sr_fp8_f32 adds the seed's upper 20 bits to what
+// it cuts off, subnormals included, and makes NaN of what is not finite.  u > 0 (a root: 2^-75 at
+// least) does not become 0.
+__device__ __forceinline__ void cut_e4m3(const float* m, const float* u, uint32_t cm, uint32_t cu,
+                                         const uint32_t* r, bool finite, u32x2& m8, u32x2& u8) {
+    const float im = pow2_code(254u - cm), iu = pow2_code(254u - cu);
+    int out[4] = {0, 0, 0, 0};
+    float sm[8], su[8];
+    int seed[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        float s = x[e] * inv;
-        if (KEEP) s = x[e] > 0.f && s < 0x1p-9f ? 0x1p-9f : s;
-        const int sd = (int)(seed[e] & 0xFFFF0000u);
-        int& o = reinterpret_cast<int*>(&out)[e / 4];
-        switch (e & 3) {
-        case 0: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 0); break;
-        case 1: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 1); break;
-        case 2: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 2); break;
-        default: o = __builtin_amdgcn_cvt_sr_fp8_f32(s, sd, o, 3);
-        }
+        sm[e] = m[e] * im;
+        su[e] = __builtin_amdgcn_fmed3f(u[e] * iu, 0x1p-9f, u[e] * 0x1p100f);
+        seed[e] = (int)(r[e] & 0xFFFF0000u);
     }
-    return out;
+    if (!finite) {  // the median of a NaN is not one
+#pragma unroll
+        for (int e = 0; e < 8; ++e) su[e] = u[e] == u[e] ? su[e] : u[e];
+    }
+#define HASTE_CUT(E)                                                                          \
+    out[0] = __builtin_amdgcn_cvt_sr_fp8_f32(sm[E], seed[E], out[0], E);                      \
+    out[1] = __builtin_amdgcn_cvt_sr_fp8_f32(sm[4 + E], seed[4 + E], out[1], E);              \
+    out[2] = __builtin_amdgcn_cvt_sr_fp8_f32(su[E], seed[(E + 1) & 3], out[2], E);            \
+    out[3] = __builtin_amdgcn_cvt_sr_fp8_f32(su[4 + E], seed[4 + ((E + 1) & 3)], out[3], E)
+    HASTE_CUT(0);
+    HASTE_CUT(1);
+    HASTE_CUT(2);
+    HASTE_CUT(3);
+#undef HASTE_CUT
+    m8 = u32x2{(uint32_t)out[0], (uint32_t)out[1]};
+    u8 = u32x2{(uint32_t)out[2], (uint32_t)out[3]};
 }
 
 __device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
@@ -152,10 +161,14 @@ __device__ __forceinline__ float adam_weight(float w, float m, float u, const Ad
     return w * a.decay - a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps);
 }
 
-template <int WT>
+// CHECK: w may be a NaN with payload bits in its lower half, which adding to could carry over.
+template <int WT, bool CHECK = true>
 __device__ __forceinline__ uint32_t sr_pair(float lo, float hi, uint32_t r_lo, uint32_t r_hi) {
     r_lo &= 0xFFFFu;
     r_hi &= 0xFFFFu;
+    if constexpr (WT == HASTE_DTYPE_BF16 && !CHECK)
+        return __builtin_amdgcn_perm(__float_as_uint(hi) + r_hi, __float_as_uint(lo) + r_lo,
+                                     0x07060302u);
     return WT == HASTE_DTYPE_BF16 ? sr_bf16(lo, r_lo) | sr_bf16(hi, r_hi) << 16
                                   : sr_f16(lo, r_lo) | sr_f16(hi, r_hi) << 16;
 }
@@ -233,6 +246,26 @@ struct AdamElems32 {
     }
 };
 
+// m and sqrt(v) of 8-bit states after a step, each operation rounded for itself: a rounding more or
+// less moves a block's scale where its largest value meets a power of two, as m' does wherever m
+// and g are the same one (bf16 gradients and e4m3 codes have few mantissas).  So does the root,
+// whose estimate s is kept unless x is past the middle between it and a neighbour.
+__device__ __forceinline__ void moments8(float* m, float* u, const float* g, float fm, float su,
+                                         const AdamArgs& a) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        m[e] = m[e] * fm + g[e] * a.c1;
+        u[e] *= su;
+        const float x = u[e] * u[e] * a.b2 + g[e] * g[e] * a.c2;
+        const float s = __builtin_amdgcn_sqrtf(x);
+        const float lo = __uint_as_float(__float_as_uint(s) - 1u),
+                    hi = __uint_as_float(__float_as_uint(s) + 1u);
+        const float up = __builtin_fmaf(-hi, s, x) > 0.f ? hi : s;
+        u[e] = __builtin_fmaf(-lo, s, x) <= 0.f ? lo : up;
+    }
+}
+
 // 8-bit states: a thread has eight elements, so 16 lanes (one DPP row) a block of 128, whose
 // maxima need no LDS.  The states are padded to whole blocks.
 template <int WT, int GT>
@@ -273,34 +306,45 @@ struct AdamElems8 {
         unpack<GT, 8>(g, gf);
         from_e4m3(m, mf);
         from_e4m3(u, uf);
-        const float fm = a.b1 * pow2_code(ms), fu = a.root_b2 * pow2_code(us);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (!FULL && i + e >= n) mf[e] = uf[e] = 0.f;
             gf[e] *= gs;
-            mf[e] = mf[e] * fm + a.c1 * gf[e];
-            uf[e] *= fu;
-            uf[e] = __builtin_amdgcn_sqrtf(uf[e] * uf[e] + a.c2 * gf[e] * gf[e]);
-            wf[e] = adam_weight(wf[e], mf[e], uf[e], a);
         }
+        moments8(mf, uf, gf, a.b1 * pow2_code(ms), pow2_code(us), a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wf[e] = adam_weight(wf[e], mf[e], uf[e], a);
         const uint32_t stream = (uint32_t)(s.n_stream >> 40);
         const uint64_t c = (uint64_t)i / 4;
         const u32x4 q0 = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
         const u32x4 q1 = philox_words((uint32_t)c + 1, (uint32_t)(c >> 32), stream, a.k0, a.k1);
         const uint32_t r[8] = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
+        uint32_t tm = row_top<false>(mf), tu = row_top<false>(uf);
+        const bool finite = !__any(max(tm, tu) >= kInfBits);
         Elems<WT, 8> out;
         if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+            // (where m and u are finite only a NaN of w itself is left, whose payload is w's)
+            if (finite) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                out.q[e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
+                for (int e = 0; e < 4; ++e)
+                    out.q[e] = sr_pair<WT, false>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    out.q[e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
+            }
         } else {
             out = pack<WT, 8>(wf);
         }
         if constexpr (FULL) store<WT, 8, WT != HASTE_DTYPE_F32>(s.w, i, out);
         else store_part<WT, 8>(s.w, i, out, n - i);
-        const uint32_t cm = scale_code(mf), cu = scale_code(uf);
-        const uint32_t ru[8] = {r[1], r[2], r[3], r[0], r[5], r[6], r[7], r[4]};
-        const u32x2 mo = cut_e4m3<false>(mf, cm, r), uo = cut_e4m3<true>(uf, cu, ru);
+        if (!finite) {
+            tm = row_top<true>(mf);
+            tu = row_top<true>(uf);
+        }
+        const uint32_t cm = scale_code(tm), cu = scale_code(tu);
+        u32x2 mo, uo;
+        cut_e4m3(mf, uf, cm, cu, r, finite, mo, uo);
         if (FULL || (i & ~(int64_t)(kBlock - 1)) < n) {
             u32x2* mp = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.m) + i);
             u32x2* up = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(s.v) + i);
@@ -488,7 +532,6 @@ extern "C" int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count
     a.c1 = (float)(1.0 - beta1);
     a.b2 = (float)beta2;
     a.c2 = (float)(1.0 - beta2);
-    a.root_b2 = (float)std::sqrt(beta2);
     a.decay = (float)(1.0 - lr * wd);
     a.lr = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     a.rcorr = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
