@@ -12,7 +12,7 @@ constexpr int kBlock = 128;    // elements of an 8-bit state that share a scale
 constexpr int kMaxSegs = 64;   // tensors of one launch: a lane to each when a wave looks its own up,
                                // and their table stays within 4 KB of kernel arguments
 constexpr int kThreads = 256;
-constexpr int kPiece = kThreads * 8;  // elements of a workgroup
+constexpr int kPiece = kThreads * 8;  // elements of a workgroup (two such pieces take the same)
 
 struct AdamSeg {
     void* w;
@@ -111,7 +111,7 @@ __device__ __forceinline__ float pow2_code(uint32_t code) { return __uint_as_flo
 
 // Eight m and u as e4m3 codes under the scales of cm and cu, m[e] rounded up by the upper half of
 // r[e] and u[e] by that of its quad's next: v_cvt_sr_fp8_f32 adds the seed's upper 20 bits to what
-// it cuts off, subnormals included, and makes NaN of what is not finite.  u > 0 (a root: 2^-75 at
+// it cuts off, subnormals included, and makes NaN of what is not finite.  u > 0 (a root: 2^-63 at
 // least) does not become 0.
 __device__ __forceinline__ void cut_e4m3(const float* m, const float* u, uint32_t cm, uint32_t cu,
                                          const uint32_t* r, bool finite, u32x2& m8, u32x2& u8) {
@@ -156,7 +156,8 @@ __device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
     }
 }
 
-// w' of one element; u = sqrt(v').  The hardware's root and reciprocal are within 1 ulp.
+// w' of one element; u = sqrt(v').  The hardware's root and reciprocal are within 1 ulp and take
+// what is below 2^-126 for 0.
 __device__ __forceinline__ float adam_weight(float w, float m, float u, const AdamArgs& a) {
     return w * a.decay - a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps);
 }
@@ -173,8 +174,9 @@ __device__ __forceinline__ uint32_t sr_pair(float lo, float hi, uint32_t r_lo, u
                                   : sr_f16(lo, r_lo) | sr_f16(hi, r_hi) << 16;
 }
 
-// 32-bit states: a piece's thread has two runs of four elements, a piece's half apart, so that every
-// 16-byte access of fp32 is next to its neighbour lane's.
+// 32-bit states: a thread has two runs of four elements, half a workgroup's apart, so that every
+// 16-byte access of fp32 is next to its neighbour lane's and lines are met whole.  A Philox call
+// serves eight elements, which two threads make each for itself.
 template <int WT, int GT>
 struct AdamElems32 {
     static constexpr int kRun = kThreads * 4;
@@ -249,7 +251,8 @@ struct AdamElems32 {
 // m and sqrt(v) of 8-bit states after a step, each operation rounded for itself: a rounding more or
 // less moves a block's scale where its largest value meets a power of two, as m' does wherever m
 // and g are the same one (bf16 gradients and e4m3 codes have few mantissas).  So does the root,
-// whose estimate s is kept unless x is past the middle between it and a neighbour.
+// whose estimate s is kept unless x is past the middle between it and a neighbour.  (Fused
+// operations and the estimate alone: 2 % faster.)
 __device__ __forceinline__ void moments8(float* m, float* u, const float* g, float fm, float su,
                                          const AdamArgs& a) {
 #pragma clang fp contract(off)
@@ -358,12 +361,13 @@ struct AdamElems8 {
     }
 };
 
-// Bound by HBM: every byte is met once.  All accesses are non-temporal (but 8-wide ones of fp32, of
-// which each touches half a line), which leaves the last-level cache to the gradients that the
-// norm has just read, and not to dirty lines: 12 layers of 768 in bf16 with 8-bit states (92 M
-// weights, norm included) 221 -> 188 us, 670 M weights 1497 -> 1350; with 32-bit states in runs of
-// four 424 -> 345 (5.8 TB/s), fp32 352 -> 281.  One piece to a workgroup and two take the same
-// within 3 %.
+// Every byte is met once.  With 32-bit states HBM bounds it: 91 M bf16 weights of 195 tensors take
+// 306 us for 2.0 GB, 6.5 TB/s with the gradients that the norm before has left in the last-level
+// cache.  With 8-bit states 670 M weights take 1068 us for 6.7 GB, 6.3 TB/s, at 55 vector
+// instructions an element, which keep the vector units as busy (10 of them Philox).  All accesses
+// are non-temporal (but 8-wide ones of fp32, of which each touches half a line), so that what is
+// met once and dirty lines do not drive those gradients out: with the norm, 8-bit 221 -> 188 us and
+// 1497 -> 1350, 32-bit 424 -> 345.
 template <int WT, int GT, bool Q8>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, const AdamArgs a) {
     using Elems = std::conditional_t<Q8, AdamElems8<WT, GT>, AdamElems32<WT, GT>>;
@@ -426,7 +430,8 @@ __device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_
 
 // part[workgroup] = the sum of squares of every gridDim-th piece, the launch's last pieces first:
 // the first tensors' gradients are then what the last-level cache holds when a step reads them
-// again from the start.
+// again from the start.  Bound by HBM: 1.34 GB of bf16 in 225 us, 6.0 TB/s; 182 MB of 195
+// tensors in 32 us, in one launch (in four of 64 tensors each 60 us).
 __global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const GradBatch b, double* part) {
     __shared__ double sums[kNormThreads / 64];
     __shared__ uint32_t piece0[kMaxGrads];

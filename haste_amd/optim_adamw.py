@@ -11,7 +11,7 @@ moments, in fp32); beside it:
     2.03 bytes an element instead of 8;
   * ``step(grad_scale=...)`` takes a factor for all gradients that is on the device, such as
     ``grad_norm``'s; a NaN there leaves parameters and states as they are.
-The tensors of a group are stepped by one launch for each 60 of them (and for each dtype of
+The tensors of a group are stepped by one launch for each 64 of them (and for each dtype of
 parameters and gradients, and each count of steps).  Random bits: Philox4x32-10 keyed by the
 seed, with the position of a tensor in its group and of an element in it as counters, so a step's
 results depend on nothing else.

@@ -584,7 +584,7 @@ int haste_rewire_ex(void* W, int32_t w_dtype, int32_t* idx, const void* grad, in
  * y and h are [N, D] contiguous.  dtype of x, res, y, h: bf16, f16 or f32; w_dtype of w
  * and b: the same or f32.  res, b may be NULL; h is required with res and unused
  * without.  stats [N, 2] (mean, rstd) is written where not NULL.  Element
- * alignment is enough for every tensor.
+ * alignment is enough for every tensor.  Outputs must not overlap inputs or each other.
  */
 int haste_layer_norm(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w,
                      const void* b, void* y, void* h, float* stats, int64_t N, int64_t D,
@@ -609,7 +609,8 @@ int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t l
  * The 2-norm over all of several tensors, and the factor that clips it:
  *   out[0] = norm = sqrt(sum g^2),  out[1] = min(1, max_norm / (norm + 1e-6)),
  * out[1] = NaN where norm is not finite (haste_adamw_step then skips its step).
- * dtype of each tensor: bf16, f16 or f32.  Sums are in a fixed order.  ws: workspace of
+ * dtype of each tensor: bf16, f16 or f32.  Squares are summed in fp32 by threads, 64 at a time,
+ * and in fp64 beyond, in a fixed order: a |g| of 1.8e19 or more makes the norm infinite.  ws: workspace of
  * haste_grad_norm_workspace_size(count) bytes (8-byte aligned).
  */
 typedef struct haste_grad_tensor {
@@ -627,7 +628,8 @@ int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, double max_
  *   g  = grad * (*grad_scale)              (1 where grad_scale is NULL)
  *   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2
  *   w' = w (1 - lr wd) - lr / (1 - beta1^step) m' / (sqrt(v' / (1 - beta2^step)) + eps)
- * in fp32.  Where *grad_scale is NaN the kernels change nothing.  w_dtype and g_dtype: bf16,
+ * in fp32 (the root of a v' below 2^-126 counts as 0).  Where *grad_scale is NaN the kernels
+ * change nothing.  w_dtype and g_dtype: bf16,
  * f16 or f32 for all of the call's tensors.  With do_sr 16-bit weights are rounded
  * stochastically, else to nearest.
  * state_bits 32: m and v are fp32 [n], m_scale and v_scale unused.
@@ -642,8 +644,8 @@ int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, double max_
  * m, and the high half of word (i + 1) & 3 for u.  A draw r in [0, 2^16) rounds up where
  * what is cut off, in units of the result's last place, plus r / 2^16 (f16 weights: the upper 13
  * bits of r over 2^13) reaches 1.
- * w and g need the alignment of their elements, m and v 16 bytes (8-bit: 8 bytes).  n == 0
- * entries are skipped.
+ * w and g need the alignment of their elements, m and v 16 bytes (8-bit: 8 bytes); n is below
+ * 2^40 and stream below 2^24.  n == 0 entries are skipped.  One launch for each 64 tensors.
  */
 typedef struct haste_adamw_tensor {
     void* w;

@@ -249,6 +249,19 @@ def test_small_roots_are_kept_above_zero(dev):
     assert (ps[0] - w).abs().max() < 3 * HYPER["lr"]
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_vanishing_gradients(dev, bits):
+    """Gradients whose squares underflow: m / eps stays far below a weight's spacing."""
+    ps, opt, _ = make(dev, [700], torch.float32, torch.float32, state_bits=bits, weight_decay=0.0)
+    w = ps[0].detach().clone()
+    ps[0].grad = torch.logspace(-44, -17, 700, device=dev)
+    for _ in range(3):
+        opt.step()
+    assert torch.equal(ps[0], w)
+    m, v = moments(opt, ps[0])
+    assert np.isfinite(m).all() and np.isfinite(v).all()
+
+
 @pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16])
 def test_rounding_is_unbiased(dev, wt):
     """Over 2000 seeds the mean of w' and of the 8-bit moments is the exact value: the mean's
