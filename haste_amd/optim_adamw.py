@@ -143,13 +143,12 @@ class AdamW(Optimizer):
 
     step.hooked = True  # Optimizer.__init__ then leaves it unwrapped
 
-    @torch.no_grad()
     def _adamw_step(self, closure=None, *, grad_scale=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_initialized() and torch._C._cuda_isCurrentStreamCapturing():
             raise RuntimeError("AdamW.step cannot be captured: the count of steps and the seed "
                                "are the host's, and a replay would repeat one step's")
         if grad_scale is not None:
@@ -169,7 +168,13 @@ class AdamW(Optimizer):
         group["seed"] += 1
         if _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, grad_scale):
             return
-        batches, device, keep, copies = self._rows(group["params"], bits)
+        with torch.no_grad():
+            self._step_any(group["params"], bits, args, sr, seed, grad_scale)
+
+    def _step_any(self, params, bits, args, sr, seed, grad_scale) -> None:
+        """The step of any parameters: those that are not plain through copies, with states made
+        where there are none yet."""
+        batches, device, keep, copies = self._rows(params, bits)
         if not batches:
             return
         scale = None
@@ -187,8 +192,7 @@ class AdamW(Optimizer):
 
     def _rows(self, params, bits):
         """The table of the step of any parameters: ([(w dtype, g dtype, step, tensors, rows)],
-        device, tensors to keep until the launch, [(parameter, contiguous copy to step)]),
-        with states made where there are none yet."""
+        device, tensors to keep until the launch, [(parameter, contiguous copy to step)])."""
         batches, stepped, copies, keep, device = {}, [], [], [], None
         for index, p in enumerate(params):
             grad = p.grad
