@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -201,6 +202,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
     {
         pybind11::gil_scoped_release no_gil;
         check(x, weight, bias, residual);
+        const c10::DeviceGuard guard(x.device());
         if (residual.defined() && residual.sizes() != x.sizes())
             residual = residual.expand(x.sizes());
         auto grad = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -83,6 +84,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     if (rows.empty()) Py_RETURN_NONE;
     const auto options = at::TensorOptions().device(c10::kCUDA, (c10::DeviceIndex)device);
     const int64_t size = haste_grad_norm_workspace_size((int32_t)n);
+    const c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
     const at::Tensor out = at::empty({2}, options.dtype(at::kFloat));
     const at::Tensor ws = at::empty({size}, options.dtype(at::kByte));
     call(haste_grad_norm(rows.data(), (int32_t)n, max_norm, out.mutable_data_ptr<float>(),
@@ -159,6 +161,8 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         if (!plain(t, &device) || t.scalar_type() != at::kFloat || t.numel() != 1) Py_RETURN_NONE;
         factor = t.const_data_ptr<float>();
     }
+    if (all.empty()) Py_RETURN_TRUE;
+    const c10::DeviceGuard guard(all[0].param.device());
     struct Group {
         int w, g;
         long long step;

@@ -455,6 +455,28 @@ def test_hooks_closure_and_groups(dev):
     assert abs(float(a[0]) - 0.9 * 1.0) < 2e-3 and abs(float(b[0]) - 0.99) < 2e-3
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_empty_parameters_schedulers_and_saved_files(dev, bits, tmp_path):
+    a = torch.nn.Parameter(torch.ones(300, device=dev, dtype=torch.bfloat16))
+    b = torch.nn.Parameter(torch.ones(0, 4, device=dev, dtype=torch.bfloat16))
+    opt = AdamW([a, b], lr=1e-2, state_bits=bits)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+    for _ in range(2):
+        a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+        norm, coef = grad_norm([a.grad, b.grad], 1.0)
+        opt.step(grad_scale=coef)
+        sched.step()
+    assert opt.state[b]["step"] == 2 and abs(opt.param_groups[0]["lr"] - 2.5e-3) < 1e-9
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    c = torch.nn.Parameter(a.detach().clone())
+    opt2 = AdamW([c, torch.nn.Parameter(b.detach().clone())], state_bits=bits)
+    opt2.load_state_dict(torch.load(tmp_path / "opt.pt", weights_only=True))
+    for o, p in ((opt, a), (opt2, c)):
+        p.grad = torch.full_like(p, 0.3)
+        o.step()
+    assert torch.equal(a, c) and opt2.param_groups[0]["seed"] == opt.param_groups[0]["seed"]
+
+
 def test_other_stream_than_the_tensors_own(dev):
     ps, opt, g = make(dev, [100000], torch.bfloat16, torch.bfloat16, state_bits=8)
     qs, opt2, _ = make(dev, [100000], torch.bfloat16, torch.bfloat16, state_bits=8)

@@ -329,3 +329,30 @@ def test_saved_rows_changed_in_place_are_noticed(dev):
         h.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_under_activation_checkpointing(dev):
+    from torch.utils.checkpoint import checkpoint
+    dat = data(20, 768, torch.bfloat16, torch.float32, dev, residual=True)
+    x, w = dat["x"].requires_grad_(True), dat["w"].requires_grad_(True)
+    f = lambda x: ops.layer_norm(x, w, dat["b"], residual=dat["res"])  # noqa: E731
+    want = torch.autograd.grad(f(x), [x, w], [dat["dy"], dat["dh"]])
+    for reentrant in (False, True):
+        out = checkpoint(f, x, use_reentrant=reentrant)
+        x.grad = w.grad = None
+        torch.autograd.backward(out, [dat["dy"], dat["dh"]])
+        assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+def test_gradients_add_up_over_uses(dev):
+    """One weight in two norms and one x as both operands: what each use gives is added."""
+    x = torch.randn(9, 96, device=dev, requires_grad=True)
+    w = torch.ones(96, device=dev, requires_grad=True)
+    y, h = ops.layer_norm(x, w, residual=x)
+    g = torch.randn_like(x)
+    (ops.layer_norm(y, w) * g).sum().backward()
+    xd, wd = x.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    ln = torch.nn.functional.layer_norm
+    (ln(ln(xd + xd, (96,), wd), (96,), wd) * g.double()).sum().backward()
+    torch.testing.assert_close(x.grad.double(), xd.grad, rtol=1e-4, atol=1e-5)
+    torch.testing.assert_close(w.grad.double(), wd.grad, rtol=1e-4, atol=1e-5)
