@@ -377,13 +377,13 @@ struct AdamElems8 {
     }
 };
 
-// Every byte is met once.  With 32-bit states HBM bounds it: 91 M bf16 weights of 195 tensors take
+// Every byte is met once, and HBM bounds it.  32-bit states: 91 M bf16 weights of 195 tensors take
 // 306 us for 2.0 GB, 6.5 TB/s with the gradients that the norm before has left in the last-level
-// cache.  With 8-bit states 670 M weights take 1068 us for 6.7 GB, 6.3 TB/s, at 55 vector
-// instructions an element, which keep the vector units as busy (10 of them Philox).  All accesses
-// are non-temporal (but 8-wide ones of fp32, of which each touches half a line), so that what is
-// met once and dirty lines do not drive those gradients out: with the norm, 8-bit 221 -> 188 us and
-// 1497 -> 1350, 32-bit 424 -> 345.
+// cache.  8-bit states: 670 M weights take 1040 us for 6.7 GB, 6.4 TB/s, at 46 vector instructions
+// an element (10 of them Philox), which keep the vector units 85 % busy; at 55 it took 1068.  All
+// accesses are non-temporal (but 8-wide ones of fp32, of which each touches half a line), so that
+// what is met once and dirty lines do not drive those gradients out: with the norm, 8-bit
+// 221 -> 188 us and 1497 -> 1350, 32-bit 424 -> 345.
 template <int WT, int GT, bool Q8>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, const AdamArgs a) {
     using Elems = std::conditional_t<Q8, AdamElems8<WT, GT>, AdamElems32<WT, GT>>;
