@@ -30,7 +30,7 @@ struct AdamBatch {
 };
 struct AdamArgs {
     float b1, c1, b2, c2;  // beta1, 1 - beta1, beta2, 1 - beta2
-    float decay, lr, rcorr, eps;  // 1 - lr wd, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+    float lr_wd, lr, rcorr, eps;  // lr wd, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
     uint32_t k0, k1;
     int32_t do_sr;
     const float* grad_scale;
@@ -164,10 +164,27 @@ __device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
     }
 }
 
-// w' of one element; u = sqrt(v').  The hardware's root and reciprocal are within 1 ulp and take
-// what is below 2^-126 for 0.
-__device__ __forceinline__ float adam_weight(float w, float m, float u, const AdamArgs& a) {
-    return w * a.decay - a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps);
+// w' = w - t, t = lr wd w + lr m / (u rcorr + eps), u = sqrt(v'): lr wd keeps its own 24 bits, where
+// a factor 1 - lr wd would keep what is left of them beside 1 (7 for lr wd = 1e-5).  The hardware's
+// root and reciprocal are within 1 ulp and take what is below 2^-126 for 0.
+__device__ __forceinline__ float adam_change(float w, float m, float u, const AdamArgs& a) {
+    return __builtin_fmaf(w, a.lr_wd, a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps));
+}
+
+// Four differences w - t cut towards zero, as a draw added to their lower bits needs them: rounded
+// to the nearest, one value in 2^18 would go the other way than the exact difference, by a whole
+// place of 16 bits.  Mode bits 0-1 are fp32's rounding: 3 towards zero, 0 to the nearest.  The
+// nearest's rest tested for its sign instead takes 5 instructions a weight: 670 M weights with 8-bit
+// states 1314 us, 1299 so, 1292 with no cut.
+__device__ __forceinline__ void sub4_towards_zero(float* w, const float* t) {
+    asm("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 3\n\t"
+        "v_sub_f32 %0, %0, %4\n\t"
+        "v_sub_f32 %1, %1, %5\n\t"
+        "v_sub_f32 %2, %2, %6\n\t"
+        "v_sub_f32 %3, %3, %7\n\t"
+        "s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 0"
+        : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])
+        : "v"(t[0]), "v"(t[1]), "v"(t[2]), "v"(t[3]));
 }
 
 // CHECK: w may be a NaN with payload bits in its lower half, which adding to could carry over.
@@ -219,7 +236,7 @@ struct AdamElems32 {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t i = piece + k * kRun + threadIdx.x * 4;
-            float wf[4], gf[4], mf[4], vf[4];
+            float wf[4], gf[4], mf[4], vf[4], tf[4];
             unpack<WT, 4>(w[k], wf);
             unpack<GT, 4>(g[k], gf);
             unpack<HASTE_DTYPE_F32, 4>(m[k], mf);
@@ -229,16 +246,19 @@ struct AdamElems32 {
                 gf[e] *= gs;
                 mf[e] = a.b1 * mf[e] + a.c1 * gf[e];
                 vf[e] = a.b2 * vf[e] + a.c2 * gf[e] * gf[e];
-                wf[e] = adam_weight(wf[e], mf[e], __builtin_amdgcn_sqrtf(vf[e]), a);
+                tf[e] = adam_change(wf[e], mf[e], __builtin_amdgcn_sqrtf(vf[e]), a);
             }
             Elems<WT, 4> out;
             if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+                sub4_towards_zero(wf, tf);
                 const uint64_t c = (uint64_t)i / 8;
                 const u32x4 q = philox_words((uint32_t)c, (uint32_t)(c >> 32), stream, a.k0, a.k1);
                 const uint32_t r0 = i & 4 ? q[2] : q[0], r1 = i & 4 ? q[3] : q[1];
                 out.q[0] = sr_pair<WT>(wf[0], wf[1], r0, r0 >> 16);
                 out.q[1] = sr_pair<WT>(wf[2], wf[3], r1, r1 >> 16);
             } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wf[e] -= tf[e];
                 out = pack<WT, 4>(wf);
             }
             const Elems<HASTE_DTYPE_F32, 4> mo = pack<HASTE_DTYPE_F32, 4>(mf),
@@ -315,7 +335,7 @@ struct AdamElems8 {
     __device__ __forceinline__ void step(const AdamSeg& s, const AdamArgs& a, float gs,
                                          int64_t piece, int64_t n) const {
         const int64_t i = piece + threadIdx.x * 8;
-        float wf[8], gf[8], mf[8], uf[8];
+        float wf[8], gf[8], mf[8], uf[8], tf[8];
         unpack<WT, 8>(w, wf);
         unpack<GT, 8>(g, gf);
         from_e4m3(m, mf);
@@ -338,7 +358,7 @@ struct AdamElems8 {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             uf[e] = __builtin_amdgcn_sqrtf(uf[e]);
-            wf[e] = adam_weight(wf[e], mf[e], uf[e], a);
+            tf[e] = adam_change(wf[e], mf[e], uf[e], a);
         }
         const uint32_t stream = (uint32_t)(s.n_stream >> 40);
         const uint64_t c = (uint64_t)i / 4;
@@ -347,6 +367,8 @@ struct AdamElems8 {
         const uint32_t r[8] = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
         Elems<WT, 8> out;
         if (WT != HASTE_DTYPE_F32 && a.do_sr) {
+            sub4_towards_zero(wf, tf);
+            sub4_towards_zero(wf + 4, tf + 4);
             // (where m and u are finite only a NaN of w itself is left, whose payload is w's)
             if (finite) {
 #pragma unroll
@@ -358,6 +380,8 @@ struct AdamElems8 {
                     out.q[e] = sr_pair<WT>(wf[2 * e], wf[2 * e + 1], r[2 * e], r[2 * e + 1]);
             }
         } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wf[e] -= tf[e];
             out = pack<WT, 8>(wf);
         }
         if constexpr (FULL) store<WT, 8, WT != HASTE_DTYPE_F32>(s.w, i, out);
@@ -553,7 +577,7 @@ extern "C" int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count
     a.c1 = (float)(1.0 - beta1);
     a.b2 = (float)beta2;
     a.c2 = (float)(1.0 - beta2);
-    a.decay = (float)(1.0 - lr * wd);
+    a.lr_wd = (float)(lr * wd);
     a.lr = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     a.rcorr = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     a.eps = (float)eps;

@@ -288,6 +288,26 @@ def test_rounding_is_unbiased(dev, wt):
         assert (np.abs(got - x) <= 0.07 * unit)[normal].all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_draws_round_the_exact_difference(dev, bits):
+    """bf16 weights of 1/2 to 2 against draws added to the float64 result.  The change, 1e-6, is off
+    by some 16 u of itself, 2^-32 of a weight's spacing: of 2^22 weights none in a thousand runs
+    rounds the other way.  Were w - t first rounded to the nearest fp32, one in 2^18 would, some 16."""
+    n = 1 << 22
+    g = torch.Generator(device=dev).manual_seed(11)
+    w = torch.rand(n, generator=g, device=dev) * 1.5 + 0.5
+    w = torch.where(torch.rand(n, generator=g, device=dev) < 0.5, -w, w).bfloat16()
+    p = torch.nn.Parameter(w)
+    opt = AdamW([p], lr=1e-6, weight_decay=0.01, state_bits=bits, seed=77)
+    p.grad = torch.randn(n, generator=g, device=dev, dtype=torch.bfloat16)
+    w0, zero = f64(p).copy(), np.zeros(n)
+    opt.step()
+    want = ref.step(w0, f64(p.grad), zero, zero, 1, 1e-6, 0.9, 0.999, 1e-8, 0.01)[0]
+    want, _ = ref.cut(want, ref.draws(np.arange(n), bits, 0, 77)[0] / 65536.0, *MANT[torch.bfloat16])
+    assert (want != w0).any()
+    assert (f64(p) != want).sum() <= 1
+
+
 def test_against_torch_adamw(dev):
     """fp32, ten steps of the same gradients: both round each step's few operations."""
     g = torch.Generator(device=dev).manual_seed(2)
