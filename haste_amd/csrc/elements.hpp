@@ -135,8 +135,9 @@ __device__ __forceinline__ Elems<DT, V> pack(const float* f) {
     } else {
 #pragma unroll
         for (int e = 0; e < V / 2; ++e)
-            v.q[e] = DT == HASTE_DTYPE_BF16 ? pack2_rne<BF16>(f[2 * e], f[2 * e + 1])
-                                            : f32_to_f16_rne(f[2 * e]) | f32_to_f16_rne(f[2 * e + 1]) << 16;
+            v.q[e] = DT == HASTE_DTYPE_BF16
+                         ? pack2_rne<BF16>(f[2 * e], f[2 * e + 1])
+                         : f32_to_f16_rne(f[2 * e]) | f32_to_f16_rne(f[2 * e + 1]) << 16;
     }
     return v;
 }

@@ -1,9 +1,9 @@
 // haste_amd._host, the Python module.  Here: the calls over many tensors, whose tables are made
-// without a Python call for each attribute of each tensor.  An AdamW step of 195 tensors with 8-bit states reads some 40
-// attributes of each: 0.9 ms in Python, more than its kernels take.
+// without a Python call for each attribute of each tensor.  An AdamW step of 195 tensors with
+// 8-bit states reads some 40 attributes of each: 0.9 ms in Python, more than its kernels take.
 //
-// grad_norm and adamw_step return None where a tensor is not plain (dense, contiguous, not negated, no
-// subclass with a dispatch of its own, on the first one's HIP device) or its state does not
+// grad_norm and adamw_step return None where a tensor is not plain (dense, contiguous, not negated,
+// no subclass with a dispatch of its own, on the first one's HIP device) or its state does not
 // fit: the callers' Python paths then copy, create or refuse.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -202,8 +202,15 @@ PyMethodDef methods[] = {
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(haste_host::layer_norm)),
      METH_FASTCALL, "layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual"},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of libhaste_ffi.so's entry points that take torch tensors.", -1,
-                      methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT,
+                      "_host",
+                      "Entry points of libhaste_ffi.so that take torch tensors.",
+                      -1,
+                      methods,
+                      nullptr,
+                      nullptr,
+                      nullptr,
+                      nullptr};
 
 }  // namespace
 

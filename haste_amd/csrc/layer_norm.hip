@@ -537,8 +537,9 @@ bool past_cache(int64_t N, int64_t D, int32_t dtype) {
 }
 
 // The partial sums of dw and db.
-int bwd_blocks(int64_t N, int64_t D, const RowShape& r) {
-    const int64_t rows = r.C ? std::max(kBwdThreads / r.tpr, 1) : 4 * kAnyRows, most = r.C ? kBwdBlocks : 64;
+int bwd_blocks(int64_t N, const RowShape& r) {
+    const int64_t rows = r.C ? std::max(kBwdThreads / r.tpr, 1) : 4 * kAnyRows;
+    const int64_t most = r.C ? kBwdBlocks : 64;
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(N, rows), most));
 }
 
@@ -647,7 +648,7 @@ extern "C" int64_t haste_layer_norm_bwd_workspace_size(int64_t N, int64_t D) {
     // (the larger of the two shapes that the rows' dtypes may take)
     int most = 1;
     for (int32_t dt : {HASTE_DTYPE_BF16, HASTE_DTYPE_F32})
-        most = std::max(most, haste::bwd_blocks(N, D, haste::bwd_shape(D, dt)));
+        most = std::max(most, haste::bwd_blocks(N, haste::bwd_shape(D, dt)));
     return most * 2 * std::max<int64_t>(D, 8) * (int64_t)sizeof(float);
 }
 
@@ -683,7 +684,7 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
     const haste::RowShape r = haste::bwd_shape(D, dtype);
-    const int blocks = haste::bwd_blocks(N, D, r);
+    const int blocks = haste::bwd_blocks(N, r);
     const bool nt = haste::past_cache(N, D, dtype);
     const char *dyc = static_cast<const char*>(dy), *dhc = static_cast<const char*>(dh),
                *hc = static_cast<const char*>(h);
@@ -701,9 +702,9 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
     do {                                                                                         \
         auto slots = [&](auto c) {                                                               \
             constexpr int C = std::min(decltype(c)::value, haste::bwd_slots(DT));                \
-            const size_t lds = r.tpr < haste::kBwdThreads && sums                                \
-                                   ? sizeof(float) * haste::row_vec(DT) * C * haste::kBwdThreads                  \
-                                   : 0;                                                          \
+            const size_t lds = r.tpr >= haste::kBwdThreads || !sums                              \
+                                   ? 0                                                           \
+                                   : sizeof(float) * haste::row_vec(DT) * C * haste::kBwdThreads; \
             auto kernel = nt ? haste::ln_bwd_kernel<DT, WT, C, true, haste::kBwdThreads>         \
                              : haste::ln_bwd_kernel<DT, WT, C, false, haste::kBwdThreads>;       \
             if constexpr (haste::wide(DT, C))                                                    \
