@@ -48,6 +48,10 @@ void check_device(const at::Tensor& t, const char* name) {
 
 void check(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias,
            const at::Tensor& residual) {
+    // (also where no gradient is recorded: the kernels are handed addresses, without the tangent)
+    for (const at::Tensor* t : {&x, &weight, &bias, &residual})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                    "layer_norm: forward-mode derivatives are not supported");
     check_device(x, "x");
     TORCH_CHECK(dtype_code(x.scalar_type()) >= 0, "unsupported dtype ", x.scalar_type());
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1,

@@ -25,7 +25,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
     """y = (h - mean) / sqrt(var + eps) * weight + bias over the last axis of h = x, or, with
     ``residual`` (of x's shape or one that broadcasts to it), (y, h) with h = x + residual.
-    Differentiable once; checks, outputs and the autograd node are native."""
+    Differentiable once, in reverse mode; checks, outputs and the autograd node are native."""
     return host().layer_norm(x, weight, bias, eps, residual)
 
 
