@@ -35,14 +35,16 @@ bool plain(const at::Tensor& t, int64_t* device) {
     return t.get_device() == *device;
 }
 
-// An entry of a state, with `n` elements of `type`; nullptr where it is anything else.
-void* state_tensor(PyObject* state, PyObject* key, at::ScalarType type, int64_t n,
+// An entry of a state, with `n` elements of `type` from a multiple of `align` bytes; nullptr where
+// it is anything else.
+void* state_tensor(PyObject* state, PyObject* key, at::ScalarType type, int64_t n, unsigned align,
                    int64_t* device) {
     PyObject* o = PyDict_GetItemWithError(state, key);
     if (!o || !THPVariable_Check(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!plain(t, device) || t.scalar_type() != type || t.numel() != n) return nullptr;
-    return t.mutable_data_ptr();
+    void* p = t.mutable_data_ptr();
+    return reinterpret_cast<uintptr_t>(p) % align ? nullptr : p;
 }
 
 struct Keys {
@@ -140,13 +142,14 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         s.row.stream = (uint32_t)i;
         const at::ScalarType type = q8 ? at::kFloat8_e4m3fn : at::kFloat;
         const int64_t size = q8 ? blocks * kStateBlock : n;
-        s.row.m = state_tensor(s.state, keys->m, type, size, &device);
-        s.row.v = state_tensor(s.state, q8 ? keys->u : keys->v, type, size, &device);
+        const unsigned align = q8 ? 8 : 16;
+        s.row.m = state_tensor(s.state, keys->m, type, size, align, &device);
+        s.row.v = state_tensor(s.state, q8 ? keys->u : keys->v, type, size, align, &device);
         if (q8) {
             s.row.m_scale = static_cast<uint8_t*>(
-                state_tensor(s.state, keys->ms, at::kFloat8_e8m0fnu, blocks, &device));
+                state_tensor(s.state, keys->ms, at::kFloat8_e8m0fnu, blocks, 1, &device));
             s.row.v_scale = static_cast<uint8_t*>(
-                state_tensor(s.state, keys->us, at::kFloat8_e8m0fnu, blocks, &device));
+                state_tensor(s.state, keys->us, at::kFloat8_e8m0fnu, blocks, 1, &device));
         }
         if (PyErr_Occurred()) return nullptr;
         if (n > 0 && (!s.row.m || !s.row.v || (q8 && (!s.row.m_scale || !s.row.v_scale))))
@@ -167,29 +170,37 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         int w, g;
         long long step;
         std::vector<haste_adamw_tensor> rows;
+        std::vector<const Stepped*> stepped;
     };
     std::vector<Group> groups;
-    for (Stepped& s : all) {
-        PyObject* step = PyLong_FromLongLong(s.step);
-        if (!step || PyDict_SetItem(s.state, keys->step, step) != 0) {
-            Py_XDECREF(step);
-            return nullptr;
-        }
-        Py_DECREF(step);
-        s.param.unsafeGetTensorImpl()->bump_version();
+    for (const Stepped& s : all) {
         Group* at = nullptr;
         for (Group& g : groups)
             if (g.w == s.w && g.g == s.g && g.step == s.step) at = &g;
         if (!at) {
-            groups.push_back(Group{s.w, s.g, s.step, {}});
+            groups.push_back(Group{s.w, s.g, s.step, {}, {}});
             at = &groups.back();
             at->rows.reserve(all.size());
+            at->stepped.reserve(all.size());
         }
         at->rows.push_back(s.row);
+        at->stepped.push_back(&s);
     }
-    for (const Group& g : groups)
+    for (const Group& g : groups) {
         call(haste_adamw_step(g.rows.data(), (int32_t)g.rows.size(), g.w, g.g, bits, lr, beta1, beta2,
                               eps, wd, g.step, sr, seed, factor, stream_of(all[0].param)));
+        // (only now: a refused step leaves the counts as they were)
+        PyObject* step = PyLong_FromLongLong(g.step);
+        if (!step) return nullptr;
+        for (const Stepped* s : g.stepped) {
+            s->param.unsafeGetTensorImpl()->bump_version();
+            if (PyDict_SetItem(s->state, keys->step, step) != 0) {
+                Py_DECREF(step);
+                return nullptr;
+            }
+        }
+        Py_DECREF(step);
+    }
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }

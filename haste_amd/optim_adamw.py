@@ -165,16 +165,15 @@ class AdamW(Optimizer):
         (beta1, beta2), sr = group["betas"], bool(group["stochastic_rounding"])
         args = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]),
                 float(group["weight_decay"]))
+        if not _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, grad_scale):
+            with torch.no_grad():
+                self._step_any(group["params"], bits, args, sr, seed, grad_scale)
         group["seed"] += 1
-        if _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, grad_scale):
-            return
-        with torch.no_grad():
-            self._step_any(group["params"], bits, args, sr, seed, grad_scale)
 
     def _step_any(self, params, bits, args, sr, seed, grad_scale) -> None:
         """The step of any parameters: those that are not plain through copies, with states made
         where there are none yet."""
-        batches, device, keep, copies = self._rows(params, bits)
+        batches, device = self._rows(params, bits)
         if not batches:
             return
         scale = None
@@ -184,16 +183,22 @@ class AdamW(Optimizer):
                                    f"on cuda:{device}")
             scale = grad_scale.data_ptr()
         stream = torch._C._cuda_getCurrentRawStream(device)
-        for w_code, g_code, step, count, rows in batches:
-            _lib.call("haste_adamw_step", rows, count, w_code, g_code, bits, *args, step, int(sr),
-                      int(seed), scale, stream)
-        for p, w in copies:
-            p.copy_(w)
+        for (w_code, g_code, step), stepped in batches.items():
+            rows = (_lib.AdamwTensor * len(stepped))(*[s[1] for s in stepped])
+            _lib.call("haste_adamw_step", rows, len(stepped), w_code, g_code, bits, *args, step,
+                      int(sr), int(seed), scale, stream)
+            # (only now: a refused step leaves the counts as they were)
+            for state, _, p, w, _ in stepped:
+                state["step"] = step
+                if w.data_ptr() != p.data_ptr():
+                    p.copy_(w)
+            # written through raw pointers: move the version counters as torch would
+            torch.autograd.graph.increment_version([s[2] for s in stepped])
 
     def _rows(self, params, bits):
-        """The table of the step of any parameters: ([(w dtype, g dtype, step, tensors, rows)],
-        device, tensors to keep until the launch, [(parameter, contiguous copy to step)])."""
-        batches, stepped, copies, keep, device = {}, [], [], [], None
+        """The tables of the step of any parameters: ({(w dtype, g dtype, step): [(state, row,
+        parameter, its contiguous tensor or copy, the gradient's)]}, device)."""
+        batches, device = {}, None
         for index, p in enumerate(params):
             grad = p.grad
             if grad is None:
@@ -218,17 +223,10 @@ class AdamW(Optimizer):
                         t.numel() != self._state_size(key, bits, p):
                     raise RuntimeError(f"AdamW: state {key} does not fit a parameter of shape "
                                        f"{list(p.shape)} with {bits}-bit states")
+                align = 1 if key.endswith("_scale") else 16 if bits == 32 else 8
+                if t.data_ptr() % align:
+                    raise RuntimeError(f"AdamW: state {key} must start at a multiple of {align} bytes")
                 row.append(t.data_ptr())
             row += [None] * (6 - len(row)) + [p.numel(), index]
-            stepped.append((state, codes, row, p))
-            keep.append((w, g))
-            if w.data_ptr() != p.data_ptr():
-                copies.append((p, w))
-        for state, codes, row, p in stepped:
-            state["step"] += 1
-            batches.setdefault((*codes, state["step"]), []).append(tuple(row))
-        if stepped:  # written through raw pointers: move the version counters as torch would
-            torch.autograd.graph.increment_version([s[3] for s in stepped])
-        return ([(*key, len(rows), (_lib.AdamwTensor * len(rows))(*rows))
-                 for key, rows in batches.items()], None if device is None else device.index, keep,
-                copies)
+            batches.setdefault((*codes, state["step"] + 1), []).append((state, tuple(row), p, w, g))
+        return batches, None if device is None else device.index

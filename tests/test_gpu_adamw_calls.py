@@ -1,0 +1,65 @@
+"""GPU: calls of AdamW and of the gradients' norm whose answers the other tests do not reach."""
+import pytest
+import torch
+
+from haste_amd.optim_adamw import AdamW
+
+pytestmark = pytest.mark.gpu
+
+
+def counts(opt, ps):
+    return [(opt.state[p].get("step"), p._version, p.detach().clone()) for p in ps], \
+        [g["seed"] for g in opt.param_groups]
+
+
+def unchanged(opt, ps, before):
+    now = counts(opt, ps)
+    assert now[1] == before[1]
+    for a, b in zip(now[0], before[0]):
+        assert a[:2] == b[:2] and torch.equal(a[2], b[2])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("plain", [True, False])
+def test_a_refused_step_moves_no_count(dev, bits, plain):
+    """Settings that the library refuses, for parameters of either path: the count of steps, the
+    version and the seed stay, and the step after it is that of an optimizer that was never refused."""
+    def make():
+        w = torch.arange(600, device=dev, dtype=torch.bfloat16).view(20, 30) / 600
+        p = torch.nn.Parameter(w if plain else w.t())
+        p.grad = torch.ones_like(p) if plain else torch.ones(20, 30, device=dev, dtype=p.dtype).t()
+        opt = AdamW([p], lr=1e-2, state_bits=bits)
+        opt.step()
+        return p, opt
+    (p, opt), (q, other) = make(), make()
+    before = counts(opt, [p])
+    opt.param_groups[0]["betas"] = (1.5, 0.9)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="betas"):
+            opt.step()
+        unchanged(opt, [p], before)
+    opt.param_groups[0]["betas"] = (0.9, 0.999)
+    opt.step()
+    other.step()
+    assert torch.equal(p, q) and opt.state[p]["step"] == 2
+
+
+def test_a_refused_tensor_stops_the_others_of_its_group(dev):
+    """States that start off 16 bytes (views of an unpadded buffer) are refused before any tensor of
+    the group is stepped, whatever its dtypes."""
+    ps = [torch.nn.Parameter(torch.ones(64, device=dev, dtype=d)) for d in (torch.bfloat16, torch.float32)]
+    opt = AdamW(ps, lr=1e-2)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    flat = torch.zeros(65, device=dev)
+    good = opt.state[ps[1]]["exp_avg"]
+    opt.state[ps[1]]["exp_avg"] = flat[1:]
+    before = counts(opt, ps)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="exp_avg .*16 bytes"):
+            opt.step()
+        unchanged(opt, ps, before)
+    opt.state[ps[1]]["exp_avg"] = good
+    opt.step()
+    assert [opt.state[p]["step"] for p in ps] == [2, 2]
