@@ -48,6 +48,7 @@ void check_device(const at::Tensor& t, const char* name) {
 
 void check(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias,
            const at::Tensor& residual) {
+    check_not_traced("layer_norm");
     // (also where no gradient is recorded: the kernels are handed addresses, without the tangent)
     for (const at::Tensor* t : {&x, &weight, &bias, &residual})
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),

@@ -68,6 +68,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     PyObject* list;
     double max_norm;
     if (!PyArg_ParseTuple(args, "O!d", &PyList_Type, &list, &max_norm)) return nullptr;
+    haste_host::check_not_traced("grad_norm");
     const Py_ssize_t n = PyList_GET_SIZE(list);
     std::vector<haste_grad_tensor> rows;
     rows.reserve((size_t)n);
@@ -115,6 +116,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "O!O!idddddpKO", &PyList_Type, &list, &PyDict_Type, &states, &bits,
                           &lr, &beta1, &beta2, &eps, &wd, &sr, &seed, &scale))
         return nullptr;
+    haste_host::check_not_traced("AdamW.step");
     std::vector<Stepped> all;
     const Py_ssize_t count = PyList_GET_SIZE(list);
     all.reserve((size_t)count);

@@ -4,8 +4,10 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/haste_ffi.h"
 
@@ -21,6 +23,15 @@ inline int dtype_code(c10::ScalarType t) {
 
 inline void* stream_of(const at::Tensor& t) {
     return c10::hip::getCurrentHIPStream(t.get_device()).stream();
+}
+
+// Refuses under torch.jit.trace and fx's tracing, whose graph would hold the empty outputs and not
+// the kernels that fill them.
+inline void check_not_traced(const char* what) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                what, ": cannot be traced (its kernels are called by address)");
 }
 
 inline void call(int rc) { TORCH_CHECK(rc == HASTE_OK, haste_last_error()); }
