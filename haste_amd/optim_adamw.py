@@ -72,8 +72,10 @@ def grad_norm(tensors: Iterable[torch.Tensor], max_norm: float = math.inf
     out = torch.empty(2, dtype=torch.float32, device=dev)
     size = _lib.lib().haste_grad_norm_workspace_size(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    _lib.call("haste_grad_norm", arr, n, float(max_norm), out.data_ptr(), ws.data_ptr(), size,
-              _C.stream_of(out))
+    # (torch's default stream is handle 0 on every device, which means the current one's)
+    with torch.cuda.device(dev):
+        _lib.call("haste_grad_norm", arr, n, float(max_norm), out.data_ptr(), ws.data_ptr(), size,
+                  _C.stream_of(out))
     return out[0], out[1]
 
 
@@ -182,7 +184,13 @@ class AdamW(Optimizer):
                 raise RuntimeError(f"AdamW: grad_scale is on {grad_scale.device}, the parameters "
                                    f"on cuda:{device}")
             scale = grad_scale.data_ptr()
-        stream = torch._C._cuda_getCurrentRawStream(device)
+        # torch's default stream is handle 0 on every device, which means the current one's
+        with torch.cuda.device(device):
+            self._launch(batches, bits, args, sr, seed, scale,
+                         torch._C._cuda_getCurrentRawStream(device))
+
+    @staticmethod
+    def _launch(batches, bits, args, sr, seed, scale, stream) -> None:
         for (w_code, g_code, step), stepped in batches.items():
             rows = (_lib.AdamwTensor * len(stepped))(*[s[1] for s in stepped])
             _lib.call("haste_adamw_step", rows, len(stepped), w_code, g_code, bits, *args, step,

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from haste_amd.optim_adamw import AdamW
+from haste_amd.optim_adamw import AdamW, grad_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,15 @@ def test_a_refused_tensor_stops_the_others_of_its_group(dev):
     opt.state[ps[1]]["exp_avg"] = good
     opt.step()
     assert [opt.state[p]["step"] for p in ps] == [2, 2]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_on_a_device_that_is_not_the_current_one(dev, bits):
+    ps = [torch.nn.Parameter(torch.linspace(-1, 1, 5000, device=f"cuda:{k}")) for k in (0, 1)]
+    for p in ps:
+        opt = AdamW([p], lr=1e-2, state_bits=bits)
+        for _ in range(2):
+            p.grad = torch.cos(p.detach() * 7)
+            opt.step(grad_scale=grad_norm([p.grad.view(50, 100).t()], 1.0)[1])
+    assert torch.equal(ps[0].cpu(), ps[1].cpu())
