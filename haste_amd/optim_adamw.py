@@ -183,6 +183,7 @@ class AdamW(Optimizer):
             if grad_scale.get_device() != device:
                 raise RuntimeError(f"AdamW: grad_scale is on {grad_scale.device}, the parameters "
                                    f"on cuda:{device}")
+            grad_scale = _dense(grad_scale, "grad_scale")
             scale = grad_scale.data_ptr()
         # torch's default stream is handle 0 on every device, which means the current one's
         with torch.cuda.device(device):
@@ -227,8 +228,8 @@ class AdamW(Optimizer):
             row = [w.data_ptr(), g.data_ptr()]
             for key, dtype in _STATE[bits].items():
                 t = state[key]
-                if t.dtype != dtype or t.device != device or not t.is_contiguous() or \
-                        t.numel() != self._state_size(key, bits, p):
+                if t.dtype != dtype or t.device != device or t.is_neg() or \
+                        not t.is_contiguous() or t.numel() != self._state_size(key, bits, p):
                     raise RuntimeError(f"AdamW: state {key} does not fit a parameter of shape "
                                        f"{list(p.shape)} with {bits}-bit states")
                 align = 1 if key.endswith("_scale") else 16 if bits == 32 else 8

@@ -75,3 +75,36 @@ def test_steps_on_a_device_that_is_not_the_current_one(dev, bits):
             p.grad = torch.cos(p.detach() * 7)
             opt.step(grad_scale=grad_norm([p.grad.view(50, 100).t()], 1.0)[1])
     assert torch.equal(ps[0].cpu(), ps[1].cpu())
+
+
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_negated_grad_scale(dev, wt, bits):
+    """A lazily negated factor counts with its sign, for plain parameters and for others."""
+    scale = torch.full((1,), 0.5, device=dev)
+    for shape in ((40, 30), (30, 40)):
+        w = torch.randn(40, 30, device=dev).to(wt)
+        grad = torch.randn(40, 30, device=dev).to(wt)
+        got = []
+        for s in (-scale, torch._neg_view(scale)):
+            p = torch.nn.Parameter(w.clone() if shape == (40, 30) else w.clone().t())
+            opt = AdamW([p], lr=1e-2, state_bits=bits)
+            for _ in range(2):
+                p.grad = grad.clone() if shape == (40, 30) else grad.t()
+                opt.step(grad_scale=s)
+            got.append(p.detach().clone())
+        assert torch.equal(*got)
+
+
+def test_a_negated_state_is_refused(dev):
+    p = torch.nn.Parameter(torch.ones(64, device=dev))
+    opt = AdamW([p])
+    for _ in range(2):
+        p.grad = torch.ones_like(p)
+        opt.step()
+        kept = p.detach().clone()
+        opt.state[p]["exp_avg"] = torch._neg_view(opt.state[p]["exp_avg"])
+        with pytest.raises(RuntimeError, match="does not fit"):
+            opt.step()
+        assert torch.equal(p, kept)
+        opt.state[p]["exp_avg"] = torch._neg_view(opt.state[p]["exp_avg"])
