@@ -166,8 +166,10 @@ __device__ __forceinline__ void from_e4m3(u32x2 c, float* f) {
 
 // w' = w - t, t = lr wd w + lr m / (u rcorr + eps), u = sqrt(v'): lr wd keeps its own 24 bits, where
 // a factor 1 - lr wd would keep what is left of them beside 1 (7 for lr wd = 1e-5).  The hardware's
-// root and reciprocal are within 1 ulp and take what is below 2^-126 for 0.
+// root and reciprocal are within 1 ulp and take what is below 2^-126 for 0.  An infinite w counts
+// in t as the largest finite one, so that w - t stays infinite (inf - inf and inf * 0 are not).
 __device__ __forceinline__ float adam_change(float w, float m, float u, const AdamArgs& a) {
+    w = __builtin_amdgcn_fmed3f(w, -__FLT_MAX__, __FLT_MAX__);
     return __builtin_fmaf(w, a.lr_wd, a.lr * m * __builtin_amdgcn_rcpf(u * a.rcorr + a.eps));
 }
 

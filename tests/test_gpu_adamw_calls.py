@@ -1,10 +1,12 @@
 """GPU: calls of AdamW and of the gradients' norm whose answers the other tests do not reach."""
+import numpy as np
 import pytest
 import torch
 
 from haste_amd.optim_adamw import AdamW, grad_norm
 
 pytestmark = pytest.mark.gpu
+INF = float("inf")
 
 
 def counts(opt, ps):
@@ -108,3 +110,28 @@ def test_a_negated_state_is_refused(dev):
             opt.step()
         assert torch.equal(p, kept)
         opt.state[p]["exp_avg"] = torch._neg_view(opt.state[p]["exp_avg"])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sr", [True, False])
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("wd", [0.0, 0.1])
+def test_infinite_weights_stay_so(dev, bits, sr, wt, wd):
+    """w (1 - lr wd) less a finite update; NaN stays NaN, and their neighbours are not touched."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    w = (torch.randn(300, generator=g, device=dev) * 0.1).to(wt)
+    grad = torch.randn(300, generator=g, device=dev).to(wt)
+    a, b = (torch.nn.Parameter(w.clone()) for _ in range(2))
+    at = torch.tensor([0, 17, 130, 299], device=dev)
+    with torch.no_grad():
+        a[at] = torch.tensor([INF, -INF, float("nan"), INF], device=dev, dtype=wt)
+    for p in (a, b):
+        opt = AdamW([p], lr=1e-2, weight_decay=wd, state_bits=bits, stochastic_rounding=sr)
+        for _ in range(2):
+            p.grad = grad
+            opt.step()
+    got = a.detach()[at].float().cpu().numpy()
+    assert np.array_equal(got, np.float32([INF, -INF, np.nan, INF]), equal_nan=True)
+    keep = torch.ones(300, dtype=torch.bool, device=dev)
+    keep[at] = False
+    assert torch.equal(a[keep], b[keep])
