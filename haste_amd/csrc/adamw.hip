@@ -442,32 +442,51 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
-// This thread's share of the squares of elements i0 .. i0 + kNormPiece of n: fp32 over its 64,
-// four sums side by side.
+// This thread's share of the squares of elements i0 .. i0 + kNormPiece of n, in fp64.
 template <int DT>
-__device__ __forceinline__ float piece_squares(const void* g, int64_t i0, int64_t n) {
+__device__ __forceinline__ double piece_squares64(const void* g, int64_t i0, int64_t n) {
+    double sum = 0.0;
+    float f[8];
+    for (int k = 0; k < kNormLoads; ++k) {
+        const int64_t at = i0 + threadIdx.x * 8 + k * (kNormThreads * 8);
+        if (at >= n) break;
+        unpack<DT, 8>(load_part<DT, 8>(g, at, n - at), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += (double)f[e] * f[e];
+    }
+    return sum;
+}
+
+// The same in fp32, four sums side by side, unless that overflows or is so small that squares may
+// have lost bits below 2^-149 (64 such losses are at most 2^-44 of a sum from 2^-100 on).
+template <int DT>
+__device__ __forceinline__ double piece_squares(const void* g, int64_t i0, int64_t n) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f}, f[8];
+    uint32_t any = 0;
+    auto add = [&](const Elems<DT, 8>& x) __attribute__((always_inline)) {
+        unpack<DT, 8>(x, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
+#pragma unroll
+        for (uint32_t q : x.q) any |= q;
+    };
     const int64_t i = i0 + threadIdx.x * 8;
     if (i0 + kNormPiece <= n) {
         Elems<DT, 8> x[kNormLoads];
 #pragma unroll
         for (int k = 0; k < kNormLoads; ++k) x[k] = load<DT, 8>(g, i + k * (kNormThreads * 8));
 #pragma unroll
-        for (int k = 0; k < kNormLoads; ++k) {
-            unpack<DT, 8>(x[k], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
-        }
+        for (int k = 0; k < kNormLoads; ++k) add(x[k]);
     } else {
         for (int k = 0; k < kNormLoads; ++k) {
             const int64_t at = i + k * (kNormThreads * 8);
             if (at >= n) break;
-            unpack<DT, 8>(load_part<DT, 8>(g, at, n - at), f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e & 3] += f[e] * f[e];
+            add(load_part<DT, 8>(g, at, n - at));
         }
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    const float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (any == 0 || (s >= 0x1p-100f && s < INFINITY)) return s;
+    return piece_squares64<DT>(g, i0, n);
 }
 
 // part[workgroup] = the sum of squares of every gridDim-th piece, the launch's last pieces first:

@@ -609,8 +609,9 @@ int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t l
  * The 2-norm over all of several tensors, and the factor that clips it:
  *   out[0] = norm = sqrt(sum g^2),  out[1] = min(1, max_norm / (norm + 1e-6)),
  * out[1] = NaN where norm is not finite (haste_adamw_step then skips its step).
- * dtype of each tensor: bf16, f16 or f32.  Squares are summed in fp32 by threads, 64 at a time,
- * and in fp64 beyond, in a fixed order: a |g| of 1.8e19 or more makes the norm infinite.  ws: workspace of
+ * dtype of each tensor: bf16, f16 or f32.  Squares are summed in fp32 by threads, 64 at a time (in
+ * fp64 where those leave fp32's range), and in fp64 beyond, in a fixed order: norm is infinite only
+ * past fp32's largest value.  ws: workspace of
  * haste_grad_norm_workspace_size(count) bytes (8-byte aligned).
  */
 typedef struct haste_grad_tensor {

@@ -135,3 +135,37 @@ def test_infinite_weights_stay_so(dev, bits, sr, wt, wd):
     keep = torch.ones(300, dtype=torch.bool, device=dev)
     keep[at] = False
     assert torch.equal(a[keep], b[keep])
+
+
+@pytest.mark.parametrize("value", [1e-22, 1e-30, 3e-19, 4e18, 1.7e19, 3e38])
+@pytest.mark.parametrize("n", [1, 64, 20000, 70000])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_norms_whose_squares_leave_fp32(dev, value, n, dt):
+    """The norm of n equal gradients is |g| sqrt(n), here below fp32's largest value unless that
+    is passed: squares from 1e-60 to 9e76 are sums of fp64, off by a few 1e-16, and the rest by
+    fp32's sums of 64 squares and the norm's own rounding, under 70 2^-24."""
+    t = torch.full((n,), value, device=dev).to(dt)
+    t[::3] *= -1
+    exact = float(t[0].double().abs()) * n ** 0.5
+    norm, coef = grad_norm([t, torch.zeros(5000, device=dev)], 1.0)
+    if exact > 3.4028235e38:
+        assert float(norm) == INF and bool(torch.isnan(coef))
+        return
+    assert abs(float(norm) - exact) <= 70 * 2.0 ** -24 * exact
+    want = min(1.0, 1.0 / (exact + 1e-6))
+    assert abs(float(coef) - want) <= 80 * 2.0 ** -24 * want
+
+
+def test_norms_of_small_beside_large(dev):
+    """One workgroup's share of each kind: what is small is not lost and not counted twice."""
+    small, large = torch.full((40000,), 1e-22, device=dev), torch.full((40000,), 2e-22, device=dev)
+    zero = torch.zeros(40000, device=dev)
+    exact = (40000 * (float(small[0].double()) ** 2 + float(large[0].double()) ** 2)) ** 0.5
+    norm, _ = grad_norm([small, zero, -zero, large])
+    assert abs(float(norm) - exact) <= 70 * 2.0 ** -24 * exact
+    one = torch.ones(1, device=dev)
+    assert float(grad_norm([small, one])[0]) == 1.0
+    bad = small.clone()
+    bad[777] = float("nan")
+    assert bool(torch.isnan(grad_norm([bad, one])[0]))
+    assert float(grad_norm([zero])[0]) == 0.0
