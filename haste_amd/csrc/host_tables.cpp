@@ -105,16 +105,17 @@ struct Stepped {
 };
 
 // adamw_step(params, state, bits, lr, beta1, beta2, eps, weight decay, stochastic rounding, seed,
-// grad_scale) -> True: steps the params that have a gradient and moves their counts of steps and
-// versions.
+// stream, grad_scale) -> True: steps the params that have a gradient, the first of them with
+// random stream `stream`, and moves their counts of steps and versions.
 PyObject* adamw_step(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
     PyObject *list, *states, *scale;
     int bits, sr;
+    unsigned stream;
     double lr, beta1, beta2, eps, wd;
     unsigned long long seed;
-    if (!PyArg_ParseTuple(args, "O!O!idddddpKO", &PyList_Type, &list, &PyDict_Type, &states, &bits,
-                          &lr, &beta1, &beta2, &eps, &wd, &sr, &seed, &scale))
+    if (!PyArg_ParseTuple(args, "O!O!idddddpKIO", &PyList_Type, &list, &PyDict_Type, &states, &bits,
+                          &lr, &beta1, &beta2, &eps, &wd, &sr, &seed, &stream, &scale))
         return nullptr;
     haste_host::check_not_traced("AdamW.step");
     std::vector<Stepped> all;
@@ -141,7 +142,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         s.row.w = p.mutable_data_ptr();
         s.row.g = grad.const_data_ptr();
         s.row.n = n;
-        s.row.stream = (uint32_t)i;
+        s.row.stream = stream + (uint32_t)i;
         const at::ScalarType type = q8 ? at::kFloat8_e4m3fn : at::kFloat;
         const int64_t size = q8 ? blocks * kStateBlock : n;
         const unsigned align = q8 ? 8 : 16;
@@ -211,7 +212,7 @@ PyMethodDef methods[] = {
     {"grad_norm", grad_norm, METH_VARARGS, "grad_norm(tensors, max_norm) -> (norm, coef) or None"},
     {"adamw_step", adamw_step, METH_VARARGS,
      "adamw_step(params, state, bits, lr, beta1, beta2, eps, weight_decay, stochastic_rounding, "
-     "seed, grad_scale) -> True or None"},
+     "seed, stream, grad_scale) -> True or None"},
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(haste_host::layer_norm)),
      METH_FASTCALL, "layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual"},
     {nullptr, nullptr, 0, nullptr}};

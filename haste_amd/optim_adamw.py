@@ -13,8 +13,8 @@ moments, in fp32); beside it:
     ``grad_norm``'s; a NaN there leaves parameters and states as they are.
 The tensors of a group are stepped by one launch for each 64 of them (and for each dtype of
 parameters and gradients, and each count of steps).  Random bits: Philox4x32-10 keyed by the
-seed, with the position of a tensor in its group and of an element in it as counters, so a step's
-results depend on nothing else.
+group's seed, with the position of a tensor among those of all groups and of an element in it as
+counters, so a step's results depend on nothing else and groups of one seed draw apart.
 
 State of a parameter (created at its first step): ``step``, an int; with 32 bits ``exp_avg`` and
 ``exp_avg_sq``, fp32 of its shape; with 8 bits ``exp_avg`` and ``rms`` (codes, of its elements in
@@ -158,24 +158,27 @@ class AdamW(Optimizer):
             if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
                 raise RuntimeError(f"grad_scale must be one float32 (got {list(grad_scale.shape)} "
                                    f"{grad_scale.dtype})")
+        stream = 0  # (of the group's first parameter)
         for group in self.param_groups:
-            self._step_group(group, grad_scale)
+            self._step_group(group, stream, grad_scale)
+            stream += len(group["params"])
         return loss
 
-    def _step_group(self, group, grad_scale) -> None:
+    def _step_group(self, group, stream, grad_scale) -> None:
         bits, seed = group["state_bits"], group["seed"]
         (beta1, beta2), sr = group["betas"], bool(group["stochastic_rounding"])
         args = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]),
                 float(group["weight_decay"]))
-        if not _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, grad_scale):
+        if not _lib.host().adamw_step(group["params"], self.state, bits, *args, sr, seed, stream,
+                                      grad_scale):
             with torch.no_grad():
-                self._step_any(group["params"], bits, args, sr, seed, grad_scale)
+                self._step_any(group["params"], bits, args, sr, seed, stream, grad_scale)
         group["seed"] += 1
 
-    def _step_any(self, params, bits, args, sr, seed, grad_scale) -> None:
+    def _step_any(self, params, bits, args, sr, seed, first, grad_scale) -> None:
         """The step of any parameters: those that are not plain through copies, with states made
         where there are none yet."""
-        batches, device = self._rows(params, bits)
+        batches, device = self._rows(params, bits, first)
         if not batches:
             return
         scale = None
@@ -204,11 +207,12 @@ class AdamW(Optimizer):
             # written through raw pointers: move the version counters as torch would
             torch.autograd.graph.increment_version([s[2] for s in stepped])
 
-    def _rows(self, params, bits):
-        """The tables of the step of any parameters: ({(w dtype, g dtype, step): [(state, row,
-        parameter, its contiguous tensor or copy, the gradient's)]}, device)."""
+    def _rows(self, params, bits, first):
+        """The tables of the step of any parameters, whose random streams count from `first`:
+        ({(w dtype, g dtype, step): [(state, row, parameter, its contiguous tensor or copy, the
+        gradient's)]}, device)."""
         batches, device = {}, None
-        for index, p in enumerate(params):
+        for index, p in enumerate(params, first):
             grad = p.grad
             if grad is None:
                 continue

@@ -169,3 +169,22 @@ def test_norms_of_small_beside_large(dev):
     bad[777] = float("nan")
     assert bool(torch.isnan(grad_norm([bad, one])[0]))
     assert float(grad_norm([zero])[0]) == 0.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("plain", [True, False])
+def test_groups_draw_for_themselves(dev, bits, plain):
+    """The same 4000 weights and gradients twice in one group and in two others of its seed: no two
+    are rounded by the same draws."""
+    g = torch.Generator(device=dev).manual_seed(6)
+    w = torch.randn(40, 100, generator=g, device=dev).to(torch.bfloat16)
+    grad = torch.randn(40, 100, generator=g, device=dev).to(torch.bfloat16)
+    ps = [torch.nn.Parameter(w.clone() if plain else w.t().contiguous().t()) for _ in range(4)]
+    opt = AdamW([dict(params=ps[:2]), dict(params=ps[2:3]), dict(params=ps[3:])], lr=1e-3, state_bits=bits)
+    for k in range(2):
+        for p in ps:
+            p.grad = grad.clone()
+        opt.step()
+        for i in range(4):
+            for j in range(i):
+                assert not torch.equal(ps[i], ps[j]), (k, i, j)
