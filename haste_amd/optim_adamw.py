@@ -116,24 +116,46 @@ class AdamW(Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         # torch casts floating-point state to the parameter's dtype: put the states back as they
-        # were saved
-        saved = {k: dict(v) for k, v in state_dict["state"].items()}
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            want = _STATE[group["state_bits"]]
-            for p in group["params"]:
-                got = saved.get(ids.pop(0))
+        # were saved.  All of it is checked before any of it replaces anything, by a hook behind
+        # the others, which sees what they made of the saved state.
+        saved = []
+        check = self.register_load_state_dict_pre_hook(
+            lambda _, state: saved.append(self._check_saved(state)))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            check.remove()
+        params = [p for group in self.param_groups for p in group["params"]]
+        for p, got in zip(params, saved[0]):
+            for key, t in got.items():
+                self.state[p][key] = t if key == "step" else t.to(device=p.device).clone()
+
+    def _check_saved(self, state_dict) -> list:
+        """What a saved state holds for each parameter, in order ({} for nothing); ValueError where
+        it does not fit them."""
+        found, groups = [], state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return found  # (torch refuses it)
+        for group, saved in zip(self.param_groups, groups):
+            bits = saved.get("state_bits")
+            if bits not in _STATE:
+                raise ValueError(f"AdamW: state_bits of the saved groups must be 8 or 32 (got {bits})")
+            for p, index in zip(group["params"], saved["params"]):
+                got = state_dict["state"].get(index)
+                found.append({})
                 if not got:
                     continue
-                for key, dtype in want.items():
+                if "step" not in got:
+                    raise ValueError("AdamW: a saved state has no step")
+                found[-1]["step"] = int(got["step"])
+                for key, dtype in _STATE[bits].items():
                     t = got.get(key)
                     if not isinstance(t, torch.Tensor) or t.dtype != dtype or \
-                            t.numel() != self._state_size(key, group["state_bits"], p):
+                            t.numel() != self._state_size(key, bits, p):
                         raise ValueError(f"AdamW: saved state {key} does not fit a parameter of "
-                                         f"shape {list(p.shape)} with {group['state_bits']}-bit states")
-                    self.state[p][key] = t.to(device=p.device).clone()
-                self.state[p]["step"] = int(got["step"])
+                                         f"shape {list(p.shape)} with {bits}-bit states")
+                    found[-1][key] = t
+        return found
 
     def step(self, closure=None, *, grad_scale=None):
         """One step, torch.optim.Optimizer.step semantics, hooks included.  ``grad_scale``: an
