@@ -91,11 +91,16 @@ class AdamW(Optimizer):
             raise ValueError(f"Invalid beta parameters: {betas}")
         if not weight_decay >= 0.0:
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
-        if state_bits not in _STATE:
-            raise ValueError(f"state_bits must be 8 or 32 (got {state_bits})")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=stochastic_rounding, seed=seed))
+
+    def add_param_group(self, param_group) -> None:
+        if isinstance(param_group, dict):  # (torch refuses anything else)
+            bits = param_group.get("state_bits", self.defaults["state_bits"])
+            if bits not in _STATE:
+                raise ValueError(f"state_bits must be 8 or 32 (got {bits})")
+        super().add_param_group(param_group)
 
     @staticmethod
     def _state_size(key: str, bits: int, p: torch.Tensor) -> int:

@@ -75,3 +75,13 @@ def test_hooks_may_change_the_state_that_is_loaded():
     assert (opt.state[w]["exp_avg"] == 2).all() and opt.state[w]["step"] == 7
     opt.load_state_dict(state)          # (as often as it is called)
     assert (opt.state[w]["exp_avg"] == 2).all()
+
+
+@pytest.mark.parametrize("later", [False, True])
+def test_state_bits_of_one_group_are_checked(later):
+    a, b = (torch.nn.Parameter(torch.ones(4)) for _ in range(2))
+    with pytest.raises(ValueError, match="state_bits"):
+        if later:
+            AdamW([a]).add_param_group(dict(params=[b], state_bits=16))
+        else:
+            AdamW([dict(params=[a]), dict(params=[b], state_bits=16)])
