@@ -158,17 +158,18 @@ __global__ __launch_bounds__(kRowThreads) void ln_dx_any_kernel(
     }
 }
 
-// sums[blockIdx.y] = dw and db of every gridDim.y-th 16 rows: 16 V columns to a workgroup.
+// sums[blockIdx.y] = dw and db of every gridDim.y-th 16 rows: 16 V columns to a workgroup, from
+// column c0 on.
 constexpr int kAnyRows = 16;
 template <int DT, int V>
 __global__ __launch_bounds__(kRowThreads) void ln_dw_any_kernel(const char* dy, int64_t lddy,
                                                                 const char* h, int64_t ldh,
                                                                 const float* stats, float* sums,
-                                                                int64_t N, int64_t D) {
+                                                                int64_t N, int64_t D, int64_t c0) {
     __shared__ float part[2 * V][kRowThreads];
     constexpr int S = kElemBytes<DT>;
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    const int64_t i = ((int64_t)blockIdx.x * 16 + x) * V;
+    const int64_t i = c0 + ((int64_t)blockIdx.x * 16 + x) * V;
     const Slot t = last_slot<V>(i, D);
     float sw[V] = {}, sb[V] = {}, a[V], n[V];
     if (i < D)
@@ -469,14 +470,14 @@ __global__ __launch_bounds__(T) void ln_bwd_kernel(
     }
 }
 
-// dw (blockIdx.y 0) and db (1) from the workgroups' sums: 64 columns a workgroup, 16 sums of
-// each side by side, joined in order.
+// dw (blockIdx.y 0) and db (1) from the workgroups' sums: 64 columns a workgroup, from column c0
+// on, 16 sums of each side by side, joined in order.
 template <int WT>
 __global__ __launch_bounds__(1024) void ln_sums_kernel(const float* __restrict__ sums, int blocks,
-                                                       void* dw, void* db, int64_t D) {
+                                                       void* dw, void* db, int64_t D, int64_t c0) {
     __shared__ float part[16][64];
     const int x = threadIdx.x & 63, k = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + x;
+    const int64_t c = c0 + (int64_t)blockIdx.x * 64 + x;
     void* out = blockIdx.y ? db : dw;
     float s = 0.f;
     if (c < D) {
@@ -561,6 +562,14 @@ int ln_rows(const char* fn, const char* what, const void* p, int64_t ld, int64_t
     return HASTE_OK;
 }
 
+// f(first, count) over launches of `count` rows or columns, `per` to a workgroup of `threads`: an axis
+// of a launch takes fewer than 2^32 threads.
+template <typename F>
+void in_launches(int64_t count, int64_t per, int threads, F f) {
+    const int64_t most = (((int64_t)1 << 32) - 1) / threads * per;
+    for (int64_t i = 0; i < count; i += most) f(i, std::min(most, count - i));
+}
+
 // f with C as a constant.
 template <typename F>
 void with_slots(int C, F f) {
@@ -611,34 +620,40 @@ extern "C" int haste_layer_norm(const void* x, int64_t ldx, const void* res, int
     HASTE_CHECK_ARG(haste::elem_aligned(stats, HASTE_DTYPE_F32), "%s: stats is misaligned", fn);
     const haste::RowShape r = haste::fwd_shape(D, dtype);
     const int threads = std::max(r.tpr, 256), rows = r.C ? threads / r.tpr : 1;
-    const dim3 grid((unsigned)haste::ceil_div(N, (int64_t)rows));
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool nt = haste::past_cache(N, D, dtype);
-    const char *xc = static_cast<const char*>(x), *rc = static_cast<const char*>(res);
-    char *yc = static_cast<char*>(y), *hc = static_cast<char*>(h);
-    auto any = [&](auto kernel) {
-        kernel<<<grid, dim3(haste::kRowThreads), 0, st>>>(xc, ldx, rc, ldres, w, b, yc, hc, stats, D,
-                                                          (float)eps);
-    };
-#define HASTE_LN_FWD(DT, WT)                                                                   \
-    do {                                                                                       \
-        auto slots = [&](auto c) {                                                             \
-            constexpr int C = decltype(c)::value;                                              \
-            if (nt)                                                                            \
-                haste::ln_fwd_kernel<DT, WT, C, true><<<grid, dim3(threads), 0, st>>>(         \
-                    xc, ldx, rc, ldres, w, b, yc, hc, stats, N, D, (float)eps, r.tpr);         \
-            else                                                                               \
-                haste::ln_fwd_kernel<DT, WT, C, false><<<grid, dim3(threads), 0, st>>>(        \
-                    xc, ldx, rc, ldres, w, b, yc, hc, stats, N, D, (float)eps, r.tpr);         \
-        };                                                                                     \
-        if (r.C)                                                                               \
-            haste::with_slots(r.C, slots);                                                     \
-        else                                                                                   \
-            any(D < haste::row_vec(DT) ? haste::ln_fwd_any_kernel<DT, WT, 1>                   \
-                                       : haste::ln_fwd_any_kernel<DT, WT, haste::row_vec(DT)>); \
+    haste::in_launches(N, rows, threads, [&](int64_t r0, int64_t n) {
+        const dim3 grid((unsigned)haste::ceil_div(n, (int64_t)rows));
+        const int64_t size = haste::elem_bytes(dtype);
+        const char *xc = static_cast<const char*>(x) + r0 * ldx * size,
+                   *rc = res ? static_cast<const char*>(res) + r0 * ldres * size : nullptr;
+        char *yc = static_cast<char*>(y) + r0 * D * size,
+             *hc = res ? static_cast<char*>(h) + r0 * D * size : nullptr;
+        float* sc = stats ? stats + 2 * r0 : nullptr;
+        auto any = [&](auto kernel) {
+            kernel<<<grid, dim3(haste::kRowThreads), 0, st>>>(xc, ldx, rc, ldres, w, b, yc, hc, sc, D,
+                                                              (float)eps);
+        };
+#define HASTE_LN_FWD(DT, WT)                                                                       \
+    do {                                                                                           \
+        auto slots = [&](auto c) {                                                                 \
+            constexpr int C = decltype(c)::value;                                                  \
+            if (nt)                                                                                \
+                haste::ln_fwd_kernel<DT, WT, C, true><<<grid, dim3(threads), 0, st>>>(             \
+                    xc, ldx, rc, ldres, w, b, yc, hc, sc, n, D, (float)eps, r.tpr);                \
+            else                                                                                   \
+                haste::ln_fwd_kernel<DT, WT, C, false><<<grid, dim3(threads), 0, st>>>(            \
+                    xc, ldx, rc, ldres, w, b, yc, hc, sc, n, D, (float)eps, r.tpr);                \
+        };                                                                                         \
+        if (r.C)                                                                                   \
+            haste::with_slots(r.C, slots);                                                         \
+        else                                                                                       \
+            any(D < haste::row_vec(DT) ? haste::ln_fwd_any_kernel<DT, WT, 1>                       \
+                                       : haste::ln_fwd_any_kernel<DT, WT, haste::row_vec(DT)>);    \
     } while (0)
-    HASTE_LN_TYPES(HASTE_LN_FWD);
+        HASTE_LN_TYPES(HASTE_LN_FWD);
 #undef HASTE_LN_FWD
+    });
     HASTE_CHECK_LAUNCH(fn);
     return HASTE_OK;
 }
@@ -689,14 +704,26 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
     const char *dyc = static_cast<const char*>(dy), *dhc = static_cast<const char*>(dh),
                *hc = static_cast<const char*>(h);
     float* sums = dw || db ? static_cast<float*>(ws) : nullptr;
-    const dim3 columns((unsigned)haste::ceil_div(D, 64), 2);
     auto any_dx = [&](auto kernel) {
-        kernel<<<dim3((unsigned)N), dim3(haste::kRowThreads), 0, st>>>(
-            dyc, lddy, dhc, lddh, hc, ldh, w, stats, static_cast<char*>(dx), D);
+        haste::in_launches(N, 1, haste::kRowThreads, [&](int64_t r0, int64_t n) {
+            const int64_t size = haste::elem_bytes(dtype);
+            kernel<<<dim3((unsigned)n), dim3(haste::kRowThreads), 0, st>>>(
+                dyc + r0 * lddy * size, lddy, dhc ? dhc + r0 * lddh * size : nullptr, lddh,
+                hc + r0 * ldh * size, ldh, w, stats + 2 * r0,
+                static_cast<char*>(dx) + r0 * D * size, D);
+        });
     };
     auto any_dw = [&](auto kernel, int V) {
-        kernel<<<dim3((unsigned)haste::ceil_div(D, (int64_t)16 * V), blocks),
-                 dim3(haste::kRowThreads), 0, st>>>(dyc, lddy, hc, ldh, stats, sums, N, D);
+        haste::in_launches(D, 16 * V, haste::kRowThreads, [&](int64_t c0, int64_t n) {
+            kernel<<<dim3((unsigned)haste::ceil_div(n, (int64_t)16 * V), blocks),
+                     dim3(haste::kRowThreads), 0, st>>>(dyc, lddy, hc, ldh, stats, sums, N, D, c0);
+        });
+    };
+    auto join = [&](auto kernel) {
+        haste::in_launches(D, 64, 1024, [&](int64_t c0, int64_t n) {
+            kernel<<<dim3((unsigned)haste::ceil_div(n, 64), 2), dim3(1024), 0, st>>>(sums, blocks, dw,
+                                                                                   db, D, c0);
+        });
     };
 #define HASTE_LN_BWD(DT, WT)                                                                     \
     do {                                                                                         \
@@ -727,8 +754,7 @@ extern "C" int haste_layer_norm_bwd(const void* dy, int64_t lddy, const void* dh
             else if (sums)                                                                       \
                 any_dw(haste::ln_dw_any_kernel<DT, V>, V);                                       \
         }                                                                                        \
-        if (sums)                                                                                \
-            haste::ln_sums_kernel<WT><<<columns, dim3(1024), 0, st>>>(sums, blocks, dw, db, D);  \
+        if (sums) join(haste::ln_sums_kernel<WT>);                                               \
     } while (0)
     HASTE_LN_TYPES(HASTE_LN_BWD);
 #undef HASTE_LN_BWD
