@@ -33,6 +33,7 @@ struct AdamArgs {
     float lr_wd, lr, rcorr, eps;  // lr wd, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
     uint32_t k0, k1;
     int32_t do_sr;
+    uint32_t blk0;  // first workgroup of the launch among those of its tensors
     const float* grad_scale;
 };
 
@@ -418,10 +419,11 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamBatch b, cons
         gs = *a.grad_scale;
         if (gs != gs) return;
     }
-    const int t = find_seg(b, blockIdx.x);
+    const uint32_t blk = a.blk0 + blockIdx.x;
+    const int t = find_seg(b, blk);
     const AdamSeg& s = b.s[t];
     const int64_t n = (int64_t)(s.n_stream & 0xFFFFFFFFFFull);
-    const int64_t i0 = (int64_t)(blockIdx.x - b.blk0[t]) * kPiece;
+    const int64_t i0 = (int64_t)(blk - b.blk0[t]) * kPiece;
     Elems x;
     if (i0 + kPiece <= n) {
         x.template fetch<true>(s, i0, n);
@@ -538,8 +540,10 @@ __global__ __launch_bounds__(kFinalThreads) void grad_norm_final_kernel(const do
     out[1] = norm < INFINITY ? fminf(1.f, max_norm / (norm + 1e-6f)) : NAN;
 }
 
+constexpr int64_t kMostBlocks = (((int64_t)1 << 32) - 1) / kThreads;  // (a launch takes 2^32 - 1 threads)
+
 template <int WT, int GT, bool Q8>
-int launch_adamw(const haste_adamw_tensor* ts, int count, const AdamArgs& a, hipStream_t st) {
+int launch_adamw(const haste_adamw_tensor* ts, int count, AdamArgs a, hipStream_t st) {
     for (int base = 0; base < count;) {
         AdamBatch b;
         b.count = 0;
@@ -554,8 +558,12 @@ int launch_adamw(const haste_adamw_tensor* ts, int count, const AdamArgs& a, hip
             HASTE_CHECK_ARG(blocks < (int64_t)1 << 31, "haste_adamw_step: tensors too large");
         }
         if (b.count == 0) break;
-        adamw_kernel<WT, GT, Q8><<<dim3((unsigned)blocks), dim3(kThreads), 0, st>>>(b, a);
-        HASTE_CHECK_LAUNCH("haste_adamw_step");
+        for (int64_t at = 0; at < blocks; at += kMostBlocks) {
+            a.blk0 = (uint32_t)at;
+            const unsigned grid = (unsigned)std::min(blocks - at, kMostBlocks);
+            adamw_kernel<WT, GT, Q8><<<dim3(grid), dim3(kThreads), 0, st>>>(b, a);
+            HASTE_CHECK_LAUNCH("haste_adamw_step");
+        }
     }
     return HASTE_OK;
 }

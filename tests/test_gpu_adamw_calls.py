@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+import adamw_reference as ref
 from haste_amd.optim_adamw import AdamW, grad_norm
 
 pytestmark = pytest.mark.gpu
@@ -188,3 +189,27 @@ def test_groups_draw_for_themselves(dev, bits, plain):
         for i in range(4):
             for j in range(i):
                 assert not torch.equal(ps[i], ps[j]), (k, i, j)
+
+
+def test_2_35_elements(dev):
+    """More than the 2^32 threads of one launch, 8 elements to each: the weights where the second
+    launch begins and at the end.  (Gradients are the weights' own memory, to have room.)"""
+    n = 2 ** 35 + 4173
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(dev)[0] < 160 * 2 ** 30:
+        pytest.skip("needs 160 GiB")
+    p = torch.nn.Parameter(torch.full((n,), 0.5, dtype=torch.bfloat16, device=dev))
+    p.grad = p.detach()
+    opt = AdamW([p], lr=1e-2, state_bits=8, seed=31)
+    opt.step()
+    zero = np.zeros(6000)
+    for at in (0, (2 ** 24 - 1) * 2048 - 3000, n - 6000):
+        w = ref.step(zero + 0.5, zero + 0.5, zero, zero, 1, 1e-2, 0.9, 0.999, 1e-8, 0.01)[0]
+        i = np.arange(at, at + 6000)
+        want, unit = ref.cut(w, ref.draws(i, 8, 0, 31)[0] / 65536.0, 7, -126)
+        got = p.detach()[at: at + 6000].double().cpu().numpy()
+        # fp32 is off by some 20 u of the change, 2^-16 of a spacing: a draw in 2^16 at most differs
+        assert (np.abs(got - want) <= 1.01 * unit).all() and (got != want).sum() <= 6, at
+    codes = opt.state[p]["exp_avg"].view(torch.uint8)
+    assert all((c != 0).all() for c in (codes[:n][-10 ** 6:], codes[: 10 ** 6])) and not codes[n:].any()
+    del p.grad
