@@ -186,7 +186,7 @@ __device__ __forceinline__ void sub4_towards_zero(float* w, const float* t) {
         "v_sub_f32 %2, %2, %6\n\t"
         "v_sub_f32 %3, %3, %7\n\t"
         "s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 0"
-        : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])
+        : "+&v"(w[0]), "+&v"(w[1]), "+&v"(w[2]), "+&v"(w[3])  // (written before all of t is read)
         : "v"(t[0]), "v"(t[1]), "v"(t[2]), "v"(t[3]));
 }
 
