@@ -405,9 +405,9 @@ struct AdamElems8 {
 };
 
 // Every byte is met once, and HBM bounds it.  32-bit states: 91 M bf16 weights of 195 tensors take
-// 306 us for 2.0 GB, 6.5 TB/s with the gradients that the norm before has left in the last-level
-// cache.  8-bit states: 670 M weights take 1040 us for 6.7 GB, 6.4 TB/s, at 46 vector instructions
-// an element (10 of them Philox), which keep the vector units 85 % busy; at 55 it took 1068.  All
+// 298 us for 2.0 GB, 6.7 TB/s with the gradients that the norm before has left in the last-level
+// cache.  8-bit states: 670 M weights take 1051 us for 6.7 GB, 6.4 TB/s, at 49 vector instructions
+// an element (10 of them Philox), which keep the vector units 88 % busy; at 55 it took 1068.  All
 // accesses are non-temporal (but 8-wide ones of fp32, of which each touches half a line), so that
 // what is met once and dirty lines do not drive those gradients out: with the norm, 8-bit
 // 221 -> 188 us and 1497 -> 1350, 32-bit 424 -> 345.
@@ -493,7 +493,7 @@ __device__ __forceinline__ double piece_squares(const void* g, int64_t i0, int64
 
 // part[workgroup] = the sum of squares of every gridDim-th piece, the launch's last pieces first:
 // the first tensors' gradients are then what the last-level cache holds when a step reads them
-// again from the start.  Bound by HBM: 1.34 GB of bf16 in 225 us, 6.0 TB/s; 182 MB of 195
+// again from the start.  Bound by HBM: 1.34 GB of bf16 in 223 us, 6.0 TB/s; 182 MB of 195
 // tensors in 32 us, in one launch (in four of 64 tensors each 60 us).
 __global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const GradBatch b, double* part) {
     __shared__ double sums[kNormThreads / 64];

@@ -584,7 +584,8 @@ int haste_rewire_ex(void* W, int32_t w_dtype, int32_t* idx, const void* grad, in
  * y and h are [N, D] contiguous.  dtype of x, res, y, h: bf16, f16 or f32; w_dtype of w
  * and b: the same or f32.  res, b may be NULL; h is required with res and unused
  * without.  stats [N, 2] (mean, rstd) is written where not NULL.  Element
- * alignment is enough for every tensor.  Outputs must not overlap inputs or each other.
+ * alignment is enough for every tensor.  Outputs must not overlap inputs or each other.  A row
+ * whose sum passes fp32's range gives NaN, one whose squared spread does gives b.
  */
 int haste_layer_norm(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w,
                      const void* b, void* y, void* h, float* stats, int64_t N, int64_t D,
@@ -629,10 +630,9 @@ int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, double max_
  *   g  = grad * (*grad_scale)              (1 where grad_scale is NULL)
  *   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2
  *   w' = w (1 - lr wd) - lr / (1 - beta1^step) m' / (sqrt(v' / (1 - beta2^step)) + eps)
- * in fp32 (the root of a v' below 2^-126 counts as 0).  Where *grad_scale is NaN the kernels
- * change nothing.  w_dtype and g_dtype: bf16,
- * f16 or f32 for all of the call's tensors.  With do_sr 16-bit weights are rounded
- * stochastically, else to nearest.
+ * in fp32 (the root of a v' below 2^-126 counts as 0; lr wd < 1 where w is infinite).  Where
+ * *grad_scale is NaN the kernels change nothing.  w_dtype and g_dtype: bf16, f16 or f32 for all
+ * of the call's tensors.  With do_sr 16-bit weights are rounded stochastically, else to nearest.
  * state_bits 32: m and v are fp32 [n], m_scale and v_scale unused.
  * state_bits 8: m holds m and v holds u = sqrt(v), both as e4m3 codes [ceil(n / 128) * 128] with
  * one E8M0 scale (2^(code - 127)) for each 128 elements in m_scale and v_scale
@@ -646,7 +646,8 @@ int haste_grad_norm(const haste_grad_tensor* tensors, int32_t count, double max_
  * what is cut off, in units of the result's last place, plus r / 2^16 (f16 weights: the upper 13
  * bits of r over 2^13) reaches 1.
  * w and g need the alignment of their elements, m and v 16 bytes (8-bit: 8 bytes); n is below
- * 2^40 and stream below 2^24.  n == 0 entries are skipped.  One launch for each 64 tensors.
+ * 2^40 and stream below 2^24.  n == 0 entries are skipped.  One launch for each 64 tensors (more
+ * from 2^35 elements on).
  */
 typedef struct haste_adamw_tensor {
     void* w;
