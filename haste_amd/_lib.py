@@ -149,6 +149,21 @@ SIGNATURES = {
     "haste_grad_norm": (ctypes.c_int, [_P, _I32, _F64, _P, _P, _I64, _P]),
     "haste_adamw_step": (ctypes.c_int, [_P, _I32, _I32, _I32, _I32, _F64, _F64, _F64, _F64, _F64,
                                         _I64, _I32, _U64, _P, _P]),
+    "haste_embedding": (ctypes.c_int, [_P, _I32, _P, _I64, _P, _I64, _I64, _I64, _F64, _I32, _P]),
+    "haste_embedding_bwd_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "haste_embedding_bwd": (ctypes.c_int, [_P, _I32, _P, _I64, _P, _I64, _I64, _I64, _F64, _I64, _I32,
+                                           _P, _I64, _P]),
+    "haste_gated_mlp_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I32, _I32, _I32]),
+    "haste_gated_mlp": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64,
+                                       _I64, _I64, _I64, _I32, _I32, _P, _I64, _P]),
+    "haste_gated_mlp_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P,
+                                           _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32,
+                                           _P, _I64, _P]),
+    "haste_label_log_probs_workspace_size": (_I64, [_I64, _I64, _I32]),
+    "haste_label_log_probs": (ctypes.c_int, [_P, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _I64, _I64,
+                                             _I32, _I32, _P, _I64, _P]),
+    "haste_label_log_probs_bwd": (ctypes.c_int, [_P, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _I64,
+                                                 _I64, _I64, _I32, _P]),
 }
 
 _lib = None

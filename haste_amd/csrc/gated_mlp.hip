@@ -1,0 +1,485 @@
+// The gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wd^T, and its gradients (gated_mlp.hpp has
+// the formulas).  Bound by its matrix products: 6 N D H operations forward, 12 N D H backward, as
+//   forward   [g | u] with h in the epilogue;  y
+//   backward  dh with dg and du in the epilogue;  dx over both;  dWg and dWu;  dWd
+// A few tokens in serving are bound by reading the weights once and take kernels of their own.
+#include <algorithm>
+
+#include "gated_mlp.hpp"
+#include "gemm.hpp"
+
+namespace haste {
+namespace {
+
+template <typename Tile, int DT, typename Epilogue>
+__global__ __launch_bounds__(Tile::kThreads, 2) void gemm_kernel(GemmArgs g, int batches, int act,
+                                                                 Epilogue out) {
+    __shared__ __attribute__((aligned(16))) char lds[Tile::kLdsBytes];
+    GemmPlace p;
+    if (!gemm_place(g, batches, &p)) return;
+    Tile t;
+    t.run(g, lds, p.tm, p.tn, p.batch, p.split);
+    const int lane = threadIdx.x & 63;
+    auto rows = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int fm = 0; fm < Tile::FM; ++fm) {
+            const int m = t.m0 + fm * 16 + (lane & 15);
+            if (m < g.M) f(fm, m);
+        }
+    };
+    if constexpr (std::is_same<Epilogue, PlainOut>::value) {
+        rows([&](int fm, int m) __attribute__((always_inline)) {
+#pragma unroll
+            for (int fn = 0; fn < Tile::FN; ++fn) {
+                const int n = t.n0 + fn * 16 + 4 * (lane >> 4);
+                if (n < g.N) out.template put<DT>(p.split, p.batch, m, n, t.acc[fn][fm]);
+            }
+        });
+    } else {
+        with_activation(act, [&](auto a) __attribute__((always_inline)) {
+            constexpr int ACT = decltype(a)::value;
+            rows([&](int fm, int m) __attribute__((always_inline)) {
+                constexpr int F = Tile::kDual ? Tile::FN / 2 : Tile::FN;
+#pragma unroll
+                for (int fn = 0; fn < F; ++fn) {
+                    const int n = t.n0 + fn * 16 + 4 * (lane >> 4);
+                    if (n >= out.ld) continue;
+                    if constexpr (Tile::kDual)
+                        out.template put<DT, ACT>(m, n, t.acc[fn][fm], t.acc[fn + F][fm]);
+                    else
+                        out.template put<DT, ACT>(m, n, t.acc[fn][fm]);
+                }
+            });
+        });
+    }
+}
+
+// --------------------------------------------------------------- a few rows ----
+// Up to 16 NG rows of x against 16 rows of the weights (of both, DUAL): the waves share K, and read
+// the weights straight into registers, at any alignment.
+template <typename T, int NG, bool DUAL, int WAVES, typename Epilogue>
+__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int64_t ldx,
+                                                             const char* w0, int64_t ldw0,
+                                                             const char* w1, int64_t ldw1, int M, int N,
+                                                             int K, int act, Epilogue out) {
+    constexpr int DT = T::code, NW = DUAL ? 2 : 1;
+    __shared__ f32x4 sums[WAVES][NG * NW][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15;
+    const int n = blockIdx.x * 16 + r;
+    const char* w[2] = {w0 + (int64_t)min(n, N - 1) * ldw0 * 2, DUAL ? w1 + (int64_t)min(n, N - 1) * ldw1 * 2 : w0};
+    f32x4 acc[NG * NW];
+#pragma unroll
+    for (int i = 0; i < NG * NW; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto piece = [](const char* p, int64_t i, int64_t count) __attribute__((always_inline)) {
+        const Elems<DT, 8> v = load_part<DT, 8>(p, i, count);
+        return u32x4{v.q[0], v.q[1], v.q[2], v.q[3]};
+    };
+#pragma unroll 4
+    for (int k0 = wave * 32; k0 < K; k0 += 32 * WAVES) {
+        const int k = k0 + 8 * (lane >> 4);
+        u32x4 fw[NW], fx[NG];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) fw[i] = piece(w[i], k, n < N ? K - k : 0);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+            fx[i] = piece(x + (int64_t)(16 * i + r) * ldx * 2, k, 16 * i + r < M ? K - k : 0);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int j = 0; j < NW; ++j) acc[i * NW + j] = mfma16x16x32<T>(fw[j], fx[i], acc[i * NW + j]);
+    }
+#pragma unroll
+    for (int i = 0; i < NG * NW; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < NG; i += WAVES) {
+        f32x4 s[NW];
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+            s[j] = sums[0][i * NW + j][lane];
+            for (int v = 1; v < WAVES; ++v) s[j] += sums[v][i * NW + j][lane];
+        }
+        const int m = 16 * i + r, col = blockIdx.x * 16 + 4 * (lane >> 4);
+        if (m >= M) continue;
+        if constexpr (DUAL) {
+            if (col < out.ld)
+                with_activation(act, [&](auto a) __attribute__((always_inline)) {
+                    out.template put<DT, decltype(a)::value>(m, col, s[0], s[1]);
+                });
+        } else {
+            if (col < N) out.template put<DT>(0, 0, m, col, s[0]);
+        }
+    }
+}
+
+// Rows [R, C] of any pitch as rows of P (a multiple of 8) elements on 16 bytes, with zeros behind C.
+__global__ __launch_bounds__(256) void pack_rows_kernel(const char* src, int64_t ld, char* dst, int64_t R,
+                                                        int64_t C, int64_t P) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pieces = P / 8;
+    if (i >= R * pieces) return;
+    const int64_t r = i / pieces, c = i % pieces * 8;
+    const Elems<HASTE_DTYPE_BF16, 8> v =
+        load_part<HASTE_DTYPE_BF16, 8>(src + r * ld * 2, c, C - c);
+    store<HASTE_DTYPE_BF16, 8>(dst, r * P + c, v);
+}
+
+// ------------------------------------------------------------------ host ----
+constexpr int64_t kMaxSide = (int64_t)1 << 20;  // a tile's rows span less than 2^31 bytes
+constexpr int kFewRows = 64;
+
+int64_t round8(int64_t n) { return ceil_div(n, 8) * 8; }
+
+// A matrix as the kernels take it.
+struct Matrix {
+    const void* p;
+    int64_t ld, rows, cols;
+};
+bool plain_rows(const Matrix& m) { return aligned16(m.p) && m.ld % 8 == 0 && m.cols % 8 == 0; }
+
+// The workspace's places, handed out in order.
+struct Space {
+    char* base;
+    int64_t used = 0;
+    void* take(int64_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += ceil_div(bytes, 256) * 256;
+        return p;
+    }
+};
+
+struct Product {
+    Matrix a[2], b[2];  // two of each where the mode has two
+    int64_t M, N, K;
+};
+
+template <int DT>
+struct TypeOf;
+template <>
+struct TypeOf<HASTE_DTYPE_BF16> {
+    typedef BF16 type;
+};
+template <>
+struct TypeOf<HASTE_DTYPE_F16> {
+    typedef F16 type;
+};
+
+template <typename Tile>
+GemmArgs gemm_args(const Product& p, int segments, int splits) {
+    GemmArgs g{};
+    for (int i = 0; i < 2; ++i) {
+        g.a.base[i] = static_cast<const char*>(p.a[i].p);
+        g.b.base[i] = static_cast<const char*>(p.b[i].p);
+    }
+    g.a.ld = p.a[0].ld;
+    g.b.ld = p.b[0].ld;
+    g.M = (int)p.M;
+    g.N = (int)p.N;
+    g.K = (int)p.K;
+    g.tiles_m = (int)ceil_div(p.M, Tile::BM);
+    g.tiles_n = (int)ceil_div(p.N, Tile::kCols);
+    g.steps = (int)ceil_div(p.K, Tile::KS);
+    g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, (int64_t)g.steps * segments));
+    return g;
+}
+
+template <typename Tile, int DT, typename Epilogue>
+void launch_tiles(const GemmArgs& g, int batches, int act, const Epilogue& out, hipStream_t st) {
+    const int64_t n = (int64_t)g.tiles_m * g.tiles_n * batches * g.splits;
+    gemm_kernel<Tile, DT, Epilogue><<<dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(Tile::kThreads), 0, st>>>(
+        g, batches, act, out);
+}
+
+// Tiles of 256 x 256 where they fill the GPU's 256 CUs, else of 128 x 128, two workgroups to a CU.
+template <GemmMode MODE>
+bool large_tiles(const Product& p) {
+    const int64_t cols = MODE == GemmMode::kDual ? 128 : 256, batches = MODE == GemmMode::kBatch ? 2 : 1;
+    return ceil_div(p.M, 256) * ceil_div(p.N, cols) * batches >= 192;
+}
+// Parts of K, where the tiles alone leave the GPU idle: at least eight steps to a part.
+template <GemmMode MODE, int DT>
+int splits_of(const Product& p) {
+    const bool large = DT != HASTE_DTYPE_F32 && large_tiles<MODE>(p);
+    const int64_t side = large ? 256 : 128, batches = MODE == GemmMode::kBatch ? 2 : 1;
+    const int64_t tiles = ceil_div(p.M, side) * ceil_div(p.N, side) * batches;
+    const int64_t steps = ceil_div(p.K, 32) * (MODE == GemmMode::kSegments ? 2 : 1);
+    if (large || tiles == 0) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / 8));
+}
+
+template <int DT, GemmMode MODE, bool AK, bool BK_, typename Epilogue>
+void product(const Product& p, int splits, int act, const Epilogue& out, hipStream_t st) {
+    constexpr int batches = MODE == GemmMode::kBatch ? 2 : 1, segments = MODE == GemmMode::kSegments ? 2 : 1;
+    if constexpr (DT == HASTE_DTYPE_F32) {
+        typedef GemmTileF32<MODE, AK, BK_> Tile;
+        launch_tiles<Tile, DT>(gemm_args<Tile>(p, segments, splits), batches, act, out, st);
+    } else {
+        typedef typename TypeOf<DT>::type T;
+        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4> Large;
+        typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2> Small;
+        if (large_tiles<MODE>(p))
+            launch_tiles<Large, DT>(gemm_args<Large>(p, segments, splits), batches, act, out, st);
+        else
+            launch_tiles<Small, DT>(gemm_args<Small>(p, segments, splits), batches, act, out, st);
+    }
+}
+
+// A product without an epilogue, its parts of K joined by a second launch.  `parts` has room for
+// plain_parts() bytes.
+template <int DT, GemmMode MODE>
+int64_t plain_parts(const Product& p) {
+    const int splits = splits_of<MODE, DT>(p);
+    return splits == 1 ? 0
+                       : splits * (MODE == GemmMode::kBatch ? 2 : 1) * p.M * (ceil_div(p.N, 4) * 4) * 4;
+}
+template <int DT, GemmMode MODE, bool AK, bool BK_>
+void plain(const Product& p, void* c0, void* c1, void* parts, hipStream_t st) {
+    const int splits = splits_of<MODE, DT>(p);
+    PlainOut out{{c0, c1}, p.N, splits > 1 ? static_cast<float*>(parts) : nullptr, (int)p.M, (int)p.N,
+                 MODE == GemmMode::kBatch ? 2 : 1};
+    product<DT, MODE, AK, BK_>(p, splits, 0, out, st);
+    if (splits > 1) {
+        const int64_t n = out.batches * p.M * ceil_div(p.N, 4);
+        sum_parts_kernel<DT><<<dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st>>>(out, splits);
+    }
+}
+
+struct Sizes {
+    int64_t N, D, H, O;
+};
+
+// A matrix with 16-byte rows: itself, or a copy in the workspace.
+template <int DT>
+Matrix packed(const Matrix& m, Space& ws, bool launch, hipStream_t st) {
+    if (DT == HASTE_DTYPE_F32 || plain_rows(m)) return m;
+    const int64_t P = round8(m.cols);
+    void* to = ws.take(m.rows * P * 2);
+    if (launch && m.rows > 0) {
+        const int64_t n = m.rows * (P / 8);
+        pack_rows_kernel<<<dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st>>>(
+            static_cast<const char*>(m.p), m.ld, static_cast<char*>(to), m.rows, m.cols, P);
+    }
+    return Matrix{to, P, m.rows, m.cols};
+}
+// Wg and Wu share a pitch in the kernels.
+template <int DT>
+void packed_pair(Matrix& g, Matrix& u, Space& ws, bool launch, hipStream_t st) {
+    if (DT != HASTE_DTYPE_F32) {
+        g = packed<DT>(g, ws, launch, st);
+        u = packed<DT>(u, ws, launch, st);
+    }
+}
+
+template <int DT>
+int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const GatedOut& out, void* y,
+                int act, char* base, bool launch, hipStream_t st) {
+    Space ws{base};
+    if constexpr (DT != HASTE_DTYPE_F32) {
+        if (s.N <= kFewRows) {
+            if (!launch) return 0;
+            typedef typename TypeOf<DT>::type T;
+            const char *xc = static_cast<const char*>(x.p), *gc = static_cast<const char*>(wg.p),
+                       *uc = static_cast<const char*>(wu.p), *dc = static_cast<const char*>(wd.p),
+                       *hc = static_cast<const char*>(out.h);
+            const dim3 g1((unsigned)ceil_div(out.ld, 16)), g2((unsigned)ceil_div(s.O, 16));
+            const PlainOut po{{y, nullptr}, s.O, nullptr, (int)s.N, (int)s.O, 1};
+            auto run = [&](auto groups) {
+                constexpr int NG = decltype(groups)::value;
+                few_rows_kernel<T, NG, true, 8, GatedOut><<<g1, dim3(512), 0, st>>>(
+                    xc, x.ld, gc, wg.ld, uc, wu.ld, (int)s.N, (int)s.H, (int)s.D, act, out);
+                few_rows_kernel<T, NG, false, 8, PlainOut><<<g2, dim3(512), 0, st>>>(
+                    hc, out.ld, dc, wd.ld, nullptr, 0, (int)s.N, (int)s.O, (int)s.H, 0, po);
+            };
+            if (s.N <= 16) run(std::integral_constant<int, 1>());
+            else if (s.N <= 32) run(std::integral_constant<int, 2>());
+            else run(std::integral_constant<int, 4>());
+            return 0;
+        }
+    }
+    x = packed<DT>(x, ws, launch, st);
+    packed_pair<DT>(wg, wu, ws, launch, st);
+    wd = packed<DT>(wd, ws, launch, st);
+    const Matrix h{out.h, out.ld, s.N, s.H};
+    const Product p1{{x, x}, {wg, wu}, s.N, s.H, s.D};
+    const Product p2{{h, h}, {wd, wd}, s.N, s.O, s.H};
+    void* parts = ws.take(plain_parts<DT, GemmMode::kPlain>(p2));
+    if (launch) {
+        product<DT, GemmMode::kDual, true, true>(p1, 1, act, out, st);
+        plain<DT, GemmMode::kPlain, true, true>(p2, y, nullptr, parts, st);
+    }
+    return ws.used;
+}
+
+struct Grads {
+    void *dx, *dwg, *dwu, *dwd;
+};
+
+template <int DT>
+int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matrix dy, const void* g,
+                 const void* u, const void* h, int64_t ld, const Grads& to, int act, char* base,
+                 bool launch, hipStream_t st) {
+    Space ws{base};
+    const int64_t bytes = s.N * ld * elem_bytes(DT);
+    void *dg = ws.take(bytes), *du = ws.take(bytes);
+    x = packed<DT>(x, ws, launch && (to.dwg || to.dwu), st);
+    packed_pair<DT>(wg, wu, ws, launch && to.dx, st);
+    wd = packed<DT>(wd, ws, launch, st);
+    dy = packed<DT>(dy, ws, launch, st);
+    const Matrix mg{dg, ld, s.N, s.H}, mu{du, ld, s.N, s.H}, mh{h, ld, s.N, s.H};
+    const Product p1{{dy, dy}, {wd, wd}, s.N, s.H, s.O};
+    const Product p2{{mg, mu}, {wg, wu}, s.N, s.D, s.H};
+    const Product p3{{mg, mu}, {x, x}, s.H, s.D, s.N};
+    const Product p4{{dy, dy}, {mh, mh}, s.O, s.H, s.N};
+    void* parts = ws.take(std::max({plain_parts<DT, GemmMode::kSegments>(p2),
+                                    plain_parts<DT, GemmMode::kBatch>(p3),
+                                    plain_parts<DT, GemmMode::kPlain>(p4)}));
+    if (launch) {
+        if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
+            const GatedGrad out{g, u, dg, du, ld};
+            product<DT, GemmMode::kPlain, true, false>(p1, 1, act, out, st);
+        }
+        if (s.N > 0 && to.dx) plain<DT, GemmMode::kSegments, true, false>(p2, to.dx, nullptr, parts, st);
+        if (to.dwg || to.dwu) plain<DT, GemmMode::kBatch, false, false>(p3, to.dwg, to.dwu, parts, st);
+        if (to.dwd) plain<DT, GemmMode::kPlain, false, false>(p4, to.dwd, nullptr, parts, st);
+    }
+    return ws.used;
+}
+
+// `call` with DT.
+#define HASTE_MLP_TYPES(call)                              \
+    (dtype == HASTE_DTYPE_F32    ? call(HASTE_DTYPE_F32)   \
+     : dtype == HASTE_DTYPE_BF16 ? call(HASTE_DTYPE_BF16)  \
+                                 : call(HASTE_DTYPE_F16))
+
+int mlp_sizes(const char* fn, int64_t N, int64_t D, int64_t H, int64_t O, int32_t dtype) {
+    HASTE_CHECK_ARG(N >= 0 && D > 0 && H > 0 && O > 0, "%s: bad sizes N=%lld D=%lld H=%lld O=%lld", fn,
+                    (long long)N, (long long)D, (long long)H, (long long)O);
+    HASTE_CHECK_ARG(D <= kMaxSide && H <= kMaxSide && O <= kMaxSide && N < (int64_t)1 << 30,
+                    "%s: too large (D, H and O up to 2^20, N below 2^30)", fn);
+    HASTE_CHECK_ARG(elem_dtype(dtype), "%s: matrices must be bf16, f16 or f32", fn);
+    return HASTE_OK;
+}
+int mlp_matrix(const char* fn, const char* what, const Matrix& m, int32_t dtype) {
+    HASTE_CHECK_ARG(m.p != nullptr && elem_aligned(m.p, dtype), "%s: %s is NULL or misaligned", fn, what);
+    HASTE_CHECK_ARG(m.ld >= m.cols && m.ld <= 4 * kMaxSide, "%s: row pitch of %s (%lld) must be %lld to 2^22",
+                    fn, what, (long long)m.ld, (long long)m.cols);
+    return HASTE_OK;
+}
+int mlp_hidden(const char* fn, const char* what, const void* p) {
+    HASTE_CHECK_ARG(p != nullptr && aligned16(p), "%s: %s is NULL or misaligned", fn, what);
+    return HASTE_OK;
+}
+int mlp_space(const char* fn, const void* ws, int64_t have, int64_t need) {
+    HASTE_CHECK_ARG(need == 0 || (ws != nullptr && aligned16(ws)), "%s: workspace is NULL or misaligned", fn);
+    if (have < need) {
+        set_error("%s: workspace too small (%lld < %lld bytes)", fn, (long long)have, (long long)need);
+        return HASTE_ERR_WORKSPACE;
+    }
+    return HASTE_OK;
+}
+int mlp_act(const char* fn, int32_t act) {
+    HASTE_CHECK_ARG(act == HASTE_ACT_SILU || act == HASTE_ACT_GELU || act == HASTE_ACT_GELU_TANH,
+                    "%s: unknown activation %d", fn, (int)act);
+    return HASTE_OK;
+}
+
+#define HASTE_TRY(expr)                  \
+    do {                                 \
+        const int rc_ = (expr);          \
+        if (rc_ != HASTE_OK) return rc_; \
+    } while (0)
+
+}  // namespace
+}  // namespace haste
+
+extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t H, int64_t O,
+                                                  int32_t dtype, int32_t backward,
+                                                  int32_t aligned) {
+    HASTE_TRY(haste::mlp_sizes("haste_gated_mlp_workspace_size", N, D, H, O, dtype));
+    const haste::Sizes s{N, D, H, O};
+    const int64_t ld = haste::round8(H);
+    // (an odd pitch: the matrix counts as one to be copied)
+    auto any = [&](int64_t rows, int64_t cols) {
+        return haste::Matrix{nullptr, aligned ? cols : cols | 1, rows, cols};
+    };
+    const haste::Matrix x = any(N, D), wg = any(H, D), wd = any(O, H), dy = any(N, O);
+#define HASTE_MLP(DT)                                                                                   \
+    (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, nullptr, ld, haste::Grads{}, \
+                                    0, nullptr, false, nullptr)                                          \
+              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{nullptr, nullptr, nullptr, ld},     \
+                                   nullptr, 0, nullptr, false, nullptr))
+    return HASTE_MLP_TYPES(HASTE_MLP);
+#undef HASTE_MLP
+}
+
+extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
+                               int64_t ldu, const void* wd, int64_t ldd, void* y, void* g, void* u,
+                               void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
+                               int32_t dtype, void* ws, int64_t ws_bytes, void* stream) {
+    const char* fn = "haste_gated_mlp";
+    HASTE_TRY(haste::mlp_sizes(fn, N, D, H, O, dtype));
+    HASTE_TRY(haste::mlp_act(fn, act));
+    if (N == 0) return HASTE_OK;
+    const haste::Sizes s{N, D, H, O};
+    const haste::Matrix mx{x, ldx, N, D}, mg{wg, ldg, H, D}, mu{wu, ldu, H, D}, md{wd, ldd, O, H};
+    HASTE_TRY(haste::mlp_matrix(fn, "x", mx, dtype));
+    HASTE_TRY(haste::mlp_matrix(fn, "the gate's weight", mg, dtype));
+    HASTE_TRY(haste::mlp_matrix(fn, "the up weight", mu, dtype));
+    HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
+    HASTE_CHECK_ARG(y != nullptr && haste::elem_aligned(y, dtype), "%s: y is NULL or misaligned", fn);
+    HASTE_TRY(haste::mlp_hidden(fn, "h", h));
+    HASTE_CHECK_ARG((g == nullptr) == (u == nullptr), "%s: g and u are written together", fn);
+    if (g) {
+        HASTE_TRY(haste::mlp_hidden(fn, "g", g));
+        HASTE_TRY(haste::mlp_hidden(fn, "u", u));
+    }
+    const haste::GatedOut out{g, u, h, haste::round8(H)};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto run = [&](char* base, bool launch) {
+#define HASTE_MLP(DT) haste::forward<DT>(s, mx, mg, mu, md, out, y, act, base, launch, st)
+        return HASTE_MLP_TYPES(HASTE_MLP);
+#undef HASTE_MLP
+    };
+    HASTE_TRY(haste::mlp_space(fn, ws, ws_bytes, run(nullptr, false)));
+    run(static_cast<char*>(ws), true);
+    HASTE_CHECK_LAUNCH(fn);
+    return HASTE_OK;
+}
+
+extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                   const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                   const void* dy, int64_t lddy, const void* g, const void* u,
+                                   const void* h, void* dx, void* dwg, void* dwu, void* dwd, int64_t N,
+                                   int64_t D, int64_t H, int64_t O, int32_t act, int32_t dtype,
+                                   void* ws, int64_t ws_bytes, void* stream) {
+    const char* fn = "haste_gated_mlp_bwd";
+    HASTE_TRY(haste::mlp_sizes(fn, N, D, H, O, dtype));
+    HASTE_TRY(haste::mlp_act(fn, act));
+    const haste::Sizes s{N, D, H, O};
+    const haste::Matrix mx{x, ldx, N, D}, mg{wg, ldg, H, D}, mu{wu, ldu, H, D}, md{wd, ldd, O, H},
+        my{dy, lddy, N, O};
+    HASTE_CHECK_ARG(haste::elem_aligned(dx, dtype) && haste::elem_aligned(dwg, dtype) &&
+                        haste::elem_aligned(dwu, dtype) && haste::elem_aligned(dwd, dtype),
+                    "%s: a gradient is misaligned", fn);
+    HASTE_CHECK_ARG((dwg == nullptr) == (dwu == nullptr), "%s: dwg and dwu are computed together", fn);
+    if (N > 0) {
+        HASTE_TRY(haste::mlp_matrix(fn, "x", mx, dtype));
+        HASTE_TRY(haste::mlp_matrix(fn, "the gate's weight", mg, dtype));
+        HASTE_TRY(haste::mlp_matrix(fn, "the up weight", mu, dtype));
+        HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
+        HASTE_TRY(haste::mlp_matrix(fn, "dy", my, dtype));
+        HASTE_TRY(haste::mlp_hidden(fn, "g", g));
+        HASTE_TRY(haste::mlp_hidden(fn, "u", u));
+        HASTE_TRY(haste::mlp_hidden(fn, "h", h));
+    }
+    const haste::Grads to{dx, dwg, dwu, dwd};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto run = [&](char* base, bool launch) {
+#define HASTE_MLP(DT) \
+    haste::backward<DT>(s, mx, mg, mu, md, my, g, u, h, haste::round8(H), to, act, base, launch, st)
+        return HASTE_MLP_TYPES(HASTE_MLP);
+#undef HASTE_MLP
+    };
+    HASTE_TRY(haste::mlp_space(fn, ws, ws_bytes, run(nullptr, false)));
+    run(static_cast<char*>(ws), true);
+    HASTE_CHECK_LAUNCH(fn);
+    return HASTE_OK;
+}

@@ -1,0 +1,348 @@
+// Products of 16-bit matrices with fp32 sums, C[m, n] = sum_k A(m, k) B(n, k), as tiles of BM x BN for
+// a workgroup of WM x WN waves, each of which holds FM x FN MFMA tiles of 16 x 16.
+//
+// K goes in steps of 32 through four stages of LDS.  Loads write LDS straight from memory, three steps
+// ahead; a wave reads the fragments of step k + 1 while its MFMAs work on step k, so neither waits
+// for the other, and one barrier a step is enough: the stage that is loaded into was last read two
+// steps ago.
+//
+// An operand is K-contiguous (element (r, k) at r * ld + k) or R-contiguous (at k * ld + r).  The
+// first kind lies in LDS as rows of 32 k's (64 bytes) and is read 16 bytes a lane; the second as
+// rows of BM (BN) r's and is read by ds_read_b64_tr_b16, which transposes 4 x 16 elements.  16-byte
+// pieces (pairs of them) are permuted within their rows so that the lanes of a read meet all banks: the
+// lanes' addresses in memory are permuted, since a load to LDS writes lane after lane.
+#pragma once
+
+#include "elements.hpp"
+
+namespace haste {
+
+// Operand rows start on 16 bytes; columns past the extent up to the next multiple of 8 are zero (K) or
+// unused (R).
+struct GemmOperand {
+    const char* base[2];
+    int64_t ld;  // elements
+};
+
+// PLAIN: one product.  DUAL: the left half of a tile's columns is B's base[0], the right half base[1],
+// each of N columns.  SEGMENTS: K is [0, K) of base[0] of both operands, then [0, K) of base[1].
+// BATCH: two products, of base[0] and base[1] of A, both with B's base[0].
+enum class GemmMode { kPlain, kDual, kSegments, kBatch };
+
+struct GemmArgs {
+    GemmOperand a, b;
+    int M, N, K;
+    int tiles_m, tiles_n;
+    int steps;   // steps of 32 of a segment
+    int splits;  // the steps are cut evenly into so many parts
+};
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// 64 lanes x 16 bytes from memory to LDS at `lds` (wave-uniform), lane after lane.  Lanes at or past the
+// resource's 2 GB write zeros.  Not the builtin: for it the compiler waits for every load in
+// flight before each read of LDS.  Nothing waits for this but wait_loads().
+__device__ __forceinline__ void load_lds16(const char* base, uint32_t voff, uint32_t lds) {
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    const i32x4 rsrc = {(int)(uint32_t)p, (int)((uint32_t)(p >> 32) & 0xFFFFu), 0x7FFFFF00, 0x00020000};
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(lds), "v"(voff), "s"(rsrc)
+        : "memory");
+}
+// Until at most n such loads of the wave are in flight and its LDS reads are done, then for the workgroup.
+template <int n>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(n) : "memory");
+}
+
+template <typename T, GemmMode MODE, bool AK, bool BK_, int FM_, int FN_, int WM_, int WN_>
+struct GemmTile {
+    static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, kWaves = WM * WN;
+    static constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, KS = 32, kStages = 4;
+    static constexpr int kThreads = 64 * kWaves;
+    static constexpr int kABytes = BM * KS * 2, kBBytes = BN * KS * 2, kStage = kABytes + kBBytes;
+    static constexpr int kLdsBytes = kStages * kStage;
+    static constexpr int kALoads = BM / 16 / kWaves, kBLoads = BN / 16 / kWaves;
+    static constexpr int kLoads = kALoads + kBLoads;
+    static constexpr bool kDual = MODE == GemmMode::kDual;
+    // columns of C to a tile
+    static constexpr int kCols = kDual ? BN / 2 : BN;
+    static_assert(BM / 16 % kWaves == 0 && BN / 16 % kWaves == 0, "loads do not divide");
+    static_assert(2 * kLoads < 63, "vmcnt");
+
+    f32x4 acc[FN][FM];
+    int m0, n0;  // first row and column of the wave's part (DUAL: of either half)
+
+    // Where a lane's 16 bytes of load j lie: row and k of their first element within the tile.
+    template <bool KC, int R>
+    static __device__ __forceinline__ void place(int j, int lane, int* r, int* k) {
+        if constexpr (KC) {
+            *r = j * 16 + lane / 4;
+            *k = 8 * ((lane & 3) ^ ((*r >> 1) & 3));
+        } else {
+            constexpr int C = R / 8;  // pieces to a row
+            const int i = j * 64 + lane, s = i % C;
+            *k = i / C;
+            const int f = ((*k & 3) | (*k >> 3 & 3) << 2) & (C / 2 - 1);
+            *r = 8 * (2 * ((s / 2) ^ f) + (s & 1));
+        }
+    }
+
+    // Fragment (16 rows from r0) of an operand's stage: lane l has row l % 16, k = 8 (l / 16) + 0..7.
+    template <bool KC, int R>
+    static __device__ __forceinline__ u32x4 fragment(const char* stage, int r0, int lane) {
+        if constexpr (KC) {
+            const int r = r0 + (lane & 15);
+            return *reinterpret_cast<const u32x4*>(stage + r * 64 +
+                                                   (((lane >> 4) ^ ((lane >> 1) & 3)) << 4));
+        } else {
+            constexpr int C = R / 8;
+            const int i = lane & 15, q = lane >> 4;
+            const int f = ((i >> 2) | q << 2) & (C / 2 - 1);
+            const char* p = stage + (q * 8 + (i >> 2)) * (R * 2) + (((r0 >> 4) ^ f) << 5) + (i & 3) * 8;
+            const u32x2 lo = lds_read_tr16(p), hi = lds_read_tr16(p + 4 * R * 2);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+    }
+
+    __device__ __forceinline__ void run(const GemmArgs& g, char* lds, int tm, int tn, int batch,
+                                        int split) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int wm = wave % WM, wn = wave / WM;
+        m0 = tm * BM + wm * FM * 16;
+        n0 = tn * kCols + wn * (kDual ? FN / 2 : FN) * 16;
+        const int all = MODE == GemmMode::kSegments ? 2 * g.steps : g.steps;
+        const int k0 = (int)((int64_t)all * split / g.splits),
+                  k1 = (int)((int64_t)all * (split + 1) / g.splits);
+        // bytes from a tile's first element
+        uint32_t off[kLoads];
+        int kpos[kLoads];
+        const char *pa[2], *pb[2];
+        const int64_t lda = g.a.ld * 2, ldb = g.b.ld * 2;
+        const int64_t a0 = AK ? tm * BM * lda : tm * BM * 2, b0 = BK_ ? tn * kCols * ldb : tn * kCols * 2;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int from = MODE == GemmMode::kBatch ? batch : MODE == GemmMode::kPlain ? 0 : x;
+            pa[x] = g.a.base[kDual ? 0 : from] + a0;
+            pb[x] = g.b.base[MODE == GemmMode::kBatch ? 0 : from] + b0;
+        }
+#pragma unroll
+        for (int j = 0; j < kALoads; ++j) {
+            int r, k;
+            place<AK, BM>(wave * kALoads + j, lane, &r, &k);
+            off[j] = tm * BM + r < g.M ? (uint32_t)(AK ? r * lda + k * 2 : k * lda + r * 2) : kOOB;
+            kpos[j] = k;
+        }
+#pragma unroll
+        for (int j = 0; j < kBLoads; ++j) {
+            int r, k;
+            place<BK_, BN>(wave * kBLoads + j, lane, &r, &k);
+            if (kDual) r = r % (BN / 2);
+            off[kALoads + j] =
+                tn * kCols + r < g.N ? (uint32_t)(BK_ ? r * ldb + k * 2 : k * ldb + r * 2) : kOOB;
+            kpos[kALoads + j] = k;
+        }
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        auto issue = [&](int kt) __attribute__((always_inline)) {
+            const bool second = MODE == GemmMode::kSegments && kt >= g.steps;
+            const int k = (second ? kt - g.steps : kt) * KS;
+            const int left = kt < k1 ? g.K - k : 0;
+            const uint32_t to = lds0 + (kt & (kStages - 1)) * kStage;
+            const char* a = pa[second] + (AK ? (int64_t)k * 2 : k * lda);
+            const char* b = pb[second] + (BK_ ? (int64_t)k * 2 : k * ldb);
+            const char* b2 = kDual ? pb[1] + (BK_ ? (int64_t)k * 2 : k * ldb) : b;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const bool is_a = j < kALoads;
+                const int i = is_a ? wave * kALoads + j : wave * kBLoads + (j - kALoads);
+                const char* p = is_a ? a : kDual && i * 16 >= BN / 2 ? b2 : b;
+                load_lds16(p, kpos[j] < left ? off[j] : kOOB, to + (is_a ? 0 : kABytes) + i * 1024);
+            }
+        };
+        u32x4 fa[2][FM], fb[2][FN];
+        auto read = [&](int kt, int set) __attribute__((always_inline)) {
+            const char* s = lds + (kt & (kStages - 1)) * kStage;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const int r = kDual ? (f / (FN / 2)) * (BN / 2) + (wn * (FN / 2) + f % (FN / 2)) * 16
+                                    : (wn * FN + f) * 16;
+                fb[set][f] = fragment<BK_, BN>(s + kABytes, r, lane);
+            }
+#pragma unroll
+            for (int f = 0; f < FM; ++f) fa[set][f] = fragment<AK, BM>(s, (wm * FM + f) * 16, lane);
+        };
+        auto multiply = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+            for (int f = 0; f < FM; ++f)
+#pragma unroll
+                for (int h = 0; h < FN; ++h)
+                    acc[h][f] = mfma16x16x32<T>(fb[set][h], fa[set][f], acc[h][f]);
+        };
+#pragma unroll
+        for (int h = 0; h < FN; ++h)
+#pragma unroll
+            for (int f = 0; f < FM; ++f) acc[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k0 < k1) {
+            issue(k0);
+            issue(k0 + 1);
+            issue(k0 + 2);
+            wait_loads<2 * kLoads>();
+            read(k0, 0);
+            // (steps past the last are zeros: loaded as such, or not multiplied)
+            auto step = [&](int kt, int set) __attribute__((always_inline)) {
+                wait_loads<kLoads>();
+                issue(kt + 3);
+                __builtin_amdgcn_sched_barrier(0);
+                read(kt + 1, 1 - set);
+                multiply(set);
+                // each read behind a few MFMAs, all of them in the step's first part
+                constexpr int reads = (AK ? FM : 2 * FM) + (BK_ ? FN : 2 * FN);
+                constexpr int per = FM * FN * 3 / 4 / reads < 1 ? 1 : FM * FN * 3 / 4 / reads;
+#pragma unroll
+                for (int i = 0; i < reads; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, per, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            for (int kt = k0; kt < k1; kt += 2) {
+                step(kt, 0);
+                step(kt + 1, 1);
+            }
+        }
+        // (LDS is written until here)
+        wait_loads<0>();
+    }
+};
+
+// The same of fp32 matrices on v_mfma_f32_16x16x4: rows of any pitch, staged through registers into
+// LDS as rows of BM (BN) r's, two steps of 16 in turn.
+template <GemmMode MODE, bool AK, bool BK_>
+struct GemmTileF32 {
+    static constexpr int FM = 4, FN = 4, WM = 2, WN = 2, BM = 128, BN = 128, KS = 16;
+    static constexpr int kThreads = 256, kPitch = BM + 4;
+    static constexpr bool kDual = MODE == GemmMode::kDual;
+    static constexpr int kCols = kDual ? BN / 2 : BN;
+    static constexpr int kLdsBytes = 2 * 2 * KS * kPitch * 4;
+    typedef Elems<HASTE_DTYPE_F32, 4> Piece;
+
+    f32x4 acc[FN][FM];
+    int m0, n0;
+
+    // Pieces t and t + 256 of an operand's step: four elements along its contiguous axis.
+    template <bool KC>
+    static __device__ __forceinline__ void place(int i, int* r, int* k) {
+        *r = KC ? i / 4 : i % 32 * 4;
+        *k = KC ? i % 4 * 4 : i / 32;
+    }
+    template <bool KC>
+    static __device__ __forceinline__ void put(float* s, int i, const Piece& v) {
+        int r, k;
+        place<KC>(i, &r, &k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s[KC ? (k + e) * kPitch + r : k * kPitch + r + e] = __uint_as_float(v.q[e]);
+    }
+    // rows [0, rows) of the tile and k's [0, left) of the step count
+    template <bool KC>
+    static __device__ __forceinline__ Piece get(const char* base, int64_t ld, int i, int rows, int left) {
+        int r, k;
+        place<KC>(i, &r, &k);
+        if (KC) return load_part<HASTE_DTYPE_F32, 4>(base, r * ld + k, r < rows ? left - k : 0);
+        return load_part<HASTE_DTYPE_F32, 4>(base, k * ld + r, k < left ? rows - r : 0);
+    }
+
+    __device__ __forceinline__ void run(const GemmArgs& g, char* lds, int tm, int tn, int batch,
+                                        int split) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = threadIdx.x;
+        const int wm = wave % WM, wn = wave / WM;
+        m0 = tm * BM + wm * FM * 16;
+        n0 = tn * kCols + wn * (kDual ? FN / 2 : FN) * 16;
+        const int all = MODE == GemmMode::kSegments ? 2 * g.steps : g.steps;
+        const int k0 = (int)((int64_t)all * split / g.splits),
+                  k1 = (int)((int64_t)all * (split + 1) / g.splits);
+        float* s = reinterpret_cast<float*>(lds);
+        auto stage = [&](int kt, int op) __attribute__((always_inline)) {
+            return s + ((kt & 1) * 2 + op) * KS * kPitch;
+        };
+        Piece a[2], b[2];
+        auto fetch = [&](int kt) __attribute__((always_inline)) {
+            const bool second = MODE == GemmMode::kSegments && kt >= g.steps;
+            const int k = (second ? kt - g.steps : kt) * KS, left = kt < k1 ? g.K - k : 0;
+            const int from = MODE == GemmMode::kBatch ? batch : second;
+            const int64_t lda = g.a.ld, ldb = g.b.ld;
+            const char* pa = g.a.base[kDual ? 0 : from] +
+                             4 * (AK ? (int64_t)tm * BM * lda + k : k * lda + (int64_t)tm * BM);
+            const int64_t b0 = 4 * (BK_ ? (int64_t)tn * kCols * ldb + k : k * ldb + (int64_t)tn * kCols);
+            const char* pb = g.b.base[MODE == GemmMode::kBatch ? 0 : from] + b0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                a[j] = get<AK>(pa, lda, t + 256 * j, g.M - tm * BM, left);
+                if (kDual)  // (K-contiguous: pieces 256 and on are rows 64 and on)
+                    b[j] = get<BK_>(g.b.base[j] + b0, ldb, t, g.N - tn * kCols, left);
+                else
+                    b[j] = get<BK_>(pb, ldb, t + 256 * j, g.N - tn * kCols, left);
+            }
+        };
+#pragma unroll
+        for (int h = 0; h < FN; ++h)
+#pragma unroll
+            for (int f = 0; f < FM; ++f) acc[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k0 < k1) fetch(k0);
+        for (int kt = k0; kt < k1; ++kt) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                put<AK>(stage(kt, 0), t + 256 * j, a[j]);
+                put<BK_>(stage(kt, 1), t + 256 * j, b[j]);
+            }
+            __syncthreads();  // (a stage is written again after the next step's)
+            fetch(kt + 1);
+#pragma unroll
+            for (int k = 0; k < KS; k += 4) {
+                const float *ra = stage(kt, 0) + (k + (lane >> 4)) * kPitch + (lane & 15),
+                            *rb = stage(kt, 1) + (k + (lane >> 4)) * kPitch + (lane & 15);
+                float fa[FM], fb[FN];
+#pragma unroll
+                for (int f = 0; f < FM; ++f) fa[f] = ra[(wm * FM + f) * 16];
+#pragma unroll
+                for (int f = 0; f < FN; ++f)
+                    fb[f] = rb[kDual ? (f / (FN / 2)) * (BN / 2) + (wn * (FN / 2) + f % (FN / 2)) * 16
+                                     : (wn * FN + f) * 16];
+#pragma unroll
+                for (int f = 0; f < FM; ++f)
+#pragma unroll
+                    for (int h = 0; h < FN; ++h)
+                        acc[h][f] =
+                            __builtin_amdgcn_mfma_f32_16x16x4f32(fb[h], fa[f], acc[h][f], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// Workgroup -> (tile row, tile column, product, split): the tiles that one XCD works on at a time
+// are eight rows by a few columns of one product, whose operands meet in its L2.
+struct GemmPlace {
+    int tm, tn, batch, split;
+};
+__device__ __forceinline__ bool gemm_place(const GemmArgs& g, int batches, GemmPlace* p) {
+    // (32 bits: a launch has fewer than 2^31 workgroups)
+    const uint32_t tiles = g.tiles_m * g.tiles_n, all = tiles * batches * g.splits;
+    const uint32_t x = blockIdx.x % 8, k = blockIdx.x / 8, lo = all / 8, rem = all % 8;
+    if (k >= lo + (x < rem ? 1 : 0)) return false;
+    const uint32_t id = x * lo + min(x, rem) + k;  // (consecutive ones on one XCD)
+    p->batch = (int)(id / (tiles * g.splits));
+    const uint32_t in_batch = id % (tiles * g.splits);
+    p->split = (int)(in_batch / tiles);
+    const int t = (int)(in_batch % tiles), rows = 8;
+    const int group = t / (rows * g.tiles_n), in = t % (rows * g.tiles_n);
+    const int height = min(rows, g.tiles_m - group * rows);
+    p->tm = group * rows + in % height;
+    p->tn = in / height;
+    return true;
+}
+
+}  // namespace haste

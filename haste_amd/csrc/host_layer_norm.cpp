@@ -5,54 +5,15 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include "../../include/haste_ffi.h"
-#include "host_tables.hpp"
+#include "host_rows.hpp"
 
 namespace haste_host {
 namespace {
 
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// t as rows [N, D] with contiguous columns, `ld` elements apart (0: one row for all), copied only
-// where it has no such view.
-struct Rows {
-    at::Tensor t;
-    int64_t ld = 0;
-};
-Rows rows_of(const at::Tensor& x, int64_t D) {
-    at::Tensor t = x.is_neg() ? x.resolve_neg() : x;
-    if (t.dim() != 2) t = t.reshape({-1, D});
-    int64_t ld = t.size(0) > 1 ? t.stride(0) : D;
-    if ((t.stride(1) != 1 && D > 1) || (ld < D && ld != 0)) {
-        t = t.contiguous();
-        ld = D;
-    }
-    return Rows{t, ld};
-}
-
-const void* ptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void* out_ptr(const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-
-void check_device(const at::Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda(), name, " must be a tensor on a HIP device (MI355X); got a ", t.device(),
-                " tensor");
-}
-
 void check(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias,
            const at::Tensor& residual) {
     check_not_traced("layer_norm");
-    // (also where no gradient is recorded: the kernels are handed addresses, without the tangent)
-    for (const at::Tensor* t : {&x, &weight, &bias, &residual})
-        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
-                                    "layer_norm: forward-mode derivatives are not supported");
+    check_no_tangent("layer_norm", {&x, &weight, &bias, &residual});
     check_device(x, "x");
     TORCH_CHECK(dtype_code(x.scalar_type()) >= 0, "unsupported dtype ", x.scalar_type());
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1,
@@ -168,29 +129,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (need & kWeight) out[1] = dw;
         if (need & kBias) out[2] = db;
         if (need & kResidual) out[4] = dx;
-        if (!at::GradMode::is_enabled()) return out;
-        // under create_graph: what is differentiated again says so, and is not taken for a constant
-        variable_list marked;
-        for (const at::Tensor& t : out)
-            if (t.defined()) marked.push_back(t.detach().set_requires_grad(true));
-        if (marked.empty()) return out;
-        const auto error = std::make_shared<torch::autograd::DelayedError>(
-            "layer_norm: its backward cannot be differentiated", (int64_t)marked.size());
-        marked = (*error)(std::move(marked));
-        size_t k = 0;
-        for (at::Tensor& t : out)
-            if (t.defined()) t = marked[k++];
+        once_differentiable("layer_norm", out);
         return out;
     }
 };
-
-// A tensor, or an undefined one for None.
-at::Tensor tensor_arg(PyObject* o, const char* name, bool optional) {
-    if (optional && o == Py_None) return at::Tensor();
-    TORCH_CHECK(THPVariable_Check(o), name, " must be a tensor on a HIP device (MI355X); got ",
-                Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
-}
 
 }  // namespace
 

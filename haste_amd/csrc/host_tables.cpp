@@ -208,13 +208,23 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
+    return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+
 PyMethodDef methods[] = {
     {"grad_norm", grad_norm, METH_VARARGS, "grad_norm(tensors, max_norm) -> (norm, coef) or None"},
     {"adamw_step", adamw_step, METH_VARARGS,
      "adamw_step(params, state, bits, lr, beta1, beta2, eps, weight_decay, stochastic_rounding, "
      "seed, stream, grad_scale) -> True or None"},
-    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(haste_host::layer_norm)),
-     METH_FASTCALL, "layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual"},
+    {"layer_norm", fast(haste_host::layer_norm), METH_FASTCALL,
+     "layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual"},
+    {"embedding", fast(haste_host::embedding), METH_FASTCALL,
+     "embedding(tokens, weight, scale, padding_idx) -> y"},
+    {"gated_mlp", fast(haste_host::gated_mlp), METH_FASTCALL,
+     "gated_mlp(x, w_gate, w_up, w_down, activation) -> y"},
+    {"label_log_probs", fast(haste_host::label_log_probs), METH_FASTCALL,
+     "label_log_probs(logits, labels, top) -> (log_probs, entropy, top_log_probs, top_labels)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT,
                       "_host",

@@ -47,5 +47,12 @@ inline PyObject* pair_of(const at::Tensor& a, const at::Tensor& b) {
 
 // layer_norm(x, weight, bias, eps, residual) -> y, or (y, h) with a residual
 PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count);
+// embedding(tokens, weight, scale, padding_idx or None) -> y
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t count);
+// gated_mlp(x, w_gate, w_up, w_down, activation code) -> y
+PyObject* gated_mlp(PyObject*, PyObject* const* args, Py_ssize_t count);
+// label_log_probs(logits, labels or None, top) -> (log_probs, entropy, top_log_probs, top_labels), None
+// for what was not asked for
+PyObject* label_log_probs(PyObject*, PyObject* const* args, Py_ssize_t count);
 
 }  // namespace haste_host

@@ -1,0 +1,500 @@
+// Log probabilities of given labels under rows of logits, the rows' entropy and their likeliest labels:
+//   m = max z, s = sum e^(z - m), log p = (z - m) - log s, H = log s - sum e^(z - m) (z - m) / s
+// and the logits' gradient dz = p (-sum_l g_l - g_H (log p + H)) + sum_{l: label l = j} g_l.
+// One pass over the logits forward and one backward, both bound by HBM: a thread keeps the running
+// maximum and sums of its part of a row, a wave the largest K keys of its part.
+#include <algorithm>
+
+#include "elements.hpp"
+
+namespace haste {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxTop = 128;
+constexpr float kGone = -150.f;  // e^x is 0 below
+
+// ------------------------------------------------------------- softmax sums ----
+// s = sum e^(z - m), t = sum e^(z - m) (z - m).  Before the first finite logit m is the lowest
+// fp32 value, not -infinity, so that z - m is a number for every z but +infinity and NaN.
+struct Sums {
+    float m, s, t;
+};
+__device__ __forceinline__ Sums no_sums() { return Sums{-3.402823466e38f, 0.f, 0.f}; }
+__device__ __forceinline__ void rescale(Sums& a, float m) {
+    const float d = fmaxf(a.m - m, kGone), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    a.t = (a.t + a.s * d) * f;
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    const float m = fmaxf(a.m, b.m);
+    rescale(a, m);
+    rescale(b, m);
+    return Sums{m, a.s + b.s, a.t + b.t};
+}
+
+// ------------------------------------------------------------ largest K keys ----
+// A label's key: its logit's order, then the lower label first.  0 is no label's.  NaN is largest.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float z, uint32_t label) {
+    uint32_t u = z == 0.f ? 0u : __float_as_uint(z);
+    u = z != z ? 0xFFFFFFFFu : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+    return (Key)u << 32 | (0xFFFFFFFFu - label);
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float(u == 0xFFFFFFFFu ? 0x7FC00000u
+                                            : u ^ ((u >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ uint32_t label_of(Key k) { return 0xFFFFFFFFu - (uint32_t)k; }
+
+// Sorts 64 R keys of a wave, largest first; key r * 64 + lane is k[r] of that lane.
+template <int R>
+__device__ __forceinline__ void sort_keys(Key (&k)[R], int lane) {
+#pragma unroll
+    for (int size = 2; size <= 64 * R; size *= 2)
+#pragma unroll
+        for (int stride = size / 2; stride > 0; stride /= 2) {
+            if (stride >= 64) {
+                const int rs = stride / 64;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (!(r & rs)) {
+                        const bool down = ((r * 64 + lane) & size) == 0;
+                        const Key a = k[r], b = k[r | rs];
+                        k[r] = (a > b) == down ? a : b;
+                        k[r | rs] = (a > b) == down ? b : a;
+                    }
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const Key o = __shfl_xor(k[r], stride);
+                    const bool most = (((r * 64 + lane) & size) == 0) == ((lane & stride) == 0);
+                    k[r] = (k[r] > o) == most ? k[r] : o;
+                }
+            }
+        }
+}
+
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wave's list of candidates in LDS, of 64 R keys.  Whenever fewer than 64 places are free it is
+// sorted and cut to its largest K, and the K-th is what a key has to exceed from then on; `shared`
+// holds the largest such bound of the workgroup.
+template <int R>
+struct Candidates {
+    Key* buf;
+    Key* shared;
+    int K, count, lane;
+    Key bound;     // (0: every key passes)
+    float least;   // its logit, NaN for none
+
+    __device__ __forceinline__ void raise(Key b) {
+        if (b > bound) {
+            bound = b;
+            least = value_of(b);
+        }
+    }
+    __device__ __forceinline__ void cut() {
+        Key k[R];
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < R; ++r) k[r] = r * 64 + lane < count ? buf[r * 64 + lane] : 0;
+        sort_keys<R>(k, lane);
+#pragma unroll
+        for (int r = 0; r < R; ++r) buf[r * 64 + lane] = k[r];
+        wave_sync();
+        if (count >= K) {
+            count = K;
+            raise(buf[K - 1]);
+            if (lane == 0) atomicMax(shared, bound);
+        }
+    }
+    // The keys of the wave's lanes; 0 for none.
+    __device__ __forceinline__ void add(Key key) {
+        const bool pass = key > bound;
+        const uint64_t mask = __ballot(pass);
+        if (!mask) return;
+        if (pass) buf[count + __popcll(mask & (((uint64_t)1 << lane) - 1))] = key;
+        count += __popcll(mask);
+        if (count > 64 * (R - 1)) cut();
+    }
+    __device__ __forceinline__ void refresh() { raise(*(volatile Key*)shared); }
+};
+
+constexpr int buffer_keys(int R) { return R ? 64 * R : 1; }
+
+// The workgroup's sums and largest keys from its waves' in wave 0's list.
+template <int R>
+struct Shared {
+    Sums sums[kWaves];
+    int count[kWaves];
+    Key bound;
+    Key buf[kWaves][buffer_keys(R)];
+};
+
+template <int R>
+__device__ __forceinline__ void join_waves(Shared<R>& sh, Sums& a, Candidates<R ? R : 2>& c) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int o = 32; o; o >>= 1) {
+        Sums b;
+        b.m = __shfl_xor(a.m, o);
+        b.s = __shfl_xor(a.s, o);
+        b.t = __shfl_xor(a.t, o);
+        a = join(a, b);
+    }
+    if (lane == 0) {
+        sh.sums[wave] = a;
+        if (R) sh.count[wave] = c.count;
+    }
+    __syncthreads();
+    a = sh.sums[0];
+    for (int w = 1; w < kWaves; ++w) a = join(a, sh.sums[w]);
+    if constexpr (R > 0) {
+        if (wave == 0) {
+            // (the bound itself is in some wave's list)
+            c.bound = sh.bound ? sh.bound - 1 : 0;
+            for (int w = 1; w < kWaves; ++w)
+                for (int i = 0; i < sh.count[w]; i += 64)
+                    c.add(i + lane < sh.count[w] ? sh.buf[w][i + lane] : 0);
+            c.cut();
+        }
+        __syncthreads();
+    }
+}
+
+struct Out {
+    float *stats, *log_probs, *entropy, *top;
+    int64_t* top_labels;
+};
+
+template <int DT>
+__device__ __forceinline__ void write_row(const void* z, const void* labels, bool wide, int64_t L,
+                                          int64_t O, int K, int64_t row, const Sums& a,
+                                          const Key* keys, const Out& out) {
+    // (a row without a finite logit has no distribution: NaN)
+    const float log_s = a.s > 0.f ? logf(a.s) : __uint_as_float(0x7FC00000u);
+    if (threadIdx.x == 0) {
+        if (out.stats) {
+            out.stats[2 * row] = a.m;
+            out.stats[2 * row + 1] = a.s > 0.f ? a.s : __uint_as_float(0x7FC00000u);
+        }
+        if (out.entropy) out.entropy[row] = log_s - a.t / a.s;
+    }
+    for (int64_t l = threadIdx.x; l < L; l += kThreads) {
+        const int64_t i = row * L + l;
+        const int64_t j = wide ? static_cast<const int64_t*>(labels)[i]
+                               : (int64_t)static_cast<const int32_t*>(labels)[i];
+        out.log_probs[i] = j >= 0 && j < O ? (load_elem<DT>(z, j) - a.m) - log_s : 0.f;
+    }
+    for (int k = threadIdx.x; k < K; k += kThreads) {
+        out.top[row * K + k] = (value_of(keys[k]) - a.m) - log_s;
+        out.top_labels[row * K + k] = label_of(keys[k]);
+    }
+}
+
+// Part `blockIdx.x % S` of row `blockIdx.x / S`.  Vectors lie on 16-byte boundaries; the row's first
+// and last may have elements of other rows in them, which are not read.
+template <int DT, int R>
+__global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz, const void* labels,
+                                                      int wide, int64_t L, int64_t O, int K, int S,
+                                                      int64_t per, Out out, Sums* part,
+                                                      Key* part_keys, int64_t row0) {
+    constexpr int SZ = kElemBytes<DT>, V = 16 / SZ;
+    __shared__ Shared<R> sh;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = row0 + blockIdx.x / S;
+    const int c = blockIdx.x % S;
+    const char* p = z + row * ldz * SZ;
+    const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / SZ);
+    const int64_t nv = (off + O + V - 1) / V;
+    const int64_t v1 = min(nv, (c + 1) * per);
+    Sums a = no_sums();
+    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0,
+                                __uint_as_float(0x7FC00000u)};
+    if (R) {
+        if (threadIdx.x == 0) sh.bound = 0;
+        __syncthreads();
+    }
+    for (int64_t v = c * per + wave * 64; v < v1; v += kThreads) {
+        const int64_t e0 = (v + lane) * V - off;
+        float f[V];
+        if (v + lane < v1 && e0 >= 0 && e0 + V <= O) {
+            unpack<DT, V>(load<DT, V>(p, e0), f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                f[e] = v + lane < v1 && e0 + e >= 0 && e0 + e < O ? load_elem<DT>(p, e0 + e)
+                                                                  : -__builtin_inff();
+        }
+        float most = f[0];
+#pragma unroll
+        for (int e = 1; e < V; ++e) most = fmaxf(most, f[e]);
+        rescale(a, fmaxf(a.m, most));
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = f[e] - a.m, x = __builtin_amdgcn_exp2f(d * kLog2e);
+            a.s += x;
+            a.t = __builtin_fmaf(x, fmaxf(d, kGone), a.t);
+        }
+        if constexpr (R > 0) {
+            // (a NaN hides from `most`, but not from the sum)
+            if (__any(!(most < top.least) || a.s != a.s)) {
+                top.refresh();
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int64_t i = e0 + e;
+                    top.add(v + lane < v1 && i >= 0 && i < O ? key_of(f[e], (uint32_t)i) : 0);
+                }
+            }
+        }
+    }
+    if (R) top.cut();
+    join_waves<R>(sh, a, top);
+    if (S == 1) {
+        write_row<DT>(p, labels, wide, L, O, K, row, a, sh.buf[0], out);
+        return;
+    }
+    if (threadIdx.x == 0) part[row * S + c] = a;
+    for (int k = threadIdx.x; k < K; k += kThreads)
+        part_keys[(row * S + c) * K + k] = sh.buf[0][k];
+}
+
+// A row's parts joined.
+template <int DT, int R>
+__global__ __launch_bounds__(kThreads) void lp_join_kernel(const char* z, int64_t ldz,
+                                                           const void* labels, int wide, int64_t L,
+                                                           int64_t O, int K, int S, Out out,
+                                                           const Sums* part, const Key* part_keys,
+                                                           int64_t row0) {
+    __shared__ Shared<R> sh;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = row0 + blockIdx.x;
+    Sums a = no_sums();
+    for (int i = threadIdx.x; i < S; i += kThreads) a = join(a, part[row * S + i]);
+    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0,
+                                __uint_as_float(0x7FC00000u)};
+    if constexpr (R > 0) {
+        if (threadIdx.x == 0) sh.bound = 0;
+        __syncthreads();
+        const int64_t n = (int64_t)S * K;
+        for (int64_t i = wave * 64; i < n; i += kThreads)
+            top.add(i + lane < n ? part_keys[row * n + i + lane] : 0);
+        top.cut();
+    }
+    join_waves<R>(sh, a, top);
+    write_row<DT>(z + row * ldz * kElemBytes<DT>, labels, wide, L, O, K, row, a, sh.buf[0], out);
+}
+
+// Elements [blockIdx.x % S * per, ...) of a row.  The labels' own elements are written again, with what
+// their labels add, after every thread's stores are done.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void lp_bwd_kernel(const char* z, int64_t ldz,
+                                                          const void* labels, int wide, int64_t L,
+                                                          const float* stats, const float* entropy,
+                                                          const float* dlp, const float* dent,
+                                                          char* dz, int64_t lddz, int64_t O, int S,
+                                                          int64_t per, int64_t row0) {
+    constexpr int SZ = kElemBytes<DT>, V = 16 / SZ;
+    const int64_t row = row0 + blockIdx.x / S, from = blockIdx.x % S * per, to = min(O, from + per);
+    z += row * ldz * SZ;
+    dz += row * lddz * SZ;
+    const float m = stats[2 * row], s = stats[2 * row + 1], H = entropy[row];
+    const float log_s = logf(s), inv = 1.f / s;
+    const float ge = dent ? dent[row] : 0.f;
+    auto label = [&](int64_t l) __attribute__((always_inline)) {
+        const int64_t i = row * L + l;
+        return wide ? static_cast<const int64_t*>(labels)[i]
+                    : (int64_t)static_cast<const int32_t*>(labels)[i];
+    };
+    float sum = 0.f;
+    if (dlp)
+        for (int64_t l = 0; l < L; ++l) {
+            const int64_t j = label(l);
+            if (j >= 0 && j < O) sum += dlp[row * L + l];
+        }
+    const float c0 = -sum - ge * H;
+    // (16-bit gradients have no use for the last bits of e^d)
+    auto base = [&](float x) __attribute__((always_inline)) {
+        const float d = x - m;
+        const float p = (DT == HASTE_DTYPE_F32 ? expf(d) : __builtin_amdgcn_exp2f(d * kLog2e)) * inv;
+        return p * __builtin_fmaf(-ge, fmaxf(d, kGone) - log_s, c0);
+    };
+    for (int64_t e0 = from + threadIdx.x * V; e0 < to; e0 += kThreads * V) {
+        float f[V];
+        unpack<DT, V>(load_part<DT, V>(z, e0, to - e0), f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = base(f[e]);
+        store_part<DT, V>(dz, e0, pack<DT, V>(f), to - e0);
+    }
+    if (!dlp) return;
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    __syncthreads();
+    for (int64_t l = threadIdx.x; l < L; l += kThreads) {
+        const int64_t j = label(l);
+        if (j < from || j >= to) continue;
+        bool first = true;
+        for (int64_t k = 0; k < l; ++k) first &= label(k) != j;
+        if (!first) continue;
+        float g = 0.f;
+        for (int64_t k = l; k < L; ++k) g += label(k) == j ? dlp[row * L + k] : 0.f;
+        store_elem<DT>(dz, j, base(load_elem<DT>(z, j)) + g);
+    }
+}
+
+// Parts of a row: eight workgroups to a compute unit where there are few rows, and at least a vector to
+// a thread.
+int parts(int64_t B, int64_t O, int32_t dtype) {
+    const int64_t vectors = ceil_div(O, 16 / elem_bytes(dtype)) + 1;
+    return (int)std::max<int64_t>(
+        1, std::min<int64_t>({ceil_div(2048, std::max<int64_t>(B, 1)), vectors / kThreads, 256}));
+}
+
+int lp_check(const char* fn, const void* z, int64_t ldz, const void* labels, int32_t label_bits,
+             int64_t L, int64_t B, int64_t O, int32_t dtype) {
+    HASTE_CHECK_ARG(B >= 0 && O > 0 && L >= 0, "%s: bad sizes B=%lld O=%lld L=%lld", fn, (long long)B,
+                    (long long)O, (long long)L);
+    HASTE_CHECK_ARG(B < (int64_t)1 << 31 && O < (int64_t)1 << 31 && L < (int64_t)1 << 31,
+                    "%s: too large", fn);
+    HASTE_CHECK_ARG(elem_dtype(dtype), "%s: logits must be bf16, f16 or f32", fn);
+    HASTE_CHECK_ARG(label_bits == 32 || label_bits == 64, "%s: labels have 32 or 64 bits", fn);
+    if (B == 0) return HASTE_OK;
+    HASTE_CHECK_ARG(z != nullptr && elem_aligned(z, dtype), "%s: logits are NULL or misaligned", fn);
+    HASTE_CHECK_ARG(ldz == 0 || ldz >= O, "%s: row pitch of the logits is short (%lld < %lld)", fn,
+                    (long long)ldz, (long long)O);
+    HASTE_CHECK_ARG(L == 0 || (labels != nullptr &&
+                               reinterpret_cast<uintptr_t>(labels) % (label_bits / 8) == 0),
+                    "%s: labels are NULL or misaligned", fn);
+    return HASTE_OK;
+}
+
+// f(first row, rows) over launches of fewer than 2^32 threads.
+template <typename F>
+void in_launches(int64_t B, int64_t S, F f) {
+    const int64_t most = (((int64_t)1 << 32) - 1) / (kThreads * S);
+    for (int64_t i = 0; i < B; i += most) f(i, std::min(most, B - i));
+}
+
+#define HASTE_LP_TYPES(call)                                                                  \
+    do {                                                                                      \
+        if (dtype == HASTE_DTYPE_F32) call(HASTE_DTYPE_F32);                                  \
+        else if (dtype == HASTE_DTYPE_BF16) call(HASTE_DTYPE_BF16);                           \
+        else call(HASTE_DTYPE_F16);                                                           \
+    } while (0)
+
+int64_t lp_workspace(int64_t B, int64_t O, int64_t K) {
+    // (fp32's parts are the most)
+    const int64_t S = parts(B, O, HASTE_DTYPE_F32);
+    return S == 1 ? 0 : ceil_div(B * S * (int64_t)sizeof(Sums), 16) * 16 + B * S * K * 8;
+}
+
+}  // namespace
+}  // namespace haste
+
+extern "C" int64_t haste_label_log_probs_workspace_size(int64_t B, int64_t O, int32_t K) {
+    if (B < 0 || O <= 0 || K < 0 || K > haste::kMaxTop || B >= (int64_t)1 << 31 ||
+        O >= (int64_t)1 << 31)
+        return HASTE_ERR_INVALID_ARG;
+    return haste::lp_workspace(B, O, K);
+}
+
+extern "C" int haste_label_log_probs(const void* z, int64_t ldz, const void* labels,
+                                     int32_t label_bits, int64_t L, float* stats, float* log_probs,
+                                     float* entropy, float* top, int64_t* top_labels, int64_t B,
+                                     int64_t O, int32_t K, int32_t dtype, void* ws, int64_t ws_bytes,
+                                     void* stream) {
+    const char* fn = "haste_label_log_probs";
+    const int rc = haste::lp_check(fn, z, ldz, labels, label_bits, L, B, O, dtype);
+    if (rc != HASTE_OK) return rc;
+    HASTE_CHECK_ARG(K >= 0 && K <= haste::kMaxTop && K <= O, "%s: top must be 0 to min(%d, O) (got %d)",
+                    fn, haste::kMaxTop, (int)K);
+    if (B == 0) return HASTE_OK;
+    HASTE_CHECK_ARG(haste::elem_aligned(stats, HASTE_DTYPE_F32) &&
+                        haste::elem_aligned(entropy, HASTE_DTYPE_F32),
+                    "%s: stats or entropy is misaligned", fn);
+    HASTE_CHECK_ARG(L == 0 || (log_probs != nullptr && haste::elem_aligned(log_probs, HASTE_DTYPE_F32)),
+                    "%s: log_probs is NULL or misaligned", fn);
+    HASTE_CHECK_ARG(K == 0 || (top != nullptr && top_labels != nullptr &&
+                               haste::elem_aligned(top, HASTE_DTYPE_F32) &&
+                               reinterpret_cast<uintptr_t>(top_labels) % 8 == 0),
+                    "%s: top or top_labels is NULL or misaligned", fn);
+    const int S = haste::parts(B, O, dtype);
+    if (S > 1) {
+        const int64_t need = haste::lp_workspace(B, O, K);
+        HASTE_CHECK_ARG(ws != nullptr && haste::aligned16(ws), "%s: workspace is NULL or misaligned",
+                        fn);
+        if (ws_bytes < need) {
+            haste::set_error("%s: workspace too small (%lld < %lld bytes)", fn, (long long)ws_bytes,
+                             (long long)need);
+            return HASTE_ERR_WORKSPACE;
+        }
+    }
+    const int64_t V = 16 / haste::elem_bytes(dtype);
+    const int64_t per = haste::ceil_div(haste::ceil_div(O, V) + 1, S);
+    auto* part = static_cast<haste::Sums*>(ws);
+    auto* keys = reinterpret_cast<haste::Key*>(
+        static_cast<char*>(ws) + haste::ceil_div(B * S * (int64_t)sizeof(haste::Sums), 16) * 16);
+    const haste::Out out{stats, log_probs, entropy, top, top_labels};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const char* zc = static_cast<const char*>(z);
+    const int wide = label_bits == 64;
+    haste::in_launches(B, S, [&](int64_t r0, int64_t n) {
+#define HASTE_LP(DT)                                                                               \
+    do {                                                                                           \
+        auto kernel = K == 0    ? haste::lp_kernel<DT, 0>                                          \
+                      : K <= 32 ? haste::lp_kernel<DT, 2>                                          \
+                                : haste::lp_kernel<DT, 4>;                                         \
+        auto join = K == 0    ? haste::lp_join_kernel<DT, 0>                                       \
+                    : K <= 32 ? haste::lp_join_kernel<DT, 2>                                       \
+                              : haste::lp_join_kernel<DT, 4>;                                      \
+        kernel<<<dim3((unsigned)(n * S)), dim3(haste::kThreads), 0, st>>>(                         \
+            zc, ldz, labels, wide, L, O, K, S, per, out, part, keys, r0);                          \
+        if (S > 1)                                                                                 \
+            join<<<dim3((unsigned)n), dim3(haste::kThreads), 0, st>>>(zc, ldz, labels, wide, L, O, \
+                                                                      K, S, out, part, keys, r0);  \
+    } while (0)
+        HASTE_LP_TYPES(HASTE_LP);
+#undef HASTE_LP
+    });
+    HASTE_CHECK_LAUNCH(fn);
+    return HASTE_OK;
+}
+
+extern "C" int haste_label_log_probs_bwd(const void* z, int64_t ldz, const void* labels,
+                                         int32_t label_bits, int64_t L, const float* stats,
+                                         const float* entropy, const float* dlp, const float* dent,
+                                         void* dz, int64_t lddz, int64_t B, int64_t O,
+                                         int32_t dtype, void* stream) {
+    const char* fn = "haste_label_log_probs_bwd";
+    const int rc = haste::lp_check(fn, z, ldz, labels, label_bits, dlp ? L : 0, B, O, dtype);
+    if (rc != HASTE_OK) return rc;
+    if (B == 0) return HASTE_OK;
+    HASTE_CHECK_ARG(stats != nullptr && entropy != nullptr &&
+                        haste::elem_aligned(stats, HASTE_DTYPE_F32) &&
+                        haste::elem_aligned(entropy, HASTE_DTYPE_F32),
+                    "%s: stats or entropy is NULL or misaligned", fn);
+    HASTE_CHECK_ARG(haste::elem_aligned(dlp, HASTE_DTYPE_F32) &&
+                        haste::elem_aligned(dent, HASTE_DTYPE_F32),
+                    "%s: a gradient is misaligned", fn);
+    HASTE_CHECK_ARG(dz != nullptr && haste::elem_aligned(dz, dtype) && lddz >= O,
+                    "%s: dz is NULL or misaligned, or its row pitch is short", fn);
+    // (32 elements to a thread)
+    const int64_t V = 16 / haste::elem_bytes(dtype), most = haste::kThreads * V * 4;
+    const int64_t S = haste::ceil_div(O, most);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    haste::in_launches(B, S, [&](int64_t r0, int64_t n) {
+#define HASTE_LP(DT)                                                                             \
+    haste::lp_bwd_kernel<DT><<<dim3((unsigned)(n * S)), dim3(haste::kThreads), 0, st>>>(         \
+        static_cast<const char*>(z), ldz, labels, label_bits == 64, L, stats, entropy, dlp,     \
+        dent, static_cast<char*>(dz), lddz, O, (int)S, most, r0)
+        HASTE_LP_TYPES(HASTE_LP);
+#undef HASTE_LP
+    });
+    HASTE_CHECK_LAUNCH(fn);
+    return HASTE_OK;
+}

@@ -1,13 +1,18 @@
-"""Public ops: ``group_ffi_mul`` (reference: shared_ffi/ops.py:7-24), ``head_tail_logits``, and
-``layer_norm`` for the encoder in front of an FFI layer."""
+"""Public ops: ``group_ffi_mul`` (reference: shared_ffi/ops.py:7-24), ``head_tail_logits``;
+``embedding``, ``layer_norm`` and ``gated_mlp`` for the encoder in front of an FFI layer; and
+``label_log_probs`` for what the layer's logits answer."""
 from typing import Optional
 
 import torch
 
 from . import bindings as _bindings
+from .embedding import embedding
+from .gated_mlp import gated_mlp
+from .label_probs import label_log_probs
 from .layer_norm import layer_norm
 
-__all__ = ["group_ffi_mul", "head_tail_logits", "layer_norm"]
+__all__ = ["group_ffi_mul", "head_tail_logits", "embedding", "layer_norm", "gated_mlp",
+           "label_log_probs"]
 
 
 def group_ffi_mul(features: torch.Tensor,

@@ -665,6 +665,87 @@ int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count, int32_t w
                      double eps, double wd, int64_t step, int32_t do_sr, uint64_t seed,
                      const float* grad_scale, void* stream);
 
+/*
+ * Embedding lookup: y[n] = RNE(scale * w[t_n]) for tokens t [N] of 32 or 64 bits (token_bits) and a
+ * table w [V, D] of row pitch ldw (elements, >= D; 0 reads one row for all); y is [N, D] contiguous.  A
+ * token outside [0, V) gives a row of zeros.  dtype of w and y: bf16, f16 or f32.
+ */
+int haste_embedding(const void* tokens, int32_t token_bits, const void* w, int64_t ldw, void* y,
+                    int64_t N, int64_t V, int64_t D, double scale, int32_t dtype, void* stream);
+
+/*
+ * Its table's gradient: dw[v] = RNE(scale * sum_{n: t_n = v} dy[n]), fp32 sums in a fixed order; rows
+ * without a token are zeros, and so is row `padding` (none where it is outside [0, V)).  dw is
+ * [V, D] contiguous, dy has row pitch lddy (0: one row for all).  ws: workspace of
+ * haste_embedding_bwd_workspace_size(N, V, D) bytes (16-byte aligned).
+ */
+int64_t haste_embedding_bwd_workspace_size(int64_t N, int64_t V, int64_t D);
+int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, int64_t lddy,
+                        void* dw, int64_t N, int64_t V, int64_t D, double scale, int64_t padding,
+                        int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * The gated feed-forward block: h = act(x wg^T) * (x wu^T), y = h wd^T, for x [N, D], wg and wu [H, D],
+ * wd [O, H] of any row pitch, y [N, O] contiguous.  Products are summed in fp32; h is rounded to
+ * dtype between them.  g = x wg^T, u = x wu^T (both or neither NULL) and h are
+ * [N, ceil8(H)] contiguous, 16-byte aligned, for the backward; their columns from H on are zeros.
+ * act: HASTE_ACT_*.  dtype of all matrices: bf16, f16 or f32.  D, H and O up to 2^20, N below 2^30.
+ * ws: workspace of haste_gated_mlp_workspace_size(N, D, H, O, dtype, backward, aligned) bytes (16-byte
+ * aligned).  16-bit rows that do not start on 16 bytes, or are no multiple of 8 long, are copied into
+ * it; with aligned != 0 there are none.
+ */
+#define HASTE_ACT_SILU 0      /* x / (1 + e^-x) */
+#define HASTE_ACT_GELU 1      /* x (1 + erf(x / sqrt 2)) / 2 */
+#define HASTE_ACT_GELU_TANH 2 /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+
+int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t H, int64_t O, int32_t dtype,
+                                       int32_t backward, int32_t aligned);
+int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
+                    int64_t ldu, const void* wd, int64_t ldd, void* y, void* g, void* u, void* h,
+                    int64_t N, int64_t D, int64_t H, int64_t O, int32_t act, int32_t dtype, void* ws,
+                    int64_t ws_bytes, void* stream);
+
+/*
+ * Its gradients, from the g, u and h of the forward:
+ *   dh = dy wd;  dg = dh u act'(g), du = dh act(g)  (rounded to dtype);
+ *   dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h,
+ * all contiguous.  dx, dwd, or dwg together with dwu may be NULL (not computed).
+ */
+int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
+                        int64_t ldu, const void* wd, int64_t ldd, const void* dy, int64_t lddy,
+                        const void* g, const void* u, const void* h, void* dx, void* dwg, void* dwu,
+                        void* dwd, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
+                        int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * Log probabilities under rows of logits z [B, O] (row pitch ldz, 0: one row for all):
+ *   log p = z - log sum_j e^z_j
+ *   log_probs[b, l] = log p of labels[b, l], 0 for labels outside [0, O)   (labels [B, L] contiguous,
+ *                     32 or 64 bits)
+ *   entropy[b] = -sum_j p_j log p_j  (p = 0 counts nothing)
+ *   top[b, k], top_labels[b, k] = log p and label of the k-th largest logit; equal logits in the order
+ *                     of their labels, NaN before all others
+ * in fp32.  A row whose logits are all -infinity, or that has a NaN or +infinity, gives NaN.
+ * K is 0 to min(128, O).  stats [B, 2] (the row's largest finite logit m, sum e^(z - m)) is for the
+ * backward; stats and entropy may be NULL.  dtype of z: bf16, f16 or f32.  ws: workspace of
+ * haste_label_log_probs_workspace_size(B, O, K) bytes (16-byte aligned).
+ */
+int64_t haste_label_log_probs_workspace_size(int64_t B, int64_t O, int32_t K);
+int haste_label_log_probs(const void* z, int64_t ldz, const void* labels, int32_t label_bits,
+                          int64_t L, float* stats, float* log_probs, float* entropy, float* top,
+                          int64_t* top_labels, int64_t B, int64_t O, int32_t K, int32_t dtype,
+                          void* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * The logits' gradient from those of log_probs (dlp [B, L]) and entropy (dent [B]), either NULL for none:
+ *   dz_j = RNE(p_j (-sum_l dlp_l - dent (log p_j + entropy)) + sum_{l: labels_l = j} dlp_l)
+ * with row pitch lddz.  stats and entropy are the forward's.
+ */
+int haste_label_log_probs_bwd(const void* z, int64_t ldz, const void* labels, int32_t label_bits,
+                              int64_t L, const float* stats, const float* entropy, const float* dlp,
+                              const float* dent, void* dz, int64_t lddz, int64_t B, int64_t O,
+                              int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
