@@ -4,6 +4,7 @@
 //   backward  dh with dg and du in the epilogue;  dx over both;  dWg and dWu;  dWd
 // A few tokens in serving are bound by reading the weights once and take kernels of their own.
 #include <algorithm>
+#include <cstdlib>
 
 #include "gated_mlp.hpp"
 #include "gemm.hpp"
@@ -20,35 +21,44 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void gemm_kernel(GemmArgs g, int
     Tile t;
     t.run(g, lds, p.tm, p.tn, p.batch, p.split);
     const int lane = threadIdx.x & 63;
+    constexpr int F = Tile::kDual ? Tile::FN / 2 : Tile::FN;
+    // f(row of tiles, row of C, first column of the lane, its sums)
     auto rows = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
         for (int fm = 0; fm < Tile::FM; ++fm) {
-            const int m = t.m0 + fm * 16 + (lane & 15);
-            if (m < g.M) f(fm, m);
+            f32x4 v[F], w[F];
+#pragma unroll
+            for (int k = 0; k < F; ++k) {
+                v[k] = t.acc[k][fm];
+                w[k] = t.acc[Tile::FN - F + k][fm];
+            }
+            const int n = t.n0 + gather_columns<F>(v, lane);
+            if (Tile::kDual) gather_columns<F>(w, lane);
+            f(fm, t.m0 + fm * 16 + (lane & 15), n, v, w);
         }
     };
     if constexpr (std::is_same<Epilogue, PlainOut>::value) {
-        rows([&](int fm, int m) __attribute__((always_inline)) {
-#pragma unroll
-            for (int fn = 0; fn < Tile::FN; ++fn) {
-                const int n = t.n0 + fn * 16 + 4 * (lane >> 4);
-                if (n < g.N) out.template put<DT>(p.split, p.batch, m, n, t.acc[fn][fm]);
-            }
+        rows([&](int, int m, int n, auto& v, auto&) __attribute__((always_inline)) {
+            if (m < g.M && n < g.N) out.template put<DT, F>(p.split, p.batch, m, n, v);
+        });
+    } else if constexpr (std::is_same<Epilogue, GatedGrad>::value) {
+        // the next rows' kept values are on their way while these are used
+        Kept<DT> slope[2], kept_act[2];
+        const int col = min(t.n0 + 16 * (lane >> 4), (int)out.ld - 16);
+        auto fetch = [&](int fm) __attribute__((always_inline)) {
+            const int64_t at = min(t.m0 + fm * 16 + (lane & 15), g.M - 1) * out.ld + col;
+            slope[fm & 1] = load_kept<DT>(out.slope, at);
+            kept_act[fm & 1] = load_kept<DT>(out.act, at);
+        };
+        fetch(0);
+        rows([&](int fm, int m, int n, auto& v, auto&) __attribute__((always_inline)) {
+            if (fm + 1 < Tile::FM) fetch(fm + 1);
+            if (m < g.M && n < out.ld) out.template put<DT, F>(m, n, v, slope[fm & 1], kept_act[fm & 1]);
         });
     } else {
         with_activation(act, [&](auto a) __attribute__((always_inline)) {
-            constexpr int ACT = decltype(a)::value;
-            rows([&](int fm, int m) __attribute__((always_inline)) {
-                constexpr int F = Tile::kDual ? Tile::FN / 2 : Tile::FN;
-#pragma unroll
-                for (int fn = 0; fn < F; ++fn) {
-                    const int n = t.n0 + fn * 16 + 4 * (lane >> 4);
-                    if (n >= out.ld) continue;
-                    if constexpr (Tile::kDual)
-                        out.template put<DT, ACT>(m, n, t.acc[fn][fm], t.acc[fn + F][fm]);
-                    else
-                        out.template put<DT, ACT>(m, n, t.acc[fn][fm]);
-                }
+            rows([&](int, int m, int n, auto& vg, auto& vu) __attribute__((always_inline)) {
+                if (m < g.M && n < out.ld) out.template put<DT, decltype(a)::value, F>(m, n, vg, vu);
             });
         });
     }
@@ -92,21 +102,21 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int
     for (int i = 0; i < NG * NW; ++i) sums[wave][i][lane] = acc[i];
     __syncthreads();
     for (int i = wave; i < NG; i += WAVES) {
-        f32x4 s[NW];
+        f32x4 s[NW][1];
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
-            s[j] = sums[0][i * NW + j][lane];
-            for (int v = 1; v < WAVES; ++v) s[j] += sums[v][i * NW + j][lane];
+            s[j][0] = sums[0][i * NW + j][lane];
+            for (int v = 1; v < WAVES; ++v) s[j][0] += sums[v][i * NW + j][lane];
         }
         const int m = 16 * i + r, col = blockIdx.x * 16 + 4 * (lane >> 4);
         if (m >= M) continue;
         if constexpr (DUAL) {
             if (col < out.ld)
                 with_activation(act, [&](auto a) __attribute__((always_inline)) {
-                    out.template put<DT, decltype(a)::value>(m, col, s[0], s[1]);
+                    out.template put<DT, decltype(a)::value, 1>(m, col, s[0], s[1]);
                 });
         } else {
-            if (col < N) out.template put<DT>(0, 0, m, col, s[0]);
+            if (col < N) out.template put<DT, 1>(0, 0, m, col, s[0]);
         }
     }
 }
@@ -127,6 +137,7 @@ constexpr int64_t kMaxSide = (int64_t)1 << 20;  // a tile's rows span less than 
 constexpr int kFewRows = 64;
 
 int64_t round8(int64_t n) { return ceil_div(n, 8) * 8; }
+int64_t round16(int64_t n) { return ceil_div(n, 16) * 16; }  // (the pitch of h and its like)
 
 // A matrix as the kernels take it.
 struct Matrix {
@@ -188,37 +199,46 @@ void launch_tiles(const GemmArgs& g, int batches, int act, const Epilogue& out, 
         g, batches, act, out);
 }
 
-// Tiles of 256 x 256 where they fill the GPU's 256 CUs, else of 128 x 128, two workgroups to a CU.
-template <GemmMode MODE>
-bool large_tiles(const Product& p) {
-    const int64_t cols = MODE == GemmMode::kDual ? 128 : 256, batches = MODE == GemmMode::kBatch ? 2 : 1;
-    return ceil_div(p.M, 256) * ceil_div(p.N, cols) * batches >= 192;
-}
-// Parts of K, where the tiles alone leave the GPU idle: at least eight steps to a part.
+// How a product is cut.  Tiles of 256 x 256 (a workgroup to a CU) where they fill most of the GPU's 256
+// CUs, by themselves or with K in parts; else of 128 x 128, two workgroups to a CU.
+struct Cut {
+    bool large;
+    int splits;
+};
 template <GemmMode MODE, int DT>
-int splits_of(const Product& p) {
-    const bool large = DT != HASTE_DTYPE_F32 && large_tiles<MODE>(p);
-    const int64_t side = large ? 256 : 128, batches = MODE == GemmMode::kBatch ? 2 : 1;
-    const int64_t tiles = ceil_div(p.M, side) * ceil_div(p.N, side) * batches;
+Cut cut_of(const Product& p, bool may_split) {
+    const int64_t batches = MODE == GemmMode::kBatch ? 2 : 1;
     const int64_t steps = ceil_div(p.K, 32) * (MODE == GemmMode::kSegments ? 2 : 1);
-    if (large || tiles == 0) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / 8));
+    auto tiles = [&](int64_t side) {
+        return ceil_div(p.M, side) * ceil_div(p.N, MODE == GemmMode::kDual ? side / 2 : side) * batches;
+    };
+    const int64_t big = tiles(256), small = tiles(128);
+    if (small == 0) return Cut{false, 1};
+    if (DT != HASTE_DTYPE_F32) {
+        if (big >= 192) return Cut{true, 1};
+        if (may_split && steps / 32 >= ceil_div(192, big)) return Cut{true, (int)(256 / big)};
+    }
+    return Cut{false, may_split ? (int)std::max<int64_t>(1, std::min(512 / small, steps / 8)) : 1};
 }
 
 template <int DT, GemmMode MODE, bool AK, bool BK_, typename Epilogue>
-void product(const Product& p, int splits, int act, const Epilogue& out, hipStream_t st) {
+void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_t st) {
     constexpr int batches = MODE == GemmMode::kBatch ? 2 : 1, segments = MODE == GemmMode::kSegments ? 2 : 1;
     if constexpr (DT == HASTE_DTYPE_F32) {
         typedef GemmTileF32<MODE, AK, BK_> Tile;
-        launch_tiles<Tile, DT>(gemm_args<Tile>(p, segments, splits), batches, act, out, st);
+        launch_tiles<Tile, DT>(gemm_args<Tile>(p, segments, cut.splits), batches, act, out, st);
     } else {
         typedef typename TypeOf<DT>::type T;
-        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4> Large;
-        typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2> Small;
-        if (large_tiles<MODE>(p))
-            launch_tiles<Large, DT>(gemm_args<Large>(p, segments, splits), batches, act, out, st);
+        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4, 4> Large;
+        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Mid;
+        typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2, 4> Small;
+        static const int tune = getenv("HASTE_TILE") ? atoi(getenv("HASTE_TILE")) : 0;
+        if (cut.large && tune)
+            launch_tiles<Mid, DT>(gemm_args<Mid>(p, segments, cut.splits), batches, act, out, st);
+        else if (cut.large)
+            launch_tiles<Large, DT>(gemm_args<Large>(p, segments, cut.splits), batches, act, out, st);
         else
-            launch_tiles<Small, DT>(gemm_args<Small>(p, segments, splits), batches, act, out, st);
+            launch_tiles<Small, DT>(gemm_args<Small>(p, segments, cut.splits), batches, act, out, st);
     }
 }
 
@@ -226,18 +246,19 @@ void product(const Product& p, int splits, int act, const Epilogue& out, hipStre
 // plain_parts() bytes.
 template <int DT, GemmMode MODE>
 int64_t plain_parts(const Product& p) {
-    const int splits = splits_of<MODE, DT>(p);
+    const int splits = cut_of<MODE, DT>(p, true).splits;
     return splits == 1 ? 0
-                       : splits * (MODE == GemmMode::kBatch ? 2 : 1) * p.M * (ceil_div(p.N, 4) * 4) * 4;
+                       : splits * (MODE == GemmMode::kBatch ? 2 : 1) * p.M * (ceil_div(p.N, 16) * 16) * 4;
 }
 template <int DT, GemmMode MODE, bool AK, bool BK_>
 void plain(const Product& p, void* c0, void* c1, void* parts, hipStream_t st) {
-    const int splits = splits_of<MODE, DT>(p);
+    const Cut cut = cut_of<MODE, DT>(p, true);
+    const int splits = cut.splits;
     PlainOut out{{c0, c1}, p.N, splits > 1 ? static_cast<float*>(parts) : nullptr, (int)p.M, (int)p.N,
                  MODE == GemmMode::kBatch ? 2 : 1};
-    product<DT, MODE, AK, BK_>(p, splits, 0, out, st);
+    product<DT, MODE, AK, BK_>(p, cut, 0, out, st);
     if (splits > 1) {
-        const int64_t n = out.batches * p.M * ceil_div(p.N, 4);
+        const int64_t n = out.batches * p.M * (out.pitch() / 4);
         sum_parts_kernel<DT><<<dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st>>>(out, splits);
     }
 }
@@ -302,7 +323,8 @@ int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const
     const Product p2{{h, h}, {wd, wd}, s.N, s.O, s.H};
     void* parts = ws.take(plain_parts<DT, GemmMode::kPlain>(p2));
     if (launch) {
-        product<DT, GemmMode::kDual, true, true>(p1, 1, act, out, st);
+        product<DT, GemmMode::kDual, true, true>(p1, cut_of<GemmMode::kDual, DT>(p1, false), act, out,
+                                                 st);
         plain<DT, GemmMode::kPlain, true, true>(p2, y, nullptr, parts, st);
     }
     return ws.used;
@@ -313,8 +335,8 @@ struct Grads {
 };
 
 template <int DT>
-int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matrix dy, const void* g,
-                 const void* u, const void* h, int64_t ld, const Grads& to, int act, char* base,
+int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matrix dy,
+                 const void* slope, const void* kept_act, const void* h, int64_t ld, const Grads& to, char* base,
                  bool launch, hipStream_t st) {
     Space ws{base};
     const int64_t bytes = s.N * ld * elem_bytes(DT);
@@ -333,8 +355,9 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
                                     plain_parts<DT, GemmMode::kPlain>(p4)}));
     if (launch) {
         if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
-            const GatedGrad out{g, u, dg, du, ld};
-            product<DT, GemmMode::kPlain, true, false>(p1, 1, act, out, st);
+            const GatedGrad out{slope, kept_act, dg, du, ld};
+            product<DT, GemmMode::kPlain, true, false>(p1, cut_of<GemmMode::kPlain, DT>(p1, false), 0, out,
+                                                       st);
         }
         if (s.N > 0 && to.dx) plain<DT, GemmMode::kSegments, true, false>(p2, to.dx, nullptr, parts, st);
         if (to.dwg || to.dwu) plain<DT, GemmMode::kBatch, false, false>(p3, to.dwg, to.dwu, parts, st);
@@ -395,7 +418,7 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
                                                   int32_t aligned) {
     HASTE_TRY(haste::mlp_sizes("haste_gated_mlp_workspace_size", N, D, H, O, dtype));
     const haste::Sizes s{N, D, H, O};
-    const int64_t ld = haste::round8(H);
+    const int64_t ld = haste::round16(H);
     // (an odd pitch: the matrix counts as one to be copied)
     auto any = [&](int64_t rows, int64_t cols) {
         return haste::Matrix{nullptr, aligned ? cols : cols | 1, rows, cols};
@@ -403,7 +426,7 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
     const haste::Matrix x = any(N, D), wg = any(H, D), wd = any(O, H), dy = any(N, O);
 #define HASTE_MLP(DT)                                                                                   \
     (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, nullptr, ld, haste::Grads{}, \
-                                    0, nullptr, false, nullptr)                                          \
+                                    nullptr, false, nullptr)                                          \
               : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{nullptr, nullptr, nullptr, ld},     \
                                    nullptr, 0, nullptr, false, nullptr))
     return HASTE_MLP_TYPES(HASTE_MLP);
@@ -411,8 +434,8 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
 }
 
 extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
-                               int64_t ldu, const void* wd, int64_t ldd, void* y, void* g, void* u,
-                               void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
+                               int64_t ldu, const void* wd, int64_t ldd, void* y, void* slope,
+                               void* kept_act, void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
                                int32_t dtype, void* ws, int64_t ws_bytes, void* stream) {
     const char* fn = "haste_gated_mlp";
     HASTE_TRY(haste::mlp_sizes(fn, N, D, H, O, dtype));
@@ -426,12 +449,13 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
     HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
     HASTE_CHECK_ARG(y != nullptr && haste::elem_aligned(y, dtype), "%s: y is NULL or misaligned", fn);
     HASTE_TRY(haste::mlp_hidden(fn, "h", h));
-    HASTE_CHECK_ARG((g == nullptr) == (u == nullptr), "%s: g and u are written together", fn);
-    if (g) {
-        HASTE_TRY(haste::mlp_hidden(fn, "g", g));
-        HASTE_TRY(haste::mlp_hidden(fn, "u", u));
+    HASTE_CHECK_ARG((slope == nullptr) == (kept_act == nullptr), "%s: slope and act are written together",
+                    fn);
+    if (slope) {
+        HASTE_TRY(haste::mlp_hidden(fn, "slope", slope));
+        HASTE_TRY(haste::mlp_hidden(fn, "act", kept_act));
     }
-    const haste::GatedOut out{g, u, h, haste::round8(H)};
+    const haste::GatedOut out{slope, kept_act, h, haste::round16(H)};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) haste::forward<DT>(s, mx, mg, mu, md, out, y, act, base, launch, st)
@@ -446,13 +470,12 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
 
 extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
                                    const void* wu, int64_t ldu, const void* wd, int64_t ldd,
-                                   const void* dy, int64_t lddy, const void* g, const void* u,
-                                   const void* h, void* dx, void* dwg, void* dwu, void* dwd, int64_t N,
-                                   int64_t D, int64_t H, int64_t O, int32_t act, int32_t dtype,
-                                   void* ws, int64_t ws_bytes, void* stream) {
+                                   const void* dy, int64_t lddy, const void* slope,
+                                   const void* kept_act, const void* h, void* dx, void* dwg, void* dwu, void* dwd, int64_t N,
+                                   int64_t D, int64_t H, int64_t O, int32_t dtype, void* ws,
+                                   int64_t ws_bytes, void* stream) {
     const char* fn = "haste_gated_mlp_bwd";
     HASTE_TRY(haste::mlp_sizes(fn, N, D, H, O, dtype));
-    HASTE_TRY(haste::mlp_act(fn, act));
     const haste::Sizes s{N, D, H, O};
     const haste::Matrix mx{x, ldx, N, D}, mg{wg, ldg, H, D}, mu{wu, ldu, H, D}, md{wd, ldd, O, H},
         my{dy, lddy, N, O};
@@ -466,15 +489,15 @@ extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, i
         HASTE_TRY(haste::mlp_matrix(fn, "the up weight", mu, dtype));
         HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
         HASTE_TRY(haste::mlp_matrix(fn, "dy", my, dtype));
-        HASTE_TRY(haste::mlp_hidden(fn, "g", g));
-        HASTE_TRY(haste::mlp_hidden(fn, "u", u));
+        HASTE_TRY(haste::mlp_hidden(fn, "slope", slope));
+        HASTE_TRY(haste::mlp_hidden(fn, "act", kept_act));
         HASTE_TRY(haste::mlp_hidden(fn, "h", h));
     }
     const haste::Grads to{dx, dwg, dwu, dwd};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) \
-    haste::backward<DT>(s, mx, mg, mu, md, my, g, u, h, haste::round8(H), to, act, base, launch, st)
+    haste::backward<DT>(s, mx, mg, mu, md, my, slope, kept_act, h, haste::round16(H), to, base, launch, st)
         return HASTE_MLP_TYPES(HASTE_MLP);
 #undef HASTE_MLP
     };

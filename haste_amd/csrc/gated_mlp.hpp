@@ -46,90 +46,150 @@ __device__ __forceinline__ void with_activation(int act, F f) {
     else f(std::integral_constant<int, HASTE_ACT_GELU_TANH>());
 }
 
-template <int DT>
-__device__ __forceinline__ void put4(void* p, int64_t at, f32x4 v, int64_t count) {
-    const float f[4] = {v[0], v[1], v[2], v[3]};
-    store_part<DT, 4>(p, at, pack<DT, 4>(f), count);
-}
-template <int DT>
-__device__ __forceinline__ f32x4 get4(const void* p, int64_t at) {
-    float f[4];
-    unpack<DT, 4>(load<DT, 4>(p, at), f);
-    return f32x4{f[0], f[1], f[2], f[3]};
+// 4 F columns side by side, the first `count` of them.
+template <int DT, int F>
+__device__ __forceinline__ void put_columns(void* p, int64_t at, const f32x4 (&v)[F], int64_t count) {
+    constexpr int V = DT == HASTE_DTYPE_F32 || F == 1 ? 4 : 8;
+#pragma unroll
+    for (int k = 0; k < 4 * F; k += V) {
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = v[(k + e) / 4][e % 4];
+        store_part<DT, V>(p, at + k, pack<DT, V>(f), count - k);
+    }
 }
 
-// Four columns from n of row m: h, and g and u where the backward will want them.  Rows of g, u and h are
-// ld apart, a multiple of 8 (16-bit) that holds them; columns past the extent come out as zeros.
-struct GatedOut {
-    void *g, *u, *h;
-    int64_t ld;
-    template <int DT, int ACT>
-    __device__ __forceinline__ void put(int64_t m, int n, f32x4 vg, f32x4 vu) const {
-        const int64_t at = m * ld + n, left = ld - n;
-        f32x4 vh;
+// What the forward keeps for the backward: fp32, or for 16-bit matrices its upper 24 bits (15 bits of
+// mantissa), rounded to nearest, three bytes each.  16 bits would add two roundings of the type's to the
+// gradients, which have two that cannot be helped (dg and du as the matrix instructions take them, and
+// their own): 3.1e-3 off in norm for bf16 instead of 2.3e-3.  fp32 costs a third more of their traffic.
+typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+typedef u32x3 __attribute__((aligned(4))) u32x3_a4;
+typedef u32x2 __attribute__((aligned(4))) u32x2_a4;
+template <int DT, int F>
+__device__ __forceinline__ void put_kept(void* p, int64_t at, const f32x4 (&v)[F]) {
+    if constexpr (DT == HASTE_DTYPE_F32) {
+        put_columns<DT, F>(p, at, v, 4 * F);
+    } else {
+        uint32_t w[3 * F];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float a, slope;
-            activation<ACT, DT == HASTE_DTYPE_F32>(vg[e], &a, &slope);
-            vh[e] = a * vu[e];
+        for (int k = 0; k < F; ++k) {
+            uint32_t r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = __float_as_uint(v[k][e]) + 0x80u;
+            w[3 * k] = __builtin_amdgcn_perm(r[1], r[0], 0x05030201u);
+            w[3 * k + 1] = __builtin_amdgcn_perm(r[2], r[1], 0x06050302u);
+            w[3 * k + 2] = __builtin_amdgcn_perm(r[3], r[2], 0x07060503u);
         }
-        if (g) {
-            put4<DT>(g, at, vg, left);
-            put4<DT>(u, at, vu, left);
-        }
-        put4<DT>(h, at, vh, left);
+        char* to = static_cast<char*>(p) + at * 3;
+        constexpr int n = 3 * F / 4 * 4;
+#pragma unroll
+        for (int k = 0; k < n; k += 4)
+            *reinterpret_cast<u32x4_a4*>(to + 4 * k) = u32x4{w[k], w[k + 1], w[k + 2], w[k + 3]};
+        if constexpr (n + 3 == 3 * F) *reinterpret_cast<u32x3_a4*>(to + 4 * n) = u32x3{w[n], w[n + 1], w[n + 2]};
+        if constexpr (n + 2 == 3 * F) *reinterpret_cast<u32x2_a4*>(to + 4 * n) = u32x2{w[n], w[n + 1]};
+    }
+}
+// Sixteen columns of it.
+template <int DT>
+struct Kept {
+    u32x4 w[DT == HASTE_DTYPE_F32 ? 4 : 3];
+};
+template <int DT>
+__device__ __forceinline__ Kept<DT> load_kept(const void* p, int64_t at) {
+    constexpr int n = DT == HASTE_DTYPE_F32 ? 4 : 3;
+    const char* from = static_cast<const char*>(p) + at * n;
+    Kept<DT> k;
+#pragma unroll
+    for (int i = 0; i < n; ++i) k.w[i] = reinterpret_cast<const u32x4_a4*>(from)[i];
+    return k;
+}
+// Columns 4 j .. 4 j + 3 of them.
+template <int DT>
+__device__ __forceinline__ f32x4 kept_columns(const Kept<DT>& k, int j) {
+    if constexpr (DT == HASTE_DTYPE_F32) return __builtin_bit_cast(f32x4, k.w[j]);
+    uint32_t w[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w[i] = k.w[(3 * j + i) / 4][(3 * j + i) % 4];
+    return f32x4{__uint_as_float(w[0] << 8), __uint_as_float(__builtin_amdgcn_perm(w[1], w[0], 0x0504030Cu)),
+                 __uint_as_float(__builtin_amdgcn_perm(w[2], w[1], 0x0403020Cu)),
+                 __uint_as_float(w[2] & 0xFFFFFF00u)};
+}
+
+// Columns n (a multiple of 4 F) and on of row m: h, and u act'(g) and act(g) where the backward will want
+// them.  Rows are ld apart, a multiple of 16 that holds them; columns past the extent come out as
+// zeros.
+struct GatedOut {
+    void *slope, *act, *h;
+    int64_t ld;
+    template <int DT, int ACT, int F>
+    __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&vg)[F], const f32x4 (&vu)[F]) const {
+        const int64_t at = m * ld + n;
+        f32x4 vh[F], vs[F], va[F];
+#pragma unroll
+        for (int k = 0; k < F; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float a, s;
+                activation<ACT, DT == HASTE_DTYPE_F32>(vg[k][e], &a, &s);
+                va[k][e] = a;
+                vs[k][e] = s * vu[k][e];
+                vh[k][e] = a * vu[k][e];
+            }
+        put_columns<DT, F>(h, at, vh, 4 * F);
+        if (!slope) return;
+        put_kept<DT, F>(slope, at, vs);
+        put_kept<DT, F>(act, at, va);
     }
 };
-// dg and du from dh and the forward's g and u.
+// dg and du from dh and what the forward kept.
 struct GatedGrad {
-    const void *g, *u;
+    const void *slope, *act;
     void *dg, *du;
     int64_t ld;
-    template <int DT, int ACT>
-    __device__ __forceinline__ void put(int64_t m, int n, f32x4 dh) const {
-        const int64_t at = m * ld + n;
-        const f32x4 vg = get4<DT>(g, at), vu = get4<DT>(u, at);
-        f32x4 a, b;
+    template <int DT, int F>
+    __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&dh)[F], const Kept<DT>& s,
+                                        const Kept<DT>& a) const {
+        f32x4 v[F];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float act, slope;
-            activation<ACT, DT == HASTE_DTYPE_F32>(vg[e], &act, &slope);
-            a[e] = dh[e] * vu[e] * slope;
-            b[e] = dh[e] * act;
-        }
-        put4<DT>(dg, at, a, 4);
-        put4<DT>(du, at, b, 4);
+        for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(s, k);
+        put_columns<DT, F>(dg, m * ld + n, v, 4 * F);
+#pragma unroll
+        for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(a, k);
+        put_columns<DT, F>(du, m * ld + n, v, 4 * F);
     }
 };
 
-// A product's result: C's rows, or where K is split fp32 parts [split][product][M][ceil4(N)].
+// A product's result: C's rows, or where K is split fp32 parts [split][product][M][ceil16(N)].
 struct PlainOut {
     void* c[2];
     int64_t ld;
     float* parts;
     int M, N, batches;
-    template <int DT>
-    __device__ __forceinline__ void put(int split, int batch, int64_t m, int n, f32x4 v) const {
-        if (parts) {
-            const int64_t pitch = (N + 3) / 4 * 4;
-            *reinterpret_cast<f32x4*>(parts + (((int64_t)split * batches + batch) * M + m) * pitch + n) = v;
-        } else {
-            put4<DT>(c[batch], m * ld + n, v, N - n);
-        }
+    __host__ __device__ int64_t pitch() const { return (N + 15) / 16 * 16; }
+    template <int DT, int F>
+    __device__ __forceinline__ void put(int split, int batch, int64_t m, int n, const f32x4 (&v)[F]) const {
+        if (parts)
+            put_columns<HASTE_DTYPE_F32, F>(parts,
+                                            (((int64_t)split * batches + batch) * M + m) * pitch() + n, v, 4 * F);
+        else
+            put_columns<DT, F>(c[batch], m * ld + n, v, N - n);
     }
 };
 
 // The parts of a split product, summed in order.
 template <int DT>
 __global__ __launch_bounds__(256) void sum_parts_kernel(PlainOut o, int splits) {
-    const int64_t pitch4 = (o.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t pitch4 = o.pitch() / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)o.batches * o.M * pitch4) return;
     const f32x4* p = reinterpret_cast<const f32x4*>(o.parts);
     const int64_t step = (int64_t)o.batches * o.M * pitch4;
-    f32x4 s = p[i];
-    for (int k = 1; k < splits; ++k) s += p[i + k * step];
+    f32x4 s[1] = {p[i]};
+    for (int k = 1; k < splits; ++k) s[0] += p[i + k * step];
     const int64_t row = i / pitch4, n = i % pitch4 * 4;
-    put4<DT>(o.c[row / o.M], row % o.M * o.ld + n, s, o.N - n);
+    const float f[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+    store_part<DT, 4>(o.c[row / o.M], row % o.M * o.ld + n, pack<DT, 4>(f), o.N - n);
 }
 
 }  // namespace haste

@@ -59,10 +59,11 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(n) : "memory");
 }
 
-template <typename T, GemmMode MODE, bool AK, bool BK_, int FM_, int FN_, int WM_, int WN_>
+template <typename T, GemmMode MODE, bool AK, bool BK_, int FM_, int FN_, int WM_, int WN_,
+          int STAGES>
 struct GemmTile {
     static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, kWaves = WM * WN;
-    static constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, KS = 32, kStages = 4;
+    static constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, KS = 32, kStages = STAGES;
     static constexpr int kThreads = 64 * kWaves;
     static constexpr int kABytes = BM * KS * 2, kBBytes = BN * KS * 2, kStage = kABytes + kBBytes;
     static constexpr int kLdsBytes = kStages * kStage;
@@ -72,10 +73,12 @@ struct GemmTile {
     // columns of C to a tile
     static constexpr int kCols = kDual ? BN / 2 : BN;
     static_assert(BM / 16 % kWaves == 0 && BN / 16 % kWaves == 0, "loads do not divide");
-    static_assert(2 * kLoads < 63, "vmcnt");
+    static_assert(kStages >= 3 && (kStages - 2) * kLoads < 63, "stages");
 
     f32x4 acc[FN][FM];
     int m0, n0;  // first row and column of the wave's part (DUAL: of either half)
+
+    static __device__ __forceinline__ int stage_of(int kt) { return (int)((uint32_t)kt % kStages); }
 
     // Where a lane's 16 bytes of load j lie: row and k of their first element within the tile.
     template <bool KC, int R>
@@ -151,7 +154,7 @@ struct GemmTile {
             const bool second = MODE == GemmMode::kSegments && kt >= g.steps;
             const int k = (second ? kt - g.steps : kt) * KS;
             const int left = kt < k1 ? g.K - k : 0;
-            const uint32_t to = lds0 + (kt & (kStages - 1)) * kStage;
+            const uint32_t to = lds0 + stage_of(kt) * kStage;
             const char* a = pa[second] + (AK ? (int64_t)k * 2 : k * lda);
             const char* b = pb[second] + (BK_ ? (int64_t)k * 2 : k * ldb);
             const char* b2 = kDual ? pb[1] + (BK_ ? (int64_t)k * 2 : k * ldb) : b;
@@ -165,7 +168,7 @@ struct GemmTile {
         };
         u32x4 fa[2][FM], fb[2][FN];
         auto read = [&](int kt, int set) __attribute__((always_inline)) {
-            const char* s = lds + (kt & (kStages - 1)) * kStage;
+            const char* s = lds + stage_of(kt) * kStage;
 #pragma unroll
             for (int f = 0; f < FN; ++f) {
                 const int r = kDual ? (f / (FN / 2)) * (BN / 2) + (wn * (FN / 2) + f % (FN / 2)) * 16
@@ -187,15 +190,14 @@ struct GemmTile {
 #pragma unroll
             for (int f = 0; f < FM; ++f) acc[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (k0 < k1) {
-            issue(k0);
-            issue(k0 + 1);
-            issue(k0 + 2);
-            wait_loads<2 * kLoads>();
+#pragma unroll
+            for (int i = 0; i < kStages - 1; ++i) issue(k0 + i);
+            wait_loads<(kStages - 2) * kLoads>();
             read(k0, 0);
             // (steps past the last are zeros: loaded as such, or not multiplied)
             auto step = [&](int kt, int set) __attribute__((always_inline)) {
-                wait_loads<kLoads>();
-                issue(kt + 3);
+                wait_loads<(kStages - 3) * kLoads>();
+                issue(kt + kStages - 1);
                 __builtin_amdgcn_sched_barrier(0);
                 read(kt + 1, 1 - set);
                 multiply(set);
@@ -322,6 +324,40 @@ struct GemmTileF32 {
         }
     }
 };
+
+// A lane holds columns 16 f + 4 q + 0..3 (q = lane / 16) of one row of C in v[f].  Exchanged among the
+// four lanes of the row so that each has 4 F columns side by side, from the returned one on: a row's
+// columns then leave in 16-byte stores of whole 64- or 128-byte lines.
+template <int F>
+__device__ __forceinline__ int gather_columns(f32x4 (&v)[F], int lane) {
+    static_assert(F == 2 || F == 4, "two or four tiles");
+    auto swap = [](f32x4& a, f32x4& b, auto op) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const auto r = op(__float_as_uint(a[e]), __float_as_uint(b[e]));
+            a[e] = __uint_as_float(r[0]);
+            b[e] = __uint_as_float(r[1]);
+        }
+    };
+    // odd rows of 16 lanes of a with even rows of b; the upper 32 lanes of a with the lower of b
+    auto by16 = [](uint32_t a, uint32_t b) __attribute__((always_inline)) {
+        return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    };
+    auto by32 = [](uint32_t a, uint32_t b) __attribute__((always_inline)) {
+        return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    };
+    const int q = lane >> 4;
+    swap(v[0], v[1], by16);
+    if constexpr (F == 2) {
+        return 16 * (q & 1) + 8 * (q >> 1);
+    } else {
+        swap(v[2], v[3], by16);
+        swap(v[0], v[2], by32);
+        swap(v[1], v[3], by32);
+        // (now v[0], v[1], v[2], v[3] are columns 0, 4, 8, 12 of the lane's sixteen)
+        return 16 * q;
+    }
+}
 
 // Workgroup -> (tile row, tile column, product, split): the tiles that one XCD works on at a time
 // are eight rows by a few columns of one product, whose operands meet in its L2.

@@ -39,13 +39,13 @@ at::Tensor workspace(int64_t N, const Weights& w, bool backward, bool is_aligned
 }
 
 struct Forward {
-    at::Tensor y, g, u, h;
+    at::Tensor y, slope, act, h;
 };
 Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up,
                 const at::Tensor& down, int act, bool keep) {
     const Weights w = weights_of(gate, up, down);
     const Rows r = matrix_of(x, w.D);
-    const int64_t N = r.t.size(0), ld = (w.H + 7) / 8 * 8;
+    const int64_t N = r.t.size(0), ld = (w.H + 15) / 16 * 16;
     const auto options = at::TensorOptions().dtype(x.scalar_type()).device(x.device());
     Forward f;
     std::vector<int64_t> shape = x.sizes().vec();
@@ -53,15 +53,17 @@ Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& u
     f.y = at::empty(shape, options);
     f.h = at::empty({N, ld}, options);
     if (keep) {
-        f.g = at::empty({N, ld}, options);
-        f.u = at::empty({N, ld}, options);
+        // (three bytes each, or fp32)
+        const bool wide = x.scalar_type() == at::kFloat;
+        f.slope = at::empty({N, wide ? ld : 3 * ld}, wide ? options : options.dtype(at::kByte));
+        f.act = at::empty_like(f.slope);
     }
     int64_t size;
     const at::Tensor ws =
         workspace(N, w, false, aligned({&r, &w.gate, &w.up, &w.down}), options, &size);
     call(haste_gated_mlp(ptr(r.t), r.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld, ptr(w.down.t),
-                         w.down.ld, out_ptr(f.y), out_ptr(f.g), out_ptr(f.u), out_ptr(f.h), N, w.D, w.H,
-                         w.O, act, w.code, out_ptr(ws), size, stream_of(x)));
+                         w.down.ld, out_ptr(f.y), out_ptr(f.slope), out_ptr(f.act), out_ptr(f.h), N,
+                         w.D, w.H, w.O, act, w.code, out_ptr(ws), size, stream_of(x)));
     return f;
 }
 
@@ -71,12 +73,11 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
                               const at::Tensor& up, const at::Tensor& down, int64_t act) {
         Forward f = haste_host::forward(x, gate, up, down, (int)act, true);
-        ctx->save_for_backward({x, gate, up, down, f.g, f.u, f.h});
+        ctx->save_for_backward({x, gate, up, down, f.slope, f.act, f.h});
         ctx->set_materialize_grads(false);
         ctx->saved_data["need"] =
             (int64_t)((x.requires_grad() ? kX : 0) | (gate.requires_grad() ? kGate : 0) |
                       (up.requires_grad() ? kUp : 0) | (down.requires_grad() ? kDown : 0));
-        ctx->saved_data["act"] = act;
         return f.y;
     }
 
@@ -105,9 +106,8 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
             call(haste_gated_mlp_bwd(ptr(x.t), x.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld,
                                      ptr(w.down.t), w.down.ld, ptr(dy.t), dy.ld, ptr(saved[4]),
                                      ptr(saved[5]), ptr(saved[6]), out_ptr(dx), out_ptr(dg),
-                                     out_ptr(du), out_ptr(dd), N, w.D, w.H, w.O,
-                                     (int)ctx->saved_data["act"].toInt(), w.code, out_ptr(ws), size,
-                                     stream_of(x.t)));
+                                     out_ptr(du), out_ptr(dd), N, w.D, w.H, w.O, w.code, out_ptr(ws),
+                                     size, stream_of(x.t)));
             out[0] = dx;
             if (need & kGate) out[1] = dg;
             if (need & kUp) out[2] = du;
