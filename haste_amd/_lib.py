@@ -154,11 +154,12 @@ SIGNATURES = {
     "haste_embedding_bwd": (ctypes.c_int, [_P, _I32, _P, _I64, _P, _I64, _I64, _I64, _F64, _I64, _I32,
                                            _P, _I64, _P]),
     "haste_gated_mlp_workspace_size": (_I64, [_I64, _I64, _I64, _I64, _I32, _I32, _I32]),
-    "haste_gated_mlp": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64,
-                                       _I64, _I64, _I64, _I32, _I32, _P, _I64, _P]),
+    "haste_gated_mlp_kept_size": (_I64, [_I64, _I64, _I32]),
+    "haste_gated_mlp": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
+                                       _I64, _I64, _I32, _I32, _P, _I64, _P]),
     "haste_gated_mlp_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P,
-                                           _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P,
-                                           _I64, _P]),
+                                           _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _I64,
+                                           _P]),
     "haste_label_log_probs_workspace_size": (_I64, [_I64, _I64, _I32]),
     "haste_label_log_probs": (ctypes.c_int, [_P, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _I64, _I64,
                                              _I32, _I32, _P, _I64, _P]),

@@ -4,7 +4,6 @@
 //   backward  dh with dg and du in the epilogue;  dx over both;  dWg and dWu;  dWd
 // A few tokens in serving are bound by reading the weights once and take kernels of their own.
 #include <algorithm>
-#include <cstdlib>
 
 #include "gated_mlp.hpp"
 #include "gemm.hpp"
@@ -46,9 +45,10 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void gemm_kernel(GemmArgs g, int
         Kept<DT> slope[2], kept_act[2];
         const int col = min(t.n0 + 16 * (lane >> 4), (int)out.ld - 16);
         auto fetch = [&](int fm) __attribute__((always_inline)) {
-            const int64_t at = min(t.m0 + fm * 16 + (lane & 15), g.M - 1) * out.ld + col;
-            slope[fm & 1] = load_kept<DT>(out.slope, at);
-            kept_act[fm & 1] = load_kept<DT>(out.act, at);
+            const int m = min(t.m0 + fm * 16 + (lane & 15), g.M - 1);
+            const char* block = out.kept.template block<DT>(m, col);
+            slope[fm & 1] = load_kept<DT>(block, m, col);
+            kept_act[fm & 1] = load_kept<DT>(block + kKeptBlock<DT>, m, col);
         };
         fetch(0);
         rows([&](int fm, int m, int n, auto& v, auto&) __attribute__((always_inline)) {
@@ -138,6 +138,7 @@ constexpr int kFewRows = 64;
 
 int64_t round8(int64_t n) { return ceil_div(n, 8) * 8; }
 int64_t round16(int64_t n) { return ceil_div(n, 16) * 16; }  // (the pitch of h and its like)
+int64_t kept_blocks(int64_t H) { return ceil_div(H, 64); }
 
 // A matrix as the kernels take it.
 struct Matrix {
@@ -230,12 +231,17 @@ void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_
     } else {
         typedef typename TypeOf<DT>::type T;
         typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4, 4> Large;
-        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Mid;
         typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2, 4> Small;
-        static const int tune = getenv("HASTE_TILE") ? atoi(getenv("HASTE_TILE")) : 0;
-        if (cut.large && tune)
-            launch_tiles<Mid, DT>(gemm_args<Mid>(p, segments, cut.splits), batches, act, out, st);
-        else if (cut.large)
+        if constexpr (!std::is_same<Epilogue, PlainOut>::value) {
+            // An epilogue that moves 8 to 10 bytes an element takes longer than a short K: two workgroups
+            // to a CU, of 256 x 128, overlap one's with the other's products (65536 x 2048 elements, K =
+            // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
+            // 1308, since they load half as much again).
+            typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
+            if (cut.large && p.K <= 1024)
+                return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);
+        }
+        if (cut.large)
             launch_tiles<Large, DT>(gemm_args<Large>(p, segments, cut.splits), batches, act, out, st);
         else
             launch_tiles<Small, DT>(gemm_args<Small>(p, segments, cut.splits), batches, act, out, st);
@@ -336,7 +342,7 @@ struct Grads {
 
 template <int DT>
 int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matrix dy,
-                 const void* slope, const void* kept_act, const void* h, int64_t ld, const Grads& to, char* base,
+                 void* kept, const void* h, int64_t ld, const Grads& to, char* base,
                  bool launch, hipStream_t st) {
     Space ws{base};
     const int64_t bytes = s.N * ld * elem_bytes(DT);
@@ -355,7 +361,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
                                     plain_parts<DT, GemmMode::kPlain>(p4)}));
     if (launch) {
         if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
-            const GatedGrad out{slope, kept_act, dg, du, ld};
+            const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld};
             product<DT, GemmMode::kPlain, true, false>(p1, cut_of<GemmMode::kPlain, DT>(p1, false), 0, out,
                                                        st);
         }
@@ -425,17 +431,23 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
     };
     const haste::Matrix x = any(N, D), wg = any(H, D), wd = any(O, H), dy = any(N, O);
 #define HASTE_MLP(DT)                                                                                   \
-    (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, nullptr, ld, haste::Grads{}, \
+    (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, ld, haste::Grads{}, \
                                     nullptr, false, nullptr)                                          \
-              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{nullptr, nullptr, nullptr, ld},     \
+              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{{nullptr, 0}, nullptr, ld},     \
                                    nullptr, 0, nullptr, false, nullptr))
     return HASTE_MLP_TYPES(HASTE_MLP);
 #undef HASTE_MLP
 }
 
+extern "C" int64_t haste_gated_mlp_kept_size(int64_t N, int64_t H, int32_t dtype) {
+    HASTE_TRY(haste::mlp_sizes("haste_gated_mlp_kept_size", N, 1, H, 1, dtype));
+    return haste::ceil_div(N, 16) * haste::kept_blocks(H) * 2 *
+           (dtype == HASTE_DTYPE_F32 ? haste::kKeptBlock<HASTE_DTYPE_F32> : haste::kKeptBlock<HASTE_DTYPE_BF16>);
+}
+
 extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
-                               int64_t ldu, const void* wd, int64_t ldd, void* y, void* slope,
-                               void* kept_act, void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
+                               int64_t ldu, const void* wd, int64_t ldd, void* y, void* kept,
+                               void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t act,
                                int32_t dtype, void* ws, int64_t ws_bytes, void* stream) {
     const char* fn = "haste_gated_mlp";
     HASTE_TRY(haste::mlp_sizes(fn, N, D, H, O, dtype));
@@ -449,13 +461,8 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
     HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
     HASTE_CHECK_ARG(y != nullptr && haste::elem_aligned(y, dtype), "%s: y is NULL or misaligned", fn);
     HASTE_TRY(haste::mlp_hidden(fn, "h", h));
-    HASTE_CHECK_ARG((slope == nullptr) == (kept_act == nullptr), "%s: slope and act are written together",
-                    fn);
-    if (slope) {
-        HASTE_TRY(haste::mlp_hidden(fn, "slope", slope));
-        HASTE_TRY(haste::mlp_hidden(fn, "act", kept_act));
-    }
-    const haste::GatedOut out{slope, kept_act, h, haste::round16(H)};
+    if (kept) HASTE_TRY(haste::mlp_hidden(fn, "kept", kept));
+    const haste::GatedOut out{{kept, haste::kept_blocks(H)}, h, haste::round16(H)};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) haste::forward<DT>(s, mx, mg, mu, md, out, y, act, base, launch, st)
@@ -470,8 +477,8 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
 
 extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
                                    const void* wu, int64_t ldu, const void* wd, int64_t ldd,
-                                   const void* dy, int64_t lddy, const void* slope,
-                                   const void* kept_act, const void* h, void* dx, void* dwg, void* dwu, void* dwd, int64_t N,
+                                   const void* dy, int64_t lddy, const void* kept,
+                                   const void* h, void* dx, void* dwg, void* dwu, void* dwd, int64_t N,
                                    int64_t D, int64_t H, int64_t O, int32_t dtype, void* ws,
                                    int64_t ws_bytes, void* stream) {
     const char* fn = "haste_gated_mlp_bwd";
@@ -489,15 +496,14 @@ extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, i
         HASTE_TRY(haste::mlp_matrix(fn, "the up weight", mu, dtype));
         HASTE_TRY(haste::mlp_matrix(fn, "the down weight", md, dtype));
         HASTE_TRY(haste::mlp_matrix(fn, "dy", my, dtype));
-        HASTE_TRY(haste::mlp_hidden(fn, "slope", slope));
-        HASTE_TRY(haste::mlp_hidden(fn, "act", kept_act));
+        HASTE_TRY(haste::mlp_hidden(fn, "kept", kept));
         HASTE_TRY(haste::mlp_hidden(fn, "h", h));
     }
     const haste::Grads to{dx, dwg, dwu, dwd};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) \
-    haste::backward<DT>(s, mx, mg, mu, md, my, slope, kept_act, h, haste::round16(H), to, base, launch, st)
+    haste::backward<DT>(s, mx, mg, mu, md, my, const_cast<void*>(kept), h, haste::round16(H), to, base, launch, st)
         return HASTE_MLP_TYPES(HASTE_MLP);
 #undef HASTE_MLP
     };

@@ -59,73 +59,95 @@ __device__ __forceinline__ void put_columns(void* p, int64_t at, const f32x4 (&v
     }
 }
 
-// What the forward keeps for the backward: fp32, or for 16-bit matrices its upper 24 bits (15 bits of
-// mantissa), rounded to nearest, three bytes each.  16 bits would add two roundings of the type's to the
-// gradients, which have two that cannot be helped (dg and du as the matrix instructions take them, and
-// their own): 3.1e-3 off in norm for bf16 instead of 2.3e-3.  fp32 costs a third more of their traffic.
-typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
-typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
-typedef u32x3 __attribute__((aligned(4))) u32x3_a4;
-typedef u32x2 __attribute__((aligned(4))) u32x2_a4;
+// What the forward keeps for the backward, s = u act'(g) and a = act(g): fp32, or for 16-bit matrices its
+// upper 24 bits (15 of mantissa), rounded to nearest.  16 bits would add two roundings of the type's
+// to the gradients, which have two that cannot be helped (dg and du as the matrix instructions take
+// them, and their own): 3.1e-3 off in norm for bf16 instead of 2.3e-3.
+//
+// Blocks of 16 rows x 64 columns, laid out for whole lines a load of a wave: 16-byte pieces of 8
+// columns' upper 16 bits (fp32: of 4 columns), rows side by side, then 16-byte pieces of 16 columns' next 8
+// bits; s, then a.
+template <int DT>
+constexpr int kKeptBlock = 16 * 64 * (DT == HASTE_DTYPE_F32 ? 4 : 3);
+struct KeptPlace {
+    void* p;
+    int64_t blocks;  // to a row of blocks
+    template <int DT>
+    __device__ __forceinline__ char* block(int64_t m, int n) const {
+        return static_cast<char*>(p) + ((m >> 4) * blocks + (n >> 6)) * (2 * kKeptBlock<DT>);
+    }
+};
+// 4 F columns from n (a multiple of 4 F) of row m, F at most 2.
 template <int DT, int F>
-__device__ __forceinline__ void put_kept(void* p, int64_t at, const f32x4 (&v)[F]) {
+__device__ __forceinline__ void put_kept(char* block, int64_t m, int n, const f32x4 (&v)[F]) {
+    static_assert(F <= 2, "a piece at most");
+    const int r = (int)(m & 15), c = n & 63;
     if constexpr (DT == HASTE_DTYPE_F32) {
-        put_columns<DT, F>(p, at, v, 4 * F);
+#pragma unroll
+        for (int k = 0; k < F; ++k)
+            *reinterpret_cast<f32x4*>(block + ((c / 4 + k) * 16 + r) * 16) = v[k];
     } else {
-        uint32_t w[3 * F];
+        uint32_t hi[2 * F], lo[F];
 #pragma unroll
         for (int k = 0; k < F; ++k) {
-            uint32_t r[4];
+            uint32_t b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = __float_as_uint(v[k][e]) + 0x80u;
-            w[3 * k] = __builtin_amdgcn_perm(r[1], r[0], 0x05030201u);
-            w[3 * k + 1] = __builtin_amdgcn_perm(r[2], r[1], 0x06050302u);
-            w[3 * k + 2] = __builtin_amdgcn_perm(r[3], r[2], 0x07060503u);
+            for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(v[k][e]) + 0x80u;
+            hi[2 * k] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
+            hi[2 * k + 1] = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
+            lo[k] = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0501u) |
+                    __builtin_amdgcn_perm(b[3], b[2], 0x05010C0Cu);
         }
-        char* to = static_cast<char*>(p) + at * 3;
-        constexpr int n = 3 * F / 4 * 4;
-#pragma unroll
-        for (int k = 0; k < n; k += 4)
-            *reinterpret_cast<u32x4_a4*>(to + 4 * k) = u32x4{w[k], w[k + 1], w[k + 2], w[k + 3]};
-        if constexpr (n + 3 == 3 * F) *reinterpret_cast<u32x3_a4*>(to + 4 * n) = u32x3{w[n], w[n + 1], w[n + 2]};
-        if constexpr (n + 2 == 3 * F) *reinterpret_cast<u32x2_a4*>(to + 4 * n) = u32x2{w[n], w[n + 1]};
+        char* to_hi = block + ((c / 8) * 16 + r) * 16 + (c & 7) * 2;
+        char* to_lo = block + 2048 + ((c / 16) * 16 + r) * 16 + (c & 15);
+        if constexpr (F == 2) {
+            *reinterpret_cast<u32x4*>(to_hi) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+            *reinterpret_cast<u32x2*>(to_lo) = u32x2{lo[0], lo[1]};
+        } else {
+            *reinterpret_cast<u32x2*>(to_hi) = u32x2{hi[0], hi[1]};
+            *reinterpret_cast<uint32_t*>(to_lo) = lo[0];
+        }
     }
 }
-// Sixteen columns of it.
+// Sixteen columns from n (a multiple of 16).
 template <int DT>
 struct Kept {
     u32x4 w[DT == HASTE_DTYPE_F32 ? 4 : 3];
 };
 template <int DT>
-__device__ __forceinline__ Kept<DT> load_kept(const void* p, int64_t at) {
-    constexpr int n = DT == HASTE_DTYPE_F32 ? 4 : 3;
-    const char* from = static_cast<const char*>(p) + at * n;
+__device__ __forceinline__ Kept<DT> load_kept(const char* block, int64_t m, int n) {
+    const int r = (int)(m & 15), c = n & 63;
     Kept<DT> k;
+    if constexpr (DT == HASTE_DTYPE_F32) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) k.w[i] = reinterpret_cast<const u32x4_a4*>(from)[i];
+        for (int i = 0; i < 4; ++i)
+            k.w[i] = *reinterpret_cast<const u32x4*>(block + ((c / 4 + i) * 16 + r) * 16);
+    } else {
+        k.w[0] = *reinterpret_cast<const u32x4*>(block + ((c / 8) * 16 + r) * 16);
+        k.w[1] = *reinterpret_cast<const u32x4*>(block + ((c / 8 + 1) * 16 + r) * 16);
+        k.w[2] = *reinterpret_cast<const u32x4*>(block + 2048 + ((c / 16) * 16 + r) * 16);
+    }
     return k;
 }
 // Columns 4 j .. 4 j + 3 of them.
 template <int DT>
 __device__ __forceinline__ f32x4 kept_columns(const Kept<DT>& k, int j) {
     if constexpr (DT == HASTE_DTYPE_F32) return __builtin_bit_cast(f32x4, k.w[j]);
-    uint32_t w[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) w[i] = k.w[(3 * j + i) / 4][(3 * j + i) % 4];
-    return f32x4{__uint_as_float(w[0] << 8), __uint_as_float(__builtin_amdgcn_perm(w[1], w[0], 0x0504030Cu)),
-                 __uint_as_float(__builtin_amdgcn_perm(w[2], w[1], 0x0403020Cu)),
-                 __uint_as_float(w[2] & 0xFFFFFF00u)};
+    const uint32_t h0 = k.w[j / 2][j % 2 * 2], h1 = k.w[j / 2][j % 2 * 2 + 1], lo = k.w[2][j];
+    return f32x4{__uint_as_float(__builtin_amdgcn_perm(h0, lo, 0x0504000Cu)),
+                 __uint_as_float(__builtin_amdgcn_perm(h0, lo, 0x0706010Cu)),
+                 __uint_as_float(__builtin_amdgcn_perm(h1, lo, 0x0504020Cu)),
+                 __uint_as_float(__builtin_amdgcn_perm(h1, lo, 0x0706030Cu))};
 }
 
-// Columns n (a multiple of 4 F) and on of row m: h, and u act'(g) and act(g) where the backward will want
-// them.  Rows are ld apart, a multiple of 16 that holds them; columns past the extent come out as
-// zeros.
+// Columns n (a multiple of 4 F) and on of row m: h, and s and a where the backward will want them.  Rows of
+// h are ld apart, a multiple of 16 that holds them; columns past the extent come out as zeros.
 struct GatedOut {
-    void *slope, *act, *h;
+    KeptPlace kept;
+    void* h;
     int64_t ld;
     template <int DT, int ACT, int F>
     __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&vg)[F], const f32x4 (&vu)[F]) const {
-        const int64_t at = m * ld + n;
         f32x4 vh[F], vs[F], va[F];
 #pragma unroll
         for (int k = 0; k < F; ++k)
@@ -137,15 +159,16 @@ struct GatedOut {
                 vs[k][e] = s * vu[k][e];
                 vh[k][e] = a * vu[k][e];
             }
-        put_columns<DT, F>(h, at, vh, 4 * F);
-        if (!slope) return;
-        put_kept<DT, F>(slope, at, vs);
-        put_kept<DT, F>(act, at, va);
+        put_columns<DT, F>(h, m * ld + n, vh, 4 * F);
+        if (!kept.p) return;
+        char* block = kept.template block<DT>(m, n);
+        put_kept<DT, F>(block, m, n, vs);
+        put_kept<DT, F>(block + kKeptBlock<DT>, m, n, va);
     }
 };
 // dg and du from dh and what the forward kept.
 struct GatedGrad {
-    const void *slope, *act;
+    KeptPlace kept;
     void *dg, *du;
     int64_t ld;
     template <int DT, int F>

@@ -39,7 +39,7 @@ at::Tensor workspace(int64_t N, const Weights& w, bool backward, bool is_aligned
 }
 
 struct Forward {
-    at::Tensor y, slope, act, h;
+    at::Tensor y, kept, h;
 };
 Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up,
                 const at::Tensor& down, int act, bool keep) {
@@ -53,16 +53,15 @@ Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& u
     f.y = at::empty(shape, options);
     f.h = at::empty({N, ld}, options);
     if (keep) {
-        // (three bytes each, or fp32)
-        const bool wide = x.scalar_type() == at::kFloat;
-        f.slope = at::empty({N, wide ? ld : 3 * ld}, wide ? options : options.dtype(at::kByte));
-        f.act = at::empty_like(f.slope);
+        const int64_t bytes = haste_gated_mlp_kept_size(N, w.H, w.code);
+        TORCH_CHECK(bytes >= 0, haste_last_error());
+        f.kept = at::empty({bytes}, options.dtype(at::kByte));
     }
     int64_t size;
     const at::Tensor ws =
         workspace(N, w, false, aligned({&r, &w.gate, &w.up, &w.down}), options, &size);
     call(haste_gated_mlp(ptr(r.t), r.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld, ptr(w.down.t),
-                         w.down.ld, out_ptr(f.y), out_ptr(f.slope), out_ptr(f.act), out_ptr(f.h), N,
+                         w.down.ld, out_ptr(f.y), out_ptr(f.kept), out_ptr(f.h), N,
                          w.D, w.H, w.O, act, w.code, out_ptr(ws), size, stream_of(x)));
     return f;
 }
@@ -73,7 +72,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
                               const at::Tensor& up, const at::Tensor& down, int64_t act) {
         Forward f = haste_host::forward(x, gate, up, down, (int)act, true);
-        ctx->save_for_backward({x, gate, up, down, f.slope, f.act, f.h});
+        ctx->save_for_backward({x, gate, up, down, f.kept, f.h});
         ctx->set_materialize_grads(false);
         ctx->saved_data["need"] =
             (int64_t)((x.requires_grad() ? kX : 0) | (gate.requires_grad() ? kGate : 0) |
@@ -105,7 +104,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
                 workspace(N, w, true, aligned({&x, &dy, &w.gate, &w.up, &w.down}), options, &size);
             call(haste_gated_mlp_bwd(ptr(x.t), x.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld,
                                      ptr(w.down.t), w.down.ld, ptr(dy.t), dy.ld, ptr(saved[4]),
-                                     ptr(saved[5]), ptr(saved[6]), out_ptr(dx), out_ptr(dg),
+                                     ptr(saved[5]), out_ptr(dx), out_ptr(dg),
                                      out_ptr(du), out_ptr(dd), N, w.D, w.H, w.O, w.code, out_ptr(ws),
                                      size, stream_of(x.t)));
             out[0] = dx;

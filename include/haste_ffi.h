@@ -688,9 +688,8 @@ int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, 
  * The gated feed-forward block: h = act(x wg^T) * (x wu^T), y = h wd^T, for x [N, D], wg and wu [H, D],
  * wd [O, H] of any row pitch, y [N, O] contiguous.  Products are summed in fp32; h is rounded to
  * dtype between them.  h [N, ceil16(H)] contiguous, 16-byte aligned; its columns from H on are zeros.
- * For the backward (both or neither NULL; the same shape and alignment): slope = u act'(g) and
- * act = act(g), with g = x wg^T and u = x wu^T; fp32 for f32, else the upper 24 bits of fp32, three
- * bytes each.
+ * kept: what the backward takes besides (NULL: nothing is kept), haste_gated_mlp_kept_size(N, H, dtype)
+ * bytes, 16-byte aligned: act(x wg^T) and act'(x wg^T) * (x wu^T) in fp32, for 16-bit types in 24 bits.
  * activation: HASTE_ACT_*.  dtype of all matrices: bf16, f16 or f32.  D, H and O up to 2^20, N below 2^30.
  * ws: workspace of haste_gated_mlp_workspace_size(N, D, H, O, dtype, backward, aligned) bytes (16-byte
  * aligned).  16-bit rows that do not start on 16 bytes, or are no multiple of 8 long, are copied into
@@ -702,21 +701,22 @@ int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, 
 
 int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t H, int64_t O, int32_t dtype,
                                        int32_t backward, int32_t aligned);
+int64_t haste_gated_mlp_kept_size(int64_t N, int64_t H, int32_t dtype);
 int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
-                    int64_t ldu, const void* wd, int64_t ldd, void* y, void* slope, void* act,
-                    void* h, int64_t N, int64_t D, int64_t H, int64_t O, int32_t activation,
+                    int64_t ldu, const void* wd, int64_t ldd, void* y, void* kept, void* h,
+                    int64_t N, int64_t D, int64_t H, int64_t O, int32_t activation,
                     int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /*
- * Its gradients, from the slope, act and h of the forward:
- *   dh = dy wd;  dg = dh slope, du = dh act  (rounded to dtype);
+ * Its gradients, from the kept and h of the forward:
+ *   dh = dy wd;  dg = dh act'(g) u, du = dh act(g)  (rounded to dtype);
  *   dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h,
  * all contiguous.  dx, dwd, or dwg together with dwu may be NULL (not computed).
  */
 int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
                         int64_t ldu, const void* wd, int64_t ldd, const void* dy, int64_t lddy,
-                        const void* slope, const void* act, const void* h, void* dx, void* dwg,
-                        void* dwu, void* dwd, int64_t N, int64_t D, int64_t H, int64_t O,
+                        const void* kept, const void* h, void* dx, void* dwg, void* dwu, void* dwd,
+                        int64_t N, int64_t D, int64_t H, int64_t O,
                         int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /*
