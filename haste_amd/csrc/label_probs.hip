@@ -28,6 +28,22 @@ __device__ __forceinline__ void rescale(Sums& a, float m) {
     a.s *= f;
     a.m = m;
 }
+// What terms of maximum m are taken relative to: 2^(z log2 e - r) takes one operation where e^(z - m) takes
+// two, with r = m log2 e rounded; `off`, the rounding, is made good in the sums.  Far from zero the
+// rounding is too large for that, and (z - m) log2 e is taken.
+constexpr float kLn2 = 0.69314718056f;
+struct Reference {
+    float r, off, scale;  // off = m log2 e - r, scale = 2^-off
+    bool far;             // (of any lane)
+};
+__device__ __forceinline__ Reference reference(float m) {
+    Reference ref{m * kLog2e, 0.f, 1.f, (bool)__any(!(fabsf(m) < 1024.f))};
+    if (!ref.far) {
+        ref.off = __builtin_fmaf(m, kLog2e, -ref.r);
+        ref.scale = __builtin_fmaf(-kLn2, ref.off, 1.f);
+    }
+    return ref;
+}
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
     const float m = fmaxf(a.m, b.m);
     rescale(a, m);
@@ -50,68 +66,56 @@ __device__ __forceinline__ float value_of(Key k) {
 }
 __device__ __forceinline__ uint32_t label_of(Key k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
-// Sorts 64 R keys of a wave, largest first; key r * 64 + lane is k[r] of that lane.
-template <int R>
-__device__ __forceinline__ void sort_keys(Key (&k)[R], int lane) {
-#pragma unroll
-    for (int size = 2; size <= 64 * R; size *= 2)
-#pragma unroll
-        for (int stride = size / 2; stride > 0; stride /= 2) {
-            if (stride >= 64) {
-                const int rs = stride / 64;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-                    if (!(r & rs)) {
-                        const bool down = ((r * 64 + lane) & size) == 0;
-                        const Key a = k[r], b = k[r | rs];
-                        k[r] = (a > b) == down ? a : b;
-                        k[r | rs] = (a > b) == down ? b : a;
-                    }
-            } else {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const Key o = __shfl_xor(k[r], stride);
-                    const bool most = (((r * 64 + lane) & size) == 0) == ((lane & stride) == 0);
-                    k[r] = (k[r] > o) == most ? k[r] : o;
-                }
-            }
-        }
-}
-
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
 
-// A wave's list of candidates in LDS, of 64 R keys.  Whenever fewer than 64 places are free it is
-// sorted and cut to its largest K, and the K-th is what a key has to exceed from then on; `shared`
-// holds the largest such bound of the workgroup.
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// A wave's list of candidates in LDS, of 64 R keys.  Whenever fewer than 64 places are free it is cut to
+// its largest K, in order, and the K-th is what a key has to exceed from then on; `shared` holds the
+// largest such bound of the workgroup.
 template <int R>
 struct Candidates {
     Key* buf;
     Key* shared;
     int K, count, lane;
-    Key bound;     // (0: every key passes)
-    float least;   // its logit, NaN for none
-
-    __device__ __forceinline__ void raise(Key b) {
-        if (b > bound) {
-            bound = b;
-            least = value_of(b);
-        }
-    }
+    Key bound;
+    // Every key goes to the place that the number of larger ones gives: fewer steps that wait for one
+    // another than a sorting network has, and as many as there are keys.
     __device__ __forceinline__ void cut() {
         Key k[R];
+        int rank[R];
         wave_sync();
 #pragma unroll
-        for (int r = 0; r < R; ++r) k[r] = r * 64 + lane < count ? buf[r * 64 + lane] : 0;
-        sort_keys<R>(k, lane);
+        for (int r = 0; r < R; ++r) {
+            k[r] = r * 64 + lane < count ? buf[r * 64 + lane] : 0;
+            rank[r] = 0;
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r) buf[r * 64 + lane] = k[r];
+        for (int r = 0; r < R; ++r) {
+            const int n = min(64, count - r * 64);
+            for (int j = 0; j < n; ++j) {
+                const Key o = (Key)lane_value((uint32_t)(k[r] >> 32), j) << 32 | lane_value((uint32_t)k[r], j);
+#pragma unroll
+                for (int q = 0; q < R; ++q) rank[q] += o > k[q] ? 1 : 0;
+            }
+        }
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r * 64 + lane < count) {
+                if (rank[r] < K) buf[rank[r]] = k[r];
+            } else if (r * 64 + lane < K) {
+                buf[r * 64 + lane] = 0;
+            }
         wave_sync();
         if (count >= K) {
             count = K;
-            raise(buf[K - 1]);
+            bound = max(bound, buf[K - 1]);
             if (lane == 0) atomicMax(shared, bound);
         }
     }
@@ -124,8 +128,27 @@ struct Candidates {
         count += __popcll(mask);
         if (count > 64 * (R - 1)) cut();
     }
-    __device__ __forceinline__ void refresh() { raise(*(volatile Key*)shared); }
+    __device__ __forceinline__ void refresh() { bound = max(bound, *(volatile Key*)shared); }
 };
+
+// The K-th largest of the wave's 64 R values, as a key that every label with such a logit exceeds.
+template <int R>
+__device__ __forceinline__ Key bound_of(const uint32_t (&u)[R], int K) {
+    int rank[R] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        for (int j = 0; j < 64; ++j) {
+            const uint32_t o = lane_value(u[r], j);
+#pragma unroll
+            for (int q = 0; q < R; ++q) rank[q] += o > u[q] ? 1 : 0;
+        }
+    // the smallest number that fewer than K exceed
+    uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int r = 0; r < R; ++r) least = rank[r] < K ? min(least, u[r]) : least;
+    for (int o = 32; o; o >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, o));
+    return (Key)least << 32;
+}
 
 constexpr int buffer_keys(int R) { return R ? 64 * R : 1; }
 
@@ -157,7 +180,7 @@ __device__ __forceinline__ void join_waves(Shared<R>& sh, Sums& a, Candidates<R 
     for (int w = 1; w < kWaves; ++w) a = join(a, sh.sums[w]);
     if constexpr (R > 0) {
         if (wave == 0) {
-            // (the bound itself is in some wave's list)
+            // (the key that is the bound may be in another wave's list)
             c.bound = sh.bound ? sh.bound - 1 : 0;
             for (int w = 1; w < kWaves; ++w)
                 for (int i = 0; i < sh.count[w]; i += 64)
@@ -206,6 +229,7 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
                                                       int64_t per, Out out, Sums* part,
                                                       Key* part_keys, int64_t row0) {
     constexpr int SZ = kElemBytes<DT>, V = 16 / SZ;
+    typedef Elems<DT, V> Vec;
     __shared__ Shared<R> sh;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t row = row0 + blockIdx.x / S;
@@ -215,46 +239,175 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
     const int64_t nv = (off + O + V - 1) / V;
     const int64_t v1 = min(nv, (c + 1) * per);
     Sums a = no_sums();
-    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0,
-                                __uint_as_float(0x7FC00000u)};
-    if (R) {
-        if (threadIdx.x == 0) sh.bound = 0;
-        __syncthreads();
-    }
-    for (int64_t v = c * per + wave * 64; v < v1; v += kThreads) {
-        const int64_t e0 = (v + lane) * V - off;
-        float f[V];
-        if (v + lane < v1 && e0 >= 0 && e0 + V <= O) {
-            unpack<DT, V>(load<DT, V>(p, e0), f);
-        } else {
+    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0};
+    // Lane's vector v; what is not the part's is -infinity.
+    auto fetch = [&](int64_t v) __attribute__((always_inline)) {
+        const int64_t e0 = v * V - off;
+        constexpr uint32_t none = DT == HASTE_DTYPE_F32    ? 0xFF800000u
+                                  : DT == HASTE_DTYPE_BF16 ? 0xFF80FF80u
+                                                           : 0xFC00FC00u;
+        Vec q;
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                f[e] = v + lane < v1 && e0 + e >= 0 && e0 + e < O ? load_elem<DT>(p, e0 + e)
-                                                                  : -__builtin_inff();
-        }
-        float most = f[0];
-#pragma unroll
-        for (int e = 1; e < V; ++e) most = fmaxf(most, f[e]);
-        rescale(a, fmaxf(a.m, most));
+        for (int i = 0; i < 4; ++i) q.q[i] = none;
+        if (v >= v1) return q;
+        if (e0 >= 0 && e0 + V <= O) return load<DT, V>(p, e0);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float d = f[e] - a.m, x = __builtin_amdgcn_exp2f(d * kLog2e);
-            a.s += x;
-            a.t = __builtin_fmaf(x, fmaxf(d, kGone), a.t);
+            if (e0 + e < 0 || e0 + e >= O) continue;
+            if constexpr (DT == HASTE_DTYPE_F32) {
+                q.q[e] = reinterpret_cast<const uint32_t*>(p)[e0 + e];
+            } else {
+                const uint32_t h = reinterpret_cast<const uint16_t*>(p)[e0 + e];
+                q.q[e / 2] = (e & 1) ? (q.q[e / 2] & 0xFFFFu) | h << 16 : (q.q[e / 2] & 0xFFFF0000u) | h;
+            }
         }
-        if constexpr (R > 0) {
-            // (a NaN hides from `most`, but not from the sum)
-            if (__any(!(most < top.least) || a.s != a.s)) {
-                top.refresh();
+        return q;
+    };
+    constexpr int U = 2, G = R ? R / 2 : 1;
+    const int64_t v0 = c * per + wave * 64;
+    float most[G];  // of the lane's logits, in G groups by turns
+#pragma unroll
+    for (int g = 0; g < G; ++g) most[g] = -__builtin_inff();
+    Reference ref = reference(a.m);
+    auto step = [&](const Vec (&q)[U]) __attribute__((always_inline)) {
+        float f[U * V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) unpack<DT, V>(q[u], f + u * V);
+        float top_of_step = -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float x = f[g * U * V / G];
+#pragma unroll
+            for (int e = 1; e < U * V / G; ++e) x = fmaxf(x, f[g * U * V / G + e]);
+            most[g] = fmaxf(most[g], x);
+            top_of_step = fmaxf(top_of_step, x);
+        }
+        // (terms up to e^2 lose nothing, and a new maximum by more is rare)
+        if (__any(top_of_step > a.m + 2.f)) {
+            rescale(a, fmaxf(a.m, top_of_step));
+            ref = reference(a.m);
+        }
+        float s = 0.f, t = 0.f;
+        if (!ref.far) {
+#pragma unroll
+            for (int e = 0; e < U * V; ++e) {
+                const float w = __builtin_fmaf(f[e], kLog2e, -ref.r), x = __builtin_amdgcn_exp2f(w);
+                s += x;
+                t = __builtin_fmaf(x, fmaxf(w, kGone), t);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < U * V; ++e) {
+                const float w = (f[e] - a.m) * kLog2e, x = __builtin_amdgcn_exp2f(w);
+                s += x;
+                t = __builtin_fmaf(x, fmaxf(w, kGone), t);
+            }
+        }
+        a.s = __builtin_fmaf(s, ref.scale, a.s);
+        a.t = __builtin_fmaf(__builtin_fmaf(-ref.off, s, t), ref.scale * kLn2, a.t);
+    };
+    // two vectors a step, the next two on their way; [in0, in1): steps whose vectors are whole
+    const int64_t stride = U * kThreads, steps = v0 < v1 ? (v1 - v0 + stride - 1) / stride : 0;
+    const int64_t whole = min(v1, (off + O) / V);  // (vectors behind it are not whole)
+    const int64_t in1 = max((int64_t)0, (whole - v0 - (U - 1) * kThreads - 64 + stride) / stride);
+    Vec q[U], next[U];
+    auto edge = [&](int64_t i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = fetch(v0 + i * stride + u * kThreads + lane);
+    };
+    int64_t i = 0;
+    if (v0 * V < off && steps > 0) {
+        edge(i++);
+        step(q);
+    }
+    if (i < in1) {
+        const char* at = p + ((v0 + i * stride + lane) * V - off) * SZ;
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = load<DT, V>(at, (int64_t)u * kThreads * V);
+        for (; i < in1; ++i) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) q[u] = next[u];
+            at += i + 1 < in1 ? stride * 16 : 0;  // (the last step's are read again)
+#pragma unroll
+            for (int u = 0; u < U; ++u) next[u] = load<DT, V>(at, (int64_t)u * kThreads * V);
+            step(q);
+        }
+    }
+    for (; i < steps; ++i) {
+        edge(i);
+        step(q);
+    }
+    {
+        float m = a.m;
+#pragma unroll
+        for (int g = 0; g < G; ++g) m = fmaxf(m, most[g]);
+        rescale(a, m);
+    }
+    if constexpr (R > 0) {
+        // K of the wave's 64 G groups reach the K-th largest of their maxima, so K labels do, and no label
+        // under it is among the K likeliest.  Only the groups that reach it are read again: a few.
+        uint32_t reach[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g)  // (a NaN hides from the maxima, but not from the sum)
+            reach[g] = (uint32_t)(key_of(a.s != a.s ? a.s : most[g], 0) >> 32);
+        const Key b = bound_of<G>(reach, K);
+        if (threadIdx.x == 0) sh.bound = 0;
+        __syncthreads();
+        if (lane == 0) atomicMax(&sh.bound, b);
+        __syncthreads();
+        top.refresh();
+        // (four of a lane's vectors at a time: their loads do not wait for one another)
+        constexpr int B = 4;
+        auto scan = [&](const int64_t (&v)[B], int n) __attribute__((always_inline)) {
+            Vec w[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k)
+                if (k < n) w[k] = fetch(v[k]);
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                if (k >= n) break;
+                float f[V];
+                unpack<DT, V>(w[k], f);
+                const float least = value_of(top.bound);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const int64_t i = e0 + e;
-                    top.add(v + lane < v1 && i >= 0 && i < O ? key_of(f[e], (uint32_t)i) : 0);
+                    if (!__any(!(f[e] < least))) continue;
+                    const int64_t i = v[k] * V - off + e;
+                    top.add(v[k] < v1 && i >= 0 && i < O ? key_of(f[e], (uint32_t)i) : 0);
+                }
+            }
+        };
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const bool in = reach[g] >= (uint32_t)(top.bound >> 32);
+            uint64_t mask = __ballot(in);
+            const int64_t n = v0 < v1 ? (v1 - v0 + kThreads - 1) / kThreads : 0;  // vectors of a lane
+            int64_t v[B];
+            if (n <= (int64_t)__popcll(mask) * G) {
+                for (int64_t j = g; j < n; j += B * G) {
+#pragma unroll
+                    for (int k = 0; k < B; ++k)
+                        v[k] = in && j + k * G < n ? v0 + (j + k * G) * kThreads + lane : v1;
+                    scan(v, (int)min((int64_t)B, (n - j + G - 1) / G));
+                }
+            } else {
+                while (mask) {
+                    int l[B];
+                    const int lanes = min(B, (int)__popcll(mask));
+#pragma unroll
+                    for (int k = 0; k < B; ++k) {
+                        l[k] = mask ? __builtin_ctzll(mask) : -1;
+                        mask &= mask - 1;
+                    }
+                    for (int64_t j = g + (int64_t)lane * G; j - (int64_t)lane * G < n; j += 64 * G) {
+#pragma unroll
+                        for (int k = 0; k < B; ++k) v[k] = l[k] >= 0 && j < n ? v0 + j * kThreads + l[k] : v1;
+                        scan(v, lanes);
+                    }
                 }
             }
         }
     }
-    if (R) top.cut();
     join_waves<R>(sh, a, top);
     if (S == 1) {
         write_row<DT>(p, labels, wide, L, O, K, row, a, sh.buf[0], out);
@@ -277,15 +430,21 @@ __global__ __launch_bounds__(kThreads) void lp_join_kernel(const char* z, int64_
     const int64_t row = row0 + blockIdx.x;
     Sums a = no_sums();
     for (int i = threadIdx.x; i < S; i += kThreads) a = join(a, part[row * S + i]);
-    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0,
-                                __uint_as_float(0x7FC00000u)};
+    Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0};
     if constexpr (R > 0) {
         if (threadIdx.x == 0) sh.bound = 0;
         __syncthreads();
         const int64_t n = (int64_t)S * K;
+        constexpr int G = R / 2;
+        uint32_t reach[G] = {};
+        for (int64_t i = threadIdx.x, j = 0; i < n; i += kThreads, ++j)
+            reach[j % G] = max(reach[j % G], (uint32_t)(part_keys[row * n + i] >> 32));
+        const Key b = bound_of<G>(reach, K);  // (as in the parts)
+        if (lane == 0) atomicMax(&sh.bound, b);
+        __syncthreads();
+        top.refresh();
         for (int64_t i = wave * 64; i < n; i += kThreads)
             top.add(i + lane < n ? part_keys[row * n + i + lane] : 0);
-        top.cut();
     }
     join_waves<R>(sh, a, top);
     write_row<DT>(z + row * ldz * kElemBytes<DT>, labels, wide, L, O, K, row, a, sh.buf[0], out);
@@ -347,12 +506,20 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(const char* z, int64_t
     }
 }
 
-// Parts of a row: eight workgroups to a compute unit where there are few rows, and at least a vector to
-// a thread.
-int parts(int64_t B, int64_t O, int32_t dtype) {
-    const int64_t vectors = ceil_div(O, 16 / elem_bytes(dtype)) + 1;
-    return (int)std::max<int64_t>(
-        1, std::min<int64_t>({ceil_div(2048, std::max<int64_t>(B, 1)), vectors / kThreads, 256}));
+// How a row is cut: `per` 16-byte vectors to a part, whole steps of a workgroup's.  Four workgroups to a CU
+// (512 rows of 131,073: 48 us, with eight 64), in as many parts as there are steps; but a row of up to 8
+// steps is not cut where there is one for each CU, since joining parts takes a launch more (5 to 8 us).
+constexpr int64_t kStep = 2 * kThreads;
+struct Cut {
+    int64_t per;
+    int parts;
+};
+Cut cut_of(int64_t B, int64_t O, int32_t dtype) {
+    const int64_t vectors = ceil_div(O, 16 / elem_bytes(dtype)) + 1, steps = ceil_div(vectors, kStep);
+    if (B >= 256 && steps <= 8) return Cut{steps * kStep, 1};
+    const int64_t parts = std::min<int64_t>({ceil_div(1024, std::max<int64_t>(B, 1)), steps, 256});
+    const int64_t per = ceil_div(steps, parts);
+    return Cut{per * kStep, (int)ceil_div(steps, per)};
 }
 
 int lp_check(const char* fn, const void* z, int64_t ldz, const void* labels, int32_t label_bits,
@@ -388,8 +555,8 @@ void in_launches(int64_t B, int64_t S, F f) {
     } while (0)
 
 int64_t lp_workspace(int64_t B, int64_t O, int64_t K) {
-    // (fp32's parts are the most)
-    const int64_t S = parts(B, O, HASTE_DTYPE_F32);
+    int64_t S = 1;
+    for (int32_t dtype : {HASTE_DTYPE_BF16, HASTE_DTYPE_F32}) S = std::max<int64_t>(S, cut_of(B, O, dtype).parts);
     return S == 1 ? 0 : ceil_div(B * S * (int64_t)sizeof(Sums), 16) * 16 + B * S * K * 8;
 }
 
@@ -423,7 +590,8 @@ extern "C" int haste_label_log_probs(const void* z, int64_t ldz, const void* lab
                                haste::elem_aligned(top, HASTE_DTYPE_F32) &&
                                reinterpret_cast<uintptr_t>(top_labels) % 8 == 0),
                     "%s: top or top_labels is NULL or misaligned", fn);
-    const int S = haste::parts(B, O, dtype);
+    const haste::Cut cut = haste::cut_of(B, O, dtype);
+    const int S = cut.parts;
     if (S > 1) {
         const int64_t need = haste::lp_workspace(B, O, K);
         HASTE_CHECK_ARG(ws != nullptr && haste::aligned16(ws), "%s: workspace is NULL or misaligned",
@@ -434,8 +602,6 @@ extern "C" int haste_label_log_probs(const void* z, int64_t ldz, const void* lab
             return HASTE_ERR_WORKSPACE;
         }
     }
-    const int64_t V = 16 / haste::elem_bytes(dtype);
-    const int64_t per = haste::ceil_div(haste::ceil_div(O, V) + 1, S);
     auto* part = static_cast<haste::Sums*>(ws);
     auto* keys = reinterpret_cast<haste::Key*>(
         static_cast<char*>(ws) + haste::ceil_div(B * S * (int64_t)sizeof(haste::Sums), 16) * 16);
@@ -453,7 +619,7 @@ extern "C" int haste_label_log_probs(const void* z, int64_t ldz, const void* lab
                     : K <= 32 ? haste::lp_join_kernel<DT, 2>                                       \
                               : haste::lp_join_kernel<DT, 4>;                                      \
         kernel<<<dim3((unsigned)(n * S)), dim3(haste::kThreads), 0, st>>>(                         \
-            zc, ldz, labels, wide, L, O, K, S, per, out, part, keys, r0);                          \
+            zc, ldz, labels, wide, L, O, K, S, cut.per, out, part, keys, r0);                          \
         if (S > 1)                                                                                 \
             join<<<dim3((unsigned)n), dim3(haste::kThreads), 0, st>>>(zc, ldz, labels, wide, L, O, \
                                                                       K, S, out, part, keys, r0);  \
