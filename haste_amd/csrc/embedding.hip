@@ -52,9 +52,11 @@ __global__ __launch_bounds__(kThreads) void emb_kernel(const void* tokens, int w
 
 // ------------------------------------------------------------------ sort ----
 // Positions by token, stable: passes over digits of the token, least significant first.  A pass
-// counts each tile's digits, turns the counts into first places (bins in order, tiles in order
-// within a bin), and moves.  Tokens that take no gradient are keyed V, behind all others.
-constexpr int kTile = 2048, kMaxBins = 1024;
+// counts each tile's digits, turns the counts into first places (digits in order, tiles in order
+// within a digit), and moves.  Tokens that take no gradient are keyed V, behind all others.
+// Up to kSmall tokens are sorted by one workgroup in LDS, all passes in one launch.
+constexpr int kTile = 1024, kMaxBins = 1024, kOwnScan = 64;
+constexpr int kSmall = 2048, kSmallThreads = 1024;
 
 __device__ __forceinline__ uint32_t sort_key(const void* tokens, bool wide, int64_t i, int64_t V,
                                              int64_t padding) {
@@ -68,119 +70,255 @@ struct SortPass {
     int64_t V, padding;
     const uint32_t *key_in, *at_in;
     uint32_t *key_out, *at_out;
-    uint32_t* counts;              // [bins][tiles]
+    uint32_t* counts;
     int64_t N;
-    int tiles, shift, bins;
+    int tiles, shift, bits;
 };
+
+// Counts lie by digit and tile for sort_scan_kernel, by tile and digit for the tiles' own sums.
+__device__ __forceinline__ int64_t count_at(const SortPass& p, int digit, int tile) {
+    return p.tiles > kOwnScan ? (int64_t)digit * p.tiles + tile : ((int64_t)tile << p.bits) + digit;
+}
 
 __global__ __launch_bounds__(kThreads) void sort_count_kernel(SortPass p) {
     __shared__ uint32_t hist[kMaxBins];
-    for (int b = threadIdx.x; b < p.bins; b += kThreads) hist[b] = 0;
+    const int bins = 1 << p.bits;
+    for (int b = threadIdx.x; b < bins; b += kThreads) hist[b] = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)blockIdx.x * kTile;
-    for (int k = threadIdx.x; k < kTile && i0 + k < p.N; k += kThreads) {
-        const uint32_t key =
-            p.tokens ? sort_key(p.tokens, p.wide, i0 + k, p.V, p.padding) : p.key_in[i0 + k];
-        atomicAdd(&hist[(key >> p.shift) & (p.bins - 1)], 1u);
+#pragma unroll
+    for (int k = 0; k < kTile; k += kThreads) {
+        const int64_t i = i0 + k + threadIdx.x;
+        if (i >= p.N) break;
+        const uint32_t key = p.tokens ? sort_key(p.tokens, p.wide, i, p.V, p.padding) : p.key_in[i];
+        atomicAdd(&hist[(key >> p.shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < p.bins; b += kThreads)
-        p.counts[(int64_t)b * p.tiles + blockIdx.x] = hist[b];
+    for (int b = threadIdx.x; b < bins; b += kThreads) p.counts[count_at(p, b, blockIdx.x)] = hist[b];
 }
 
-// counts [n] to the sums of those before, one workgroup.
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int64_t n) {
-    __shared__ uint32_t wave_sum[16];
+// The sum of x over the threads before, and over all of them in `all`.  share [THREADS / 64].
+template <int THREADS>
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* share, uint32_t* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t in = x;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t y = __shfl_up(in, o);
+        if (lane >= o) in += y;
+    }
+    __syncthreads();
+    if (lane == 63) share[wave] = in;
+    __syncthreads();
+    uint32_t before = in - x;
+    *all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        before += w < wave ? share[w] : 0;
+        *all += share[w];
+    }
+    return before;
+}
+
+// counts [n] to the sums of those before, one workgroup (for more than kOwnScan tiles).
+__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int64_t n) {
+    __shared__ uint32_t share[16];
     uint32_t base = 0;
     for (int64_t i0 = 0; i0 < n; i0 += 4096) {
         const int64_t i = i0 + threadIdx.x * 4;
-        uint32_t c[4], s = 0;
+        uint32_t c[4], s = 0, all;
         for (int k = 0; k < 4; ++k) {
             c[k] = i + k < n ? counts[i + k] : 0;
             s += c[k];
         }
-        uint32_t in = s;
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t x = __shfl_up(in, o);
-            if (lane >= o) in += x;
-        }
-        if (lane == 63) wave_sum[wave] = in;
-        __syncthreads();
-        uint32_t before = base, all = 0;
-        for (int w = 0; w < 16; ++w) {
-            before += w < wave ? wave_sum[w] : 0;
-            all += wave_sum[w];
-        }
-        uint32_t at = before + in - s;
+        uint32_t at = base + sum_before<1024>(s, share, &all);
         for (int k = 0; k < 4; ++k) {
             if (i + k < n) counts[i + k] = at;
             at += c[k];
         }
         base += all;
-        __syncthreads();
     }
+}
+
+// The lanes of the wave with the same digit, of those `in`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool in) {
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot((d >> b & 1) != 0);
+        same &= (d >> b & 1) ? set : ~set;
+    }
+    return same;
+}
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// The place of a lane's key, from the next place of its digit in the wave's keys (in order).
+__device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, int bits, bool in, int lane) {
+    const uint64_t same = same_digit(d, bits, in);
+    uint32_t at = 0;
+    if (in) at = next[d] + __popcll(same & (((uint64_t)1 << lane) - 1));
+    wave_sync();
+    // (the last of them moves the place on, after all have read it)
+    if (in && (same >> lane) == 1) next[d] += __popcll(same);
+    wave_sync();
+    return at;
 }
 
 __global__ __launch_bounds__(kThreads) void sort_move_kernel(SortPass p) {
     constexpr int kWaves = kThreads / 64, kPer = kTile / kWaves;
     __shared__ uint32_t next[kWaves][kMaxBins];  // counts of the waves' parts, then their next places
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int b = threadIdx.x; b < kWaves * kMaxBins; b += kThreads) (&next[0][0])[b] = 0;
-    __syncthreads();
+    __shared__ uint32_t share[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << p.bits;
+    // (all loads first: none of them waits for another)
     const int64_t i0 = (int64_t)blockIdx.x * kTile + wave * kPer;
-    uint32_t key[kPer / 64];
+    uint32_t key[kPer / 64], from[kPer / 64];
 #pragma unroll
     for (int k = 0; k < kPer / 64; ++k) {
-        const int64_t i = i0 + k * 64 + lane;
-        key[k] = 0;
-        if (i < p.N) {
-            key[k] = p.tokens ? sort_key(p.tokens, p.wide, i, p.V, p.padding) : p.key_in[i];
-            atomicAdd(&next[wave][(key[k] >> p.shift) & (p.bins - 1)], 1u);
+        const int64_t i = min(i0 + k * 64 + lane, p.N - 1);
+        key[k] = p.tokens ? sort_key(p.tokens, p.wide, i, p.V, p.padding) : p.key_in[i];
+        from[k] = p.at_in ? p.at_in[i] : (uint32_t)i;
+    }
+    constexpr int kOwn = kMaxBins / kThreads;  // digits to a thread
+    uint32_t before[kOwn] = {}, sum[kOwn] = {};
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int b = j * kThreads + threadIdx.x;
+        if (b >= bins) break;
+        if (p.tiles > kOwnScan) {
+            before[j] = p.counts[count_at(p, b, blockIdx.x)];
+        } else {  // summed here: a launch less than by sort_scan_kernel
+#pragma unroll 16
+            for (int t = 0; t < p.tiles; ++t) {
+                const uint32_t c = p.counts[count_at(p, b, t)];
+                before[j] += t < (int)blockIdx.x ? c : 0;
+                sum[j] += c;
+            }
         }
     }
+    for (int b = lane; b < bins; b += 64) next[wave][b] = 0;
+    wave_sync();
+#pragma unroll
+    for (int k = 0; k < kPer / 64; ++k)
+        if (i0 + k * 64 + lane < p.N) atomicAdd(&next[wave][(key[k] >> p.shift) & (bins - 1)], 1u);
     __syncthreads();
-    for (int b = threadIdx.x; b < p.bins; b += kThreads) {
-        uint32_t at = p.counts[(int64_t)b * p.tiles + blockIdx.x];
-        for (int w = 0; w < kWaves; ++w) {
-            const uint32_t c = next[w][b];
-            next[w][b] = at;
-            at += c;
+    uint32_t base = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int b = j * kThreads + threadIdx.x;
+        if (j * kThreads >= bins) break;
+        uint32_t at = before[j], all;
+        if (p.tiles <= kOwnScan) {
+            at += base + sum_before<kThreads>(sum[j], share, &all);
+            base += all;
         }
+        if (b < bins)
+            for (int w = 0; w < kWaves; ++w) {
+                const uint32_t c = next[w][b];
+                next[w][b] = at;
+                at += c;
+            }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kPer / 64; ++k) {
-        const int64_t i = i0 + k * 64 + lane;
-        const bool in = i < p.N;
-        const uint32_t d = (key[k] >> p.shift) & (p.bins - 1);
-        // the wave's lanes with the same digit
-        uint64_t same = __ballot(in);
-        for (int b = 1; b < p.bins; b *= 2) {
-            const uint64_t set = __ballot((d & b) != 0);
-            same &= (d & b) ? set : ~set;
-        }
+        const bool in = i0 + k * 64 + lane < p.N;
+        const uint32_t at = take_place(next[wave], (key[k] >> p.shift) & (bins - 1), p.bits, in, lane);
         if (in) {
-            const uint32_t rank = __popcll(same & (((uint64_t)1 << lane) - 1));
-            const uint32_t at = next[wave][d] + rank;
             p.key_out[at] = key[k];
-            p.at_out[at] = p.at_in ? p.at_in[i] : (uint32_t)i;
+            p.at_out[at] = from[k];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        // (the last of them moves the place on, after all have read it)
-        if (in && (same >> lane) == 1) next[wave][d] += __popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// first[v] = first sorted place whose key is at least v, for v = 0 .. V.
+// All passes over N <= kSmall tokens.
+__global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(SortPass p, int passes) {
+    constexpr int kWaves = kSmallThreads / 64, kPer = kSmall / kWaves / 64, kBins = 512;
+    __shared__ uint32_t keys[kSmall], places[kSmall];
+    __shared__ uint32_t next[kWaves][kBins];
+    __shared__ uint32_t share[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << p.bits, N = (int)p.N;
+    // a wave's keys are side by side, as many to each as the tokens give
+    const int per = (N + kWaves * 64 - 1) / (kWaves * 64), i0 = wave * per * 64;
+    uint32_t key[kPer], at[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = i0 + k * 64 + lane;
+        at[k] = i;
+        key[k] = k < per && i < N ? sort_key(p.tokens, p.wide, i, p.V, p.padding) : 0;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * p.bits;
+        for (int b = threadIdx.x; b < kWaves * kBins; b += kSmallThreads) (&next[0][0])[b] = 0;
+        __syncthreads();
+        // a key's place among the wave's of its digit; their counts are left in `next`
+        uint32_t to[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (k >= per) break;
+            to[k] = take_place(next[wave], (key[k] >> shift) & (bins - 1), p.bits,
+                               i0 + k * 64 + lane < N, lane);
+        }
+        __syncthreads();
+        uint32_t sum = 0, all;
+        const int b = threadIdx.x;
+        if (b < bins)
+            for (int w = 0; w < kWaves; ++w) sum += next[w][b];
+        uint32_t first = sum_before<kSmallThreads>(sum, share, &all);
+        if (b < bins)
+            for (int w = 0; w < kWaves; ++w) {
+                const uint32_t c = next[w][b];
+                next[w][b] = first;
+                first += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (k >= per || i0 + k * 64 + lane >= N) break;
+            const uint32_t place = next[wave][(key[k] >> shift) & (bins - 1)] + to[k];
+            keys[place] = key[k];
+            places[place] = at[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int i = i0 + k * 64 + lane;
+            if (k < per && i < N) {
+                key[k] = keys[i];
+                at[k] = places[i];
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = i0 + k * 64 + lane;
+        if (k < per && i < N) {
+            p.key_out[i] = key[k];
+            p.at_out[i] = at[k];
+        }
+    }
+}
+
+// first[v] = first sorted place whose key is at least v, for v = 0 .. V: by halving, first among 1024
+// keys in LDS and then between two of them.
 __global__ __launch_bounds__(kThreads) void emb_first_kernel(const uint32_t* key, int64_t N, int64_t V,
                                                              uint32_t* first) {
+    constexpr int kSamples = 1024;
+    __shared__ uint32_t sample[kSamples];
+    const int64_t step = (N + kSamples - 1) / kSamples;
+    const int n = step ? (int)((N + step - 1) / step) : 0;  // keys 0, step, 2 step, ...
+    for (int k = threadIdx.x; k < n; k += kThreads) sample[k] = key[k * step];
+    __syncthreads();
     const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (v > V) return;
-    int64_t lo = 0, hi = N;
+    int a = 0, b = n;  // samples under v: [0, a)
+    while (a < b) {
+        const int mid = (a + b) / 2;
+        if (sample[mid] < (uint32_t)v) a = mid + 1;
+        else b = mid;
+    }
+    int64_t lo = a ? (a - 1) * step + 1 : 0, hi = min(N, a * step);
     while (lo < hi) {
         const int64_t mid = (lo + hi) / 2;
         if (key[mid] < (uint32_t)v) lo = mid + 1;
@@ -190,108 +328,163 @@ __global__ __launch_bounds__(kThreads) void emb_first_kernel(const uint32_t* key
 }
 
 // -------------------------------------------------------------- gradient ----
-// A token met at most `window` times is summed by one group of threads.  The sorted places of one met
-// more often are cut where multiples of `window` lie; the parts are summed each for itself and
-// joined in order by a second launch.  A window has parts of at most two such tokens: of the one at
-// its first place (slot 0), and of another at its last (slot 1).
-template <int DT, int V>
-__device__ __forceinline__ void add_rows(const char* dy, int64_t lddy, const uint32_t* at, int64_t b,
-                                         int64_t e, int64_t col, float* sum) {
-#pragma unroll 8
-    for (int64_t i = b; i < e; ++i) {
-        float f[V];
-        const char* row = dy + (int64_t)at[i] * lddy * kElemBytes<DT>;
-        if constexpr (V == 1) f[0] = load_elem<DT>(row, col);
-        else unpack<DT, V>(load<DT, V>(row, col), f);
-#pragma unroll
-        for (int k = 0; k < V; ++k) sum[k] += f[k];
+// A group of tpr threads sums rows of dy, C vectors of a row to a thread at a time.  A token met up to
+// kLight times is summed by one group, one met up to `window` times by a workgroup's groups together.
+// The sorted places of one met more often are cut where multiples of `window` lie; the parts are
+// summed each by a workgroup, in the same launch, and joined in order by a second.  A window has parts
+// of at most two such tokens: of the one at its first place (slot 0), and of another at its last
+// (slot 1).
+constexpr int kLight = 16;
+struct Gradient {
+    const char* dy;
+    int64_t lddy;
+    const uint32_t *key, *at, *first;
+    float* parts;
+    char* dw;
+    int64_t rows, D, window, windows;
+    float scale;
+    int tpr;
+};
+
+template <int DT, int V, int C>
+struct Columns {
+    float f[C][V];
+    // column vectors c0, c0 + tpr, ... of a group's thread; the last of a row shares elements
+    static __device__ __forceinline__ int64_t at(const Gradient& g, int64_t c0, int c) {
+        return min((c0 + c * g.tpr) * V, g.D - V);
     }
-}
-template <int DT, int V>
-__device__ __forceinline__ void put_row(char* dw, int64_t v, int64_t D, int64_t col, float* f,
-                                        float scale) {
+    __device__ __forceinline__ void sum(const Gradient& g, int64_t c0, int64_t b, int64_t e) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] *= scale;
-    char* row = dw + v * D * kElemBytes<DT>;
-    if constexpr (V == 1) store_elem<DT>(row, col, f[0]);
-    else store<DT, V>(row, col, pack<DT, V>(f));
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[c][k] = 0.f;
+#pragma unroll 4
+        for (int64_t i = b; i < e; ++i) {
+            const char* row = g.dy + (int64_t)g.at[i] * g.lddy * kElemBytes<DT>;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float x[V];
+                if constexpr (V == 1) x[0] = load_elem<DT>(row, at(g, c0, c));
+                else unpack<DT, V>(load<DT, V>(row, at(g, c0, c)), x);
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[c][k] += x[k];
+            }
+        }
+    }
+    __device__ __forceinline__ void put(const Gradient& g, int64_t c0, int64_t v) const {
+        char* row = g.dw + v * g.D * kElemBytes<DT>;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float x[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[k] = f[c][k] * g.scale;
+            if ((c0 + c * g.tpr) * V >= g.D) continue;
+            if constexpr (V == 1) store_elem<DT>(row, at(g, c0, c), x[0]);
+            else store<DT, V>(row, at(g, c0, c), pack<DT, V>(x));
+        }
+    }
+};
+
+// Rows [b, e) of the sorted places summed by all groups, into the first group's s.  Every thread calls.
+template <int DT, int V, int C>
+__device__ __forceinline__ void sum_together(const Gradient& g, Columns<DT, V, C>& s, float* share,
+                                             int64_t c0, int64_t b, int64_t e) {
+    const int groups = kThreads / g.tpr, group = threadIdx.x / g.tpr;
+    const int64_t n = e - b;
+    s.sum(g, c0, b + n * group / groups, b + n * (group + 1) / groups);
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) share[(c * V + k) * kThreads + threadIdx.x] = s.f[c][k];
+    __syncthreads();
+    if (group == 0)
+        for (int o = 1; o < groups; ++o)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int k = 0; k < V; ++k) s.f[c][k] += share[(c * V + k) * kThreads + o * g.tpr + threadIdx.x];
 }
 
-template <int DT, int V>
-__global__ __launch_bounds__(kThreads) void emb_grad_kernel(const char* dy, int64_t lddy,
-                                                            const uint32_t* at, const uint32_t* first,
-                                                            char* dw, int64_t rows, int64_t D,
-                                                            int64_t window, float scale, int tpr) {
-    const int64_t v = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
-    if (v >= rows) return;
-    const int64_t b = first[v], e = first[v + 1];
-    if (e - b > window) return;
-    for (int64_t i = (int64_t)(threadIdx.x % tpr) * V; i < D; i += tpr * V) {
-        const int64_t col = min(i, D - V);
-        float sum[V] = {};
-        add_rows<DT, V>(dy, lddy, at, b, e, col, sum);
-        put_row<DT, V>(dw, v, D, col, sum, scale);
+// The first workgroups take the windows; the others rows of the table, `stride` apart (frequent
+// tokens tend to lie side by side).
+template <int DT, int V, int C>
+__global__ __launch_bounds__(kThreads) void emb_grad_kernel(Gradient g, int windows, int64_t row0,
+                                                            int64_t rows, int64_t stride) {
+    __shared__ float share[C * V * kThreads];
+    __shared__ int lengths[kThreads];
+    const int groups = kThreads / g.tpr, group = threadIdx.x / g.tpr, lane = threadIdx.x % g.tpr;
+    Columns<DT, V, C> s;
+    if ((int)blockIdx.x >= windows) {
+        const int64_t r = blockIdx.x - windows + group * stride, v = row0 + r;
+        const bool mine = r < rows;
+        const int64_t b = mine ? g.first[v] : 0, e = mine ? g.first[v + 1] : 0;
+        if (mine && e - b <= kLight)
+            for (int64_t c0 = lane; c0 * V < g.D; c0 += C * g.tpr) {
+                s.sum(g, c0, b, e);
+                s.put(g, c0, v);
+            }
+        if (lane == 0) lengths[group] = (int)(e - b);
+        if (!__syncthreads_or(e - b > kLight)) return;
+        for (int k = 0; k < groups; ++k) {
+            if (lengths[k] <= kLight || lengths[k] > g.window) continue;
+            const int64_t u = row0 + blockIdx.x - windows + k * stride, ub = g.first[u];
+            for (int64_t i = 0; i * V < g.D; i += C * g.tpr) {
+                sum_together(g, s, share, i + lane, ub, ub + lengths[k]);
+                if (group == 0) s.put(g, i + lane, u);
+            }
+        }
+        return;
     }
-}
-
-template <int DT, int V>
-__global__ __launch_bounds__(kThreads) void emb_windows_kernel(const char* dy, int64_t lddy,
-                                                               const uint32_t* key, const uint32_t* at,
-                                                               const uint32_t* first, float* parts,
-                                                               int64_t rows, int64_t D, int64_t window,
-                                                               int tpr) {
-    const int64_t w = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
-    const int64_t live = first[rows], from = w * window, to = min(live, from + window);
+    const int64_t w = blockIdx.x;
+    const int64_t live = g.first[g.rows], from = w * g.window, to = min(live, from + g.window);
     for (int slot = 0; slot < 2 && from < live; ++slot) {
-        const int64_t v = key[slot ? to - 1 : from];
-        const int64_t b0 = first[v], e0 = first[v + 1];
-        if (e0 - b0 <= window || (slot && b0 <= from)) continue;
-        for (int64_t i = (int64_t)(threadIdx.x % tpr) * V; i < D; i += tpr * V) {
-            const int64_t col = min(i, D - V);
-            float sum[V] = {};
-            add_rows<DT, V>(dy, lddy, at, max(b0, from), min(e0, to), col, sum);
-            float* p = parts + (2 * w + slot) * D + col;
+        const int64_t v = g.key[slot ? to - 1 : from];
+        const int64_t b0 = g.first[v], e0 = g.first[v + 1];
+        if (e0 - b0 <= g.window || (slot && b0 <= from)) continue;
+        for (int64_t i = 0; i * V < g.D; i += C * g.tpr) {
+            sum_together(g, s, share, i + lane, max(b0, from), min(e0, to));
+            float* p = g.parts + (2 * w + slot) * g.D;
+            if (group == 0)
 #pragma unroll
-            for (int k = 0; k < V; ++k) p[k] = sum[k];
+                for (int c = 0; c < C; ++c)
+                    if ((i + lane + c * g.tpr) * V < g.D)
+#pragma unroll
+                        for (int k = 0; k < V; ++k) p[s.at(g, i + lane, c) + k] = s.f[c][k];
         }
     }
 }
 
 // A workgroup to a window: the token that starts in it, if it is one of those.
-constexpr int kJoinThreads = 1024;
 template <int DT, int V>
-__global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(const float* parts,
-                                                                const uint32_t* key,
-                                                                const uint32_t* first, char* dw,
-                                                                int64_t rows, int64_t D,
-                                                                int64_t window, float scale, int tpr) {
-    __shared__ float share[kJoinThreads * V];
-    const int64_t w = blockIdx.x;
-    const int64_t live = first[rows], from = w * window, to = min(live, from + window);
-    const int groups = kJoinThreads / tpr, group = threadIdx.x / tpr;
+__global__ __launch_bounds__(kThreads) void emb_join_kernel(Gradient g) {
+    __shared__ float share[kThreads * V];
+    const int64_t w = blockIdx.x, live = g.first[g.rows], from = w * g.window, to = min(live, from + g.window);
+    const int groups = kThreads / g.tpr, group = threadIdx.x / g.tpr, lane = threadIdx.x % g.tpr;
     for (int slot = 0; slot < 2 && from < live; ++slot) {
-        const int64_t v = key[slot ? to - 1 : from];
-        const int64_t b0 = first[v], e0 = first[v + 1];
-        if (e0 - b0 <= window || (slot ? b0 <= from : b0 < from)) continue;
-        const int64_t n = (e0 - 1) / window - w + 1;  // parts, cut evenly among the groups
+        const int64_t v = g.key[slot ? to - 1 : from];
+        const int64_t b0 = g.first[v], e0 = g.first[v + 1];
+        if (e0 - b0 <= g.window || (slot ? b0 <= from : b0 < from)) continue;
+        const int64_t n = (e0 - 1) / g.window - w + 1;  // parts, cut evenly among the groups
         const int64_t x0 = n * group / groups, x1 = n * (group + 1) / groups;
-        for (int64_t i0 = 0; i0 < D; i0 += tpr * V) {
-            const int64_t i = i0 + (int64_t)(threadIdx.x % tpr) * V, col = min(i, D - V);
-            float sum[V] = {};
-#pragma unroll 4
+        for (int64_t i0 = 0; i0 < g.D; i0 += g.tpr * V) {
+            const int64_t i = i0 + (int64_t)lane * V;
+            Columns<DT, V, 1> s{};
+            const int64_t col = s.at(g, i / V, 0);
+#pragma unroll 8
             for (int64_t x = x0; x < x1; ++x) {
-                const float* p = parts + (2 * (w + x) + (x == 0 ? slot : 0)) * D + col;
+                const float* p = g.parts + (2 * (w + x) + (x == 0 ? slot : 0)) * g.D + col;
 #pragma unroll
-                for (int k = 0; k < V; ++k) sum[k] += p[k];
+                for (int k = 0; k < V; ++k) s.f[0][k] += p[k];
             }
 #pragma unroll
-            for (int k = 0; k < V; ++k) share[threadIdx.x * V + k] = sum[k];
+            for (int k = 0; k < V; ++k) share[threadIdx.x * V + k] = s.f[0][k];
             __syncthreads();
-            if (group == 0 && i < D) {
-                for (int g = 1; g < groups; ++g)
+            if (group == 0 && i < g.D) {
+                for (int o = 1; o < groups; ++o)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) sum[k] += share[(g * tpr + threadIdx.x) * V + k];
-                put_row<DT, V>(dw, v, D, col, sum, scale);
+                    for (int k = 0; k < V; ++k) s.f[0][k] += share[(o * g.tpr + threadIdx.x) * V + k];
+                s.put(g, i / V, v);
             }
             __syncthreads();
         }
@@ -299,8 +492,8 @@ __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(const float* par
 }
 
 // ------------------------------------------------------------------ host ----
-// Places to a window: 2048 windows at most.
-int64_t window_of(int64_t N) { return std::max<int64_t>(64, ceil_div(N, 2048)); }
+// Places to a window: 1024 windows at most.
+int64_t window_of(int64_t N) { return std::max<int64_t>(256, ceil_div(N, 1024)); }
 
 struct Plan {
     int passes, bits;
@@ -311,7 +504,8 @@ Plan plan(int64_t N, int64_t V, int64_t D) {
     Plan p;
     int bits = 1;
     while ((V >> bits) != 0) ++bits;
-    p.passes = (bits + 9) / 10;
+    const int most = N <= kSmall ? 9 : 10;
+    p.passes = (bits + most - 1) / most;
     p.bits = (bits + p.passes - 1) / p.passes;
     p.tiles = ceil_div(N, kTile);
     p.windows = ceil_div(N, window_of(N));
@@ -377,6 +571,26 @@ int threads_of(int64_t D, int32_t dtype) {
     return row_threads(ceil_div(D, V));
 }
 
+// Threads to a row and vectors of it to a thread at a time: the pair that leaves the fewest idle, and
+// among those the one with the fewest threads (more rows to a wave).
+struct GroupShape {
+    int tpr, columns;
+};
+GroupShape group_shape(int64_t D, int32_t dtype) {
+    const int64_t V = D < 16 / elem_bytes(dtype) ? 1 : 16 / elem_bytes(dtype), n = ceil_div(D, V);
+    GroupShape best{64, 1};
+    int64_t least = INT64_MAX;
+    for (int tpr = 1; tpr <= 64; tpr *= 2)
+        for (int c = 1; c <= 3; ++c) {
+            const int64_t taken = ceil_div(n, tpr * c) * tpr * c * (tpr * c < n && tpr < 64 ? 4 : 1);
+            if (taken < least) {
+                least = taken;
+                best = GroupShape{tpr, c};
+            }
+        }
+    return best;
+}
+
 // f(first, count) over launches of `count` groups of tpr threads, fewer than 2^32 threads each.
 template <typename F>
 void in_launches(int64_t count, int tpr, F f) {
@@ -440,49 +654,56 @@ extern "C" int haste_embedding_bwd(const void* tokens, int32_t token_bits, const
     auto words = [&](int64_t at) { return reinterpret_cast<uint32_t*>(base + at); };
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint32_t *key = words(p.key[0]), *at = words(p.at[0]), *first = words(p.first);
-    for (int k = 0; k < p.passes && N > 0; ++k) {
-        haste::SortPass s{};
-        if (k == 0) s.tokens = tokens;
-        s.wide = token_bits == 64;
-        s.V = V;
-        s.padding = padding;
+    haste::SortPass s{};
+    s.tokens = tokens;
+    s.wide = token_bits == 64;
+    s.V = V;
+    s.padding = padding;
+    s.N = N;
+    s.bits = p.bits;
+    if (N > 0 && N <= haste::kSmall) {
+        s.key_out = key;
+        s.at_out = at;
+        haste::sort_small_kernel<<<dim3(1), dim3(haste::kSmallThreads), 0, st>>>(s, p.passes);
+    }
+    for (int k = 0; k < p.passes && N > haste::kSmall; ++k) {
+        s.tokens = k ? nullptr : tokens;
         s.key_in = key;
         s.at_in = k ? at : nullptr;
         key = s.key_out = words(p.key[(k + 1) % 2]);
         at = s.at_out = words(p.at[(k + 1) % 2]);
         s.counts = words(p.counts);
-        s.N = N;
         s.tiles = (int)p.tiles;
         s.shift = k * p.bits;
-        s.bins = 1 << p.bits;
         const dim3 grid((unsigned)p.tiles), block(haste::kThreads);
         haste::sort_count_kernel<<<grid, block, 0, st>>>(s);
-        haste::sort_scan_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.counts, p.tiles << p.bits);
+        if (p.tiles > haste::kOwnScan)
+            haste::sort_scan_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.counts, p.tiles << p.bits);
         haste::sort_move_kernel<<<grid, block, 0, st>>>(s);
     }
     haste::emb_first_kernel<<<dim3((unsigned)haste::ceil_div(V + 1, haste::kThreads)),
                               dim3(haste::kThreads), 0, st>>>(key, N, V, first);
-    const int tpr = haste::threads_of(D, dtype), per = haste::kThreads / tpr;
-    const int64_t window = haste::window_of(N);
-    float* parts = reinterpret_cast<float*>(base + p.parts);
-    const char* dyc = static_cast<const char*>(dy);
-    char* dwc = static_cast<char*>(dw);
-    const int64_t size = haste::elem_bytes(dtype);
+    const haste::GroupShape shape = haste::group_shape(D, dtype);
+    const int per = haste::kThreads / shape.tpr;
+    const haste::Gradient g{static_cast<const char*>(dy), lddy, key, at, first,
+                            reinterpret_cast<float*>(base + p.parts), static_cast<char*>(dw), V, D,
+                            haste::window_of(N), p.windows, (float)scale, shape.tpr};
+    // (a single window holds no token more often than it is long)
+    const int windows = p.windows > 1 ? (int)p.windows : 0;
 #define HASTE_EMB(DT, VEC)                                                                           \
     do {                                                                                             \
-        haste::in_launches(V, tpr, [&](int64_t v0, int64_t n) {                                      \
-            haste::emb_grad_kernel<DT, VEC><<<dim3((unsigned)haste::ceil_div(n, per)),               \
-                                              dim3(haste::kThreads), 0, st>>>(                       \
-                dyc, lddy, at, first + v0, dwc + v0 * D * size, n, D, window, (float)scale, tpr);    \
+        auto kernel = shape.columns == 1   ? haste::emb_grad_kernel<DT, VEC, 1>                      \
+                      : shape.columns == 2 ? haste::emb_grad_kernel<DT, VEC, 2>                      \
+                                           : haste::emb_grad_kernel<DT, VEC, 3>;                     \
+        haste::in_launches(V, shape.tpr, [&](int64_t v0, int64_t n) {                                \
+            const int first_windows = v0 == 0 ? windows : 0;                                         \
+            const int64_t stride = haste::ceil_div(n, per);                                          \
+            kernel<<<dim3((unsigned)(first_windows + stride)), dim3(haste::kThreads), 0, st>>>(      \
+                g, first_windows, v0, n, stride);                                                    \
         });                                                                                          \
-        if (p.windows > 1) {                                                                         \
-            haste::emb_windows_kernel<DT, VEC><<<dim3((unsigned)haste::ceil_div(p.windows, per)),    \
-                                                 dim3(haste::kThreads), 0, st>>>(                    \
-                dyc, lddy, key, at, first, parts, V, D, window, tpr);                                \
-            haste::emb_join_kernel<DT, VEC><<<dim3((unsigned)p.windows), dim3(haste::kJoinThreads),  \
-                                              0, st>>>(parts, key, first, dwc, V, D, window,         \
-                                                       (float)scale, tpr);                           \
-        }                                                                                            \
+        if (windows)                                                                                 \
+            haste::emb_join_kernel<DT, VEC>                                                          \
+                <<<dim3((unsigned)p.windows), dim3(haste::kThreads), 0, st>>>(g);                    \
     } while (0)
     HASTE_EMB_TYPES(HASTE_EMB);
 #undef HASTE_EMB
