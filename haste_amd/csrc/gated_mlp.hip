@@ -121,15 +121,28 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int
     }
 }
 
-// Rows [R, C] of any pitch as rows of P (a multiple of 8) elements on 16 bytes, with zeros behind C.
-__global__ __launch_bounds__(256) void pack_rows_kernel(const char* src, int64_t ld, char* dst, int64_t R,
-                                                        int64_t C, int64_t P) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pieces = P / 8;
-    if (i >= R * pieces) return;
+// Matrices [R, C] of any pitch as rows of P (a multiple of 8) elements on 16 bytes, with zeros behind C;
+// one launch for all that a call has.
+constexpr int kMaxPacks = 5;
+struct Packs {
+    struct {
+        const char* src;
+        char* dst;
+        int64_t ld, R, C, P;
+        uint32_t block0;  // its first workgroup
+    } m[kMaxPacks];
+    int count;
+};
+__global__ __launch_bounds__(256) void pack_rows_kernel(Packs p) {
+    int k = 0;
+    for (int j = 1; j < p.count; ++j) k = blockIdx.x >= p.m[j].block0 ? j : k;
+    const auto& m = p.m[k];
+    const int64_t i = (int64_t)(blockIdx.x - m.block0) * 256 + threadIdx.x, pieces = m.P / 8;
+    if (i >= m.R * pieces) return;
     const int64_t r = i / pieces, c = i % pieces * 8;
     const Elems<HASTE_DTYPE_BF16, 8> v =
-        load_part<HASTE_DTYPE_BF16, 8>(src + r * ld * 2, c, C - c);
-    store<HASTE_DTYPE_BF16, 8>(dst, r * P + c, v);
+        load_part<HASTE_DTYPE_BF16, 8>(m.src + r * m.ld * 2, c, m.C - c);
+    store<HASTE_DTYPE_BF16, 8>(m.dst, r * m.P + c, v);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -201,25 +214,32 @@ void launch_tiles(const GemmArgs& g, int batches, int act, const Epilogue& out, 
 }
 
 // How a product is cut.  Tiles of 256 x 256 (a workgroup to a CU) where they fill most of the GPU's 256
-// CUs, by themselves or with K in parts; else of 128 x 128, two workgroups to a CU.
+// CUs, by themselves or with K in parts; else of 128 x 128, two workgroups to a CU; else, where those
+// leave half of the CUs idle, of 64 x 128: the time is then that of a tile's steps and epilogue (509 rows,
+// H = 2048: 28.8 -> 24.9 us for the block; 512 rows, H = 8192, with the first rule left out: 162 -> 198).
+enum class Tiles { kLarge, kSmall, kLow };
 struct Cut {
-    bool large;
+    Tiles tiles;
     int splits;
 };
 template <GemmMode MODE, int DT>
 Cut cut_of(const Product& p, bool may_split) {
     const int64_t batches = MODE == GemmMode::kBatch ? 2 : 1;
     const int64_t steps = ceil_div(p.K, 32) * (MODE == GemmMode::kSegments ? 2 : 1);
-    auto tiles = [&](int64_t side) {
-        return ceil_div(p.M, side) * ceil_div(p.N, MODE == GemmMode::kDual ? side / 2 : side) * batches;
+    auto tiles = [&](int64_t rows, int64_t cols) {
+        return ceil_div(p.M, rows) * ceil_div(p.N, MODE == GemmMode::kDual ? cols / 2 : cols) * batches;
     };
-    const int64_t big = tiles(256), small = tiles(128);
-    if (small == 0) return Cut{false, 1};
-    if (DT != HASTE_DTYPE_F32) {
-        if (big >= 192) return Cut{true, 1};
-        if (may_split && steps / 32 >= ceil_div(192, big)) return Cut{true, (int)(256 / big)};
-    }
-    return Cut{false, may_split ? (int)std::max<int64_t>(1, std::min(512 / small, steps / 8)) : 1};
+    const int64_t big = tiles(256, 256), small = tiles(128, 128), low = tiles(64, 128);
+    // (16 steps to a part at least)
+    auto splits = [&](int64_t n) {
+        return may_split ? std::max<int64_t>(1, std::min(256 / n, steps / 16)) : 1;
+    };
+    if (small == 0) return Cut{Tiles::kSmall, 1};
+    if (DT == HASTE_DTYPE_F32) return Cut{Tiles::kSmall, (int)splits(small)};
+    if (big >= 192) return Cut{Tiles::kLarge, 1};
+    if (may_split && steps / 32 >= ceil_div(192, big)) return Cut{Tiles::kLarge, (int)(256 / big)};
+    if (small * splits(small) <= 128) return Cut{Tiles::kLow, (int)splits(low)};
+    return Cut{Tiles::kSmall, (int)splits(small)};
 }
 
 template <int DT, GemmMode MODE, bool AK, bool BK_, typename Epilogue>
@@ -238,13 +258,16 @@ void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_
             // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
             // 1308, since they load half as much again).
             typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
-            if (cut.large && p.K <= 1024)
+            if (cut.tiles == Tiles::kLarge && p.K <= 1024)
                 return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);
         }
-        if (cut.large)
+        typedef GemmTile<T, MODE, AK, BK_, 2, 4, 2, 2, 4> Low;
+        if (cut.tiles == Tiles::kLarge)
             launch_tiles<Large, DT>(gemm_args<Large>(p, segments, cut.splits), batches, act, out, st);
-        else
+        else if (cut.tiles == Tiles::kSmall)
             launch_tiles<Small, DT>(gemm_args<Small>(p, segments, cut.splits), batches, act, out, st);
+        else
+            launch_tiles<Low, DT>(gemm_args<Low>(p, segments, cut.splits), batches, act, out, st);
     }
 }
 
@@ -273,27 +296,26 @@ struct Sizes {
     int64_t N, D, H, O;
 };
 
-// A matrix with 16-byte rows: itself, or a copy in the workspace.
-template <int DT>
-Matrix packed(const Matrix& m, Space& ws, bool launch, hipStream_t st) {
-    if (DT == HASTE_DTYPE_F32 || plain_rows(m)) return m;
-    const int64_t P = round8(m.cols);
-    void* to = ws.take(m.rows * P * 2);
-    if (launch && m.rows > 0) {
-        const int64_t n = m.rows * (P / 8);
-        pack_rows_kernel<<<dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st>>>(
-            static_cast<const char*>(m.p), m.ld, static_cast<char*>(to), m.rows, m.cols, P);
+// Matrices with 16-byte rows: themselves, or copies in the workspace, made by one launch.
+struct Packer {
+    Packs packs{};
+    uint32_t blocks = 0;
+    template <int DT>
+    Matrix add(const Matrix& m, Space& ws, bool used) {
+        if (DT == HASTE_DTYPE_F32 || plain_rows(m)) return m;
+        const int64_t P = round8(m.cols);
+        void* to = ws.take(m.rows * P * 2);
+        if (used && m.rows > 0) {
+            packs.m[packs.count++] = {static_cast<const char*>(m.p), static_cast<char*>(to), m.ld,
+                                      m.rows, m.cols, P, blocks};
+            blocks += (uint32_t)ceil_div(m.rows * (P / 8), 256);
+        }
+        return Matrix{to, P, m.rows, m.cols};
     }
-    return Matrix{to, P, m.rows, m.cols};
-}
-// Wg and Wu share a pitch in the kernels.
-template <int DT>
-void packed_pair(Matrix& g, Matrix& u, Space& ws, bool launch, hipStream_t st) {
-    if (DT != HASTE_DTYPE_F32) {
-        g = packed<DT>(g, ws, launch, st);
-        u = packed<DT>(u, ws, launch, st);
+    void launch(hipStream_t st) const {
+        if (blocks) pack_rows_kernel<<<dim3(blocks), dim3(256), 0, st>>>(packs);
     }
-}
+};
 
 template <int DT>
 int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const GatedOut& out, void* y,
@@ -312,7 +334,7 @@ int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const
                 constexpr int NG = decltype(groups)::value;
                 few_rows_kernel<T, NG, true, 8, GatedOut><<<g1, dim3(512), 0, st>>>(
                     xc, x.ld, gc, wg.ld, uc, wu.ld, (int)s.N, (int)s.H, (int)s.D, act, out);
-                few_rows_kernel<T, NG, false, 8, PlainOut><<<g2, dim3(512), 0, st>>>(
+                few_rows_kernel<T, NG, false, 16, PlainOut><<<g2, dim3(1024), 0, st>>>(
                     hc, out.ld, dc, wd.ld, nullptr, 0, (int)s.N, (int)s.O, (int)s.H, 0, po);
             };
             if (s.N <= 16) run(std::integral_constant<int, 1>());
@@ -321,14 +343,17 @@ int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const
             return 0;
         }
     }
-    x = packed<DT>(x, ws, launch, st);
-    packed_pair<DT>(wg, wu, ws, launch, st);
-    wd = packed<DT>(wd, ws, launch, st);
+    Packer packer;
+    x = packer.add<DT>(x, ws, true);
+    wg = packer.add<DT>(wg, ws, true);
+    wu = packer.add<DT>(wu, ws, true);
+    wd = packer.add<DT>(wd, ws, true);
     const Matrix h{out.h, out.ld, s.N, s.H};
     const Product p1{{x, x}, {wg, wu}, s.N, s.H, s.D};
     const Product p2{{h, h}, {wd, wd}, s.N, s.O, s.H};
     void* parts = ws.take(plain_parts<DT, GemmMode::kPlain>(p2));
     if (launch) {
+        packer.launch(st);
         product<DT, GemmMode::kDual, true, true>(p1, cut_of<GemmMode::kDual, DT>(p1, false), act, out,
                                                  st);
         plain<DT, GemmMode::kPlain, true, true>(p2, y, nullptr, parts, st);
@@ -347,10 +372,12 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
     Space ws{base};
     const int64_t bytes = s.N * ld * elem_bytes(DT);
     void *dg = ws.take(bytes), *du = ws.take(bytes);
-    x = packed<DT>(x, ws, launch && (to.dwg || to.dwu), st);
-    packed_pair<DT>(wg, wu, ws, launch && to.dx, st);
-    wd = packed<DT>(wd, ws, launch, st);
-    dy = packed<DT>(dy, ws, launch, st);
+    Packer packer;
+    x = packer.add<DT>(x, ws, to.dwg || to.dwu);
+    wg = packer.add<DT>(wg, ws, to.dx);
+    wu = packer.add<DT>(wu, ws, to.dx);
+    wd = packer.add<DT>(wd, ws, to.dx || to.dwg || to.dwu);
+    dy = packer.add<DT>(dy, ws, true);
     const Matrix mg{dg, ld, s.N, s.H}, mu{du, ld, s.N, s.H}, mh{h, ld, s.N, s.H};
     const Product p1{{dy, dy}, {wd, wd}, s.N, s.H, s.O};
     const Product p2{{mg, mu}, {wg, wu}, s.N, s.D, s.H};
@@ -360,6 +387,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
                                     plain_parts<DT, GemmMode::kBatch>(p3),
                                     plain_parts<DT, GemmMode::kPlain>(p4)}));
     if (launch) {
+        packer.launch(st);
         if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
             const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld};
             product<DT, GemmMode::kPlain, true, false>(p1, cut_of<GemmMode::kPlain, DT>(p1, false), 0, out,

@@ -23,10 +23,27 @@ __device__ __forceinline__ void activation(float g, float* a, float* slope) {
         *a = g * s;
         *slope = s * __builtin_fmaf(g, 1.f - s, 1.f);
     } else if constexpr (ACT == HASTE_ACT_GELU) {
-        const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+        float cdf, e;  // the normal distribution at g, e^(-g^2 / 2)
+        if constexpr (PRECISE) {
+            cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+            e = expf(-0.5f * g * g);
+        } else {
+            // erfc(x) e^(x^2), x = |g| / sqrt 2, as a polynomial in t = 1 / (1 + x / 2): a least-squares fit
+            // with weights driven to equal errors, 1.5e-6 of its value up to x = 9.5 (e^(-x^2) is 0 in fp32
+            // behind).  A fifth of erfcf's operations, which took 5 of 15 us at 509 rows.
+            const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35355339059f, fabsf(g), 1.f));
+            float q = 0.08912339f;
+            q = __builtin_fmaf(q, t, -0.35997868f);
+            q = __builtin_fmaf(q, t, 0.393769f);
+            q = __builtin_fmaf(q, t, 0.03466602f);
+            q = __builtin_fmaf(q, t, 0.28271684f);
+            q = __builtin_fmaf(q, t, 0.27735418f);
+            q = __builtin_fmaf(q, t, 0.28234804f);
+            e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
+            const float tail = 0.5f * q * t * e;
+            cdf = g < 0.f ? tail : 1.f - tail;
+        }
         *a = g * cdf;
-        const float e = PRECISE ? expf(-0.5f * g * g)
-                                : __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
         *slope = __builtin_fmaf(g * 0.39894228040143268f, e, cdf);
     } else {
         // 0.5 (1 + tanh(t)) = sigmoid(2 t), t = sqrt(2 / pi) (g + 0.044715 g^3)

@@ -4,8 +4,8 @@ strides and the kernels that a size takes (few rows, small and large tiles, K in
 Tolerances: u = 2^-24, U_d half a step of the type.  A product of K terms is off by (K + 2) u of its
 terms' absolute sum, whatever the order, and by its operands' errors times the other operand.  What
 lies between the products is rounded to the type: h, and for the backward dg and du; u act'(g) and act(g)
-are kept in 24 bits (2^-17 of their size; fp32: none lost).  act is within 8 u of its size and moves by at
-most 1.2 |dg|; act' moves by at most 1.2 |dg|."""
+are kept in 24 bits (2^-17 of their size; fp32: none lost).  act is within 8 u of its size (16-bit gelu: 1.5e-6, 25 u,
+of its tail besides) and moves by at most 1.2 |dg|; act' moves by at most 1.2 |dg|."""
 import math
 
 import pytest
@@ -45,7 +45,8 @@ def reference(x, wg, wu, wd, name, dy=None):
     g, u = mm(X, G.t()), mm(X, Up.t())
     eg, eu = ((D + 2) * U * mm(X.abs(), w.abs().t()) for w in (G, Up))
     a, s = act(name, g)
-    ea = 1.2 * eg + 16 * U * (a.abs() + g.abs() * 0.1)
+    ka = 16 if dt is torch.float32 or name != "gelu" else 42
+    ea = 1.2 * eg + ka * U * (a.abs() + g.abs() * 0.1)
     h = a * u
     eh = ea * (u.abs() + eu) + a.abs() * eu + ud * h.abs() + tiny
     y = mm(h, Dn.t())
@@ -56,7 +57,7 @@ def reference(x, wg, wu, wd, name, dy=None):
         N, O = Y.shape
         dh = mm(Y, Dn)
         edh = (O + 2) * U * mm(Y.abs(), Dn.abs())
-        ea, es = 1.2 * eg + 16 * U * (a.abs() + 0.1 * g.abs()), 1.2 * eg + 16 * U * (s.abs() + 0.1)
+        ea, es = 1.2 * eg + ka * U * (a.abs() + 0.1 * g.abs()), 1.2 * eg + ka * U * (s.abs() + 0.1)
         kept = 0.0 if dt is torch.float32 else 2.0 ** -17
         eus = eu * s.abs() + u.abs() * es + eu * es
         eus, ea = 1.05 * eus + kept * (u * s).abs(), 1.05 * ea + kept * a.abs()
