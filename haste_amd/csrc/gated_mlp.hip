@@ -66,37 +66,79 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void gemm_kernel(GemmArgs g, int
 
 // --------------------------------------------------------------- a few rows ----
 // Up to 16 NG rows of x against 16 rows of the weights (of both, DUAL): the waves share K, and read
-// the weights straight into registers, at any alignment.
+// the weights straight into registers, at any alignment.  fp32 weights are split there; x is too (DUAL), or
+// comes as its parts, `plane` bytes apart.
 template <typename T, int NG, bool DUAL, int WAVES, typename Epilogue>
-__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int64_t ldx,
+__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int64_t ldx, int64_t plane,
                                                              const char* w0, int64_t ldw0,
                                                              const char* w1, int64_t ldw1, int M, int N,
                                                              int K, int act, Epilogue out) {
-    constexpr int DT = T::code, NW = DUAL ? 2 : 1;
+    constexpr int DT = T::code, NW = DUAL ? 2 : 1, P = DT == HASTE_DTYPE_F32 ? 3 : 1, SZ = kElemBytes<DT>;
+    typedef typename std::conditional<P == 3, BF16, T>::type MT;
     __shared__ f32x4 sums[WAVES][NG * NW][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15;
     const int n = blockIdx.x * 16 + r;
-    const char* w[2] = {w0 + (int64_t)min(n, N - 1) * ldw0 * 2, DUAL ? w1 + (int64_t)min(n, N - 1) * ldw1 * 2 : w0};
+    const char* w[2] = {w0 + (int64_t)min(n, N - 1) * ldw0 * SZ,
+                        DUAL ? w1 + (int64_t)min(n, N - 1) * ldw1 * SZ : w0};
     f32x4 acc[NG * NW];
 #pragma unroll
     for (int i = 0; i < NG * NW; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Piece {
+        u32x4 p[P];
+    };
+    // eight elements: one fragment, or three
     auto piece = [](const char* p, int64_t i, int64_t count) __attribute__((always_inline)) {
-        const Elems<DT, 8> v = load_part<DT, 8>(p, i, count);
-        return u32x4{v.q[0], v.q[1], v.q[2], v.q[3]};
+        Piece f;
+        if constexpr (P == 1) {
+            const Elems<DT, 8> v = load_part<DT, 8>(p, i, count);
+            f.p[0] = u32x4{v.q[0], v.q[1], v.q[2], v.q[3]};
+        } else {
+            float v[8];
+            unpack<DT, 8>(load_part<DT, 8>(p, i, count), v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t lo[3], hi[3];
+                split_f32(v[2 * k], lo);
+                split_f32(v[2 * k + 1], hi);
+#pragma unroll
+                for (int j = 0; j < P; ++j) f.p[j][k] = lo[j] | hi[j] << 16;
+            }
+        }
+        return f;
+    };
+    auto rows = [&](int i, int k) __attribute__((always_inline)) {
+        const int m = 16 * i + r, count = m < M ? K - k : 0;
+        if constexpr (P == 1 || DUAL) return piece(x + (int64_t)m * ldx * SZ, k, count);
+        Piece f;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const Elems<HASTE_DTYPE_BF16, 8> v =
+                load_part<HASTE_DTYPE_BF16, 8>(x + j * plane + (int64_t)m * ldx * 2, k, count);
+            f.p[j] = u32x4{v.q[0], v.q[1], v.q[2], v.q[3]};
+        }
+        return f;
     };
 #pragma unroll 4
     for (int k0 = wave * 32; k0 < K; k0 += 32 * WAVES) {
         const int k = k0 + 8 * (lane >> 4);
-        u32x4 fw[NW], fx[NG];
+        Piece fw[NW], fx[NG];
 #pragma unroll
         for (int i = 0; i < NW; ++i) fw[i] = piece(w[i], k, n < N ? K - k : 0);
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
-            fx[i] = piece(x + (int64_t)(16 * i + r) * ldx * 2, k, 16 * i + r < M ? K - k : 0);
+        for (int i = 0; i < NG; ++i) fx[i] = rows(i, k);
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
-            for (int j = 0; j < NW; ++j) acc[i * NW + j] = mfma16x16x32<T>(fw[j], fx[i], acc[i * NW + j]);
+            for (int j = 0; j < NW; ++j) {
+                f32x4& c = acc[i * NW + j];
+                if constexpr (P == 1) {
+                    c = mfma16x16x32<MT>(fw[j].p[0], fx[i].p[0], c);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 6; ++q)
+                        c = mfma16x16x32<MT>(fw[j].p[kPartsOfB >> (2 * q) & 3], fx[i].p[kPartsOfA >> (2 * q) & 3], c);
+                }
+            }
     }
 #pragma unroll
     for (int i = 0; i < NG * NW; ++i) sums[wave][i][lane] = acc[i];
@@ -122,7 +164,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int
 }
 
 // Matrices [R, C] of any pitch as rows of P (a multiple of 8) elements on 16 bytes, with zeros behind C;
-// one launch for all that a call has.
+// fp32 ones as their three parts.  One launch for all that a call has.
 constexpr int kMaxPacks = 5;
 struct Packs {
     struct {
@@ -133,16 +175,24 @@ struct Packs {
     } m[kMaxPacks];
     int count;
 };
+template <bool F32>
 __global__ __launch_bounds__(256) void pack_rows_kernel(Packs p) {
+    constexpr int DT = F32 ? HASTE_DTYPE_F32 : HASTE_DTYPE_BF16;
     int k = 0;
     for (int j = 1; j < p.count; ++j) k = blockIdx.x >= p.m[j].block0 ? j : k;
     const auto& m = p.m[k];
     const int64_t i = (int64_t)(blockIdx.x - m.block0) * 256 + threadIdx.x, pieces = m.P / 8;
     if (i >= m.R * pieces) return;
     const int64_t r = i / pieces, c = i % pieces * 8;
-    const Elems<HASTE_DTYPE_BF16, 8> v =
-        load_part<HASTE_DTYPE_BF16, 8>(m.src + r * m.ld * 2, c, m.C - c);
-    store<HASTE_DTYPE_BF16, 8>(m.dst, r * m.P + c, v);
+    const Elems<DT, 8> v = load_part<DT, 8>(m.src + r * m.ld * kElemBytes<DT>, c, m.C - c);
+    if constexpr (F32) {
+        float f[8];
+        unpack<DT, 8>(v, f);
+        const f32x4 w[2] = {{f[0], f[1], f[2], f[3]}, {f[4], f[5], f[6], f[7]}};
+        put_operand<DT, 2>(m.dst, m.R * m.P * 2, r * m.P + c, w);
+    } else {
+        store<DT, 8>(m.dst, r * m.P + c, v);
+    }
 }
 
 // ------------------------------------------------------------------ host ----
@@ -152,11 +202,16 @@ constexpr int kFewRows = 64;
 int64_t round8(int64_t n) { return ceil_div(n, 8) * 8; }
 int64_t round16(int64_t n) { return ceil_div(n, 16) * 16; }  // (the pitch of h and its like)
 int64_t kept_blocks(int64_t H) { return ceil_div(H, 64); }
+// h, dg or du: of the type, fp32 as three bf16 parts.
+int64_t hidden_bytes(int64_t N, int64_t ld, int32_t dtype) {
+    return N * ld * 2 * (dtype == HASTE_DTYPE_F32 ? 3 : 1);
+}
 
 // A matrix as the kernels take it.
 struct Matrix {
     const void* p;
     int64_t ld, rows, cols;
+    int64_t plane = 0;  // fp32 as three parts: bytes between them
 };
 bool plain_rows(const Matrix& m) { return aligned16(m.p) && m.ld % 8 == 0 && m.cols % 8 == 0; }
 
@@ -186,6 +241,10 @@ template <>
 struct TypeOf<HASTE_DTYPE_F16> {
     typedef F16 type;
 };
+template <>
+struct TypeOf<HASTE_DTYPE_F32> {
+    typedef F32Parts type;
+};
 
 template <typename Tile>
 GemmArgs gemm_args(const Product& p, int segments, int splits) {
@@ -196,13 +255,15 @@ GemmArgs gemm_args(const Product& p, int segments, int splits) {
     }
     g.a.ld = p.a[0].ld;
     g.b.ld = p.b[0].ld;
+    g.a.plane = p.a[0].plane;
+    g.b.plane = p.b[0].plane;
     g.M = (int)p.M;
     g.N = (int)p.N;
     g.K = (int)p.K;
     g.tiles_m = (int)ceil_div(p.M, Tile::BM);
     g.tiles_n = (int)ceil_div(p.N, Tile::kCols);
     g.steps = (int)ceil_div(p.K, Tile::KS);
-    g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, (int64_t)g.steps * segments));
+    g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, (int64_t)g.steps * segments * Tile::kProducts));
     return g;
 }
 
@@ -225,7 +286,8 @@ struct Cut {
 template <GemmMode MODE, int DT>
 Cut cut_of(const Product& p, bool may_split) {
     const int64_t batches = MODE == GemmMode::kBatch ? 2 : 1;
-    const int64_t steps = ceil_div(p.K, 32) * (MODE == GemmMode::kSegments ? 2 : 1);
+    const int64_t products = DT == HASTE_DTYPE_F32 ? 6 : 1;
+    const int64_t steps = ceil_div(p.K, 32) * (MODE == GemmMode::kSegments ? 2 : 1) * products;
     auto tiles = [&](int64_t rows, int64_t cols) {
         return ceil_div(p.M, rows) * ceil_div(p.N, MODE == GemmMode::kDual ? cols / 2 : cols) * batches;
     };
@@ -235,7 +297,6 @@ Cut cut_of(const Product& p, bool may_split) {
         return may_split ? std::max<int64_t>(1, std::min(256 / n, steps / 16)) : 1;
     };
     if (small == 0) return Cut{Tiles::kSmall, 1};
-    if (DT == HASTE_DTYPE_F32) return Cut{Tiles::kSmall, (int)splits(small)};
     if (big >= 192) return Cut{Tiles::kLarge, 1};
     if (may_split && steps / 32 >= ceil_div(192, big)) return Cut{Tiles::kLarge, (int)(256 / big)};
     if (small * splits(small) <= 128) return Cut{Tiles::kLow, (int)splits(low)};
@@ -245,30 +306,25 @@ Cut cut_of(const Product& p, bool may_split) {
 template <int DT, GemmMode MODE, bool AK, bool BK_, typename Epilogue>
 void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_t st) {
     constexpr int batches = MODE == GemmMode::kBatch ? 2 : 1, segments = MODE == GemmMode::kSegments ? 2 : 1;
-    if constexpr (DT == HASTE_DTYPE_F32) {
-        typedef GemmTileF32<MODE, AK, BK_> Tile;
-        launch_tiles<Tile, DT>(gemm_args<Tile>(p, segments, cut.splits), batches, act, out, st);
-    } else {
-        typedef typename TypeOf<DT>::type T;
-        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4, 4> Large;
-        typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2, 4> Small;
-        if constexpr (!std::is_same<Epilogue, PlainOut>::value) {
-            // An epilogue that moves 8 to 10 bytes an element takes longer than a short K: two workgroups
-            // to a CU, of 256 x 128, overlap one's with the other's products (65536 x 2048 elements, K =
-            // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
-            // 1308, since they load half as much again).
-            typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
-            if (cut.tiles == Tiles::kLarge && p.K <= 1024)
-                return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);
-        }
-        typedef GemmTile<T, MODE, AK, BK_, 2, 4, 2, 2, 4> Low;
-        if (cut.tiles == Tiles::kLarge)
-            launch_tiles<Large, DT>(gemm_args<Large>(p, segments, cut.splits), batches, act, out, st);
-        else if (cut.tiles == Tiles::kSmall)
-            launch_tiles<Small, DT>(gemm_args<Small>(p, segments, cut.splits), batches, act, out, st);
-        else
-            launch_tiles<Low, DT>(gemm_args<Low>(p, segments, cut.splits), batches, act, out, st);
+    typedef typename TypeOf<DT>::type T;
+    typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4, 4> Large;
+    typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2, 4> Small;
+    if constexpr (!std::is_same<Epilogue, PlainOut>::value) {
+        // An epilogue that moves 8 to 10 bytes an element takes longer than a short K: two workgroups
+        // to a CU, of 256 x 128, overlap one's with the other's products (65536 x 2048 elements, K =
+        // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
+        // 1308, since they load half as much again).
+        typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
+        if (cut.tiles == Tiles::kLarge && DT != HASTE_DTYPE_F32 && p.K <= 1024)
+            return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);
     }
+    typedef GemmTile<T, MODE, AK, BK_, 2, 4, 2, 2, 4> Low;
+    if (cut.tiles == Tiles::kLarge)
+        launch_tiles<Large, DT>(gemm_args<Large>(p, segments, cut.splits), batches, act, out, st);
+    else if (cut.tiles == Tiles::kSmall)
+        launch_tiles<Small, DT>(gemm_args<Small>(p, segments, cut.splits), batches, act, out, st);
+    else
+        launch_tiles<Low, DT>(gemm_args<Low>(p, segments, cut.splits), batches, act, out, st);
 }
 
 // A product without an epilogue, its parts of K joined by a second launch.  `parts` has room for
@@ -296,24 +352,27 @@ struct Sizes {
     int64_t N, D, H, O;
 };
 
-// Matrices with 16-byte rows: themselves, or copies in the workspace, made by one launch.
+// Matrices with 16-byte rows (fp32: their parts): themselves, or copies in the workspace, made by one launch.
 struct Packer {
     Packs packs{};
     uint32_t blocks = 0;
     template <int DT>
     Matrix add(const Matrix& m, Space& ws, bool used) {
-        if (DT == HASTE_DTYPE_F32 || plain_rows(m)) return m;
-        const int64_t P = round8(m.cols);
-        void* to = ws.take(m.rows * P * 2);
+        constexpr bool parts = DT == HASTE_DTYPE_F32;
+        if (!parts && plain_rows(m)) return m;
+        const int64_t P = round8(m.cols), plane = parts ? m.rows * P * 2 : 0;
+        void* to = ws.take(m.rows * P * 2 * (parts ? 3 : 1));
         if (used && m.rows > 0) {
             packs.m[packs.count++] = {static_cast<const char*>(m.p), static_cast<char*>(to), m.ld,
                                       m.rows, m.cols, P, blocks};
             blocks += (uint32_t)ceil_div(m.rows * (P / 8), 256);
         }
-        return Matrix{to, P, m.rows, m.cols};
+        return Matrix{to, P, m.rows, m.cols, plane};
     }
+    template <int DT>
     void launch(hipStream_t st) const {
-        if (blocks) pack_rows_kernel<<<dim3(blocks), dim3(256), 0, st>>>(packs);
+        if (blocks)
+            pack_rows_kernel<DT == HASTE_DTYPE_F32><<<dim3(blocks), dim3(256), 0, st>>>(packs);
     }
 };
 
@@ -321,39 +380,37 @@ template <int DT>
 int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const GatedOut& out, void* y,
                 int act, char* base, bool launch, hipStream_t st) {
     Space ws{base};
-    if constexpr (DT != HASTE_DTYPE_F32) {
-        if (s.N <= kFewRows) {
-            if (!launch) return 0;
-            typedef typename TypeOf<DT>::type T;
-            const char *xc = static_cast<const char*>(x.p), *gc = static_cast<const char*>(wg.p),
-                       *uc = static_cast<const char*>(wu.p), *dc = static_cast<const char*>(wd.p),
-                       *hc = static_cast<const char*>(out.h);
-            const dim3 g1((unsigned)ceil_div(out.ld, 16)), g2((unsigned)ceil_div(s.O, 16));
-            const PlainOut po{{y, nullptr}, s.O, nullptr, (int)s.N, (int)s.O, 1};
-            auto run = [&](auto groups) {
-                constexpr int NG = decltype(groups)::value;
-                few_rows_kernel<T, NG, true, 8, GatedOut><<<g1, dim3(512), 0, st>>>(
-                    xc, x.ld, gc, wg.ld, uc, wu.ld, (int)s.N, (int)s.H, (int)s.D, act, out);
-                few_rows_kernel<T, NG, false, 16, PlainOut><<<g2, dim3(1024), 0, st>>>(
-                    hc, out.ld, dc, wd.ld, nullptr, 0, (int)s.N, (int)s.O, (int)s.H, 0, po);
-            };
-            if (s.N <= 16) run(std::integral_constant<int, 1>());
-            else if (s.N <= 32) run(std::integral_constant<int, 2>());
-            else run(std::integral_constant<int, 4>());
-            return 0;
-        }
+    if (s.N <= kFewRows) {
+        if (!launch) return 0;
+        typedef typename TypeOf<DT>::type T;
+        const char *xc = static_cast<const char*>(x.p), *gc = static_cast<const char*>(wg.p),
+                   *uc = static_cast<const char*>(wu.p), *dc = static_cast<const char*>(wd.p),
+                   *hc = static_cast<const char*>(out.h);
+        const dim3 g1((unsigned)ceil_div(out.ld, 16)), g2((unsigned)ceil_div(s.O, 16));
+        const PlainOut po{{y, nullptr}, s.O, nullptr, (int)s.N, (int)s.O, 1};
+        auto run = [&](auto groups) {
+            constexpr int NG = decltype(groups)::value;
+            few_rows_kernel<T, NG, true, 8, GatedOut><<<g1, dim3(512), 0, st>>>(
+                xc, x.ld, 0, gc, wg.ld, uc, wu.ld, (int)s.N, (int)s.H, (int)s.D, act, out);
+            few_rows_kernel<T, NG, false, 16, PlainOut><<<g2, dim3(1024), 0, st>>>(
+                hc, out.ld, out.plane, dc, wd.ld, nullptr, 0, (int)s.N, (int)s.O, (int)s.H, 0, po);
+        };
+        if (s.N <= 16) run(std::integral_constant<int, 1>());
+        else if (s.N <= 32) run(std::integral_constant<int, 2>());
+        else run(std::integral_constant<int, 4>());
+        return 0;
     }
     Packer packer;
     x = packer.add<DT>(x, ws, true);
     wg = packer.add<DT>(wg, ws, true);
     wu = packer.add<DT>(wu, ws, true);
     wd = packer.add<DT>(wd, ws, true);
-    const Matrix h{out.h, out.ld, s.N, s.H};
+    const Matrix h{out.h, out.ld, s.N, s.H, out.plane};
     const Product p1{{x, x}, {wg, wu}, s.N, s.H, s.D};
     const Product p2{{h, h}, {wd, wd}, s.N, s.O, s.H};
     void* parts = ws.take(plain_parts<DT, GemmMode::kPlain>(p2));
     if (launch) {
-        packer.launch(st);
+        packer.launch<DT>(st);
         product<DT, GemmMode::kDual, true, true>(p1, cut_of<GemmMode::kDual, DT>(p1, false), act, out,
                                                  st);
         plain<DT, GemmMode::kPlain, true, true>(p2, y, nullptr, parts, st);
@@ -370,7 +427,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
                  void* kept, const void* h, int64_t ld, const Grads& to, char* base,
                  bool launch, hipStream_t st) {
     Space ws{base};
-    const int64_t bytes = s.N * ld * elem_bytes(DT);
+    const int64_t plane = DT == HASTE_DTYPE_F32 ? s.N * ld * 2 : 0, bytes = hidden_bytes(s.N, ld, DT);
     void *dg = ws.take(bytes), *du = ws.take(bytes);
     Packer packer;
     x = packer.add<DT>(x, ws, to.dwg || to.dwu);
@@ -378,7 +435,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
     wu = packer.add<DT>(wu, ws, to.dx);
     wd = packer.add<DT>(wd, ws, to.dx || to.dwg || to.dwu);
     dy = packer.add<DT>(dy, ws, true);
-    const Matrix mg{dg, ld, s.N, s.H}, mu{du, ld, s.N, s.H}, mh{h, ld, s.N, s.H};
+    const Matrix mg{dg, ld, s.N, s.H, plane}, mu{du, ld, s.N, s.H, plane}, mh{h, ld, s.N, s.H, plane};
     const Product p1{{dy, dy}, {wd, wd}, s.N, s.H, s.O};
     const Product p2{{mg, mu}, {wg, wu}, s.N, s.D, s.H};
     const Product p3{{mg, mu}, {x, x}, s.H, s.D, s.N};
@@ -387,9 +444,9 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
                                     plain_parts<DT, GemmMode::kBatch>(p3),
                                     plain_parts<DT, GemmMode::kPlain>(p4)}));
     if (launch) {
-        packer.launch(st);
+        packer.launch<DT>(st);
         if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
-            const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld};
+            const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld, plane};
             product<DT, GemmMode::kPlain, true, false>(p1, cut_of<GemmMode::kPlain, DT>(p1, false), 0, out,
                                                        st);
         }
@@ -461,7 +518,7 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
 #define HASTE_MLP(DT)                                                                                   \
     (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, ld, haste::Grads{}, \
                                     nullptr, false, nullptr)                                          \
-              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{{nullptr, 0}, nullptr, ld},     \
+              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{{nullptr, 0}, nullptr, ld, 0},     \
                                    nullptr, 0, nullptr, false, nullptr))
     return HASTE_MLP_TYPES(HASTE_MLP);
 #undef HASTE_MLP
@@ -490,7 +547,8 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
     HASTE_CHECK_ARG(y != nullptr && haste::elem_aligned(y, dtype), "%s: y is NULL or misaligned", fn);
     HASTE_TRY(haste::mlp_hidden(fn, "h", h));
     if (kept) HASTE_TRY(haste::mlp_hidden(fn, "kept", kept));
-    const haste::GatedOut out{{kept, haste::kept_blocks(H)}, h, haste::round16(H)};
+    const haste::GatedOut out{{kept, haste::kept_blocks(H)}, h, haste::round16(H),
+                              dtype == HASTE_DTYPE_F32 ? N * haste::round16(H) * 2 : 0};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) haste::forward<DT>(s, mx, mg, mu, md, out, y, act, base, launch, st)

@@ -76,6 +76,42 @@ __device__ __forceinline__ void put_columns(void* p, int64_t at, const f32x4 (&v
     }
 }
 
+// fp32 as three bf16 parts, the rest rounded to nearest each time (gemm.hpp).  What is not finite is its
+// own first part; what would round to infinity is cut instead.
+__device__ __forceinline__ void split_f32(float a, uint32_t (&u)[3]) {
+    u[0] = f32_to_bf16_rne(a);
+    const uint32_t bits = __float_as_uint(a);
+    const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+    if (finite && (u[0] & 0x7FFFu) == 0x7F80u) u[0] = bits >> 16;
+    const float r = finite ? a - bf16_bits_to_f32(u[0]) : 0.f;
+    u[1] = f32_to_bf16_rne(r);
+    u[2] = f32_to_bf16_rne(r - bf16_bits_to_f32(u[1]));
+}
+// 4 F columns of a matrix that is an operand of the next product: of its type, or three parts.
+template <int DT, int F>
+__device__ __forceinline__ void put_operand(void* p, int64_t plane, int64_t at, const f32x4 (&v)[F]) {
+    if constexpr (DT == HASTE_DTYPE_F32) {
+        uint32_t w[3][2 * F];
+#pragma unroll
+        for (int k = 0; k < 2 * F; ++k) {
+            uint32_t lo[3], hi[3];
+            split_f32(v[k / 2][k % 2 * 2], lo);
+            split_f32(v[k / 2][k % 2 * 2 + 1], hi);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) w[i][k] = lo[i] | hi[i] << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            char* to = static_cast<char*>(p) + i * plane + at * 2;
+#pragma unroll
+            for (int k = 0; k < 2 * F; k += 2)
+                *reinterpret_cast<u32x2*>(to + 4 * k) = u32x2{w[i][k], w[i][k + 1]};
+        }
+    } else {
+        put_columns<DT, F>(p, at, v, 4 * F);
+    }
+}
+
 // What the forward keeps for the backward, s = u act'(g) and a = act(g): fp32, or for 16-bit matrices its
 // upper 24 bits (15 of mantissa), rounded to nearest.  16 bits would add two roundings of the type's
 // to the gradients, which have two that cannot be helped (dg and du as the matrix instructions take
@@ -162,7 +198,7 @@ __device__ __forceinline__ f32x4 kept_columns(const Kept<DT>& k, int j) {
 struct GatedOut {
     KeptPlace kept;
     void* h;
-    int64_t ld;
+    int64_t ld, plane;
     template <int DT, int ACT, int F>
     __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&vg)[F], const f32x4 (&vu)[F]) const {
         f32x4 vh[F], vs[F], va[F];
@@ -176,7 +212,7 @@ struct GatedOut {
                 vs[k][e] = s * vu[k][e];
                 vh[k][e] = a * vu[k][e];
             }
-        put_columns<DT, F>(h, m * ld + n, vh, 4 * F);
+        put_operand<DT, F>(h, plane, m * ld + n, vh);
         if (!kept.p) return;
         char* block = kept.template block<DT>(m, n);
         put_kept<DT, F>(block, m, n, vs);
@@ -187,17 +223,17 @@ struct GatedOut {
 struct GatedGrad {
     KeptPlace kept;
     void *dg, *du;
-    int64_t ld;
+    int64_t ld, plane;
     template <int DT, int F>
     __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&dh)[F], const Kept<DT>& s,
                                         const Kept<DT>& a) const {
         f32x4 v[F];
 #pragma unroll
         for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(s, k);
-        put_columns<DT, F>(dg, m * ld + n, v, 4 * F);
+        put_operand<DT, F>(dg, plane, m * ld + n, v);
 #pragma unroll
         for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(a, k);
-        put_columns<DT, F>(du, m * ld + n, v, 4 * F);
+        put_operand<DT, F>(du, plane, m * ld + n, v);
     }
 };
 

@@ -1,6 +1,11 @@
 // Products of 16-bit matrices with fp32 sums, C[m, n] = sum_k A(m, k) B(n, k), as tiles of BM x BN for
 // a workgroup of WM x WN waves, each of which holds FM x FN MFMA tiles of 16 x 16.
 //
+// fp32 matrices come as three bf16 parts, a = a0 + a1 + a2 (each the rest rounded to nearest, so that
+// |a1| <= 2^-9 |a| and |a2| <= 2^-18 |a|), and their product as the six of the parts' products that are not
+// under 2^-26 of it: a2 b0 + a0 b2 + a1 b1 + a1 b0 + a0 b1 + a0 b0, one behind the other along K.  Six
+// bf16 products take less time than one on the fp32 matrix instructions, whose rate is a sixteenth.
+//
 // K goes in steps of 32 through four stages of LDS.  Loads write LDS straight from memory, three steps
 // ahead; a wave reads the fragments of step k + 1 while its MFMAs work on step k, so neither waits
 // for the other, and one barrier a step is enough: the stage that is loaded into was last read two
@@ -13,6 +18,8 @@
 // lanes' addresses in memory are permuted, since a load to LDS writes lane after lane.
 #pragma once
 
+#include <type_traits>
+
 #include "elements.hpp"
 
 namespace haste {
@@ -21,7 +28,8 @@ namespace haste {
 // unused (R).
 struct GemmOperand {
     const char* base[2];
-    int64_t ld;  // elements
+    int64_t ld;     // elements
+    int64_t plane;  // bytes between the parts of an fp32 matrix
 };
 
 // PLAIN: one product.  DUAL: the left half of a tile's columns is B's base[0], the right half base[1],
@@ -44,7 +52,9 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 // flight before each read of LDS.  Nothing waits for this but wait_loads().
 __device__ __forceinline__ void load_lds16(const char* base, uint32_t voff, uint32_t lds) {
     const uint64_t p = reinterpret_cast<uint64_t>(base);
-    const i32x4 rsrc = {(int)(uint32_t)p, (int)((uint32_t)(p >> 32) & 0xFFFFu), 0x7FFFFF00, 0x00020000};
+    const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
+                        __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xFFFFu)), 0x7FFFFF00,
+                        0x00020000};
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0\n\t"
@@ -59,9 +69,21 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(n) : "memory");
 }
 
+// The fp32 form's six products: which part of A and of B (two bits each).
+constexpr uint32_t kPartsOfA = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10;
+constexpr uint32_t kPartsOfB = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
+
+// T: BF16, F16, or F32Parts.
+struct F32Parts {
+    static constexpr int code = HASTE_DTYPE_F32;
+};
+
 template <typename T, GemmMode MODE, bool AK, bool BK_, int FM_, int FN_, int WM_, int WN_,
           int STAGES>
 struct GemmTile {
+    static constexpr bool kParts = std::is_same<T, F32Parts>::value;
+    static constexpr int kProducts = kParts ? 6 : 1;
+    typedef typename std::conditional<kParts, BF16, T>::type M_;
     static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, kWaves = WM * WN;
     static constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, KS = 32, kStages = STAGES;
     static constexpr int kThreads = 64 * kWaves;
@@ -118,9 +140,9 @@ struct GemmTile {
         const int wm = wave % WM, wn = wave / WM;
         m0 = tm * BM + wm * FM * 16;
         n0 = tn * kCols + wn * (kDual ? FN / 2 : FN) * 16;
-        const int all = MODE == GemmMode::kSegments ? 2 * g.steps : g.steps;
-        const int k0 = (int)((int64_t)all * split / g.splits),
-                  k1 = (int)((int64_t)all * (split + 1) / g.splits);
+        const int all = (MODE == GemmMode::kSegments ? 2 : 1) * kProducts * g.steps;
+        const int k0 = __builtin_amdgcn_readfirstlane((int)((int64_t)all * split / g.splits)),
+                  k1 = __builtin_amdgcn_readfirstlane((int)((int64_t)all * (split + 1) / g.splits));
         // bytes from a tile's first element
         uint32_t off[kLoads];
         int kpos[kLoads];
@@ -150,14 +172,26 @@ struct GemmTile {
             kpos[kALoads + j] = k;
         }
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        // the next step to be loaded: step `k_in` of run `part` over K
+        int part = __builtin_amdgcn_readfirstlane(k0 / max(g.steps, 1)), k_in = k0 - part * g.steps;
         auto issue = [&](int kt) __attribute__((always_inline)) {
-            const bool second = MODE == GemmMode::kSegments && kt >= g.steps;
-            const int k = (second ? kt - g.steps : kt) * KS;
+            const bool second = MODE == GemmMode::kSegments && part >= kProducts;
+            const int k = k_in * KS;
             const int left = kt < k1 ? g.K - k : 0;
             const uint32_t to = lds0 + stage_of(kt) * kStage;
-            const char* a = pa[second] + (AK ? (int64_t)k * 2 : k * lda);
-            const char* b = pb[second] + (BK_ ? (int64_t)k * 2 : k * ldb);
-            const char* b2 = kDual ? pb[1] + (BK_ ? (int64_t)k * 2 : k * ldb) : b;
+            int64_t pa_off = AK ? (int64_t)k * 2 : k * lda, pb_off = BK_ ? (int64_t)k * 2 : k * ldb;
+            if (kParts) {
+                const int product = second ? part - kProducts : part;
+                pa_off += (kPartsOfA >> (2 * product) & 3) * g.a.plane;
+                pb_off += (kPartsOfB >> (2 * product) & 3) * g.b.plane;
+            }
+            const char* a = (second ? pa[1] : pa[0]) + pa_off;
+            const char* b = (second ? pb[1] : pb[0]) + pb_off;
+            const char* b2 = kDual ? pb[1] + pb_off : b;
+            if (++k_in == g.steps) {
+                k_in = 0;
+                ++part;
+            }
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 const bool is_a = j < kALoads;
@@ -183,7 +217,7 @@ struct GemmTile {
             for (int f = 0; f < FM; ++f)
 #pragma unroll
                 for (int h = 0; h < FN; ++h)
-                    acc[h][f] = mfma16x16x32<T>(fb[set][h], fa[set][f], acc[h][f]);
+                    acc[h][f] = mfma16x16x32<M_>(fb[set][h], fa[set][f], acc[h][f]);
         };
 #pragma unroll
         for (int h = 0; h < FN; ++h)
@@ -218,110 +252,6 @@ struct GemmTile {
         }
         // (LDS is written until here)
         wait_loads<0>();
-    }
-};
-
-// The same of fp32 matrices on v_mfma_f32_16x16x4: rows of any pitch, staged through registers into
-// LDS as rows of BM (BN) r's, two steps of 16 in turn.
-template <GemmMode MODE, bool AK, bool BK_>
-struct GemmTileF32 {
-    static constexpr int FM = 4, FN = 4, WM = 2, WN = 2, BM = 128, BN = 128, KS = 16;
-    static constexpr int kThreads = 256, kPitch = BM + 4;
-    static constexpr bool kDual = MODE == GemmMode::kDual;
-    static constexpr int kCols = kDual ? BN / 2 : BN;
-    static constexpr int kLdsBytes = 2 * 2 * KS * kPitch * 4;
-    typedef Elems<HASTE_DTYPE_F32, 4> Piece;
-
-    f32x4 acc[FN][FM];
-    int m0, n0;
-
-    // Pieces t and t + 256 of an operand's step: four elements along its contiguous axis.
-    template <bool KC>
-    static __device__ __forceinline__ void place(int i, int* r, int* k) {
-        *r = KC ? i / 4 : i % 32 * 4;
-        *k = KC ? i % 4 * 4 : i / 32;
-    }
-    template <bool KC>
-    static __device__ __forceinline__ void put(float* s, int i, const Piece& v) {
-        int r, k;
-        place<KC>(i, &r, &k);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            s[KC ? (k + e) * kPitch + r : k * kPitch + r + e] = __uint_as_float(v.q[e]);
-    }
-    // rows [0, rows) of the tile and k's [0, left) of the step count
-    template <bool KC>
-    static __device__ __forceinline__ Piece get(const char* base, int64_t ld, int i, int rows, int left) {
-        int r, k;
-        place<KC>(i, &r, &k);
-        if (KC) return load_part<HASTE_DTYPE_F32, 4>(base, r * ld + k, r < rows ? left - k : 0);
-        return load_part<HASTE_DTYPE_F32, 4>(base, k * ld + r, k < left ? rows - r : 0);
-    }
-
-    __device__ __forceinline__ void run(const GemmArgs& g, char* lds, int tm, int tn, int batch,
-                                        int split) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = threadIdx.x;
-        const int wm = wave % WM, wn = wave / WM;
-        m0 = tm * BM + wm * FM * 16;
-        n0 = tn * kCols + wn * (kDual ? FN / 2 : FN) * 16;
-        const int all = MODE == GemmMode::kSegments ? 2 * g.steps : g.steps;
-        const int k0 = (int)((int64_t)all * split / g.splits),
-                  k1 = (int)((int64_t)all * (split + 1) / g.splits);
-        float* s = reinterpret_cast<float*>(lds);
-        auto stage = [&](int kt, int op) __attribute__((always_inline)) {
-            return s + ((kt & 1) * 2 + op) * KS * kPitch;
-        };
-        Piece a[2], b[2];
-        auto fetch = [&](int kt) __attribute__((always_inline)) {
-            const bool second = MODE == GemmMode::kSegments && kt >= g.steps;
-            const int k = (second ? kt - g.steps : kt) * KS, left = kt < k1 ? g.K - k : 0;
-            const int from = MODE == GemmMode::kBatch ? batch : second;
-            const int64_t lda = g.a.ld, ldb = g.b.ld;
-            const char* pa = g.a.base[kDual ? 0 : from] +
-                             4 * (AK ? (int64_t)tm * BM * lda + k : k * lda + (int64_t)tm * BM);
-            const int64_t b0 = 4 * (BK_ ? (int64_t)tn * kCols * ldb + k : k * ldb + (int64_t)tn * kCols);
-            const char* pb = g.b.base[MODE == GemmMode::kBatch ? 0 : from] + b0;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                a[j] = get<AK>(pa, lda, t + 256 * j, g.M - tm * BM, left);
-                if (kDual)  // (K-contiguous: pieces 256 and on are rows 64 and on)
-                    b[j] = get<BK_>(g.b.base[j] + b0, ldb, t, g.N - tn * kCols, left);
-                else
-                    b[j] = get<BK_>(pb, ldb, t + 256 * j, g.N - tn * kCols, left);
-            }
-        };
-#pragma unroll
-        for (int h = 0; h < FN; ++h)
-#pragma unroll
-            for (int f = 0; f < FM; ++f) acc[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (k0 < k1) fetch(k0);
-        for (int kt = k0; kt < k1; ++kt) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                put<AK>(stage(kt, 0), t + 256 * j, a[j]);
-                put<BK_>(stage(kt, 1), t + 256 * j, b[j]);
-            }
-            __syncthreads();  // (a stage is written again after the next step's)
-            fetch(kt + 1);
-#pragma unroll
-            for (int k = 0; k < KS; k += 4) {
-                const float *ra = stage(kt, 0) + (k + (lane >> 4)) * kPitch + (lane & 15),
-                            *rb = stage(kt, 1) + (k + (lane >> 4)) * kPitch + (lane & 15);
-                float fa[FM], fb[FN];
-#pragma unroll
-                for (int f = 0; f < FM; ++f) fa[f] = ra[(wm * FM + f) * 16];
-#pragma unroll
-                for (int f = 0; f < FN; ++f)
-                    fb[f] = rb[kDual ? (f / (FN / 2)) * (BN / 2) + (wn * (FN / 2) + f % (FN / 2)) * 16
-                                     : (wn * FN + f) * 16];
-#pragma unroll
-                for (int f = 0; f < FM; ++f)
-#pragma unroll
-                    for (int h = 0; h < FN; ++h)
-                        acc[h][f] =
-                            __builtin_amdgcn_mfma_f32_16x16x4f32(fb[h], fa[f], acc[h][f], 0, 0, 0);
-            }
-        }
     }
 };
 

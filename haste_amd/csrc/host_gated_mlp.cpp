@@ -51,7 +51,9 @@ Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& u
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = w.O;
     f.y = at::empty(shape, options);
-    f.h = at::empty({N, ld}, options);
+    // (fp32: three bf16 parts)
+    const bool wide = x.scalar_type() == at::kFloat;
+    f.h = at::empty({wide ? 3 * N : N, ld}, wide ? options.dtype(at::kBFloat16) : options);
     if (keep) {
         const int64_t bytes = haste_gated_mlp_kept_size(N, w.H, w.code);
         TORCH_CHECK(bytes >= 0, haste_last_error());
