@@ -2,6 +2,7 @@
 // dW[v] = s sum_{n: t_n = v} dy[n], summed in fp32 in the order of n (no float atomics).
 // Both are bound by HBM; the gradient's table is written once, rows without a token among it.
 #include <algorithm>
+#include <type_traits>
 
 #include "elements.hpp"
 
@@ -120,24 +121,20 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* share, uint
     return before;
 }
 
-// counts [n] to the sums of those before, one workgroup (for more than kOwnScan tiles).
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int64_t n) {
-    __shared__ uint32_t share[16];
+// A digit's counts to the sums of the tiles' before, and its sum behind all counts (for more than
+// kOwnScan tiles).
+__global__ __launch_bounds__(kThreads) void sort_scan_kernel(uint32_t* counts, int tiles) {
+    __shared__ uint32_t share[kThreads / 64];
+    uint32_t* c = counts + (int64_t)blockIdx.x * tiles;
     uint32_t base = 0;
-    for (int64_t i0 = 0; i0 < n; i0 += 4096) {
-        const int64_t i = i0 + threadIdx.x * 4;
-        uint32_t c[4], s = 0, all;
-        for (int k = 0; k < 4; ++k) {
-            c[k] = i + k < n ? counts[i + k] : 0;
-            s += c[k];
-        }
-        uint32_t at = base + sum_before<1024>(s, share, &all);
-        for (int k = 0; k < 4; ++k) {
-            if (i + k < n) counts[i + k] = at;
-            at += c[k];
-        }
+    for (int t0 = 0; t0 < tiles; t0 += kThreads) {
+        const int t = t0 + threadIdx.x;
+        uint32_t all;
+        const uint32_t at = base + sum_before<kThreads>(t < tiles ? c[t] : 0, share, &all);
+        if (t < tiles) c[t] = at;
         base += all;
     }
+    if (threadIdx.x == 0) counts[(int64_t)gridDim.x * tiles + blockIdx.x] = base;
 }
 
 // The lanes of the wave with the same digit, of those `in`.
@@ -187,6 +184,7 @@ __global__ __launch_bounds__(kThreads) void sort_move_kernel(SortPass p) {
         if (b >= bins) break;
         if (p.tiles > kOwnScan) {
             before[j] = p.counts[count_at(p, b, blockIdx.x)];
+            sum[j] = p.counts[(int64_t)bins * p.tiles + b];
         } else {  // summed here: a launch less than by sort_scan_kernel
 #pragma unroll 16
             for (int t = 0; t < p.tiles; ++t) {
@@ -207,11 +205,9 @@ __global__ __launch_bounds__(kThreads) void sort_move_kernel(SortPass p) {
     for (int j = 0; j < kOwn; ++j) {
         const int b = j * kThreads + threadIdx.x;
         if (j * kThreads >= bins) break;
-        uint32_t at = before[j], all;
-        if (p.tiles <= kOwnScan) {
-            at += base + sum_before<kThreads>(sum[j], share, &all);
-            base += all;
-        }
+        uint32_t all;
+        uint32_t at = base + before[j] + sum_before<kThreads>(sum[j], share, &all);
+        base += all;
         if (b < bins)
             for (int w = 0; w < kWaves; ++w) {
                 const uint32_t c = next[w][b];
@@ -329,12 +325,11 @@ __global__ __launch_bounds__(kThreads) void emb_first_kernel(const uint32_t* key
 
 // -------------------------------------------------------------- gradient ----
 // A group of tpr threads sums rows of dy, C vectors of a row to a thread at a time.  A token met up to
-// kLight times is summed by one group, one met up to `window` times by a workgroup's groups together.
+// `light` times is summed by one group, one met up to `window` times by a workgroup's groups together.
 // The sorted places of one met more often are cut where multiples of `window` lie; the parts are
 // summed each by a workgroup, in the same launch, and joined in order by a second.  A window has parts
 // of at most two such tokens: of the one at its first place (slot 0), and of another at its last
 // (slot 1).
-constexpr int kLight = 16;
 struct Gradient {
     const char* dy;
     int64_t lddy;
@@ -343,11 +338,12 @@ struct Gradient {
     char* dw;
     int64_t rows, D, window, windows;
     float scale;
-    int tpr;
+    int tpr, light;
 };
 
 template <int DT, int V, int C>
 struct Columns {
+    static constexpr int kAhead = 4;
     float f[C][V];
     // column vectors c0, c0 + tpr, ... of a group's thread; the last of a row shares elements
     static __device__ __forceinline__ int64_t at(const Gradient& g, int64_t c0, int c) {
@@ -358,18 +354,40 @@ struct Columns {
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int k = 0; k < V; ++k) f[c][k] = 0.f;
-#pragma unroll 4
-        for (int64_t i = b; i < e; ++i) {
-            const char* row = g.dy + (int64_t)g.at[i] * g.lddy * kElemBytes<DT>;
+        // (rows whose loads do not wait for one another: four, or what is left)
+        int64_t i = b;
+        for (; i + kAhead <= e; i += kAhead) add<kAhead>(g, c0, i);
+        if (kAhead > 2 && i + 2 <= e) {
+            add<2>(g, c0, i);
+            i += 2;
+        }
+        for (; i < e; ++i) add<1>(g, c0, i);
+    }
+    template <int n>
+    __device__ __forceinline__ void add(const Gradient& g, int64_t c0, int64_t i) {
+        typename std::conditional<V == 1, float, Elems<DT, V == 1 ? 4 : V>>::type x[n][C];
+        uint32_t at_row[n];
+#pragma unroll
+        for (int j = 0; j < n; ++j) at_row[j] = g.at[i + j];
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const char* row = g.dy + (int64_t)at_row[j] * g.lddy * kElemBytes<DT>;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                float x[V];
-                if constexpr (V == 1) x[0] = load_elem<DT>(row, at(g, c0, c));
-                else unpack<DT, V>(load<DT, V>(row, at(g, c0, c)), x);
-#pragma unroll
-                for (int k = 0; k < V; ++k) f[c][k] += x[k];
+                if constexpr (V == 1) x[j][c] = load_elem<DT>(row, at(g, c0, c));
+                else x[j][c] = load<DT, V>(row, at(g, c0, c));
             }
         }
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float y[V];
+                if constexpr (V == 1) y[0] = x[j][c];
+                else unpack<DT, V>(x[j][c], y);
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[c][k] += y[k];
+            }
     }
     __device__ __forceinline__ void put(const Gradient& g, int64_t c0, int64_t v) const {
         char* row = g.dw + v * g.D * kElemBytes<DT>;
@@ -419,15 +437,15 @@ __global__ __launch_bounds__(kThreads) void emb_grad_kernel(Gradient g, int wind
         const int64_t r = blockIdx.x - windows + group * stride, v = row0 + r;
         const bool mine = r < rows;
         const int64_t b = mine ? g.first[v] : 0, e = mine ? g.first[v + 1] : 0;
-        if (mine && e - b <= kLight)
+        if (mine && e - b <= g.light)
             for (int64_t c0 = lane; c0 * V < g.D; c0 += C * g.tpr) {
                 s.sum(g, c0, b, e);
                 s.put(g, c0, v);
             }
         if (lane == 0) lengths[group] = (int)(e - b);
-        if (!__syncthreads_or(e - b > kLight)) return;
+        if (!__syncthreads_or(e - b > g.light)) return;
         for (int k = 0; k < groups; ++k) {
-            if (lengths[k] <= kLight || lengths[k] > g.window) continue;
+            if (lengths[k] <= g.light || lengths[k] > g.window) continue;
             const int64_t u = row0 + blockIdx.x - windows + k * stride, ub = g.first[u];
             for (int64_t i = 0; i * V < g.D; i += C * g.tpr) {
                 sum_together(g, s, share, i + lane, ub, ub + lengths[k]);
@@ -519,7 +537,7 @@ Plan plan(int64_t N, int64_t V, int64_t D) {
         p.key[k] = take(4 * N);
         p.at[k] = take(4 * N);
     }
-    p.counts = take(4 * (p.tiles << p.bits));
+    p.counts = take(4 * ((p.tiles + 1) << p.bits));
     p.first = take(4 * (V + 1));
     p.parts = take(8 * p.windows * D);
     p.bytes = next;
@@ -678,7 +696,7 @@ extern "C" int haste_embedding_bwd(const void* tokens, int32_t token_bits, const
         const dim3 grid((unsigned)p.tiles), block(haste::kThreads);
         haste::sort_count_kernel<<<grid, block, 0, st>>>(s);
         if (p.tiles > haste::kOwnScan)
-            haste::sort_scan_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.counts, p.tiles << p.bits);
+            haste::sort_scan_kernel<<<dim3(1u << p.bits), block, 0, st>>>(s.counts, s.tiles);
         haste::sort_move_kernel<<<grid, block, 0, st>>>(s);
     }
     haste::emb_first_kernel<<<dim3((unsigned)haste::ceil_div(V + 1, haste::kThreads)),
@@ -687,7 +705,8 @@ extern "C" int haste_embedding_bwd(const void* tokens, int32_t token_bits, const
     const int per = haste::kThreads / shape.tpr;
     const haste::Gradient g{static_cast<const char*>(dy), lddy, key, at, first,
                             reinterpret_cast<float*>(base + p.parts), static_cast<char*>(dw), V, D,
-                            haste::window_of(N), p.windows, (float)scale, shape.tpr};
+                            haste::window_of(N), p.windows, (float)scale, shape.tpr,
+                            std::min(16 * 64 / shape.tpr, 128)};  // (narrow rows: many groups)
     // (a single window holds no token more often than it is long)
     const int windows = p.windows > 1 ? (int)p.windows : 0;
 #define HASTE_EMB(DT, VEC)                                                                           \
