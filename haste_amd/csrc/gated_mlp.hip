@@ -468,6 +468,8 @@ int mlp_sizes(const char* fn, int64_t N, int64_t D, int64_t H, int64_t O, int32_
                     (long long)N, (long long)D, (long long)H, (long long)O);
     HASTE_CHECK_ARG(D <= kMaxSide && H <= kMaxSide && O <= kMaxSide && N < (int64_t)1 << 30,
                     "%s: too large (D, H and O up to 2^20, N below 2^30)", fn);
+    // (a launch over the pieces of x or dy has fewer than 2^32 threads)
+    HASTE_CHECK_ARG(N * std::max(D, O) < (int64_t)1 << 34, "%s: too large (N D and N O below 2^34)", fn);
     HASTE_CHECK_ARG(elem_dtype(dtype), "%s: matrices must be bf16, f16 or f32", fn);
     return HASTE_OK;
 }

@@ -115,6 +115,10 @@ void check(const at::Tensor& logits, const at::Tensor& labels, int64_t top) {
                                                     logits.sizes().slice(0, logits.dim() - 1),
                 "label_log_probs: labels must be [..., L] for logits [..., O] (got ", labels.sizes(),
                 " for ", logits.sizes(), ")");
+    TORCH_CHECK(labels.size(-1) <= HASTE_MAX_GRAD_LABELS || !logits.requires_grad() ||
+                    !at::GradMode::is_enabled(),
+                "label_log_probs: at most ", HASTE_MAX_GRAD_LABELS, " labels a row with a gradient (got ",
+                labels.size(-1), ")");
 }
 
 }  // namespace

@@ -639,6 +639,9 @@ extern "C" int haste_label_log_probs_bwd(const void* z, int64_t ldz, const void*
     const char* fn = "haste_label_log_probs_bwd";
     const int rc = haste::lp_check(fn, z, ldz, labels, label_bits, dlp ? L : 0, B, O, dtype);
     if (rc != HASTE_OK) return rc;
+    // (a row's labels are compared with one another)
+    HASTE_CHECK_ARG(!dlp || L <= HASTE_MAX_GRAD_LABELS, "%s: at most %d labels a row (got %lld)", fn,
+                    HASTE_MAX_GRAD_LABELS, (long long)L);
     if (B == 0) return HASTE_OK;
     HASTE_CHECK_ARG(stats != nullptr && entropy != nullptr &&
                         haste::elem_aligned(stats, HASTE_DTYPE_F32) &&

@@ -693,7 +693,8 @@ int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, 
  * bytes, 16-byte aligned: act(x wg^T) and act'(x wg^T) * (x wu^T) in fp32, for 16-bit types in 24 bits.
  * activation: HASTE_ACT_*.  dtype of all matrices: bf16, f16 or f32 (each
  * product of f32 matrices is six of their bf16 parts: its rounding is fp32's, but an infinity may
- * come out as NaN).  D, H and O up to 2^20, N below 2^30.
+ * come out as NaN).  D, H and O up to 2^20, N below 2^30, N D and N O below
+ * 2^34.
  * ws: workspace of haste_gated_mlp_workspace_size(N, D, H, O, dtype, backward, aligned) bytes (16-byte
  * aligned).  16-bit rows that do not start on 16 bytes, or are no multiple of 8 long, are copied into
  * it; with aligned != 0 there are none.
@@ -744,8 +745,9 @@ int haste_label_log_probs(const void* z, int64_t ldz, const void* labels, int32_
 /*
  * The logits' gradient from those of log_probs (dlp [B, L]) and entropy (dent [B]), either NULL for none:
  *   dz_j = RNE(p_j (-sum_l dlp_l - dent (log p_j + entropy)) + sum_{l: labels_l = j} dlp_l)
- * with row pitch lddz.  stats and entropy are the forward's.
+ * with row pitch lddz.  stats and entropy are the forward's.  L up to HASTE_MAX_GRAD_LABELS.
  */
+#define HASTE_MAX_GRAD_LABELS 4096
 int haste_label_log_probs_bwd(const void* z, int64_t ldz, const void* labels, int32_t label_bits,
                               int64_t L, const float* stats, const float* entropy, const float* dlp,
                               const float* dent, void* dz, int64_t lddz, int64_t B, int64_t O,

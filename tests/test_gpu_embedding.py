@@ -72,7 +72,28 @@ def test_counts(dev, N, V):
     check(*data(N, V, 40, torch.bfloat16, dev, seed=N + V), padding=0 if N % 2 else None)
 
 
-@pytest.mark.parametrize("times", [1, 63, 64, 65, 66, 127, 128, 129, 191, 192, 193, 1000, 5000])
+@pytest.mark.parametrize("N,V", [(65536, 32000), (65537, 32000), (100000, 70001), (300000, 513)])
+def test_tokens_by_their_rank(dev, N, V):
+    """The sort's forms past 64 tiles, and tokens of every frequency."""
+    tokens, w, dy = data(N, V, 24, torch.float32, dev, seed=N)
+    tokens = torch.exp(torch.rand(N, device=dev).double() * torch.tensor(V, device=dev).log()).long() - 1
+    check(tokens.clamp_(0, V - 1), w, dy)
+
+
+@pytest.mark.parametrize("D", [4, 8, 24, 100])
+def test_narrow_rows_of_frequent_tokens(dev, D):
+    """Rows of few threads: many tokens to a workgroup, summed by a group or together."""
+    g = torch.Generator(device=dev).manual_seed(D)
+    counts = torch.randint(0, 400, (700,), generator=g, device=dev)
+    tokens = torch.arange(700, device=dev).repeat_interleave(counts)
+    tokens = tokens[torch.randperm(len(tokens), generator=g, device=dev)]
+    for dt in (torch.bfloat16, torch.float32):
+        check(tokens, torch.randn(700, D, generator=g, device=dev).to(dt),
+              torch.randn(len(tokens), D, generator=g, device=dev).to(dt))
+
+
+@pytest.mark.parametrize("times", [1, 15, 16, 17, 63, 64, 65, 66, 127, 128, 129, 191, 192, 193, 255, 256, 257,
+                                   511, 512, 513, 1000, 5000])
 def test_a_token_met_many_times(dev, times):
     """Parts of a frequent token that begin and end anywhere in a window, next to others."""
     g = torch.Generator(device=dev).manual_seed(times)
@@ -84,7 +105,7 @@ def test_a_token_met_many_times(dev, times):
 
 
 def test_one_token_200000_times(dev):
-    """More places than 2048 windows of 64.  Whole numbers: every partial sum is exact."""
+    """More places than 1024 windows of 192.  Whole numbers: every partial sum is exact."""
     N = 200000
     w = torch.zeros(3, 24, device=dev, requires_grad=True)
     dy = torch.randint(-3, 4, (N, 24), device=dev).float()

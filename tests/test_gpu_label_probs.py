@@ -190,6 +190,11 @@ def test_labels_twice_and_outside(dev):
     check(z, labels, 0, dlp, dent)
     got = check(z, labels, 0, dlp, None)
     assert not got["dz"][5].any() and not got["dz"][6].any()
+    # every label asked for, without a gradient, and as many as may have one
+    z, _, _, _ = data(3, 9000, 1, torch.float32, dev)
+    check(z, torch.arange(9000, device=dev).expand(3, 9000))
+    z, labels, dlp, dent = data(3, 5000, 4096, torch.float32, dev)
+    check(z, labels, 0, dlp, dent)
     # many labels, more than threads
     z, labels, dlp, dent = data(3, 900, 700, torch.float32, dev)
     check(z, labels, 0, dlp, dent)
@@ -317,6 +322,8 @@ def test_refusals(dev):
     with pytest.raises(RuntimeError, match="last axis"):
         ops.label_log_probs(z[:, :0], None)
     z = z.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="4096 labels"):
+        ops.label_log_probs(z, labels.repeat(1, 2049))
     r = ops.label_log_probs(z, labels)
     g, = torch.autograd.grad([r.log_probs], [z], [dlp.requires_grad_(True)], create_graph=True)
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
