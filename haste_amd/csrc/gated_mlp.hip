@@ -3,6 +3,10 @@
 //   forward   [g | u] with h in the epilogue;  y
 //   backward  dh with dg and du in the epilogue;  dx over both;  dWg and dWu;  dWd
 // A few tokens in serving are bound by reading the weights once and take kernels of their own.
+// Measured in bf16 at widths 768 and 2048: one row 4.8 + 4.9 us (9.4 MB, two launches' latency); 509 rows 11 + 10
+// + 4 us (latency of few workgroups); 65,536 rows forward 565 to 626 (412 GFLOP, and 1.07 GB written) + 233 us,
+// backward 430 to 455 + 427 + 410 + 224 us.  At 16,384 rows, widths 4096 and 8192: 1913 + 978 and 1126 + 1944 +
+// 1823 + 917 us, 1.13 to 1.2 PFLOP/s.
 #include <algorithm>
 
 #include "gated_mlp.hpp"

@@ -2,6 +2,8 @@
 //   forward   g = x Wg^T, u = x Wu^T, h = act(g) u;  y = h Wd^T
 //   backward  dh = dy Wd, dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu,
 //             dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+// The epilogues of h and of dg and du are bound by what they move, 8 and 10 bytes an element for 16-bit
+// matrices (65,536 x 2048: 1.07 GB and 1.34 GB, 220 and 270 us of HBM, in part under the products).
 #pragma once
 
 #include <type_traits>

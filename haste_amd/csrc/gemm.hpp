@@ -6,10 +6,15 @@
 // under 2^-26 of it: a2 b0 + a0 b2 + a1 b1 + a1 b0 + a0 b1 + a0 b0, one behind the other along K.  Six
 // bf16 products take less time than one on the fp32 matrix instructions, whose rate is a sixteenth.
 //
-// K goes in steps of 32 through four stages of LDS.  Loads write LDS straight from memory, three steps
-// ahead; a wave reads the fragments of step k + 1 while its MFMAs work on step k, so neither waits
-// for the other, and one barrier a step is enough: the stage that is loaded into was last read two
-// steps ago.
+// K goes in steps of 32 through four stages of LDS (three where two workgroups of 256 x 128 share it).  Loads
+// write LDS straight from memory, all but one of the stages ahead; a wave reads the fragments of step k + 1
+// while its MFMAs work on step k, so neither waits for the other, and one barrier a step is enough: the
+// stage that is loaded into was last read two steps ago.
+//
+// Measured in bf16: 16384 x 4096 x 8192 at 1.12 to 1.21 PFLOP/s by operands' order, 65536 x 768 x 2048 at 0.89
+// (y) to 1.0 (dWg, dWu).  The matrix units bound the large ones: fed without a pause they draw the card's
+// power and its clock falls to 1.7 GHz; a library product of 8192^3 reaches 1.37.  No bank conflicts were
+// counted in LDS.
 //
 // An operand is K-contiguous (element (r, k) at r * ld + k) or R-contiguous (at k * ld + r).  The
 // first kind lies in LDS as rows of 32 k's (64 bytes) and is read 16 bytes a lane; the second as

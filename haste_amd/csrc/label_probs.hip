@@ -1,8 +1,11 @@
 // Log probabilities of given labels under rows of logits, the rows' entropy and their likeliest labels:
 //   m = max z, s = sum e^(z - m), log p = (z - m) - log s, H = log s - sum e^(z - m) (z - m) / s
 // and the logits' gradient dz = p (-sum_l g_l - g_H (log p + H)) + sum_{l: label l = j} g_l.
-// One pass over the logits forward and one backward, both bound by HBM: a thread keeps the running
-// maximum and sums of its part of a row, a wave the largest K keys of its part.
+// One pass over the logits forward and one backward: a thread keeps the running maximum and sums of its
+// part of a row, a wave the largest K keys of its part.  Measured on bf16 logits: 512 rows of 670,091 forward
+// 158 us (686 MB, 4.3 TB/s) and backward 226 us (1.4 GB, 6.1 TB/s, in part from the last-level cache), bound
+// by HBM; 512 rows of 131,073 with entropy and ten labels 41 us (134 MB, 3.2 TB/s), bound by some 14 vector
+// instructions an element.  One row of 131,073: 10 us and 6 us to join its parts, latency.
 #include <algorithm>
 
 #include "elements.hpp"

@@ -29,7 +29,7 @@ def label_log_probs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None,
     """For logits [..., O] and labels [..., L] (int64 or int32; entries outside [0, O) stand for no
     label and give 0): log softmax at the labels, the rows' entropy, and the ``top`` (up to 128)
     largest log probabilities with their labels, equal logits in the labels' order.  Differentiable
-    once, in reverse mode, through ``log_probs`` (of up to 4096 labels a row) and ``entropy``.  Labels with a logit of -infinity are
-    ruled out: they have log probability -infinity, no part in the entropy and no gradient.  A row
-    that rules out all of them, or has a NaN or +infinity, gives NaN."""
+    once, in reverse mode, through ``log_probs`` (of up to 4096 labels a row) and ``entropy``.  Labels
+    with a logit of -infinity are ruled out: they have log probability -infinity, no part in the entropy
+    and no gradient.  A row that rules out all of them, or has a NaN or +infinity, gives NaN."""
     return LabelLogProbs(*host().label_log_probs(logits, labels, top))

@@ -693,8 +693,7 @@ int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, 
  * bytes, 16-byte aligned: act(x wg^T) and act'(x wg^T) * (x wu^T) in fp32, for 16-bit types in 24 bits.
  * activation: HASTE_ACT_*.  dtype of all matrices: bf16, f16 or f32 (each
  * product of f32 matrices is six of their bf16 parts: its rounding is fp32's, but an infinity may
- * come out as NaN).  D, H and O up to 2^20, N below 2^30, N D and N O below
- * 2^34.
+ * come out as NaN).  D, H and O up to 2^20, N below 2^30, N D and N O below 2^34.
  * ws: workspace of haste_gated_mlp_workspace_size(N, D, H, O, dtype, backward, aligned) bytes (16-byte
  * aligned).  16-bit rows that do not start on 16 bytes, or are no multiple of 8 long, are copied into
  * it; with aligned != 0 there are none.
