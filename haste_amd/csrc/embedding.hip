@@ -1,5 +1,5 @@
 // Embedding lookup with scaling, y[n] = s W[t_n], and the table's gradient by sorted tokens,
-// dW[v] = s sum_{n: t_n = v} dy[n], summed in fp32 in the order of n (no float atomics).
+// dW[v] = s sum_{n: t_n = v} dy[n], summed in fp32 in a fixed order (no float atomics).
 // Both are bound by HBM; the gradient's table is written once, rows without a token among it.
 // Measured at 65,536 tokens of 32,000 in bf16 rows of 768: lookup 30 us (142 MB, 4.8 TB/s); gradient 85 us
 // in seven launches: sort 23, first places 5, sums 37 (132 MB, 3.6 TB/s: rows of dy in the tokens'

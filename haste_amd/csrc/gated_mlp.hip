@@ -313,13 +313,13 @@ void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_
     typedef typename TypeOf<DT>::type T;
     typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 4, 4> Large;
     typedef GemmTile<T, MODE, AK, BK_, 4, 4, 2, 2, 4> Small;
-    if constexpr (!std::is_same<Epilogue, PlainOut>::value) {
+    if constexpr (!std::is_same<Epilogue, PlainOut>::value && DT != HASTE_DTYPE_F32) {
         // An epilogue that moves 8 to 10 bytes an element takes longer than a short K: two workgroups
         // to a CU, of 256 x 128, overlap one's with the other's products (65536 x 2048 elements, K =
         // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
         // 1308, since they load half as much again).
         typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
-        if (cut.tiles == Tiles::kLarge && DT != HASTE_DTYPE_F32 && p.K <= 1024)
+        if (cut.tiles == Tiles::kLarge && p.K <= 1024)
             return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);
     }
     typedef GemmTile<T, MODE, AK, BK_, 2, 4, 2, 2, 4> Low;

@@ -31,5 +31,6 @@ def label_log_probs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None,
     largest log probabilities with their labels, equal logits in the labels' order.  Differentiable
     once, in reverse mode, through ``log_probs`` (of up to 4096 labels a row) and ``entropy``.  Labels
     with a logit of -infinity are ruled out: they have log probability -infinity, no part in the entropy
-    and no gradient.  A row that rules out all of them, or has a NaN or +infinity, gives NaN."""
+    and no gradient but that of their own log probability, where ``labels`` ask for it.  A row that
+    rules out all of them, or has a NaN or +infinity, gives NaN."""
     return LabelLogProbs(*host().label_log_probs(logits, labels, top))
