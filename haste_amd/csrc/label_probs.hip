@@ -57,10 +57,12 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 // ------------------------------------------------------------ largest K keys ----
 // A label's key: its logit's order, then the lower label first.  0 is no label's.  NaN is largest.
 typedef unsigned long long Key;
+__device__ __forceinline__ uint32_t order_of(float z) {
+    const uint32_t u = z == 0.f ? 0u : __float_as_uint(z);
+    return z != z ? 0xFFFFFFFFu : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
 __device__ __forceinline__ Key key_of(float z, uint32_t label) {
-    uint32_t u = z == 0.f ? 0u : __float_as_uint(z);
-    u = z != z ? 0xFFFFFFFFu : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-    return (Key)u << 32 | (0xFFFFFFFFu - label);
+    return (Key)order_of(z) << 32 | (0xFFFFFFFFu - label);
 }
 __device__ __forceinline__ float value_of(Key k) {
     const uint32_t u = (uint32_t)(k >> 32);
@@ -131,28 +133,31 @@ struct Candidates {
         count += __popcll(mask);
         if (count > 64 * (R - 1)) cut();
     }
-    __device__ __forceinline__ void refresh() { bound = max(bound, *(volatile Key*)shared); }
 };
 
-// The K-th largest of the wave's 64 R values, as a key that every label with such a logit exceeds.
-template <int R>
-__device__ __forceinline__ Key bound_of(const uint32_t (&u)[R], int K) {
-    int rank[R] = {};
+// The K-th largest of the workgroup's values, one to a thread (u; `share` has room for them), by halving: a
+// key that every label of such an order exceeds.  Orders are taken to the bits that the logits' type has.
+// Every thread calls.
+template <int DT>
+__device__ __forceinline__ Key bound_of(uint32_t u, uint32_t* share, int K) {
+    constexpr int bits = DT == HASTE_DTYPE_F32 ? 32 : DT == HASTE_DTYPE_BF16 ? 16 : 19;
+    share[threadIdx.x] = u;
+    __syncthreads();
+    uint32_t x[kWaves], least = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        for (int j = 0; j < 64; ++j) {
-            const uint32_t o = lane_value(u[r], j);
+    for (int w = 0; w < kWaves; ++w) x[w] = share[w * 64 + (threadIdx.x & 63)];
 #pragma unroll
-            for (int q = 0; q < R; ++q) rank[q] += o > u[q] ? 1 : 0;
-        }
-    // the smallest number that fewer than K exceed
-    uint32_t least = 0xFFFFFFFFu;
+    for (int b = 31; b >= 32 - bits; --b) {
+        const uint32_t more = least | 1u << b;
+        int reach = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) least = rank[r] < K ? min(least, u[r]) : least;
-    for (int o = 32; o; o >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, o));
+        for (int w = 0; w < kWaves; ++w) reach += __popcll(__ballot(x[w] >= more));
+        least = reach >= K ? more : least;
+    }
     return (Key)least << 32;
 }
 
+constexpr int kWindows = 8;  // a thread's windows of steps, at most
 constexpr int buffer_keys(int R) { return R ? 64 * R : 1; }
 
 // The workgroup's sums and largest keys from its waves' in wave 0's list.
@@ -234,7 +239,10 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
     constexpr int SZ = kElemBytes<DT>, V = 16 / SZ;
     typedef Elems<DT, V> Vec;
     __shared__ Shared<R> sh;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // a thread's largest logit of each window of its steps (as orders), and those that are read again
+    __shared__ uint32_t seen[R ? kWindows : 1][R ? kThreads : 1], share[R ? kThreads : 1];
+    __shared__ uint16_t list[R ? kWaves : 1][R ? 64 * kWindows : 1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t row = row0 + blockIdx.x / S;
     const int c = blockIdx.x % S;
     const char* p = z + row * ldz * SZ;
@@ -266,25 +274,29 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
         }
         return q;
     };
-    constexpr int U = 2, G = R ? R / 2 : 1;
-    const int64_t v0 = c * per + wave * 64;
-    float most[G];  // of the lane's logits, in G groups by turns
-#pragma unroll
-    for (int g = 0; g < G; ++g) most[g] = -__builtin_inff();
+    constexpr int U = 2;
+    const int64_t v0 = c * per + wave * 64, stride = U * kThreads,
+                  steps = v0 < v1 ? (v1 - v0 + stride - 1) / stride : 0;
+    const int length = (int)((steps + kWindows - 1) / kWindows);  // steps to a window
+    float all = -__builtin_inff(), most = all;  // the largest of the lane's logits, and of the window's
+    int window = 0, left = length;
+    auto close = [&]() __attribute__((always_inline)) {
+        all = fmaxf(all, most);
+        if constexpr (R > 0) {
+            seen[window++][threadIdx.x] = order_of(most);
+            most = -__builtin_inff();
+            left = length;
+        }
+    };
     Reference ref = reference(a.m);
     auto step = [&](const Vec (&q)[U]) __attribute__((always_inline)) {
         float f[U * V];
 #pragma unroll
         for (int u = 0; u < U; ++u) unpack<DT, V>(q[u], f + u * V);
-        float top_of_step = -__builtin_inff();
+        float top_of_step = f[0];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            float x = f[g * U * V / G];
-#pragma unroll
-            for (int e = 1; e < U * V / G; ++e) x = fmaxf(x, f[g * U * V / G + e]);
-            most[g] = fmaxf(most[g], x);
-            top_of_step = fmaxf(top_of_step, x);
-        }
+        for (int e = 1; e < U * V; ++e) top_of_step = fmaxf(top_of_step, f[e]);
+        most = fmaxf(most, top_of_step);
         // (terms up to e^2 lose nothing, and a new maximum by more is rare)
         if (__any(top_of_step > a.m + 2.f)) {
             rescale(a, fmaxf(a.m, top_of_step));
@@ -308,9 +320,9 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
         }
         a.s = __builtin_fmaf(s, ref.scale, a.s);
         a.t = __builtin_fmaf(__builtin_fmaf(-ref.off, s, t), ref.scale * kLn2, a.t);
+        if (R > 0 && --left == 0) close();
     };
-    // two vectors a step, the next two on their way; [in0, in1): steps whose vectors are whole
-    const int64_t stride = U * kThreads, steps = v0 < v1 ? (v1 - v0 + stride - 1) / stride : 0;
+    // two vectors a step, the next two on their way; steps up to in1 have whole vectors only
     const int64_t whole = min(v1, (off + O) / V);  // (vectors behind it are not whole)
     const int64_t in1 = max((int64_t)0, (whole - v0 - (U - 1) * kThreads - 64 + stride) / stride);
     Vec q[U], next[U];
@@ -340,32 +352,41 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
         edge(i);
         step(q);
     }
-    {
-        float m = a.m;
-#pragma unroll
-        for (int g = 0; g < G; ++g) m = fmaxf(m, most[g]);
-        rescale(a, m);
-    }
+    if (R == 0 || left < length) close();
+    rescale(a, fmaxf(a.m, all));
     if constexpr (R > 0) {
-        // K of the wave's 64 G groups reach the K-th largest of their maxima, so K labels do, and no label
-        // under it is among the K likeliest.  Only the groups that reach it are read again: a few.
-        uint32_t reach[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g)  // (a NaN hides from the maxima, but not from the sum)
-            reach[g] = (uint32_t)(key_of(a.s != a.s ? a.s : most[g], 0) >> 32);
-        const Key b = bound_of<G>(reach, K);
+        // K of the threads reach the K-th largest of their maxima, so K labels do, and no label under it is
+        // among the K likeliest.  Only the threads' windows that reach it are read again: a few.
         if (threadIdx.x == 0) sh.bound = 0;
-        __syncthreads();
-        if (lane == 0) atomicMax(&sh.bound, b);
-        __syncthreads();
-        top.refresh();
-        // (four of a lane's vectors at a time: their loads do not wait for one another)
-        constexpr int B = 4;
-        auto scan = [&](const int64_t (&v)[B], int n) __attribute__((always_inline)) {
+        // (a NaN hides from the maxima, but not from the sum)
+        const bool hidden = a.s != a.s;
+        top.bound = bound_of<DT>(order_of(hidden ? a.s : all), share, K);
+        if (lane == 0) atomicMax(&sh.bound, top.bound);
+        int found = 0;
+        for (int w = 0; w < window; ++w) {
+            const bool in = hidden || seen[w][threadIdx.x] >= (uint32_t)(top.bound >> 32);
+            const uint64_t mask = __ballot(in);
+            if (in) list[wave][found + __popcll(mask & (((uint64_t)1 << lane) - 1))] = w * 64 + lane;
+            found += __popcll(mask);
+        }
+        wave_sync();
+        // (two vectors of a lane at a time: their loads do not wait for one another)
+        constexpr int B = 2;
+        const int vectors = length * U, items = found * vectors;
+        for (int i0 = 0; i0 < items; i0 += 64 * B) {
+            const int n = items - i0 > 64 ? 2 : 1;
             Vec w[B];
+            int64_t v[B];
 #pragma unroll
-            for (int k = 0; k < B; ++k)
-                if (k < n) w[k] = fetch(v[k]);
+            for (int k = 0; k < B; ++k) {
+                if (k >= n) break;
+                const uint32_t i = i0 + k * 64 + lane, x = min(i / vectors, (uint32_t)found - 1);
+                const int at = list[wave][x];
+                v[k] = i < (uint32_t)items
+                           ? v0 + ((int64_t)(at >> 6) * vectors + i % vectors) * kThreads + (at & 63)
+                           : v1;
+                w[k] = fetch(v[k]);
+            }
 #pragma unroll
             for (int k = 0; k < B; ++k) {
                 if (k >= n) break;
@@ -375,38 +396,8 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     if (!__any(!(f[e] < least))) continue;
-                    const int64_t i = v[k] * V - off + e;
-                    top.add(v[k] < v1 && i >= 0 && i < O ? key_of(f[e], (uint32_t)i) : 0);
-                }
-            }
-        };
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const bool in = reach[g] >= (uint32_t)(top.bound >> 32);
-            uint64_t mask = __ballot(in);
-            const int64_t n = v0 < v1 ? (v1 - v0 + kThreads - 1) / kThreads : 0;  // vectors of a lane
-            int64_t v[B];
-            if (n <= (int64_t)__popcll(mask) * G) {
-                for (int64_t j = g; j < n; j += B * G) {
-#pragma unroll
-                    for (int k = 0; k < B; ++k)
-                        v[k] = in && j + k * G < n ? v0 + (j + k * G) * kThreads + lane : v1;
-                    scan(v, (int)min((int64_t)B, (n - j + G - 1) / G));
-                }
-            } else {
-                while (mask) {
-                    int l[B];
-                    const int lanes = min(B, (int)__popcll(mask));
-#pragma unroll
-                    for (int k = 0; k < B; ++k) {
-                        l[k] = mask ? __builtin_ctzll(mask) : -1;
-                        mask &= mask - 1;
-                    }
-                    for (int64_t j = g + (int64_t)lane * G; j - (int64_t)lane * G < n; j += 64 * G) {
-#pragma unroll
-                        for (int k = 0; k < B; ++k) v[k] = l[k] >= 0 && j < n ? v0 + j * kThreads + l[k] : v1;
-                        scan(v, lanes);
-                    }
+                    const int64_t j = v[k] * V - off + e;
+                    top.add(v[k] < v1 && j >= 0 && j < O ? key_of(f[e], (uint32_t)j) : 0);
                 }
             }
         }
@@ -429,6 +420,7 @@ __global__ __launch_bounds__(kThreads) void lp_join_kernel(const char* z, int64_
                                                            const Sums* part, const Key* part_keys,
                                                            int64_t row0) {
     __shared__ Shared<R> sh;
+    __shared__ uint32_t share[R ? kThreads : 1];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t row = row0 + blockIdx.x;
     Sums a = no_sums();
@@ -436,16 +428,12 @@ __global__ __launch_bounds__(kThreads) void lp_join_kernel(const char* z, int64_
     Candidates<R ? R : 2> top{sh.buf[wave], &sh.bound, K, 0, lane, 0};
     if constexpr (R > 0) {
         if (threadIdx.x == 0) sh.bound = 0;
-        __syncthreads();
         const int64_t n = (int64_t)S * K;
-        constexpr int G = R / 2;
-        uint32_t reach[G] = {};
-        for (int64_t i = threadIdx.x, j = 0; i < n; i += kThreads, ++j)
-            reach[j % G] = max(reach[j % G], (uint32_t)(part_keys[row * n + i] >> 32));
-        const Key b = bound_of<G>(reach, K);  // (as in the parts)
-        if (lane == 0) atomicMax(&sh.bound, b);
-        __syncthreads();
-        top.refresh();
+        uint32_t most = 0;
+        for (int64_t i = threadIdx.x; i < n; i += kThreads)
+            most = max(most, (uint32_t)(part_keys[row * n + i] >> 32));
+        top.bound = bound_of<DT>(most, share, K);  // (as in the parts)
+        if (lane == 0) atomicMax(&sh.bound, top.bound);
         for (int64_t i = wave * 64; i < n; i += kThreads)
             top.add(i + lane < n ? part_keys[row * n + i + lane] : 0);
     }
