@@ -4,8 +4,8 @@
 // One pass over the logits forward and one backward: a thread keeps the running maximum and sums of its
 // part of a row, a wave the largest K keys of its part.  Measured on bf16 logits: 512 rows of 670,091 forward
 // 158 us (686 MB, 4.3 TB/s) and backward 226 us (1.4 GB, 6.1 TB/s, in part from the last-level cache), bound
-// by HBM; 512 rows of 131,073 with entropy and ten labels 41 us (134 MB, 3.2 TB/s), bound by some 14 vector
-// instructions an element.  One row of 131,073: 10 us and 6 us to join its parts, latency.
+// by HBM; 512 rows of 131,073 with ten labels 30 us (139 MB, 4.6 TB/s) and 6.6 us to join two parts each: the
+// pass takes about 22 of the 30, finding the labels the rest.  One row of 131,073: 8 us and 5 us, latency.
 #include <algorithm>
 
 #include "elements.hpp"
@@ -157,7 +157,9 @@ __device__ __forceinline__ Key bound_of(uint32_t u, uint32_t* share, int K) {
     return (Key)least << 32;
 }
 
-constexpr int kWindows = 8;  // a thread's windows of steps, at most
+// A thread's windows of steps, at most.  More re-read less and keep more: 512 x 131,073 with the 100
+// likeliest 59 us, with 4 windows 63; 4096 x 20,000 with 10 53 us, with 16 windows 60.
+constexpr int kWindows = 8;
 constexpr int buffer_keys(int R) { return R ? 64 * R : 1; }
 
 // The workgroup's sums and largest keys from its waves' in wave 0's list.
@@ -497,9 +499,10 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(const char* z, int64_t
     }
 }
 
-// How a row is cut: `per` 16-byte vectors to a part, whole steps of a workgroup's.  Four workgroups to a CU
-// (512 rows of 131,073: 48 us, with eight 64), in as many parts as there are steps; but a row of up to 8
-// steps is not cut where there is one for each CU, since joining parts takes a launch more (5 to 8 us).
+// How a row is cut: `per` 16-byte vectors to a part, whole steps of a workgroup's.  Two workgroups to a CU (512
+// rows of 131,073 with ten labels: 30.5 us, with four 36.4, with eight 42; 1000 rows without: 48 and 58), in as
+// many parts as there are steps; but a row of up to 8 steps is not cut where there is one for each CU, since
+// joining parts takes a launch more (5 to 8 us).
 constexpr int64_t kStep = 2 * kThreads;
 struct Cut {
     int64_t per;
@@ -508,7 +511,7 @@ struct Cut {
 Cut cut_of(int64_t B, int64_t O, int32_t dtype) {
     const int64_t vectors = ceil_div(O, 16 / elem_bytes(dtype)) + 1, steps = ceil_div(vectors, kStep);
     if (B >= 256 && steps <= 8) return Cut{steps * kStep, 1};
-    const int64_t parts = std::min<int64_t>({ceil_div(1024, std::max<int64_t>(B, 1)), steps, 256});
+    const int64_t parts = std::min<int64_t>({ceil_div(512, std::max<int64_t>(B, 1)), steps, 256});
     const int64_t per = ceil_div(steps, parts);
     return Cut{per * kStep, (int)ceil_div(steps, per)};
 }
