@@ -3,9 +3,9 @@
 // and the logits' gradient dz = p (-sum_l g_l - g_H (log p + H)) + sum_{l: label l = j} g_l.
 // One pass over the logits forward and one backward: a thread keeps the running maximum and sums of its
 // part of a row, a wave the largest K keys of its part.  Measured on bf16 logits: 512 rows of 670,091 forward
-// 158 us (686 MB, 4.3 TB/s) and backward 226 us (1.4 GB, 6.1 TB/s, in part from the last-level cache), bound
-// by HBM; 512 rows of 131,073 with ten labels 30 us (139 MB, 4.6 TB/s) and 6.6 us to join two parts each: the
-// pass takes about 22 of the 30, finding the labels the rest.  One row of 131,073: 8 us and 5 us, latency.
+// 150 us (686 MB, 4.6 TB/s) and backward 228 us (1.4 GB, 6.0 TB/s, in part from the last-level cache), bound
+// by HBM; 512 rows of 131,073 with ten labels 31 us (139 MB, 4.5 TB/s), some 6 of them to find the labels.  One
+// row of 131,073: 8 us, and 5 us to join its parts, latency.
 #include <algorithm>
 
 #include "elements.hpp"
@@ -157,8 +157,8 @@ __device__ __forceinline__ Key bound_of(uint32_t u, uint32_t* share, int K) {
     return (Key)least << 32;
 }
 
-// A thread's windows of steps, at most.  More re-read less and keep more: 512 x 131,073 with the 100
-// likeliest 59 us, with 4 windows 63; 4096 x 20,000 with 10 53 us, with 16 windows 60.
+// A thread's windows of steps, at most.  More re-read less and keep more: with four workgroups to a CU 512 x
+// 131,073 with the 100 likeliest took 59 us, with 4 windows 63; 4096 x 20,000 with 10 53 us, with 16 windows 60.
 constexpr int kWindows = 8;
 constexpr int buffer_keys(int R) { return R ? 64 * R : 1; }
 
@@ -360,9 +360,10 @@ __global__ __launch_bounds__(kThreads) void lp_kernel(const char* z, int64_t ldz
         // K of the threads reach the K-th largest of their maxima, so K labels do, and no label under it is
         // among the K likeliest.  Only the threads' windows that reach it are read again: a few.
         if (threadIdx.x == 0) sh.bound = 0;
-        // (a NaN hides from the maxima, but not from the sum)
+        // (a NaN hides from the maxima, but not from the sum; it is not what bounds, since +infinity makes the
+        // sum one too)
         const bool hidden = a.s != a.s;
-        top.bound = bound_of<DT>(order_of(hidden ? a.s : all), share, K);
+        top.bound = bound_of<DT>(order_of(all), share, K);
         if (lane == 0) atomicMax(&sh.bound, top.bound);
         int found = 0;
         for (int w = 0; w < window; ++w) {

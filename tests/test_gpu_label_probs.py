@@ -117,6 +117,27 @@ def test_few_and_many_rows(dev, B, O, top):
     check(z, labels, top, dlp, dent)
 
 
+@pytest.mark.parametrize("B,O,dt", [(520, 70001, torch.bfloat16), (513, 40009, torch.float16),
+                                    (260, 60013, torch.float32)])
+@pytest.mark.parametrize("top", [1, 10, 100])
+def test_long_parts(dev, B, O, dt, top):
+    """Parts of many steps, whose likeliest labels are found again by windows of them."""
+    z, _, _, _ = data(B, O, 1, dt, dev, seed=top, pitch=5)
+    i = torch.arange(O, device=dev)
+    z[3] = -1.5                                # all equal
+    z[4], z[5] = (i / O).to(dt), (-i / O).to(dt)
+    z[6] = (i * 7919 % 13).to(dt)              # many of each
+    z[7], z[7, O - 3:] = -INF, 2.0             # three left, at the end
+    z[8, O // 2 : O // 2 + 300] = 9.0          # side by side
+    check(z, None, top)
+    z[9, 12345] = z[9, O - 1] = math.nan
+    z[10, 23456] = INF
+    got = run(z, None, top)
+    order = torch.sort(z[9:11].double(), dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(got["top_labels"][9:11], order)
+    assert got["top_log_probs"][9:11].isnan().all()
+
+
 @pytest.mark.parametrize("kind", ["equal", "ascending", "descending", "steps", "zeros", "two"])
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("top", [1, 5, 32, 128])
@@ -167,6 +188,17 @@ def test_rows_without_a_distribution(dev, dt):
     assert got["top_labels"][1].tolist() == list(range(6))
     assert got["top_labels"][3, :2].tolist() == [2500, 2900]
     assert got["top_labels"][4, 0] == 17 and got["top_labels"][6].tolist() == list(range(6))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("O", [1, 9, 700, 5003, 40001])
+def test_infinity_is_the_likeliest(dev, dt, O):
+    """One label at +infinity and no NaN, or one NaN: it is the first of any number of labels."""
+    z, _, _, _ = data(6, O, 1, dt, dev)
+    at = torch.tensor([0, O // 2, O - 1] * 2, device=dev)
+    z[torch.arange(6, device=dev), at] = torch.tensor([INF] * 3 + [math.nan] * 3, device=dev, dtype=dt)
+    for top in {1, min(2, O)}:
+        assert torch.equal(run(z, None, top)["top_labels"][:, 0], at)
 
 
 @pytest.mark.parametrize("scale", [1e-3, 30.0, 1e4, 1e38])
