@@ -231,7 +231,7 @@ struct Space {
 };
 
 struct Product {
-    Matrix a[2], b[2];  // two of each where the mode has two
+    Matrix a[2], b[2];  // two of each where the mode has two, of one pitch
     int64_t M, N, K;
 };
 
@@ -361,9 +361,9 @@ struct Packer {
     Packs packs{};
     uint32_t blocks = 0;
     template <int DT>
-    Matrix add(const Matrix& m, Space& ws, bool used) {
+    Matrix add(const Matrix& m, Space& ws, bool used, bool as_it_lies = true) {
         constexpr bool parts = DT == HASTE_DTYPE_F32;
-        if (!parts && plain_rows(m)) return m;
+        if (!parts && as_it_lies && plain_rows(m)) return m;
         const int64_t P = round8(m.cols), plane = parts ? m.rows * P * 2 : 0;
         void* to = ws.take(m.rows * P * 2 * (parts ? 3 : 1));
         if (used && m.rows > 0) {
@@ -372,6 +372,13 @@ struct Packer {
             blocks += (uint32_t)ceil_div(m.rows * (P / 8), 256);
         }
         return Matrix{to, P, m.rows, m.cols, plane};
+    }
+    // Two operands of one product, which have one pitch: both as they lie or both as copies.
+    template <int DT>
+    void add_pair(Matrix& a, Matrix& b, Space& ws, bool used) {
+        const bool as_they_lie = plain_rows(a) && plain_rows(b) && a.ld == b.ld;
+        a = add<DT>(a, ws, used, as_they_lie);
+        b = add<DT>(b, ws, used, as_they_lie);
     }
     template <int DT>
     void launch(hipStream_t st) const {
@@ -406,8 +413,7 @@ int64_t forward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, const
     }
     Packer packer;
     x = packer.add<DT>(x, ws, true);
-    wg = packer.add<DT>(wg, ws, true);
-    wu = packer.add<DT>(wu, ws, true);
+    packer.add_pair<DT>(wg, wu, ws, true);
     wd = packer.add<DT>(wd, ws, true);
     const Matrix h{out.h, out.ld, s.N, s.H, out.plane};
     const Product p1{{x, x}, {wg, wu}, s.N, s.H, s.D};
@@ -435,8 +441,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
     void *dg = ws.take(bytes), *du = ws.take(bytes);
     Packer packer;
     x = packer.add<DT>(x, ws, to.dwg || to.dwu);
-    wg = packer.add<DT>(wg, ws, to.dx);
-    wu = packer.add<DT>(wu, ws, to.dx);
+    packer.add_pair<DT>(wg, wu, ws, to.dx);
     wd = packer.add<DT>(wd, ws, to.dx || to.dwg || to.dwu);
     dy = packer.add<DT>(dy, ws, true);
     const Matrix mg{dg, ld, s.N, s.H, plane}, mu{du, ld, s.N, s.H, plane}, mh{h, ld, s.N, s.H, plane};

@@ -23,8 +23,10 @@ Weights weights_of(const at::Tensor& gate, const at::Tensor& up, const at::Tenso
                    dtype_code(gate.scalar_type())};
 }
 
-// Whether the kernels take all of these rows where they lie (16-bit: on 16 bytes).
-bool aligned(std::initializer_list<const Rows*> rows) {
+// Whether the kernels take all of these rows where they lie (16-bit: on 16 bytes, both projections at one
+// pitch).
+bool aligned(const Weights& w, std::initializer_list<const Rows*> rows) {
+    if (w.gate.ld != w.up.ld) return false;
     for (const Rows* r : rows)
         if (reinterpret_cast<uintptr_t>(ptr(r->t)) % 16 != 0 || r->ld % 8 != 0 || r->t.size(1) % 8 != 0)
             return false;
@@ -61,7 +63,7 @@ Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& u
     }
     int64_t size;
     const at::Tensor ws =
-        workspace(N, w, false, aligned({&r, &w.gate, &w.up, &w.down}), options, &size);
+        workspace(N, w, false, aligned(w, {&r, &w.gate, &w.up, &w.down}), options, &size);
     call(haste_gated_mlp(ptr(r.t), r.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld, ptr(w.down.t),
                          w.down.ld, out_ptr(f.y), out_ptr(f.kept), out_ptr(f.h), N,
                          w.D, w.H, w.O, act, w.code, out_ptr(ws), size, stream_of(x)));
@@ -103,7 +105,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
             if (need & kDown) dd = at::empty({w.O, w.H}, options);
             int64_t size;
             const at::Tensor ws =
-                workspace(N, w, true, aligned({&x, &dy, &w.gate, &w.up, &w.down}), options, &size);
+                workspace(N, w, true, aligned(w, {&x, &dy, &w.gate, &w.up, &w.down}), options, &size);
             call(haste_gated_mlp_bwd(ptr(x.t), x.ld, ptr(w.gate.t), w.gate.ld, ptr(w.up.t), w.up.ld,
                                      ptr(w.down.t), w.down.ld, ptr(dy.t), dy.ld, ptr(saved[4]),
                                      ptr(saved[5]), out_ptr(dx), out_ptr(dg),

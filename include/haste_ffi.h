@@ -696,7 +696,7 @@ int haste_embedding_bwd(const void* tokens, int32_t token_bits, const void* dy, 
  * come out as NaN).  D, H and O up to 2^20, N below 2^30, N D and N O below 2^34.
  * ws: workspace of haste_gated_mlp_workspace_size(N, D, H, O, dtype, backward, aligned) bytes (16-byte
  * aligned).  16-bit rows that do not start on 16 bytes, or are no multiple of 8 long, are copied into
- * it; with aligned != 0 there are none.
+ * it, and so are wg and wu of two pitches; with aligned != 0 there are none of either.
  */
 #define HASTE_ACT_SILU 0      /* x / (1 + e^-x) */
 #define HASTE_ACT_GELU 1      /* x (1 + erf(x / sqrt 2)) / 2 */

@@ -84,6 +84,9 @@ def test_gated_mlp_sizes():
     need = size(100, 8, 16, 8, BF16, 1, 0)
     assert _call("haste_gated_mlp_bwd", MLP_BWD, x=66, dy=66, wg=66, wu=66, wd=66, ws_bytes=need - 1) == WS
     assert _call("haste_gated_mlp", MLP, N=0) == OK
+    # two pitches of the projections: both are copied
+    assert _call("haste_gated_mlp", MLP, ldu=16, ws_bytes=size(100, 8, 16, 8, BF16, 0, 1)) == WS
+    assert _call("haste_gated_mlp_bwd", MLP_BWD, ldg=16, ws_bytes=size(100, 8, 16, 8, BF16, 1, 1)) == WS
 
 
 LP = dict(z=64, ldz=50, labels=64, bits=64, L=2, stats=None, lp=64, ent=64, top=64, top_labels=64, B=4, O=50,

@@ -190,6 +190,22 @@ def test_layouts(dev, kind, dt, N):
     check(d)
 
 
+@pytest.mark.parametrize("pads", [(0, 8), (8, 0), (16, 8), (0, 3), (3, 0), (5, 8), (8, 5)])
+@pytest.mark.parametrize("N,H", [(40, 96), (200, 96), (600, 1001)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_projections_of_two_pitches(dev, pads, N, H, dt):
+    """w_gate and w_up with rows at different pitches: the bits of plain ones."""
+    d = data(N, 64, H, 72, dt, dev, seed=1)
+    want = run(d)
+    for k, pad in zip(("wg", "wu"), pads):
+        wide = torch.full((H, 64 + pad), float("nan"), dtype=dt, device=dev)
+        wide[:, :64] = d[k]
+        d[k] = wide[:, :64]
+    got = run(d)
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+
+
 def test_pitches_with_rubbish_between_rows(dev):
     """What lies between rows that are read in place is not taken for zeros."""
     for dt in (torch.bfloat16, torch.float16):
