@@ -32,6 +32,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(4);
         if (!grads[0].defined()) return out;
+        check_gradients("embedding", grads);
         const at::Tensor tokens = ctx->get_saved_variables()[0];
         {
             const at::AutoGradMode off(false);

@@ -87,6 +87,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(5);
         if (!grads[0].defined()) return out;
+        check_gradients("gated_mlp", grads);
         const int64_t need = ctx->saved_data["need"].toInt();
         const variable_list saved = ctx->get_saved_variables();
         {

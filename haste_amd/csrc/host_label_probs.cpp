@@ -62,6 +62,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(3);
+        check_gradients("label_log_probs", grads);
         const bool given = ctx->saved_data["labels"].toBool();
         const at::Tensor dent = dense(grads[0]), dlp = given ? dense(grads[1]) : at::Tensor();
         if (!dent.defined() && !dlp.defined()) return out;

@@ -90,6 +90,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_gradients("layer_norm", grads);
         at::Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : at::Tensor();
         const int64_t need = ctx->saved_data["need"].toInt();
         const variable_list saved = ctx->get_saved_variables();

@@ -60,6 +60,12 @@ inline void check_no_tangent(const char* what, std::initializer_list<const at::T
                                     ": forward-mode derivatives are not supported");
 }
 
+// A backward's own checks: a tangent may come with its gradients alone, and a tracer run over it alone.
+inline void check_gradients(const char* what, const variable_list& grads) {
+    check_not_traced(what);
+    for (const at::Tensor& g : grads) check_no_tangent(what, {&g});
+}
+
 // A backward's results under create_graph: what is differentiated again says so, and is not taken for a
 // constant.
 inline void once_differentiable(const char* what, variable_list& out) {
