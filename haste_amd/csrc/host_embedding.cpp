@@ -90,7 +90,7 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t count) {
             if (padding < 0) padding += V;
         }
         const c10::DeviceGuard guard(weight.device());
-        tokens = tokens.contiguous();
+        tokens = dense(tokens);
         y = at::GradMode::is_enabled() && weight.requires_grad()
                 ? Embedding::apply(tokens, weight, scale, padding)
                 : forward(tokens, weight, scale);

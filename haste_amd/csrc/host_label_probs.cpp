@@ -37,11 +37,6 @@ Forward forward(const at::Tensor& logits, const at::Tensor& labels, int64_t top,
     return f;
 }
 
-// A gradient as contiguous fp32, or undefined.
-at::Tensor dense(const at::Tensor& g) {
-    return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).contiguous() : g;
-}
-
 struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& logits,
                                  const std::optional<at::Tensor>& labels_arg, int64_t top) {
@@ -136,7 +131,7 @@ PyObject* label_log_probs(PyObject*, PyObject* const* args, Py_ssize_t count) {
         pybind11::gil_scoped_release no_gil;
         check(logits, labels, top);
         const c10::DeviceGuard guard(logits.device());
-        if (labels.defined()) labels = labels.contiguous();
+        labels = dense(labels);
         if (at::GradMode::is_enabled() && logits.requires_grad()) {
             const variable_list out =
                 LabelLogProbs::apply(logits, std::optional<at::Tensor>(labels), top);

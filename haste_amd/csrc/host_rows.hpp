@@ -37,6 +37,11 @@ inline Rows rows_of(const at::Tensor& x, int64_t D) {
     return Rows{t, ld};
 }
 
+// t contiguous and with its sign applied, or undefined.
+inline at::Tensor dense(const at::Tensor& t) {
+    return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t;
+}
+
 inline const void* ptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 inline void* out_ptr(const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
