@@ -440,10 +440,12 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
     const int64_t plane = DT == HASTE_DTYPE_F32 ? s.N * ld * 2 : 0, bytes = hidden_bytes(s.N, ld, DT);
     void *dg = ws.take(bytes), *du = ws.take(bytes);
     Packer packer;
-    x = packer.add<DT>(x, ws, to.dwg || to.dwu);
-    packer.add_pair<DT>(wg, wu, ws, to.dx);
-    wd = packer.add<DT>(wd, ws, to.dx || to.dwg || to.dwu);
-    dy = packer.add<DT>(dy, ws, true);
+    if (s.N > 0) {  // (without rows the products of K = 0 read nothing)
+        x = packer.add<DT>(x, ws, to.dwg || to.dwu);
+        packer.add_pair<DT>(wg, wu, ws, to.dx);
+        wd = packer.add<DT>(wd, ws, to.dx || to.dwg || to.dwu);
+        dy = packer.add<DT>(dy, ws, true);
+    }
     const Matrix mg{dg, ld, s.N, s.H, plane}, mu{du, ld, s.N, s.H, plane}, mh{h, ld, s.N, s.H, plane};
     const Product p1{{dy, dy}, {wd, wd}, s.N, s.H, s.O};
     const Product p2{{mg, mu}, {wg, wu}, s.N, s.D, s.H};
@@ -596,6 +598,7 @@ extern "C" int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, i
         HASTE_TRY(haste::mlp_hidden(fn, "kept", kept));
         HASTE_TRY(haste::mlp_hidden(fn, "h", h));
     }
+    if (N == 0 && !dwg && !dwd) return HASTE_OK;
     const haste::Grads to{dx, dwg, dwu, dwd};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {

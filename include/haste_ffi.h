@@ -714,7 +714,8 @@ int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64_t ldg, con
  * Its gradients, from the kept and h of the forward:
  *   dh = dy wd;  dg = dh act'(g) u, du = dh act(g)  (rounded to dtype);
  *   dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h,
- * all contiguous.  dx, dwd, or dwg together with dwu may be NULL (not computed).
+ * all contiguous.  dx, dwd, or dwg together with dwu may be NULL (not computed).  With N = 0 nothing is
+ * read, and the weights' gradients are zeros.
  */
 int haste_gated_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
                         int64_t ldu, const void* wd, int64_t ldd, const void* dy, int64_t lddy,
