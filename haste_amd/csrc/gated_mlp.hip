@@ -457,7 +457,7 @@ int64_t backward(const Sizes& s, Matrix x, Matrix wg, Matrix wu, Matrix wd, Matr
     if (launch) {
         packer.launch<DT>(st);
         if (s.N > 0 && (to.dx || to.dwg || to.dwu)) {
-            const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld, plane};
+            const GatedGrad out{{kept, kept_blocks(s.H)}, dg, du, ld, plane, (int)s.H};
             product<DT, GemmMode::kPlain, true, false>(p1, cut_of<GemmMode::kPlain, DT>(p1, false), 0, out,
                                                        st);
         }
@@ -531,7 +531,7 @@ extern "C" int64_t haste_gated_mlp_workspace_size(int64_t N, int64_t D, int64_t 
 #define HASTE_MLP(DT)                                                                                   \
     (backward ? haste::backward<DT>(s, x, wg, wg, wd, dy, nullptr, nullptr, ld, haste::Grads{}, \
                                     nullptr, false, nullptr)                                          \
-              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{{nullptr, 0}, nullptr, ld, 0},     \
+              : haste::forward<DT>(s, x, wg, wg, wd, haste::GatedOut{{nullptr, 0}, nullptr, ld, 0, (int)H},     \
                                    nullptr, 0, nullptr, false, nullptr))
     return HASTE_MLP_TYPES(HASTE_MLP);
 #undef HASTE_MLP
@@ -561,7 +561,7 @@ extern "C" int haste_gated_mlp(const void* x, int64_t ldx, const void* wg, int64
     HASTE_TRY(haste::mlp_hidden(fn, "h", h));
     if (kept) HASTE_TRY(haste::mlp_hidden(fn, "kept", kept));
     const haste::GatedOut out{{kept, haste::kept_blocks(H)}, h, haste::round16(H),
-                              dtype == HASTE_DTYPE_F32 ? N * haste::round16(H) * 2 : 0};
+                              dtype == HASTE_DTYPE_F32 ? N * haste::round16(H) * 2 : 0, (int)H};
     hipStream_t st = static_cast<hipStream_t>(stream);
     auto run = [&](char* base, bool launch) {
 #define HASTE_MLP(DT) haste::forward<DT>(s, mx, mg, mu, md, out, y, act, base, launch, st)

@@ -195,12 +195,24 @@ __device__ __forceinline__ f32x4 kept_columns(const Kept<DT>& k, int j) {
                  __uint_as_float(__builtin_amdgcn_perm(h1, lo, 0x0706030Cu))};
 }
 
+// Columns n and on, those from H on as zeros.  They come out of products with zeros, but a row with an infinity
+// makes those NaN, and the next product would take that to all of the row.
+template <int F>
+__device__ __forceinline__ void zero_from(f32x4 (&v)[F], int n, int H) {
+    if (n + 4 * F <= H) return;
+#pragma unroll
+    for (int k = 0; k < F; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = n + 4 * k + e < H ? v[k][e] : 0.f;
+}
+
 // Columns n (a multiple of 4 F) and on of row m: h, and s and a where the backward will want them.  Rows of
-// h are ld apart, a multiple of 16 that holds them; columns past the extent come out as zeros.
+// h are ld apart, a multiple of 16 that holds them; columns from H on come out as zeros.
 struct GatedOut {
     KeptPlace kept;
     void* h;
     int64_t ld, plane;
+    int H;
     template <int DT, int ACT, int F>
     __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&vg)[F], const f32x4 (&vu)[F]) const {
         f32x4 vh[F], vs[F], va[F];
@@ -214,6 +226,7 @@ struct GatedOut {
                 vs[k][e] = s * vu[k][e];
                 vh[k][e] = a * vu[k][e];
             }
+        zero_from<F>(vh, n, H);
         put_operand<DT, F>(h, plane, m * ld + n, vh);
         if (!kept.p) return;
         char* block = kept.template block<DT>(m, n);
@@ -226,15 +239,18 @@ struct GatedGrad {
     KeptPlace kept;
     void *dg, *du;
     int64_t ld, plane;
+    int H;
     template <int DT, int F>
     __device__ __forceinline__ void put(int64_t m, int n, const f32x4 (&dh)[F], const Kept<DT>& s,
                                         const Kept<DT>& a) const {
         f32x4 v[F];
 #pragma unroll
         for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(s, k);
+        zero_from<F>(v, n, H);
         put_operand<DT, F>(dg, plane, m * ld + n, v);
 #pragma unroll
         for (int k = 0; k < F; ++k) v[k] = dh[k] * kept_columns<DT>(a, k);
+        zero_from<F>(v, n, H);
         put_operand<DT, F>(du, plane, m * ld + n, v);
     }
 };

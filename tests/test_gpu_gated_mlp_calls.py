@@ -20,3 +20,39 @@ def test_no_rows(dev, dt, sizes):
         got = torch.autograd.grad([y], [x, *w], [torch.zeros_like(y)])
         assert y.shape == (0, O) and [g.shape for g in got] == [t.shape for t in (x, *w)]
         assert not any(g.any() for g in got)     # (NaN counts as true)
+
+
+def positive(N, D, H, O, dt, dev):
+    """Everything above zero: sums of infinities of one sign are infinite."""
+    g = torch.Generator(device=dev).manual_seed(N + H)
+    r = lambda *s: (torch.rand(*s, generator=g, device=dev) * 0.5 + 0.25).to(dt)  # noqa: E731
+    return dict(x=r(N, D), wg=r(H, D), wu=r(H, D), wd=r(O, H), dy=r(N, O))
+
+
+@pytest.mark.parametrize("N", [40, 70, 300])
+@pytest.mark.parametrize("H", [3, 8, 13, 1003])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh"])
+def test_an_infinite_input_among_positive_ones(dev, N, H, dt, name):
+    """Both projections, h and y of its row are +infinity, whatever the hidden width."""
+    d = positive(N, 8, H, 5, dt, dev)
+    clean = ops.gated_mlp(d["x"], d["wg"], d["wu"], d["wd"], activation=name)
+    d["x"][7, 2] = float("inf")
+    y = ops.gated_mlp(d["x"], d["wg"], d["wu"], d["wd"], activation=name)
+    assert (y[7] == float("inf")).all(), y[7]
+    keep = torch.arange(N, device=dev) != 7
+    assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("N", [40, 300])
+@pytest.mark.parametrize("H", [3, 8, 13, 1003])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_an_infinite_gradient_among_positive_ones(dev, N, H, dt):
+    """With gates above zero silu rises: dh, dg, du and dx of the row are +infinity."""
+    d = positive(N, 8, H, 5, dt, dev)
+    x = d["x"].requires_grad_(True)
+    y = ops.gated_mlp(x, d["wg"], d["wu"], d["wd"])
+    d["dy"][7, 2] = float("inf")
+    dx, = torch.autograd.grad([y], [x], [d["dy"]])
+    assert (dx[7] == float("inf")).all(), dx[7]
+    assert dx[torch.arange(N, device=dev) != 7].isfinite().all()
