@@ -70,7 +70,7 @@ Forward forward(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& u
     return f;
 }
 
-enum { kX = 1, kGate = 2, kUp = 4, kDown = 8 };
+enum { kX, kGate, kUp, kDown };  // the node's inputs
 
 struct GatedMlp : torch::autograd::Function<GatedMlp> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
@@ -78,9 +78,6 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
         Forward f = haste_host::forward(x, gate, up, down, (int)act, true);
         ctx->save_for_backward({x, gate, up, down, f.kept, f.h});
         ctx->set_materialize_grads(false);
-        ctx->saved_data["need"] =
-            (int64_t)((x.requires_grad() ? kX : 0) | (gate.requires_grad() ? kGate : 0) |
-                      (up.requires_grad() ? kUp : 0) | (down.requires_grad() ? kDown : 0));
         return f.y;
     }
 
@@ -88,7 +85,9 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
         variable_list out(5);
         if (!grads[0].defined()) return out;
         check_gradients("gated_mlp", grads);
-        const int64_t need = ctx->saved_data["need"].toInt();
+        // (what the engine wants now: autograd.grad may ask for fewer than require one)
+        const bool need_x = ctx->needs_input_grad(kX), need_gate = ctx->needs_input_grad(kGate),
+                   need_up = ctx->needs_input_grad(kUp), need_down = ctx->needs_input_grad(kDown);
         const variable_list saved = ctx->get_saved_variables();
         {
             const at::AutoGradMode off(false);
@@ -98,12 +97,12 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
             const auto options =
                 at::TensorOptions().dtype(x.t.scalar_type()).device(x.t.device());
             at::Tensor dx, dg, du, dd;
-            if (need & kX) dx = at::empty(saved[0].sizes(), options);
-            if (need & (kGate | kUp)) {
+            if (need_x) dx = at::empty(saved[0].sizes(), options);
+            if (need_gate || need_up) {
                 dg = at::empty({w.H, w.D}, options);
                 du = at::empty({w.H, w.D}, options);
             }
-            if (need & kDown) dd = at::empty({w.O, w.H}, options);
+            if (need_down) dd = at::empty({w.O, w.H}, options);
             int64_t size;
             const at::Tensor ws =
                 workspace(N, w, true, aligned(w, {&x, &dy, &w.gate, &w.up, &w.down}), options, &size);
@@ -113,8 +112,8 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
                                      out_ptr(du), out_ptr(dd), N, w.D, w.H, w.O, w.code, out_ptr(ws),
                                      size, stream_of(x.t)));
             out[0] = dx;
-            if (need & kGate) out[1] = dg;
-            if (need & kUp) out[2] = du;
+            if (need_gate) out[1] = dg;
+            if (need_up) out[2] = du;
             out[3] = dd;
         }
         once_differentiable("gated_mlp", out);

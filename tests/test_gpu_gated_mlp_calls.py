@@ -56,3 +56,25 @@ def test_an_infinite_gradient_among_positive_ones(dev, N, H, dt):
     dx, = torch.autograd.grad([y], [x], [d["dy"]])
     assert (dx[7] == float("inf")).all(), dx[7]
     assert dx[torch.arange(N, device=dev) != 7].isfinite().all()
+
+
+def test_gradients_that_the_engine_does_not_want(dev):
+    """autograd.grad of some inputs takes no memory for the others' gradients, and gives the same bits."""
+    N, D, H, O = 80, 1024, 4096, 1024
+    g = torch.Generator(device=dev).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(torch.bfloat16)  # noqa: E731
+    leaves = [t.requires_grad_(True) for t in (r(N, D), r(H, D), r(H, D), r(O, H))]
+    dy = r(N, O)
+    want = torch.autograd.grad([ops.gated_mlp(*leaves)], leaves, [dy])
+    weight = H * D * 2                                     # bytes of any one weight's gradient
+    for some in ([0], [3], [0, 3]):
+        y = ops.gated_mlp(*leaves)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(dev)
+        before = torch.cuda.memory_allocated(dev)
+        got = torch.autograd.grad([y], [leaves[k] for k in some], [dy])
+        torch.cuda.synchronize()
+        # what is returned, and a workspace: dg, du and the parts of the products, all under two weights' size
+        room = (weight if 3 in some else 0) + 2 * weight
+        assert torch.cuda.max_memory_allocated(dev) - before < room, some
+        assert all(torch.equal(a, want[k]) for a, k in zip(got, some))
