@@ -11,6 +11,7 @@
 
 #include "gated_mlp.hpp"
 #include "gemm.hpp"
+#include "launches.hpp"
 
 namespace haste {
 namespace {
@@ -168,7 +169,8 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(const char* x, int
 }
 
 // Matrices [R, C] of any pitch as rows of P (a multiple of 8) elements on 16 bytes, with zeros behind C;
-// fp32 ones as their three parts.  One launch for all that a call has.
+// fp32 ones as their three parts.  One launch for all that a call has (or as many as they need: `first` is
+// the launch's first workgroup).
 constexpr int kMaxPacks = 5;
 struct Packs {
     struct {
@@ -180,12 +182,13 @@ struct Packs {
     int count;
 };
 template <bool F32>
-__global__ __launch_bounds__(256) void pack_rows_kernel(Packs p) {
+__global__ __launch_bounds__(256) void pack_rows_kernel(Packs p, uint32_t first) {
     constexpr int DT = F32 ? HASTE_DTYPE_F32 : HASTE_DTYPE_BF16;
+    const uint32_t block = first + blockIdx.x;
     int k = 0;
-    for (int j = 1; j < p.count; ++j) k = blockIdx.x >= p.m[j].block0 ? j : k;
+    for (int j = 1; j < p.count; ++j) k = block >= p.m[j].block0 ? j : k;
     const auto& m = p.m[k];
-    const int64_t i = (int64_t)(blockIdx.x - m.block0) * 256 + threadIdx.x, pieces = m.P / 8;
+    const int64_t i = (int64_t)(block - m.block0) * 256 + threadIdx.x, pieces = m.P / 8;
     if (i >= m.R * pieces) return;
     const int64_t r = i / pieces, c = i % pieces * 8;
     const Elems<DT, 8> v = load_part<DT, 8>(m.src + r * m.ld * kElemBytes<DT>, c, m.C - c);
@@ -359,7 +362,7 @@ struct Sizes {
 // Matrices with 16-byte rows (fp32: their parts): themselves, or copies in the workspace, made by one launch.
 struct Packer {
     Packs packs{};
-    uint32_t blocks = 0;
+    uint32_t blocks = 0;  // (five matrices of up to 2^40 elements, 2^11 to a workgroup: under 2^32)
     template <int DT>
     Matrix add(const Matrix& m, Space& ws, bool used, bool as_it_lies = true) {
         constexpr bool parts = DT == HASTE_DTYPE_F32;
@@ -382,8 +385,10 @@ struct Packer {
     }
     template <int DT>
     void launch(hipStream_t st) const {
-        if (blocks)
-            pack_rows_kernel<DT == HASTE_DTYPE_F32><<<dim3(blocks), dim3(256), 0, st>>>(packs);
+        in_launches_of(blocks, 256, [&](int64_t first, int64_t count) {
+            pack_rows_kernel<DT == HASTE_DTYPE_F32>
+                <<<dim3((unsigned)count), dim3(256), 0, st>>>(packs, (uint32_t)first);
+        });
     }
 };
 
@@ -479,7 +484,7 @@ int mlp_sizes(const char* fn, int64_t N, int64_t D, int64_t H, int64_t O, int32_
                     (long long)N, (long long)D, (long long)H, (long long)O);
     HASTE_CHECK_ARG(D <= kMaxSide && H <= kMaxSide && O <= kMaxSide && N < (int64_t)1 << 30,
                     "%s: too large (D, H and O up to 2^20, N below 2^30)", fn);
-    // (a launch over the pieces of x or dy has fewer than 2^32 threads)
+    // (so that a product's launch has fewer than 2^32 threads, 512 to a tile of 256 x 256)
     HASTE_CHECK_ARG(N * std::max(D, O) < (int64_t)1 << 34, "%s: too large (N D and N O below 2^34)", fn);
     HASTE_CHECK_ARG(elem_dtype(dtype), "%s: matrices must be bf16, f16 or f32", fn);
     return HASTE_OK;

@@ -1,4 +1,7 @@
 """CPU: calls of the gated block's C entry points that start no kernel and say so."""
+import os
+import subprocess
+
 import pytest
 
 from haste_amd import _lib
@@ -17,3 +20,13 @@ def test_backward_of_no_rows_takes_no_weights(dt, D, H, O):
     for weight in (None, 66):
         assert L.haste_gated_mlp_bwd(None, D, weight, D, weight, D, weight, H, None, O, None, None, None, None,
                                      None, None, 0, D, H, O, dt, None, 0, None) == _lib.HASTE_OK, _lib.last_error()
+
+
+def test_how_copies_are_cut_into_launches(tmp_path):
+    """The arithmetic, on the CPU: tests/native/launches_check.cpp."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "launches_check")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(here, "native", "launches_check.cpp"),
+                    "-o", exe], check=True, timeout=120)
+    out = subprocess.run([exe], check=True, capture_output=True, text=True, timeout=60).stdout
+    assert "launches_check OK" in out

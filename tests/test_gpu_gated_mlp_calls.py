@@ -78,3 +78,34 @@ def test_gradients_that_the_engine_does_not_want(dev):
         room = (weight if 3 in some else 0) + 2 * weight
         assert torch.cuda.max_memory_allocated(dev) - before < room, some
         assert all(torch.equal(a, want[k]) for a, k in zip(got, some))
+
+
+def test_copies_of_more_than_a_launch(dev):
+    """Two projections of 2^34 elements each, whose rows do not start on 16 bytes: their copies take 2^32 threads and
+    more.  Every weight is a power of two of its row and column, so that both projections are known exactly."""
+    N, H, D = 65, 1 << 17, (1 << 17) + 1
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(dev)[0] < 170 << 30:
+        pytest.skip("needs 170 GiB")
+    # x is 1 in three columns; a weight is 2^-(row mod 8) there (the up projection: 2^-(row mod 4)), else rubbish
+    # that a zero of x takes out
+    cols = [0, D // 2, D - 1]
+    x = torch.zeros(N, D, device=dev, dtype=torch.bfloat16)
+    x[:, cols] = 1
+    rows = torch.arange(H, device=dev)
+    w = []
+    for mod in (8, 4):
+        t = torch.full((H, D), 3.0, device=dev, dtype=torch.bfloat16)
+        for c in cols:
+            t[:, c] = torch.exp2(-(rows % mod).float())
+        w.append(t)
+    down = torch.zeros(8, H, device=dev, dtype=torch.bfloat16)
+    pick = torch.tensor([0, 1, 7, 4096, 70001, H // 2 + 5, H - 2, H - 1], device=dev)
+    down[torch.arange(8, device=dev), pick] = 1
+    y = ops.gated_mlp(x, *w, down)
+    del w, t
+    g, u = (3 * torch.exp2(-(pick % mod).double()) for mod in (8, 4))
+    h = g * torch.sigmoid(g) * u
+    # (act within 2^-20 of itself, h rounded to bf16, then exact)
+    assert ((y.double() - h).abs() <= h * (2.0 ** -8 + 2.0 ** -19)).all()
+    torch.cuda.empty_cache()
