@@ -472,11 +472,12 @@ __global__ __launch_bounds__(kThreads) void lp_bwd_kernel(const char* z, int64_t
             if (j >= 0 && j < O) sum += dlp[row * L + l];
         }
     const float c0 = -sum - ge * H;
-    // (16-bit gradients have no use for the last bits of e^d)
+    // (16-bit gradients have no use for the last bits of e^d.  The instruction gives 0 for what is under 2^-126,
+    // where bf16 has values yet once the factor, up to some hundreds, is in: it takes 2^24 e^d.)
     auto base = [&](float x) __attribute__((always_inline)) {
-        const float d = x - m;
-        const float p = (DT == HASTE_DTYPE_F32 ? expf(d) : __builtin_amdgcn_exp2f(d * kLog2e)) * inv;
-        return p * __builtin_fmaf(-ge, fmaxf(d, kGone) - log_s, c0);
+        const float d = x - m, by = __builtin_fmaf(-ge, fmaxf(d, kGone) - log_s, c0);
+        if constexpr (DT == HASTE_DTYPE_F32) return expf(d) * inv * by;
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(d, kLog2e, 24.f)) * inv * by * 0x1p-24f;
     };
     for (int64_t e0 = from + threadIdx.x * V; e0 < to; e0 += kThreads * V) {
         float f[V];
