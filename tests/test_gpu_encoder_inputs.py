@@ -27,3 +27,15 @@ def test_lazily_negated_tokens_and_labels(dev, dt):
                           torch.autograd.grad([lp], [x], [torch.ones_like(lp)])[0]])
         for a, b in zip(*grads):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N", [262143, 262144, 262145, 400000])
+def test_one_token_in_more_than_1024_windows(dev, N):
+    """Windows are 256 places, and longer from 262,144 tokens on.  Whole numbers: every partial sum is exact."""
+    g = torch.Generator(device=dev).manual_seed(N)
+    w = torch.zeros(5, 24, device=dev, requires_grad=True)
+    tokens = torch.where(torch.rand(N, generator=g, device=dev) < 0.97, 2, 4)
+    dy = torch.randint(-3, 4, (N, 24), generator=g, device=dev).float()
+    dw, = torch.autograd.grad([ops.embedding(tokens, w)], [w], [dy])
+    for v in range(5):
+        assert torch.equal(dw[v], dy[tokens == v].sum(0)), v
