@@ -45,6 +45,12 @@ void clear_error();
         }                                                                         \
     } while (0)
 
+#define HASTE_TRY(expr)                  \
+    do {                                 \
+        const int rc_ = (expr);          \
+        if (rc_ != HASTE_OK) return rc_; \
+    } while (0)
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -117,6 +123,12 @@ __device__ __forceinline__ uint32_t pack2_rne<BF16>(float a, float b) {
 template <>
 __device__ __forceinline__ uint32_t pack2_rne<F16>(float a, float b) {
     return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+}
+
+// Until the wave's LDS accesses before are done, for those after.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // ---------------------------------------------------------------- MFMA ------

@@ -149,10 +149,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool in) {
     }
     return same;
 }
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
+
 // The place of a lane's key, from the next place of its digit in the wave's keys (in order).
 __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t d, int bits, bool in, int lane) {
     const uint64_t same = same_digit(d, bits, in);
@@ -568,12 +565,6 @@ int check_rows(const char* fn, const char* what, const void* p, int64_t ld, int6
                     (long long)ld, (long long)D);
     return HASTE_OK;
 }
-
-#define HASTE_TRY(expr)                  \
-    do {                                 \
-        const int rc_ = (expr);          \
-        if (rc_ != HASTE_OK) return rc_; \
-    } while (0)
 
 // `call` with DT and V: 16-byte vectors, or elements where a row is shorter than one.
 #define HASTE_EMB_TYPES(call)                                                \

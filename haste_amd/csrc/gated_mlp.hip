@@ -513,12 +513,6 @@ int mlp_act(const char* fn, int32_t act) {
     return HASTE_OK;
 }
 
-#define HASTE_TRY(expr)                  \
-    do {                                 \
-        const int rc_ = (expr);          \
-        if (rc_ != HASTE_OK) return rc_; \
-    } while (0)
-
 }  // namespace
 }  // namespace haste
 

@@ -71,11 +71,6 @@ __device__ __forceinline__ float value_of(Key k) {
 }
 __device__ __forceinline__ uint32_t label_of(Key k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }

@@ -579,12 +579,6 @@ void with_slots(int C, F f) {
     else f(std::integral_constant<int, 4>());
 }
 
-#define HASTE_TRY(expr)                        \
-    do {                                       \
-        const int rc_ = (expr);                \
-        if (rc_ != HASTE_OK) return rc_;       \
-    } while (0)
-
 // `call` with DT and WT for the types of a call.
 #define HASTE_LN_TYPES(call)                                                                 \
     do {                                                                                     \
