@@ -320,7 +320,8 @@ void product(const Product& p, Cut cut, int act, const Epilogue& out, hipStream_
         // An epilogue that moves 8 to 10 bytes an element takes longer than a short K: two workgroups
         // to a CU, of 256 x 128, overlap one's with the other's products (65536 x 2048 elements, K =
         // 768: h 585 -> 565 us, dg and du 473 -> 430; 16384 x 8192, K = 4096: 1922 -> 2193, 1131 ->
-        // 1308, since they load half as much again).
+        // 1308, since they load half as much again).  In between, for the whole forward of 65536 x 2048:
+        // K = 1280 1097 -> 1119 us, 1536 1245 -> 1284, 2048 1549 -> 1635; 16384 x 8192: K = 1280 the same.
         typedef GemmTile<T, MODE, AK, BK_, 8, 4, 2, 2, 3> Half;
         if (cut.tiles == Tiles::kLarge && p.K <= 1024)
             return launch_tiles<Half, DT>(gemm_args<Half>(p, segments, cut.splits), batches, act, out, st);

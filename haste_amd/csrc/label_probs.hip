@@ -643,7 +643,7 @@ extern "C" int haste_label_log_probs_bwd(const void* z, int64_t ldz, const void*
                     "%s: a gradient is misaligned", fn);
     HASTE_CHECK_ARG(dz != nullptr && haste::elem_aligned(dz, dtype) && lddz >= O,
                     "%s: dz is NULL or misaligned, or its row pitch is short", fn);
-    // (32 elements to a thread)
+    // (four vectors to a thread)
     const int64_t V = 16 / haste::elem_bytes(dtype), most = haste::kThreads * V * 4;
     const int64_t S = haste::ceil_div(O, most);
     hipStream_t st = static_cast<hipStream_t>(stream);

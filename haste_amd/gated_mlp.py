@@ -5,8 +5,9 @@
   y = (act(x w_gate^T) * (x w_up^T)) w_down^T
 
 with both projections, the activation and their product in one kernel, and the gradients of x and
-all three weights.  Sums are fp32; what lies between the products (the hidden values and the gradients
-of the projections) is rounded to x's dtype, as the matrix instructions take it.  The backward needs
+all three weights (those that autograd wants; w_gate's and w_up's come together).  Sums are fp32; what lies
+between the products (the hidden values and the gradients of the projections) is rounded to x's dtype, as the matrix
+instructions take it (float16: past 65,504 they are infinite).  The backward needs
 8 bytes for each hidden value of 16-bit matrices, 14 of float32.  x and the weights: bfloat16,
 float16 or float32, all of one dtype; each float32 product is six of bfloat16 parts, whose rounding is
 float32's, but where an infinity comes in a NaN may come out.

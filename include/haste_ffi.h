@@ -666,7 +666,7 @@ int haste_adamw_step(const haste_adamw_tensor* tensors, int32_t count, int32_t w
                      const float* grad_scale, void* stream);
 
 /*
- * Embedding lookup: y[n] = RNE(scale * w[t_n]) for tokens t [N] of 32 or 64 bits (token_bits) and a
+ * Embedding lookup: y[n] = RNE(scale * w[t_n]), scale rounded to fp32, for tokens t [N] of 32 or 64 bits (token_bits) and a
  * table w [V, D] of row pitch ldw (elements, >= D; 0 reads one row for all); y is [N, D] contiguous.  A
  * token outside [0, V) gives a row of zeros.  dtype of w and y: bf16, f16 or f32.
  */
